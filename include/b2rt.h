@@ -405,6 +405,111 @@ int b2_mse_loss_fwd(const b2_mse_args* args, b2_stream_t stream);
 int b2_mse_loss_bwd(const b2_mse_args* args, b2_stream_t stream);
 uint64_t b2_mse_loss_workspace_bytes(int64_t n);
 
+/* ------------------------------------------------------------------------------------------ */
+/* 4-bit weights: OCP microscaling MXFP4 (E2M1 codes, one E8M0 scale per 32 columns)            */
+/* ------------------------------------------------------------------------------------------ */
+
+/* An MXFP4 matrix of `rows` x `cols`:
+ *   codes  [rows][b2_mx4_code_bytes(cols)]: two E2M1 codes a byte, the even column in the low nibble; rows are
+ *          padded with zero codes to a multiple of 32 columns, so each row is a multiple of 16 bytes;
+ *   scales [ceil(rows/128)][ceil(cols/128)][32][4][4] (b2_mx4_scale_bytes): the E8M0 scale (2^(code - 127)) of
+ *          row r, block j = col / 32 lies at [r / 128][j / 4][r % 32][(r % 128) / 32][j % 4], the order in which
+ *          the tensor core's scale columns are filled; scales of rows and blocks past the end are 0.
+ * Quantisation: scale = 2^(floor(log2(largest magnitude of the block)) - 2), at least 2^-127; each element is
+ * divided by it (exactly) and rounded to the nearest of 0, .5, 1, 1.5, 2, 3, 4, 6, ties to the even code,
+ * magnitudes above 6 become 6. A block that holds an infinity or a NaN gets the NaN scale (255) and zero codes, so
+ * the whole block reads back as NaN. */
+typedef struct b2_mx4_args {
+  const void* x;      /* quantize: input [rows][cols], unit column stride, row stride ld */
+  uint8_t* codes;     /* 16-byte aligned */
+  uint8_t* scales;    /* 16-byte aligned */
+  void* out;          /* dequantize: output [rows][cols], unit column stride, row stride ld */
+  int64_t rows, cols, ld;
+  int32_t dtype;      /* of x / out: F32, BF16 or F16 */
+  int32_t pad_;
+} b2_mx4_args;
+int b2_mx4_quantize(const b2_mx4_args* args, b2_stream_t stream);
+int b2_mx4_dequantize(const b2_mx4_args* args, b2_stream_t stream);
+int64_t b2_mx4_code_bytes(int64_t cols);
+int64_t b2_mx4_scale_bytes(int64_t rows, int64_t cols);
+
+/* Linear over a frozen MXFP4 weight W [N][K], with the LoRA side path as one more term of the same product.
+ *   transpose_w == 0 (forward): out[M][N] = A W^T + bias[N] + lora_h[M][r] lora_b[N][r]^T, A an MXFP4 matrix [M][K]
+ *                               (x_codes, x_scales); the element products are exact, the sums fp32;
+ *   transpose_w == 1 (dX):      out[M][K] = x[M][N] W + lora_h[M][r] lora_b[r][K], x bf16 (the straight-through
+ *                               gradient of the quantised activation).
+ * out is bf16 with row stride out_ld, bias bf16. lora_r = 0: no side path; else 8..64, a multiple of 8, bf16 rows
+ * with leading dims lora_h_ld / lora_b_ld.
+ * workspace: b2_mx4_gemm_workspace_bytes() bytes, 16-byte aligned (0: none needed). */
+typedef struct b2_mx4_gemm_args {
+  const uint8_t* x_codes; /* forward */
+  const uint8_t* x_scales;
+  const void* x;          /* dX */
+  const uint8_t* w_codes;
+  const uint8_t* w_scales;
+  const void* bias;       /* NULL: none (forward only) */
+  void* out;
+  const void* lora_h;
+  const void* lora_b;
+  void* workspace;
+  int64_t M, N, K;
+  int64_t x_ld, out_ld, lora_h_ld, lora_b_ld;
+  int32_t lora_r;
+  int32_t transpose_w;
+} b2_mx4_gemm_args;
+int b2_mx4_gemm(const b2_mx4_gemm_args* args, b2_stream_t stream);
+uint64_t b2_mx4_gemm_workspace_bytes(const b2_mx4_gemm_args* args);
+
+/* ------------------------------------------------------------------------------------------ */
+/* Attention with a learned relative position bias                                              */
+/* ------------------------------------------------------------------------------------------ */
+
+#define B2_BIAS_MAX_BUCKETS 128
+#define B2_BIAS_MAX_DISTANCE 1024
+
+/* Bucket of the relative position `rel` = key position - query position. One-sided (bidirectional == 0):
+ * n = max(-rel, 0) over nb = num_buckets buckets; two-sided: n = |rel| over nb = num_buckets / 2, plus nb where
+ * rel > 0. The first nb / 2 distances have a bucket each; distance n beyond gets
+ * first + floor((nb - first) * log(n / first) / log(max_distance / first)), first = nb / 2, at most nb - 1, in exact
+ * arithmetic. Needs 2 <= nb, num_buckets <= B2_BIAS_MAX_BUCKETS (even when two-sided) and
+ * nb / 2 < max_distance <= B2_BIAS_MAX_DISTANCE; -1 otherwise. */
+int b2_bias_bucket(int64_t rel, int32_t num_buckets, int32_t max_distance, int32_t bidirectional);
+
+/* O = softmax(scale * Q K^T + bias) V with bias[h][i][j] = table[bucket(j - i - q_offset)][h], keys masked by
+ * key_mask (bytes [B][Sk], 0 = masked; row stride mask_sb) and, when causal, keys j > i + q_offset. A row whose keys
+ * are all masked gives zeros (lse -inf) and zero gradients; K and V at masked positions are never used, whatever they
+ * hold. Query head h reads key/value head h / (H / Hk). Tensors are [B, heads, S, D] with (batch, head, seq) strides
+ * in elements and unit stride along D; lse and delta are fp32 [B, H, Sq].
+ * Backward: dQ, dK, dV, and (dtable != NULL) dtable[n][h] = sum of dS over the pairs in bucket n, fp32
+ * [num_buckets][H], every sum in a fixed order.
+ * workspace: b2_bias_attn_workspace_bytes(args, backward) bytes, 16-byte aligned (0: none needed). */
+typedef struct b2_bias_attn_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* o;
+  float* lse;             /* forward: may be NULL */
+  const float* table;     /* fp32 [num_buckets][H] contiguous */
+  const uint8_t* key_mask; /* NULL: none */
+  const void* d_o;
+  void* dq;
+  void* dk;
+  void* dv;
+  float* dtable;          /* NULL: not wanted */
+  void* workspace;
+  int64_t B, H, Hk, Sq, Sk, D;
+  int64_t q_s[3], k_s[3], v_s[3], o_s[3], do_s[3], dq_s[3], dk_s[3], dv_s[3];
+  int64_t mask_sb;
+  int64_t q_offset;
+  float scale;
+  int32_t num_buckets, max_distance;
+  int32_t bidirectional, causal;
+  int32_t dtype;          /* F32, BF16 or F16: q, k, v, o, dO, dq, dk, dv */
+} b2_bias_attn_args;
+int b2_bias_attn_fwd(const b2_bias_attn_args* args, b2_stream_t stream);
+int b2_bias_attn_bwd(const b2_bias_attn_args* args, b2_stream_t stream);
+uint64_t b2_bias_attn_workspace_bytes(const b2_bias_attn_args* args, int32_t backward);
+
 #ifdef __cplusplus
 }
 #endif

@@ -379,6 +379,11 @@ def int8_mlp(x, q1, s1, b1, q2, s2, b2):
     return _Int8GeluMLP.apply(x, q1, s1, b1, q2, s2, b2)
 
 
+# ---- 4-bit linears and relative-position-bias attention -------------------------------------------
+
+from .bias_attention import bucket_bias_attention, relative_position_bucket  # noqa: E402
+from .mx4 import Mx4, mx4_dequantize, mx4_linear, mx4_lora_linear, mx4_quantize  # noqa: E402
+
 if os.environ.get("B2_DISABLE", "0") in ("", "0"):
     enable(True)
 

@@ -3,7 +3,7 @@
 Produces, in this package directory (both git-ignored, both shipped with the source tree):
   libb2rt.so   the C-ABI library (include/b2rt.h): runtime, slab allocator, every CUDA kernel,
                compiled with nvcc for sm_100a only (-gencode arch=compute_100a,code=sm_100a);
-  _b2ops.so    the ATen operator shim (csrc/shim/ops.cpp), linked against libb2rt.so and libtorch.
+  _b2ops.so    the ATen operator shim (csrc/shim/*.cpp), linked against libb2rt.so and libtorch.
 
 Incremental: an object is rebuilt when its source or any header under csrc/ or include/ is newer.
 """
@@ -73,17 +73,27 @@ def build_ops(verbose=False):
     import torch
     from torch.utils import cpp_extension as ce
 
-    src = os.path.join(CSRC, "shim", "ops.cpp")
-    if not _stale(OPS, [src, LIB] + _headers()):
+    srcs = sorted(glob.glob(os.path.join(CSRC, "shim", "*.cpp")))
+    if not _stale(OPS, srcs + [LIB] + _headers()):
         return OPS
     inc = ce.include_paths(device_type="cuda")
     libdirs = ce.library_paths(device_type="cuda")
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
-           "-DTORCH_API_INCLUDE_EXTENSION_H", "-DTORCH_EXTENSION_NAME=_b2ops"]
+    flags = ["-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
+             "-DTORCH_API_INCLUDE_EXTENSION_H", "-DTORCH_EXTENSION_NAME=_b2ops"]
     for i in inc:
-        cmd += ["-isystem", i]
-    cmd += [src, "-o", OPS, f"-L{HERE}", "-lb2rt", "-Wl,-rpath,$ORIGIN"]
+        flags += ["-isystem", i]
+    os.makedirs(BUILD, exist_ok=True)
+    objs, todo = [], []
+    for s in srcs:
+        o = os.path.join(BUILD, "shim_" + os.path.basename(s) + ".o")
+        objs.append(o)
+        if _stale(o, [s] + _headers()):
+            todo.append(["g++", *flags, "-c", s, "-o", o])
+    if todo:
+        with cf.ThreadPoolExecutor(max_workers=len(todo)) as ex:
+            list(ex.map(_run, todo))
+    cmd = ["g++", "-shared", *objs, "-o", OPS, f"-L{HERE}", "-lb2rt", "-Wl,-rpath,$ORIGIN"]
     for d in libdirs:
         if "torch" in d:
             cmd += [f"-L{d}", f"-Wl,-rpath,{d}"]

@@ -1,0 +1,93 @@
+// Attention with a learned relative position bias: parameters and device helpers shared by the SIMT and the
+// tensor-core kernels.
+//
+//   x_ij = scale q_i.k_j + table[bucket(j - i - q_offset)][h]      keys j masked by key_mask, and j > i + q_offset
+//   P = softmax_j(x), O = P V                                      when causal
+//   dP = dO V^T, delta_i = sum_d dO O, dS = P (dP - delta), dQ = scale dS K, dK = scale dS^T Q, dV = P^T dO,
+//   dtable[n][h] = sum of dS over batch and over the pairs whose bucket is n
+//
+// The bias depends on j - i alone and is constant beyond +-max_distance, so a kernel holds it as one vector per head
+// in shared memory. Everything is kept in units of log2 (x * log2 e) so that the exponential is one exp2.
+#pragma once
+
+#include "common.cuh"
+
+namespace b2 {
+namespace bias_attn {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+struct Params {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* o;
+  float* lse;
+  const float* table;
+  const uint8_t* mask;
+  const void* d_o;
+  void* dq;
+  void* dk;
+  void* dv;
+  const float* delta;   // [B*H*Sq] rowsum(dO * O)
+  float* dtab;          // [B*H][query tiles][num_buckets] partial sums, NULL: not wanted
+  float* part_o;        // [nsplit][B*H*Sq][D] unnormalised outputs of the key splits
+  float2* part_ml;      // [nsplit][B*H*Sq] (running maximum in log2 units, sum)
+  int64_t q_s[3], k_s[3], v_s[3], o_s[3], do_s[3], dq_s[3], dk_s[3], dv_s[3];
+  int64_t mask_sb;
+  int B, H, Hk, Sq, Sk, D;
+  int q_off;
+  int R;                // max_distance
+  int nb;               // num_buckets
+  int bidir, causal;
+  int nsplit;           // key splits of the forward (grid.z)
+  int nthr;
+  uint16_t thr[B2_BIAS_MAX_BUCKETS];  // bucket of a one-sided distance n = number of thresholds <= n
+  float scale;
+  int* err;
+};
+
+// Bucket of the relative position rel (|rel| <= R).
+__device__ __forceinline__ int bucket_of(const Params& p, int rel) {
+  const int n = p.bidir ? abs(rel) : max(-rel, 0);
+  int c = 0;
+  for (int i = 0; i < p.nthr; ++i) c += (n >= (int)p.thr[i]) ? 1 : 0;
+  return c + (p.bidir && rel > 0 ? p.nb / 2 : 0);
+}
+
+// Bias of head h at a relative position, in log2 units; -inf where the causal mask hides the key.
+__device__ __forceinline__ float bias_at(const Params& p, int h, int rel) {
+  if (p.causal && rel > 0) return -INFINITY;
+  const int r = max(-p.R, min(p.R, rel));
+  return p.table[(int64_t)bucket_of(p, r) * p.H + h] * kLog2e;
+}
+
+template <typename T>
+__device__ __forceinline__ const T* row_of(const void* base, const int64_t* s, int b, int h, int64_t i) {
+  return (const T*)base + b * s[0] + h * s[1] + i * s[2];
+}
+template <typename T>
+__device__ __forceinline__ T* row_of(void* base, const int64_t* s, int b, int h, int64_t i) {
+  return (T*)base + b * s[0] + h * s[1] + i * s[2];
+}
+
+// First key past the last one that query row i may see.
+__device__ __forceinline__ int key_end(const Params& p, int64_t last_row) {
+  if (!p.causal) return p.Sk;
+  const int64_t e = last_row + p.q_off + 1;
+  return e < 0 ? 0 : (e < p.Sk ? (int)e : p.Sk);
+}
+
+int simt_fwd(const Params& p, int dtype, cudaStream_t st);   // bias_attn_simt.cu
+int simt_bwd(const Params& p, int dtype, cudaStream_t st);
+constexpr int kSimtTile = 64;
+
+// More than the default 48 KB of shared memory, set once per kernel and device.
+template <typename K>
+int allow_smem(K kern, int bytes, const char* what) {
+  return check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), what);
+}
+
+}  // namespace bias_attn
+}  // namespace b2

@@ -1,0 +1,430 @@
+// Relative-position-bias attention on the FMA pipe: fp32 inputs, and 16-bit inputs whose layout the tensor-core
+// kernels do not take. A block of 256 threads works on 64 x 64 tiles held in shared memory as fp32, each thread on
+// 4 x 4 scores and on 4 rows x DP / 16 columns of the outputs; every operand read is a 16-byte shared-memory load
+// whose bank pattern is conflict-free (rows padded by 4 floats). Forward: one pass with the running maximum and sum,
+// the key axis split over blockIdx.z when there are few query tiles. Backward: one kernel owns query tiles (dQ and the
+// bias gradient), one owns key tiles (dK, dV, summed over the query heads that share them), so every sum has one owner
+// and a fixed order.
+#include "bias_attn.cuh"
+
+namespace b2 {
+namespace bias_attn {
+namespace {
+
+constexpr int T64 = kSimtTile;
+constexpr int PS = T64 + 4;
+
+template <int DP>
+struct Smem {
+  static constexpr int LD = DP + 4;
+  static constexpr int TILE = T64 * LD;  // floats of a 64-row operand tile
+};
+
+// 64 rows of an operand -> fp32 tile, zeros past the end of the rows, past D, and (keep != NULL) in masked rows.
+template <typename T, int DP>
+__device__ __forceinline__ void load_tile(float* dst, const void* base, const int64_t* s, int b, int h, int r0, int rows,
+                                          int D, float mul, const uint8_t* keep) {
+  for (int e = threadIdx.x; e < T64 * DP; e += 256) {
+    const int r = e / DP, d = e % DP;
+    float v = 0.f;
+    if (r0 + r < rows && d < D && (keep == nullptr || keep[r])) v = to_f32<T>(row_of<T>(base, s, b, h, r0 + r)[d]) * mul;
+    dst[r * Smem<DP>::LD + d] = v;
+  }
+}
+
+// acc[i][j] += A[ty*4 + i] . B[tx + 16 j] over DP columns
+template <int DP>
+__device__ __forceinline__ void dot_tile(const float* A, const float* B, int ty, int tx, float (&acc)[4][4]) {
+  constexpr int LD = Smem<DP>::LD;
+#pragma unroll 4
+  for (int d = 0; d < DP; d += 4) {
+    float4 a[4], c[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(A + (ty * 4 + i) * LD + d);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c[j] = *reinterpret_cast<const float4*>(B + (tx + 16 * j) * LD + d);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        acc[i][j] = fmaf(a[i].x, c[j].x, acc[i][j]);
+        acc[i][j] = fmaf(a[i].y, c[j].y, acc[i][j]);
+        acc[i][j] = fmaf(a[i].z, c[j].z, acc[i][j]);
+        acc[i][j] = fmaf(a[i].w, c[j].w, acc[i][j]);
+      }
+  }
+}
+
+// acc[i][c*4 + e] += sum_k P[ty*4 + i][k] * V[k][tx*4 + 64 c + e]
+template <int DP>
+__device__ __forceinline__ void pv_tile(const float* P, const float* V, int ty, int tx, float (&acc)[4][DP / 16]) {
+  constexpr int LD = Smem<DP>::LD;
+#pragma unroll 2
+  for (int k = 0; k < T64; k += 4) {
+    float4 pr[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) pr[i] = *reinterpret_cast<const float4*>(P + (ty * 4 + i) * PS + k);
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+      for (int c = 0; c < DP / 64; ++c) {
+        const float4 w = *reinterpret_cast<const float4*>(V + (k + kk) * LD + tx * 4 + 64 * c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float pv = reinterpret_cast<const float*>(&pr[i])[kk];
+          acc[i][c * 4 + 0] = fmaf(pv, w.x, acc[i][c * 4 + 0]);
+          acc[i][c * 4 + 1] = fmaf(pv, w.y, acc[i][c * 4 + 1]);
+          acc[i][c * 4 + 2] = fmaf(pv, w.z, acc[i][c * 4 + 2]);
+          acc[i][c * 4 + 3] = fmaf(pv, w.w, acc[i][c * 4 + 3]);
+        }
+      }
+  }
+}
+
+__device__ __forceinline__ float max16(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+__device__ __forceinline__ float sum16(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// keep[j] for the 64 keys from k0; returns whether any is left.
+__device__ __forceinline__ bool load_keep(const Params& p, int b, int k0, uint8_t* keep) {
+  bool any = false;
+  if (threadIdx.x < T64) {
+    const int j = k0 + threadIdx.x;
+    const bool ok = j < p.Sk && (p.mask == nullptr || p.mask[(int64_t)b * p.mask_sb + j] != 0);
+    keep[threadIdx.x] = ok;
+    any = ok;
+  }
+  return __syncthreads_or(any);
+}
+
+__device__ __forceinline__ void fill_bias(const Params& p, int h, float* bias) {
+  for (int i = threadIdx.x; i <= 2 * p.R; i += 256) bias[i] = bias_at(p, h, i - p.R);
+}
+__device__ __forceinline__ float bias_get(const Params& p, const float* bias, int rel) {
+  if (p.causal && rel > 0) return -INFINITY;
+  return bias[max(-p.R, min(p.R, rel)) + p.R];
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) fwd_kernel(const __grid_constant__ Params p) {
+  extern __shared__ float4 sm4[];
+  float* Qs = reinterpret_cast<float*>(sm4);
+  float* Ks = Qs + Smem<DP>::TILE;
+  float* Vs = Ks + Smem<DP>::TILE;
+  float* Ps = Vs + Smem<DP>::TILE;
+  float* bias = Ps + T64 * PS;
+  uint8_t* keep = reinterpret_cast<uint8_t*>(bias + 2 * p.R + 1);
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int q0 = blockIdx.x * T64;
+  const int b = blockIdx.y / p.H, h = blockIdx.y % p.H, hk = h / (p.H / p.Hk);
+  fill_bias(p, h, bias);
+  load_tile<T, DP>(Qs, p.q, p.q_s, b, h, q0, p.Sq, p.D, p.scale * kLog2e, nullptr);
+  float m[4], l[4], acc[4][DP / 16];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    m[i] = -INFINITY, l[i] = 0.f;
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) acc[i][c] = 0.f;
+  }
+  const int nt = (key_end(p, min(q0 + T64, p.Sq) - 1) + T64 - 1) / T64;
+  const int per = (nt + p.nsplit - 1) / p.nsplit;
+  const int t1 = min(nt, ((int)blockIdx.z + 1) * per);
+  for (int t = blockIdx.z * per; t < t1; ++t) {
+    const int k0 = t * T64;
+    __syncthreads();
+    if (!load_keep(p, b, k0, keep)) continue;
+    load_tile<T, DP>(Ks, p.k, p.k_s, b, hk, k0, p.Sk, p.D, 1.f, keep);
+    load_tile<T, DP>(Vs, p.v, p.v_s, b, hk, k0, p.Sk, p.D, 1.f, keep);
+    __syncthreads();
+    float s[4][4] = {};
+    dot_tile<DP>(Qs, Ks, ty, tx, s);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int qi = q0 + ty * 4 + i;
+      float mx = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int c = tx + 16 * j;
+        s[i][j] = keep[c] ? s[i][j] + bias_get(p, bias, k0 + c - qi - p.q_off) : -INFINITY;
+        mx = fmaxf(mx, s[i][j]);
+      }
+      mx = fmaxf(m[i], max16(mx));
+      const float ref = mx == -INFINITY ? 0.f : mx;  // nothing seen yet: exp2(-inf - 0) = 0
+      const float alpha = exp2f(m[i] - ref);
+      m[i] = mx;
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float e = exp2f(s[i][j] - ref);
+        Ps[(ty * 4 + i) * PS + tx + 16 * j] = e;
+        sum += e;
+      }
+      l[i] = l[i] * alpha + sum16(sum);
+#pragma unroll
+      for (int c = 0; c < DP / 16; ++c) acc[i][c] *= alpha;
+    }
+    __syncwarp();  // a warp's 8 rows of P are read by the same warp
+    pv_tile<DP>(Ps, Vs, ty, tx, acc);
+  }
+  const int64_t nrow = (int64_t)p.B * p.H * p.Sq;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int qi = q0 + ty * 4 + i;
+    if (qi >= p.Sq) continue;
+    const int64_t row = (int64_t)blockIdx.y * p.Sq + qi;
+    if (p.nsplit > 1) {
+      const int64_t pr = (int64_t)blockIdx.z * nrow + row;
+      if (tx == 0) p.part_ml[pr] = make_float2(m[i], l[i]);
+#pragma unroll
+      for (int c = 0; c < DP / 16; ++c) {
+        const int d = tx * 4 + 64 * (c >> 2) + (c & 3);
+        if (d < p.D) p.part_o[pr * p.D + d] = acc[i][c];
+      }
+    } else {
+      const float inv = l[i] > 0.f ? 1.f / l[i] : 0.f;
+      T* o = row_of<T>(p.o, p.o_s, b, h, qi);
+#pragma unroll
+      for (int c = 0; c < DP / 16; ++c) {
+        const int d = tx * 4 + 64 * (c >> 2) + (c & 3);
+        if (d < p.D) o[d] = from_f32<T>(acc[i][c] * inv);
+      }
+      if (tx == 0 && p.lse) p.lse[row] = l[i] > 0.f ? (m[i] + log2f(l[i])) * kLn2 : -INFINITY;
+    }
+  }
+}
+
+// dQ and the bias gradient: a block owns 64 query rows of one head and walks the keys.
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) dq_kernel(const __grid_constant__ Params p) {
+  extern __shared__ float4 sm4[];
+  float* Qs = reinterpret_cast<float*>(sm4);
+  float* Gs = Qs + Smem<DP>::TILE;  // dO
+  float* Ks = Gs + Smem<DP>::TILE;
+  float* Vs = Ks + Smem<DP>::TILE;
+  float* Ps = Vs + Smem<DP>::TILE;  // dS
+  float* bias = Ps + T64 * PS;
+  float* diag = bias + 2 * p.R + 1;                       // 127 diagonal sums of a tile
+  int* dbk = reinterpret_cast<int*>(diag + 2 * T64);      // and their buckets
+  uint8_t* keep = reinterpret_cast<uint8_t*>(dbk + 2 * T64);
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int q0 = blockIdx.x * T64;
+  const int b = blockIdx.y / p.H, h = blockIdx.y % p.H, hk = h / (p.H / p.Hk);
+  fill_bias(p, h, bias);
+  load_tile<T, DP>(Qs, p.q, p.q_s, b, h, q0, p.Sq, p.D, p.scale * kLog2e, nullptr);
+  load_tile<T, DP>(Gs, p.d_o, p.do_s, b, h, q0, p.Sq, p.D, 1.f, nullptr);
+  float L[4], dl[4], acc[4][DP / 16];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int qi = q0 + ty * 4 + i;
+    const int64_t row = (int64_t)blockIdx.y * p.Sq + qi;
+    // rows past the end and rows with no key: exp2(x - inf) = 0
+    L[i] = qi < p.Sq ? p.lse[row] * kLog2e : INFINITY;
+    if (L[i] == -INFINITY) L[i] = INFINITY;
+    dl[i] = qi < p.Sq ? p.delta[row] : 0.f;
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) acc[i][c] = 0.f;
+  }
+  float db = 0.f;  // thread n: sum of dS over bucket n
+  const int nt = (key_end(p, min(q0 + T64, p.Sq) - 1) + T64 - 1) / T64;
+  for (int t = 0; t < nt; ++t) {
+    const int k0 = t * T64;
+    __syncthreads();
+    if (!load_keep(p, b, k0, keep)) continue;
+    load_tile<T, DP>(Ks, p.k, p.k_s, b, hk, k0, p.Sk, p.D, 1.f, keep);
+    load_tile<T, DP>(Vs, p.v, p.v_s, b, hk, k0, p.Sk, p.D, 1.f, keep);
+    __syncthreads();
+    float s[4][4] = {}, dp[4][4] = {};
+    dot_tile<DP>(Qs, Ks, ty, tx, s);
+    dot_tile<DP>(Gs, Vs, ty, tx, dp);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int qi = q0 + ty * 4 + i;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int c = tx + 16 * j;
+        const float x = keep[c] ? s[i][j] + bias_get(p, bias, k0 + c - qi - p.q_off) : -INFINITY;
+        Ps[(ty * 4 + i) * PS + c] = exp2f(x - L[i]) * (dp[i][j] - dl[i]);
+      }
+    }
+    if (p.dtab) {
+      __syncthreads();
+      if (threadIdx.x < 2 * T64 - 1) {
+        const int d = (int)threadIdx.x - (T64 - 1);  // key - query inside the tile
+        float a = 0.f;
+        for (int r = max(0, -d); r < min(T64, T64 - d); ++r) a += Ps[r * PS + r + d];
+        diag[threadIdx.x] = a;
+        dbk[threadIdx.x] = bucket_of(p, max(-p.R, min(p.R, k0 + d - q0 - p.q_off)));
+      }
+      __syncthreads();
+      if ((int)threadIdx.x < p.nb)
+        for (int i = 0; i < 2 * T64 - 1; ++i) db += dbk[i] == (int)threadIdx.x ? diag[i] : 0.f;
+    } else {
+      __syncwarp();
+    }
+    pv_tile<DP>(Ps, Ks, ty, tx, acc);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int qi = q0 + ty * 4 + i;
+    if (qi >= p.Sq || !p.dq) continue;
+    T* o = row_of<T>(p.dq, p.dq_s, b, h, qi);
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+      const int d = tx * 4 + 64 * (c >> 2) + (c & 3);
+      if (d < p.D) o[d] = from_f32<T>(acc[i][c] * p.scale);
+    }
+  }
+  if (p.dtab && (int)threadIdx.x < p.nb)
+    p.dtab[((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * p.nb + threadIdx.x] = db;
+}
+
+// dK, dV: a block owns 64 keys of one key/value head and walks the queries of every head that shares it.
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) dkv_kernel(const __grid_constant__ Params p) {
+  extern __shared__ float4 sm4[];
+  float* Ks = reinterpret_cast<float*>(sm4);
+  float* Vs = Ks + Smem<DP>::TILE;
+  float* Qs = Vs + Smem<DP>::TILE;
+  float* Gs = Qs + Smem<DP>::TILE;  // dO
+  float* Pt = Gs + Smem<DP>::TILE;  // P^T
+  float* St = Pt + T64 * PS;        // dS^T
+  float* bias = St + T64 * PS;
+  float* Lq = bias + 2 * p.R + 1;
+  float* Dq = Lq + T64;
+  uint8_t* keep = reinterpret_cast<uint8_t*>(Dq + T64);
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int k0 = blockIdx.x * T64;
+  const int b = blockIdx.y / p.Hk, hk = blockIdx.y % p.Hk, G = p.H / p.Hk;
+  const bool some = load_keep(p, b, k0, keep);
+  load_tile<T, DP>(Ks, p.k, p.k_s, b, hk, k0, p.Sk, p.D, 1.f, keep);
+  load_tile<T, DP>(Vs, p.v, p.v_s, b, hk, k0, p.Sk, p.D, 1.f, keep);
+  float dk[4][DP / 16] = {}, dv[4][DP / 16] = {};
+  // causal: the first query row that sees key k0
+  const int64_t first = p.causal ? max((int64_t)0, (int64_t)k0 - p.q_off) : 0;
+  const int nt = (p.Sq + T64 - 1) / T64;
+  for (int g = 0; g < G && some; ++g) {
+    const int h = hk * G + g;
+    __syncthreads();
+    fill_bias(p, h, bias);
+    for (int t = (int)min((int64_t)nt, first / T64); t < nt; ++t) {
+      const int q0 = t * T64;
+      __syncthreads();
+      load_tile<T, DP>(Qs, p.q, p.q_s, b, h, q0, p.Sq, p.D, 1.f, nullptr);
+      load_tile<T, DP>(Gs, p.d_o, p.do_s, b, h, q0, p.Sq, p.D, 1.f, nullptr);
+      if (threadIdx.x < T64) {
+        const int qi = q0 + threadIdx.x;
+        const int64_t row = ((int64_t)b * p.H + h) * p.Sq + qi;
+        float L = qi < p.Sq ? p.lse[row] * kLog2e : INFINITY;
+        Lq[threadIdx.x] = L == -INFINITY ? INFINITY : L;
+        Dq[threadIdx.x] = qi < p.Sq ? p.delta[row] : 0.f;
+      }
+      __syncthreads();
+      float s[4][4] = {}, dp[4][4] = {};
+      dot_tile<DP>(Ks, Qs, ty, tx, s);
+      dot_tile<DP>(Vs, Gs, ty, tx, dp);
+      const float sl2 = p.scale * kLog2e;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = ty * 4 + i;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int c = tx + 16 * j;
+          const float x = keep[r] ? fmaf(s[i][j], sl2, bias_get(p, bias, k0 + r - (q0 + c) - p.q_off)) : -INFINITY;
+          const float e = exp2f(x - Lq[c]);
+          Pt[r * PS + c] = e;
+          St[r * PS + c] = e * (dp[i][j] - Dq[c]);
+        }
+      }
+      __syncwarp();
+      pv_tile<DP>(Pt, Gs, ty, tx, dv);
+      pv_tile<DP>(St, Qs, ty, tx, dk);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int kj = k0 + ty * 4 + i;
+    if (kj >= p.Sk) continue;
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+      const int d = tx * 4 + 64 * (c >> 2) + (c & 3);
+      if (d >= p.D) continue;
+      if (p.dk) row_of<T>(p.dk, p.dk_s, b, hk, kj)[d] = from_f32<T>(dk[i][c] * p.scale);
+      if (p.dv) row_of<T>(p.dv, p.dv_s, b, hk, kj)[d] = from_f32<T>(dv[i][c]);
+    }
+  }
+}
+
+template <int DP>
+int smem_bytes(const Params& p, int tiles, int ps) {
+  return (tiles * Smem<DP>::TILE + ps * T64 * PS + 2 * p.R + 1 + 4 * T64 + 4) * 4 + T64;
+}
+
+template <typename T, int DP>
+int fwd_t(const Params& p, cudaStream_t st) {
+  const int sm = smem_bytes<DP>(p, 3, 1);
+  if (int rc = allow_smem(fwd_kernel<T, DP>, sm, "bias_attn_fwd_simt")) return rc;
+  {
+    LaunchScope ls("bias_attn_fwd_simt", st);
+    dim3 grid((p.Sq + T64 - 1) / T64, p.B * p.H, p.nsplit);
+    fwd_kernel<T, DP><<<grid, 256, sm, st>>>(p);
+  }
+  return after_launch("bias_attn_fwd_simt");
+}
+
+template <typename T, int DP>
+int bwd_t(const Params& p, cudaStream_t st) {
+  const int sq = smem_bytes<DP>(p, 4, 1), sk = smem_bytes<DP>(p, 4, 2);
+  if (p.dq || p.dtab) {
+    if (int rc = allow_smem(dq_kernel<T, DP>, sq, "bias_attn_dq_simt")) return rc;
+    {
+      LaunchScope ls("bias_attn_dq_simt", st);
+      dq_kernel<T, DP><<<dim3((p.Sq + T64 - 1) / T64, p.B * p.H), 256, sq, st>>>(p);
+    }
+    if (int rc = after_launch("bias_attn_dq_simt")) return rc;
+  }
+  if (p.dk || p.dv) {
+    if (int rc = allow_smem(dkv_kernel<T, DP>, sk, "bias_attn_dkv_simt")) return rc;
+    {
+      LaunchScope ls("bias_attn_dkv_simt", st);
+      dkv_kernel<T, DP><<<dim3((p.Sk + T64 - 1) / T64, p.B * p.Hk), 256, sk, st>>>(p);
+    }
+    if (int rc = after_launch("bias_attn_dkv_simt")) return rc;
+  }
+  return 0;
+}
+
+template <typename T>
+int fwd_d(const Params& p, cudaStream_t st) {
+  return p.D <= 64 ? fwd_t<T, 64>(p, st) : fwd_t<T, 128>(p, st);
+}
+template <typename T>
+int bwd_d(const Params& p, cudaStream_t st) {
+  return p.D <= 64 ? bwd_t<T, 64>(p, st) : bwd_t<T, 128>(p, st);
+}
+
+}  // namespace
+
+int simt_fwd(const Params& p, int dtype, cudaStream_t st) {
+  switch (dtype) {
+    case B2_F32: return fwd_d<float>(p, st);
+    case B2_BF16: return fwd_d<__nv_bfloat16>(p, st);
+    default: return fwd_d<__half>(p, st);
+  }
+}
+int simt_bwd(const Params& p, int dtype, cudaStream_t st) {
+  switch (dtype) {
+    case B2_F32: return bwd_d<float>(p, st);
+    case B2_BF16: return bwd_d<__nv_bfloat16>(p, st);
+    default: return bwd_d<__half>(p, st);
+  }
+}
+
+}  // namespace bias_attn
+}  // namespace b2

@@ -1,0 +1,335 @@
+// MXFP4 (OCP microscaling): quantisation of a matrix to E2M1 codes with one power-of-two scale per 32 columns, and
+// reading it back.
+//
+// A block's scale is 2^(floor(log2(amax)) - 2): with the fp32 exponent field e of amax that is the E8M0 code
+// max(e - 2, 0), and multiplying by 2^(127 - code) divides exactly. The E2M1 rounding (nearest, ties to even,
+// saturating) is the cvt.rn.satfinite.e2m1x2 instruction; reading back is one exact product per element.
+#include "common.cuh"
+
+namespace b2 {
+namespace {
+
+constexpr int kBlk = 32;  // columns per scale
+
+// Byte of the scale of (row, block of 32 columns) in the tiled scale array (see b2_mx4_args).
+__host__ __device__ __forceinline__ int64_t scale_at(int64_t row, int64_t blk, int64_t nkb) {
+  return ((row >> 7) * nkb + (blk >> 2)) * 512 + (row & 31) * 16 + ((row & 127) >> 5) * 4 + (blk & 3);
+}
+
+__device__ __forceinline__ float e8m0_to_f32(uint32_t code) {
+  if (code == 255u) return __uint_as_float(0x7FC00000u);
+  return code ? __uint_as_float(code << 23) : __uint_as_float(0x00400000u);  // code 0: 2^-127
+}
+
+// Eight floats -> eight E2M1 codes, element 0 in the lowest nibble.
+__device__ __forceinline__ uint32_t e2m1x8(const float* v) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+      "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+      : "=r"(r)
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return r;
+}
+
+// Eight codes -> four half2 (exact: every E2M1 value is a half).
+__device__ __forceinline__ void e2m1x8_to_half2(uint32_t c, __half2* h) {
+  uint32_t o[4];
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+      : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3])
+      : "r"(c));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = *reinterpret_cast<__half2*>(&o[i]);
+}
+
+// Eight consecutive elements at p as floats; `n` (< 8 at a ragged end) of them exist.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(const T* p, int n, float* v) {
+  if (VEC) {
+    if constexpr (sizeof(T) == 4) {
+      const float4 a = *reinterpret_cast<const float4*>(p), b = *(reinterpret_cast<const float4*>(p) + 1);
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+      const uint4 raw = *reinterpret_cast<const uint4*>(p);
+      const T* t = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(t[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32<T>(p[i]) : 0.f;
+  }
+}
+
+// Four lanes own a block of 32 columns, eight columns each. The grid covers the padded scale array (rows to a
+// multiple of 128, blocks to a multiple of 4), whose padding is written as zeros here.
+// VEC: every 8-column group that exists is whole and 16-byte aligned.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) mx4_quantize_k(const T* __restrict__ x, uint8_t* __restrict__ codes,
+                                                      uint8_t* __restrict__ scales, int64_t rows, int64_t cols,
+                                                      int64_t x_ld, int64_t nkb) {
+  const int64_t groups = nkb * 16;  // 8-column groups per padded row
+  const int64_t total = (rows + 127) / 128 * 128 * groups;
+  const int64_t cb = (cols + kBlk - 1) / kBlk * 16;  // code bytes per row
+  // total is a multiple of 32, so whole warps leave the loop together
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / groups, g = i - row * groups;
+    const int64_t c0 = g * 8;
+    float v[8];
+    float am = 0.f;
+    bool bad = false;
+    const bool in = row < rows && c0 < cols;
+    if (in) {
+      load8<T, VEC>(x + row * x_ld + c0, (int)min((int64_t)8, cols - c0), v);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float a = fabsf(v[k]);
+        bad |= !(a <= 3.402823466e38f);
+        am = fmaxf(am, a);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = 0.f;
+    }
+    am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 1));
+    am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 2));
+    uint32_t b = bad ? 1u : 0u;
+    b |= __shfl_xor_sync(0xffffffffu, b, 1);
+    b |= __shfl_xor_sync(0xffffffffu, b, 2);
+    const int e = (int)(__float_as_uint(am) >> 23);
+    const uint32_t code = b ? 255u : (uint32_t)max(e - 2, 0);
+    if (row < rows && c0 < cb * 2) {
+      const float inv = b ? 0.f : __uint_as_float((254u - code) << 23);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = b ? 0.f : v[k] * inv;
+      *reinterpret_cast<uint32_t*>(codes + row * cb + g * 4) = e2m1x8(v);
+    }
+    if ((g & 3) == 0) scales[scale_at(row, g >> 2, nkb)] = (row < rows && c0 < cols) ? (uint8_t)code : (uint8_t)0;
+  }
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) mx4_dequantize_k(const uint8_t* __restrict__ codes,
+                                                        const uint8_t* __restrict__ scales, T* __restrict__ out,
+                                                        int64_t rows, int64_t cols, int64_t ld, int64_t nkb) {
+  const int64_t groups = (cols + 7) / 8;
+  const int64_t cb = (cols + kBlk - 1) / kBlk * 16;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * groups; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / groups, g = i - row * groups;
+    const uint32_t c = *reinterpret_cast<const uint32_t*>(codes + row * cb + g * 4);
+    const float s = e8m0_to_f32(scales[scale_at(row, g >> 2, nkb)]);
+    __half2 h[4];
+    e2m1x8_to_half2(c, h);
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 f = __half22float2(h[k]);
+      v[2 * k] = f.x * s, v[2 * k + 1] = f.y * s;
+    }
+    T* o = out + row * ld + g * 8;
+    if (VEC) {
+      if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
+        *(reinterpret_cast<float4*>(o) + 1) = make_float4(v[4], v[5], v[6], v[7]);
+      } else {
+        uint4 raw;
+        T* t = reinterpret_cast<T*>(&raw);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) t[k] = from_f32<T>(v[k]);
+        *reinterpret_cast<uint4*>(o) = raw;
+      }
+    } else {
+      const int n = (int)min((int64_t)8, cols - g * 8);
+      for (int k = 0; k < n; ++k) o[k] = from_f32<T>(v[k]);
+    }
+  }
+}
+
+template <typename T>
+int quantize_t(const b2_mx4_args* a, cudaStream_t st) {
+  const int64_t nkb = (a->cols + 127) / 128;
+  const int64_t work = (a->rows + 127) / 128 * 128 * nkb * 16;
+  const bool vec = a->cols % 8 == 0 && ((uintptr_t)a->x & 15) == 0 && (a->ld * (int64_t)sizeof(T)) % 16 == 0;
+  const int grid = grid_for(work, 256, 16);
+  {
+    LaunchScope ls("mx4_quantize", st);
+    if (vec)
+      mx4_quantize_k<T, true><<<grid, 256, 0, st>>>((const T*)a->x, a->codes, a->scales, a->rows, a->cols, a->ld, nkb);
+    else
+      mx4_quantize_k<T, false><<<grid, 256, 0, st>>>((const T*)a->x, a->codes, a->scales, a->rows, a->cols, a->ld, nkb);
+  }
+  return after_launch("mx4_quantize");
+}
+
+template <typename T>
+int dequantize_t(const b2_mx4_args* a, cudaStream_t st) {
+  const int64_t nkb = (a->cols + 127) / 128;
+  const int grid = grid_for(a->rows * ((a->cols + 7) / 8), 256, 16);
+  const bool vec = a->cols % 8 == 0 && ((uintptr_t)a->out & 15) == 0 && (a->ld * (int64_t)sizeof(T)) % 16 == 0;
+  {
+    LaunchScope ls("mx4_dequantize", st);
+    if (vec)
+      mx4_dequantize_k<T, true><<<grid, 256, 0, st>>>(a->codes, a->scales, (T*)a->out, a->rows, a->cols, a->ld, nkb);
+    else
+      mx4_dequantize_k<T, false><<<grid, 256, 0, st>>>(a->codes, a->scales, (T*)a->out, a->rows, a->cols, a->ld, nkb);
+  }
+  return after_launch("mx4_dequantize");
+}
+
+int check(const b2_mx4_args* a, const void* data, const char* what) {
+  if (!a) return fail(B2_ERR_ARG, std::string(what) + ": null arguments");
+  if (a->rows < 0 || a->cols < 0) return fail(B2_ERR_ARG, std::string(what) + ": negative size");
+  if (a->dtype != B2_F32 && a->dtype != B2_BF16 && a->dtype != B2_F16)
+    return fail(B2_ERR_ARG, std::string(what) + ": dtype must be F32, BF16 or F16");
+  if (a->rows == 0 || a->cols == 0) return 0;
+  if (a->ld < a->cols && a->rows > 1) return fail(B2_ERR_ARG, std::string(what) + ": ld smaller than cols");
+  if (!data || !a->codes || !a->scales) return fail(B2_ERR_ARG, std::string(what) + ": null pointer");
+  if (((uintptr_t)a->codes | (uintptr_t)a->scales) & 15)
+    return fail(B2_ERR_ARG, std::string(what) + ": codes and scales must be 16-byte aligned");
+  if ((uintptr_t)data % dtype_size(a->dtype)) return fail(B2_ERR_ARG, std::string(what) + ": unaligned data pointer");
+  return ensure_init();
+}
+
+}  // namespace
+}  // namespace b2
+
+extern "C" int64_t b2_mx4_code_bytes(int64_t cols) { return cols <= 0 ? 0 : (cols + 31) / 32 * 16; }
+extern "C" int64_t b2_mx4_scale_bytes(int64_t rows, int64_t cols) {
+  return rows <= 0 || cols <= 0 ? 0 : (rows + 127) / 128 * ((cols + 127) / 128) * 512;
+}
+
+extern "C" int b2_mx4_quantize(const b2_mx4_args* a, b2_stream_t stream) {
+  using namespace b2;
+  if (int rc = check(a, a ? a->x : nullptr, "mx4_quantize")) return rc;
+  if (a->rows == 0 || a->cols == 0) return 0;
+  cudaStream_t st = (cudaStream_t)stream;
+  switch (a->dtype) {
+    case B2_F32: return quantize_t<float>(a, st);
+    case B2_BF16: return quantize_t<__nv_bfloat16>(a, st);
+    default: return quantize_t<__half>(a, st);
+  }
+}
+
+extern "C" int b2_mx4_dequantize(const b2_mx4_args* a, b2_stream_t stream) {
+  using namespace b2;
+  if (int rc = check(a, a ? a->out : nullptr, "mx4_dequantize")) return rc;
+  if (a->rows == 0 || a->cols == 0) return 0;
+  cudaStream_t st = (cudaStream_t)stream;
+  switch (a->dtype) {
+    case B2_F32: return dequantize_t<float>(a, st);
+    case B2_BF16: return dequantize_t<__nv_bfloat16>(a, st);
+    default: return dequantize_t<__half>(a, st);
+  }
+}
+
+// ---- product ------------------------------------------------------------------------------------------------------
+// Every MXFP4 value that quantisation makes is a bf16 value, so the product of the bf16 read-backs is the product of
+// the codes. Both operands are expanded into the workspace, the LoRA operands beside them as r more terms of the
+// reduction, and multiplied by the bf16 GEMM, which sums in fp32 and rounds once.
+namespace b2 {
+namespace {
+
+int64_t pad_to(int64_t k, int64_t m) { return (k + m - 1) / m * m; }
+uint64_t up16(uint64_t v) { return (v + 15) / 16 * 16; }
+
+int expand(const uint8_t* codes, const uint8_t* scales, void* out, int64_t rows, int64_t cols, int64_t ld, cudaStream_t st) {
+  b2_mx4_args d{};
+  d.codes = const_cast<uint8_t*>(codes), d.scales = const_cast<uint8_t*>(scales), d.out = out;
+  d.rows = rows, d.cols = cols, d.ld = ld, d.dtype = B2_BF16;
+  return b2_mx4_dequantize(&d, st);
+}
+int copy2d(void* dst, int64_t dld, const void* src, int64_t sld, int64_t rows, int64_t cols, cudaStream_t st) {
+  return check_cuda(cudaMemcpy2DAsync(dst, dld * 2, src, sld * 2, cols * 2, rows, cudaMemcpyDeviceToDevice, st), "mx4_gemm copy");
+}
+
+int gemm_check(const b2_mx4_gemm_args* a) {
+  if (!a) return fail(B2_ERR_ARG, "mx4_gemm: null arguments");
+  if (a->M < 0 || a->N < 0 || a->K < 0) return fail(B2_ERR_ARG, "mx4_gemm: negative size");
+  if (a->M == 0 || a->N == 0 || a->K == 0) return 0;
+  if (!a->w_codes || !a->w_scales || !a->out || (a->transpose_w ? !a->x : (!a->x_codes || !a->x_scales)))
+    return fail(B2_ERR_ARG, "mx4_gemm: null pointer");
+  if (((uintptr_t)a->w_codes | (uintptr_t)a->w_scales | (uintptr_t)a->x_codes | (uintptr_t)a->x_scales) & 15)
+    return fail(B2_ERR_ARG, "mx4_gemm: codes and scales must be 16-byte aligned");
+  if (a->out_ld < (a->transpose_w ? a->K : a->N)) return fail(B2_ERR_ARG, "mx4_gemm: out_ld smaller than a row");
+  if (a->transpose_w && a->x_ld < a->N) return fail(B2_ERR_ARG, "mx4_gemm: x_ld smaller than a row");
+  if (a->lora_r) {
+    if (a->lora_r < 8 || a->lora_r > 64 || a->lora_r % 8 || !a->lora_h || !a->lora_b || a->lora_h_ld % 8 || a->lora_b_ld % 8 ||
+        (((uintptr_t)a->lora_h | (uintptr_t)a->lora_b) & 15))
+      return fail(B2_ERR_ARG, "mx4_gemm: lora_r must be 8..64 and a multiple of 8, with 16-byte aligned operands and rows");
+  }
+  return 0;
+}
+
+// Operand buffers of the expanded product: A [M][lda], W [wrows][ldw].
+struct Expanded {
+  int64_t kp, lda, ldw, wrows;
+  bool copy_x;
+};
+Expanded expanded(const b2_mx4_gemm_args* a) {
+  Expanded e;
+  e.kp = pad_to(a->K, 32);
+  if (a->transpose_w) {
+    e.copy_x = a->lora_r != 0;
+    e.lda = pad_to(a->N + a->lora_r, 8), e.ldw = e.kp, e.wrows = a->N + a->lora_r;
+  } else {
+    e.copy_x = true;
+    e.lda = e.ldw = e.kp + a->lora_r, e.wrows = a->N;
+  }
+  return e;
+}
+
+}  // namespace
+}  // namespace b2
+
+extern "C" uint64_t b2_mx4_gemm_workspace_bytes(const b2_mx4_gemm_args* a) {
+  using namespace b2;
+  if (!a || a->M <= 0 || a->N <= 0 || a->K <= 0) return 0;
+  const Expanded e = expanded(a);
+  return up16((uint64_t)e.wrows * e.ldw * 2) + (e.copy_x ? up16((uint64_t)a->M * e.lda * 2) : 0);
+}
+
+extern "C" int b2_mx4_gemm(const b2_mx4_gemm_args* a, b2_stream_t stream) {
+  using namespace b2;
+  if (int rc = gemm_check(a)) return rc;
+  if (a->M == 0 || a->N == 0 || a->K == 0) return 0;
+  if (int rc = ensure_init()) return rc;
+  if (!a->workspace || ((uintptr_t)a->workspace & 15))
+    return fail(B2_ERR_ARG, "mx4_gemm: a 16-byte aligned workspace of b2_mx4_gemm_workspace_bytes() is required");
+  cudaStream_t st = (cudaStream_t)stream;
+  const Expanded e = expanded(a);
+  const int r = a->lora_r;
+  uint16_t* w = (uint16_t*)a->workspace;
+  uint16_t* x = (uint16_t*)((char*)a->workspace + up16((uint64_t)e.wrows * e.ldw * 2));
+  if (int rc = expand(a->w_codes, a->w_scales, w, a->N, e.kp, e.ldw, st)) return rc;
+  b2_gemm_args g{};
+  g.b = w, g.c = a->out, g.M = a->M, g.batch = 1, g.alpha = 1.f, g.dtype = B2_BF16;
+  g.c_sm = a->out_ld, g.c_sn = 1;
+  if (a->transpose_w) {
+    g.a = a->x, g.a_sm = a->x_ld, g.a_sk = 1;
+    g.N = a->K, g.K = a->N + r, g.b_sk = e.ldw, g.b_sn = 1;
+    if (r) {
+      if (int rc = copy2d(w + a->N * e.ldw, e.ldw, a->lora_b, a->lora_b_ld, r, a->K, st)) return rc;
+      if (int rc = copy2d(x, e.lda, a->x, a->x_ld, a->M, a->N, st)) return rc;
+      if (int rc = copy2d(x + a->N, e.lda, a->lora_h, a->lora_h_ld, a->M, r, st)) return rc;
+      g.a = x, g.a_sm = e.lda;
+    }
+  } else {
+    if (int rc = expand(a->x_codes, a->x_scales, x, a->M, e.kp, e.lda, st)) return rc;
+    if (r) {
+      if (int rc = copy2d(w + e.kp, e.ldw, a->lora_b, a->lora_b_ld, a->N, r, st)) return rc;
+      if (int rc = copy2d(x + e.kp, e.lda, a->lora_h, a->lora_h_ld, a->M, r, st)) return rc;
+    }
+    g.a = x, g.a_sm = e.lda, g.a_sk = 1;
+    g.N = a->N, g.K = e.kp + r, g.b_sn = e.ldw, g.b_sk = 1;
+    if (a->bias) g.bias = a->bias, g.bias_sn = 1, g.has_bias = 1, g.beta = 1.f;
+  }
+  return b2_gemm(&g, st);
+}

@@ -30,33 +30,9 @@
 #include <string>
 #include <vector>
 
-#include "../../../include/b2rt.h"
+#include "shim.h"
 
 namespace {
-
-std::string b2_error() {
-  char buf[1024];
-  b2rt_last_error(buf, sizeof(buf));
-  return std::string(buf);
-}
-
-void b2_check(int rc, const char* what) { TORCH_CHECK(rc == 0, "b200 ", what, " failed: ", b2_error()); }
-
-void count(const char* name) { b2rt_count_op(name); }
-void count_fallback(const std::string& name) { b2rt_count_op(("fallback:" + name).c_str()); }
-
-b2_stream_t cur_stream() { return (b2_stream_t)at::cuda::getCurrentCUDAStream().stream(); }
-
-int dtype_code(at::ScalarType t) {
-  switch (t) {
-    case at::kFloat: return B2_F32;
-    case at::kBFloat16: return B2_BF16;
-    case at::kHalf: return B2_F16;
-    case at::kDouble: return B2_F64;
-    default: return -1;
-  }
-}
-bool is_row_dtype(at::ScalarType t) { return t == at::kFloat || t == at::kBFloat16 || t == at::kHalf; }
 
 std::atomic<int> g_force_simt{0};     // bit0: gemm, bit1: attention
 std::atomic<int> g_attn_policy{-1};  // 0 off, 1 on, 2 auto (-1: read the environment)
