@@ -496,6 +496,9 @@ typedef struct b2_bias_attn_args {
   void* dk;
   void* dv;
   float* dtable;          /* NULL: not wanted */
+  float* o32;             /* fp32 [B, H, Sq, D] contiguous, may be NULL. Forward: O, computed to about 2^-17 and not
+                             rounded, is also written here. Backward: read in place of o for delta = rowsum(dO O); dS
+                             cancels over each row, so the rounding of O would stay in the bias gradient */
   void* workspace;
   int64_t B, H, Hk, Sq, Sk, D;
   int64_t q_s[3], k_s[3], v_s[3], o_s[3], do_s[3], dq_s[3], dk_s[3], dv_s[3];

@@ -260,6 +260,18 @@ def test_gradients_wanted_one_at_a_time(dt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("S", [200, 512])
+def test_bias_gradient_keeps_fp32_accuracy(dt, S):
+    """With 16-bit tensors the bias gradient is still a sum of fp32 dS: the two exponent terms carry |x| 2^-23 each
+    (|x| < 16 here) and delta is a sum of D fp32 products, so it is within 2^-17 of the magnitudes of dP - delta's sums."""
+    q, k, v, go, table, m = _case(2, 4, 4, S, S, 64, dt, S, "tail")
+    ref = ot.bias_attention(q, k, v, table, key_mask=m, go=go)
+    got = _run(q, k, v, table, m, go)["dtable"].cpu().double()
+    assert bool(((got - ref["dtable"]).abs() <= 2.0 ** -17 * (ref["dtable_abs"] + ref["ds_abs"]) + 1e-9).all())
+
+
+@pytest.mark.gpu
 def test_refusals():
     import torch_vulkan_b200 as tv
 

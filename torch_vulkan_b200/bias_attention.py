@@ -20,8 +20,9 @@ class _BucketBiasAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, key_mask, max_distance, bidirectional, causal, scale, q_offset):
         args = (max_distance, bidirectional, causal, scale, q_offset)
-        o, lse = torch.ops.b2.bias_attn_fwd(q, k, v, table, key_mask, *args)
-        ctx.save_for_backward(q, k, v, o, lse, table, key_mask)
+        # a backward keeps the unrounded output: its dS cancels over each row
+        o, lse, o32 = torch.ops.b2.bias_attn_fwd(q, k, v, table, key_mask, *args, any(ctx.needs_input_grad[:4]))
+        ctx.save_for_backward(q, k, v, o if o32 is None else o32, lse, table, key_mask)
         ctx.args = args
         return o
 

@@ -58,7 +58,10 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Pa
   T* o = row_of<T>(p.o, p.o_s, (int)(bh / p.H), (int)(bh % p.H), i);
 #pragma unroll
   for (int c = 0; c < 4; ++c)
-    if (lane + 32 * c < p.D) o[lane + 32 * c] = from_f32<T>(acc[c] * inv);
+    if (lane + 32 * c < p.D) {
+      o[lane + 32 * c] = from_f32<T>(acc[c] * inv);
+      if (p.o32) p.o32[row * p.D + lane + 32 * c] = acc[c] * inv;
+    }
   if (lane == 0 && p.lse) p.lse[row] = l > 0.f ? (M + log2f(l)) * kLn2 : -INFINITY;
 }
 
@@ -71,9 +74,10 @@ __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ Para
   if (row >= nrow) return;
   const int64_t i = row % p.Sq, bh = row / p.Sq;
   const T* o = row_of<T>((const void*)p.o, p.o_s, (int)(bh / p.H), (int)(bh % p.H), i);
+  const float* o32 = p.o32 ? p.o32 + row * p.D : nullptr;
   const T* g = row_of<T>(p.d_o, p.do_s, (int)(bh / p.H), (int)(bh % p.H), i);
   float s = 0.f;
-  for (int d = lane; d < p.D; d += 32) s = fmaf(to_f32<T>(o[d]), to_f32<T>(g[d]), s);
+  for (int d = lane; d < p.D; d += 32) s = fmaf(o32 ? o32[d] : to_f32<T>(o[d]), to_f32<T>(g[d]), s);
   s = warp_sum(s);
   if (lane == 0) delta[row] = s;
 }
@@ -128,30 +132,44 @@ int check(const b2_bias_attn_args* a, bool bwd) {
     return fail(B2_ERR_ARG, std::string(w) + ": num_buckets must be 2..128 (two-sided: even, 4..128) and max_distance "
                                              "above half a side's buckets and at most 1024");
   if (a->B == 0 || a->H == 0 || a->Sq == 0) return 0;
-  if (!a->q || !a->o || !a->table || (a->Sk > 0 && (!a->k || !a->v)))
+  if ((uintptr_t)a->o32 & 15) return fail(B2_ERR_ARG, std::string(w) + ": o32 must be 16-byte aligned");
+  if (!a->q || (!a->o && !(bwd && a->o32)) || !a->table || (a->Sk > 0 && (!a->k || !a->v)))
     return fail(B2_ERR_ARG, std::string(w) + ": null tensor");
   if (bwd && (!a->d_o || !a->lse)) return fail(B2_ERR_ARG, std::string(w) + ": dO and lse are required");
   return 0;
 }
 
 struct Plan {
+  bool tc = false;
   int nsplit = 1;
   int ntq = 0;               // query tiles of the bias-gradient partial sums
+  int sq_pad = 0;            // tensor-core backward: rows of (lse, delta) per head
   uint64_t part_o = 0, part_ml = 0, delta = 0, dtab = 0, bytes = 0;  // offsets into the workspace
 };
 
 uint64_t up16(uint64_t v) { return (v + 15) / 16 * 16; }
 
+// Key splits of the forward: as many waves of blocks as the SMs need, times the key tiles a block walks plus about four
+// tiles' worth of set-up and joining; at least two tiles a split.
+int pick_splits(int64_t blocks, int64_t tk) {
+  const int64_t sms = device_info().sm_count > 0 ? device_info().sm_count : 148;
+  int best = 1;
+  int64_t best_cost = INT64_MAX;
+  for (int64_t ns = 1; ns <= std::max<int64_t>(1, std::min<int64_t>(tk / 2, 64)); ++ns) {
+    const int64_t cost = (blocks * ns + sms - 1) / sms * ((tk + ns - 1) / ns + 4) + (ns > 1 ? 2 : 0);
+    if (cost < best_cost) best_cost = cost, best = (int)ns;
+  }
+  return best;
+}
+
 Plan make_plan(const b2_bias_attn_args* a, bool bwd) {
   Plan pl;
   const int64_t rows = a->B * a->H * a->Sq;
-  const int tile = kSimtTile;
+  pl.tc = bwd ? tc_bwd_eligible(a) : tc_fwd_eligible(a);
+  const int tile = pl.tc ? kTcTile : kSimtTile;
   const int64_t tq = (a->Sq + tile - 1) / tile, tk = (a->Sk + tile - 1) / tile;
   if (!bwd) {
-    // few query tiles and many key tiles: split the keys so that every SM has a block, at least four tiles each
-    const int64_t blocks = tq * a->B * a->H;
-    const int64_t sms = device_info().sm_count > 0 ? device_info().sm_count : 148;
-    if (blocks < sms) pl.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>(sms / blocks, tk / 4));
+    pl.nsplit = pick_splits(tq * a->B * a->H, tk);
     if (pl.nsplit > 1) {
       pl.part_o = 0;
       pl.part_ml = up16((uint64_t)pl.nsplit * rows * a->D * 4);
@@ -160,7 +178,8 @@ Plan make_plan(const b2_bias_attn_args* a, bool bwd) {
   } else {
     pl.ntq = (int)tq;
     pl.delta = 0;
-    pl.dtab = up16((uint64_t)rows * 4);
+    pl.sq_pad = (int)((a->Sq + kTcPad - 1) / kTcPad * kTcPad);
+    pl.dtab = pl.tc ? (uint64_t)(a->B * a->H) * pl.sq_pad * 8 : up16((uint64_t)rows * 4);
     pl.bytes = pl.dtab + (a->dtable ? up16((uint64_t)(a->B * a->H * tq) * a->num_buckets * 4) : 0);
   }
   return pl;
@@ -168,7 +187,7 @@ Plan make_plan(const b2_bias_attn_args* a, bool bwd) {
 
 Params make_params(const b2_bias_attn_args* a) {
   Params p{};
-  p.q = a->q, p.k = a->k, p.v = a->v, p.o = a->o, p.lse = a->lse, p.table = a->table, p.mask = a->key_mask;
+  p.q = a->q, p.k = a->k, p.v = a->v, p.o = a->o, p.o32 = a->o32, p.lse = a->lse, p.table = a->table, p.mask = a->key_mask;
   p.d_o = a->d_o, p.dq = a->dq, p.dk = a->dk, p.dv = a->dv;
   for (int i = 0; i < 3; ++i) {
     p.q_s[i] = a->q_s[i], p.k_s[i] = a->k_s[i], p.v_s[i] = a->v_s[i], p.o_s[i] = a->o_s[i];
@@ -244,7 +263,7 @@ extern "C" int b2_bias_bucket(int64_t rel, int32_t num_buckets, int32_t max_dist
 extern "C" uint64_t b2_bias_attn_workspace_bytes(const b2_bias_attn_args* a, int32_t backward) {
   using namespace b2::bias_attn;
   if (!a || a->B <= 0 || a->H <= 0 || a->Sq <= 0 || a->Sk <= 0) return 0;
-  if (check(a, false)) return 0;
+  if (check(a, backward != 0)) return 0;
   b2::ensure_init();
   return make_plan(a, backward != 0).bytes;
 }
@@ -262,7 +281,7 @@ extern "C" int b2_bias_attn_fwd(const b2_bias_attn_args* a, b2_stream_t stream) 
   p.nsplit = pl.nsplit;
   p.part_o = (float*)((char*)a->workspace + pl.part_o);
   p.part_ml = (float2*)((char*)a->workspace + pl.part_ml);
-  if (int rc = simt_fwd(p, a->dtype, st)) return rc;
+  if (int rc = pl.tc ? tc_fwd(p, a->dtype == B2_BF16, st) : simt_fwd(p, a->dtype, st)) return rc;
   return p.nsplit > 1 ? by_dtype<Combine>(a->dtype, p, st) : 0;
 }
 
@@ -289,8 +308,12 @@ extern "C" int b2_bias_attn_bwd(const b2_bias_attn_args* a, b2_stream_t stream) 
   float* delta = (float*)((char*)a->workspace + pl.delta);
   p.delta = delta;
   p.dtab = a->dtable ? (float*)((char*)a->workspace + pl.dtab) : nullptr;
-  if (int rc = by_dtype<Delta>(a->dtype, p, delta, st)) return rc;
-  if (int rc = simt_bwd(p, a->dtype, st)) return rc;
+  if (pl.tc) {
+    if (int rc = tc_bwd(p, a->dtype == B2_BF16, (float2*)delta, pl.sq_pad, st)) return rc;
+  } else {
+    if (int rc = by_dtype<Delta>(a->dtype, p, delta, st)) return rc;
+    if (int rc = simt_bwd(p, a->dtype, st)) return rc;
+  }
   if (a->dtable) {
     {
       LaunchScope ls("bias_attn_dtable", st);

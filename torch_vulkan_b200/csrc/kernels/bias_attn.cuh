@@ -23,6 +23,7 @@ struct Params {
   const void* k;
   const void* v;
   void* o;
+  float* o32;           // unrounded O [B*H*Sq][D], NULL: not kept
   float* lse;
   const float* table;
   const uint8_t* mask;
@@ -82,6 +83,12 @@ __device__ __forceinline__ int key_end(const Params& p, int64_t last_row) {
 int simt_fwd(const Params& p, int dtype, cudaStream_t st);   // bias_attn_simt.cu
 int simt_bwd(const Params& p, int dtype, cudaStream_t st);
 constexpr int kSimtTile = 64;
+bool tc_fwd_eligible(const b2_bias_attn_args* a);            // bias_attn_tc.cu
+bool tc_bwd_eligible(const b2_bias_attn_args* a);
+int tc_fwd(const Params& p, bool bf16, cudaStream_t st);
+int tc_bwd(const Params& p, bool bf16, float2* lsed, int sq_pad, cudaStream_t st);
+constexpr int kTcTile = 128;
+constexpr int kTcPad = 384;  // (lse, delta) rows are padded to a multiple of every tile height
 
 // More than the default 48 KB of shared memory, set once per kernel and device.
 template <typename K>

@@ -193,7 +193,10 @@ __global__ void __launch_bounds__(256) fwd_kernel(const __grid_constant__ Params
 #pragma unroll
       for (int c = 0; c < DP / 16; ++c) {
         const int d = tx * 4 + 64 * (c >> 2) + (c & 3);
-        if (d < p.D) o[d] = from_f32<T>(acc[i][c] * inv);
+        if (d < p.D) {
+          o[d] = from_f32<T>(acc[i][c] * inv);
+          if (p.o32) p.o32[row * p.D + d] = acc[i][c] * inv;
+        }
       }
       if (tx == 0 && p.lse) p.lse[row] = l[i] > 0.f ? (m[i] + log2f(l[i])) * kLn2 : -INFINITY;
     }

@@ -1,0 +1,996 @@
+// Relative-position-bias attention on the tensor cores (tcgen05 + TMEM + TMA), bf16 / f16, head dim up to 128 in
+// multiples of 8 (columns past D are filled with zeros by the tile loads and clipped by the tile stores).
+//
+// The bias of a 128-row tile against a key tile depends on key - query alone: it is a slice of one vector of
+// 2 max_distance + 509 floats per head in shared memory, which thread = row reads at consecutive addresses across the
+// lanes (no bank conflicts); tiles wholly beyond max_distance take one constant instead. The causal mask is part of the
+// vector (-inf), the key mask one bit per key from a ballot, and fully hidden tiles at the end are not walked.
+#include "bias_attn.cuh"
+#include "tc_ptx.cuh"
+
+namespace b2 {
+
+bool make_tmap(CUtensorMap* m, CUtensorMapDataType dt, int rank, const void* base, const uint64_t* dims,
+               const uint64_t* strides_bytes, const uint32_t* box, CUtensorMapSwizzle sw);  // gemm_tc.cu
+
+namespace bias_attn {
+namespace {
+
+constexpr int kPad = 254;  // a tile that reaches within max_distance spans at most 254 more positions on either side
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if (BF16) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+  }
+  __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+
+template <bool BF16>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if (BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  return __half22float2(*reinterpret_cast<__half2*>(&w));
+}
+
+__device__ __forceinline__ int vec_len(const Params& p) { return 2 * p.R + 2 * kPad + 1; }
+inline int vec_bytes(const Params& p) { return (2 * p.R + 2 * kPad + 1 + 3) / 4 * 16; }
+
+// vec[rel + R + kPad] = bias of head h at rel, log2 units
+__device__ __forceinline__ void fill_vec(const Params& p, int h, float* vec, int tid, int n) {
+  for (int i = tid; i < vec_len(p); i += n) vec[i] = bias_at(p, h, i - p.R - kPad);
+}
+
+// One bit per key of the 32 keys from k: inside [0, Sk) and not masked. Whole warp.
+__device__ __forceinline__ uint32_t key_bits(const Params& p, int b, int k) {
+  const int j = k + (threadIdx.x & 31);
+  const bool ok = j < p.Sk && (p.mask == nullptr || p.mask[(int64_t)b * p.mask_sb + j] != 0);
+  return __ballot_sync(0xffffffffu, ok);
+}
+
+// One past the last key below `end` that the mask leaves (whole block of nthreads; contains block barriers).
+__device__ __forceinline__ int trim_end(const Params& p, int b, int end, int nthreads) {
+  if (p.mask == nullptr) return end;
+  const uint8_t* m = p.mask + (int64_t)b * p.mask_sb;
+  while (end > 0) {
+    const int j = end - 1 - (int)threadIdx.x;
+    const bool any = (int)threadIdx.x < nthreads && j >= 0 && m[j] != 0;
+    if (__syncthreads_or(any)) {
+      // a key among the last nthreads: the exact end does not matter, tiles are dropped whole
+      return end;
+    }
+    end -= nthreads;
+  }
+  return 0;
+}
+
+// ==================================================================================================
+// forward: two softmax warpgroups take the key tiles in turn, each with its own S and O in TMEM
+// ==================================================================================================
+template <int D>
+struct Fwd {
+  static constexpr int BQ = 128, BK = 128, DCH = D / 64;
+  static constexpr int Q_BYTES = BQ * D * 2, KV_BYTES = BK * D * 2;
+  static constexpr int NS = D == 64 ? 4 : 2;  // K / V ring depth
+  static constexpr int OFF_Q = 0, OFF_K = Q_BYTES, OFF_V = OFF_K + NS * KV_BYTES, OFF_BAR = OFF_V + NS * KV_BYTES;
+  static constexpr int OFF_VEC = OFF_BAR + 256;
+  static constexpr int THREADS = 320;
+  static constexpr uint32_t T_S = 0, T_O = 256, TMEM_COLS = 512;
+};
+
+// PREC (o32 wanted, for a backward): P enters the product as two 16-bit numbers, P = hi + lo, so that O is good to about
+// 2^-17 before its rounding. delta = rowsum(dO O) is made from it, and dS = P (dP - delta) cancels over a row: with P
+// rounded once, the bias gradient (a sum of dS over many rows) keeps errors of a few 1e-3 of itself.
+template <int D, bool BF16, bool PREC>
+__global__ void __launch_bounds__(320, 1)
+    bias_fwd_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO,
+                const __grid_constant__ Params p) {
+  using C = Fwd<D>;
+  constexpr int NS = C::NS;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+  uint64_t* q_full = bar;
+  uint64_t* k_full = bar + 1;         // [NS]
+  uint64_t* k_empty = k_full + NS;    // [NS]
+  uint64_t* v_full = k_empty + NS;    // [NS]
+  uint64_t* v_empty = v_full + NS;    // [NS]
+  uint64_t* s_full = v_empty + NS;    // [2] S of tile t in S[t & 1]
+  uint64_t* p_full = s_full + 2;      // [2] P of tile t in TMEM over S[t & 1]
+  uint64_t* o_upd = p_full + 2;       // [2] P V of tile t done
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_upd + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(o_upd + 3);
+  float* vec = reinterpret_cast<float*>(smem + C::OFF_VEC);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // causal: the tiles with the most keys start first
+  const int qt = p.causal ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x;
+  const int q0 = qt * C::BQ;
+  const int b = (int)blockIdx.y / p.H, h = (int)blockIdx.y % p.H, hk = h / (p.H / p.Hk);
+
+  if (threadIdx.x == 0) {
+    tc::mbar_init(q_full, 1);
+    for (int i = 0; i < NS; ++i) {
+      tc::mbar_init(&k_full[i], 1), tc::mbar_init(&k_empty[i], 1);
+      tc::mbar_init(&v_full[i], 1), tc::mbar_init(&v_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) tc::mbar_init(&s_full[i], 1), tc::mbar_init(&p_full[i], 128), tc::mbar_init(&o_upd[i], 1);
+    *abort_flag = 0;
+    tc::fence_barrier_init();
+  }
+  tc::pdl_wait();
+  if (warp == 1) {
+    tc::tmem_alloc(tmem_slot, C::TMEM_COLS);
+    tc::tmem_relinquish();
+  }
+  fill_vec(p, h, vec, threadIdx.x, C::THREADS);
+  const int end = trim_end(p, b, key_end(p, min(q0 + C::BQ, p.Sq) - 1), C::THREADS);
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tbase = *tmem_slot;
+  tc::pdl_trigger();
+  const int ntiles = (end + C::BK - 1) / C::BK;
+  const int per = (ntiles + p.nsplit - 1) / p.nsplit;
+  const int t0 = (int)blockIdx.z * per;
+  const int n = max(0, min(per, ntiles - t0));  // tiles of this block: t0 .. t0 + n
+
+  if (warp == 0) {
+    if (lane == 0 && n > 0) {
+      // ---------------- producer ----------------
+      bool ok = true;
+      tc::mbar_arrive_expect_tx(q_full, C::Q_BYTES);
+      for (int c = 0; c < C::DCH; ++c) tc::tma_load_4d(smem + C::OFF_Q + c * (C::BQ * 128), &tmQ, q_full, c * 64, q0, h, b);
+      int issued_k[NS] = {}, issued_v[NS] = {};
+      for (int t = 0; t < n; ++t) {
+        const int s = t % NS, k0 = (t0 + t) * C::BK;
+        const uint32_t ph = (uint32_t)((t / NS) & 1) ^ 1;
+        if (!tc::mbar_wait(&k_empty[s], ph, p.err) || *abort_flag) { ok = false; break; }
+        tc::mbar_arrive_expect_tx(&k_full[s], C::KV_BYTES);
+        for (int c = 0; c < C::DCH; ++c)
+          tc::tma_load_4d(smem + C::OFF_K + s * C::KV_BYTES + c * (C::BK * 128), &tmK, &k_full[s], c * 64, k0, hk, b);
+        issued_k[s]++;
+        if (!tc::mbar_wait(&v_empty[s], ph, p.err) || *abort_flag) { ok = false; break; }
+        tc::mbar_arrive_expect_tx(&v_full[s], C::KV_BYTES);
+        for (int c = 0; c < C::DCH; ++c)
+          tc::tma_load_4d(smem + C::OFF_V + s * C::KV_BYTES + c * (C::BK * 128), &tmV, &v_full[s], c * 64, k0, hk, b);
+        issued_v[s]++;
+      }
+      if (!ok) {
+        *abort_flag = 1;
+        tc::mbar_wait(q_full, 0, nullptr);
+        for (int s = 0; s < NS; ++s) {
+          if (issued_k[s]) tc::mbar_wait(&k_full[s], (uint32_t)((issued_k[s] - 1) & 1), nullptr);
+          if (issued_v[s]) tc::mbar_wait(&v_full[s], (uint32_t)((issued_v[s] - 1) & 1), nullptr);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && n > 0) {
+      // ---------------- MMA issuer: S_t = Q K_t^T into S[t & 1]; O[t & 1] += P_t V_t with P_t read from TMEM; then
+      // S_t+2 over P_t's columns (MMAs of one thread execute in order) ----------------
+      constexpr uint32_t IDESC_S = tc::idesc_f16(128, C::BK, BF16, false, false);
+      constexpr uint32_t IDESC_O = tc::idesc_f16(128, D, BF16, false, true);
+      const tc::SDesc qd = tc::sdesc_parts(tc::smem_u32(smem + C::OFF_Q), 16, 1024);
+      bool ok = tc::mbar_wait(q_full, 0, p.err);
+      auto issue_s = [&](int t) -> bool {
+        const int ks = t % NS;
+        if (!tc::mbar_wait(&k_full[ks], (uint32_t)((t / NS) & 1), p.err)) return false;
+        tc::tc_fence_after();
+        const tc::SDesc kd = tc::sdesc_parts(tc::smem_u32(smem + C::OFF_K + ks * C::KV_BYTES), 16, 1024);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t off = (k >> 2) * (C::BK * 128) + (k & 3) * 32;
+          tc::mma_f16_ss(tbase + C::T_S + (t & 1) * 128, tc::sdesc_at(qd, off), tc::sdesc_at(kd, off), IDESC_S, k > 0 ? 1u : 0u);
+        }
+        tc::mma_commit(&s_full[t & 1]);
+        tc::mma_commit(&k_empty[ks]);
+        return true;
+      };
+      if (ok) ok = issue_s(0);
+      if (ok && n > 1) ok = issue_s(1);
+      for (int t = 0; t < n && ok; ++t) {
+        const int s = t & 1, vs = t % NS;
+        if (!tc::mbar_wait(&p_full[s], (uint32_t)((t >> 1) & 1), p.err) ||
+            !tc::mbar_wait(&v_full[vs], (uint32_t)((t / NS) & 1), p.err)) {
+          ok = false;
+          break;
+        }
+        tc::tc_fence_after();
+        const tc::SDesc vd = tc::sdesc_parts(tc::smem_u32(smem + C::OFF_V + vs * C::KV_BYTES), C::BK * 128, 1024);
+#pragma unroll
+        for (int k = 0; k < C::BK / 16; ++k)
+          tc::mma_f16_ts(tbase + C::T_O + s * 128, tbase + C::T_S + s * 128 + k * 8, tc::sdesc_at(vd, k * 2048), IDESC_O,
+                         (k > 0 || t >= 2) ? 1u : 0u);
+        if (PREC) {
+#pragma unroll
+          for (int k = 0; k < C::BK / 16; ++k)
+            tc::mma_f16_ts(tbase + C::T_O + s * 128, tbase + C::T_S + s * 128 + 64 + k * 8, tc::sdesc_at(vd, k * 2048), IDESC_O, 1u);
+        }
+        tc::mma_commit(&o_upd[s]);
+        tc::mma_commit(&v_empty[vs]);
+        if (t + 2 < n && !issue_s(t + 2)) ok = false;
+      }
+      if (!ok) *abort_flag = 1;
+    }
+  } else {
+    // ---------------- softmax warpgroups: thread = query row ----------------
+    const int g = (warp - 2) >> 2, quarter = warp & 3;
+    const int r = quarter * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+    const uint32_t t_s = tbase + C::T_S + g * 128, t_o = tbase + C::T_O + g * 128;
+    const float sl2 = p.scale * kLog2e;
+    const float2 sl22 = make_float2(sl2, sl2);
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    int kb = 0;
+    for (int t = g; t < n; t += 2, ++kb) {
+      const int k0 = (t0 + t) * C::BK;
+      uint32_t bits[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) bits[c] = key_bits(p, b, k0 + c * 32);
+      const bool full = (bits[0] & bits[1] & bits[2] & bits[3]) == 0xffffffffu;
+      if (!tc::mbar_wait(&s_full[g], (uint32_t)(kb & 1), p.err) || *abort_flag) {
+        ok = false;
+        break;
+      }
+      tc::tc_fence_after();
+      uint32_t sr[128];
+      __syncwarp();
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tc::tmem_ld32(t_s + c * 32 + lane_off, sr + 32 * c);
+      tc::tmem_wait_ld();
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tc::reg_fence32(sr + 32 * c);
+      // bias: x = s * scale_log2 + bias. rel of column 0 against this tile's first row
+      const int rel0 = k0 - q0 - p.q_off;
+      const bool near = rel0 - 127 < p.R && rel0 + 127 > -p.R;
+      float cst = 0.f;
+      if (near) {
+        const float* bv = vec + (rel0 - r + p.R + kPad);
+#pragma unroll
+        for (int e = 0; e < 128; e += 2) {
+          const float2 x = __ffma2_rn(make_float2(__uint_as_float(sr[e]), __uint_as_float(sr[e + 1])), sl22,
+                                      make_float2(bv[e], bv[e + 1]));
+          sr[e] = __float_as_uint(x.x), sr[e + 1] = __float_as_uint(x.y);
+        }
+      } else {
+        cst = rel0 > 0 ? vec[vec_len(p) - 1] : vec[0];
+      }
+      if (!full) {
+#pragma unroll
+        for (int e = 0; e < 128; ++e)
+          if (!((bits[e >> 5] >> (e & 31)) & 1u)) sr[e] = __float_as_uint(-INFINITY);
+      }
+      float mx8[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) mx8[e] = __uint_as_float(sr[e]);
+#pragma unroll
+      for (int e = 8; e < 128; ++e) mx8[e & 7] = fmaxf(mx8[e & 7], __uint_as_float(sr[e]));
+      const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])),
+                             fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
+      const float mul = near ? 1.f : sl2;  // scale > 0
+      const float m_blk = fmaf(mx, mul, cst);
+      // keep the old maximum unless the new one is more than 2^8 larger
+      const bool need = m_blk > m + 8.f || (m == -INFINITY && m_blk > -INFINITY);
+      float alpha = 1.f;
+      if (need) {
+        alpha = (m == -INFINITY) ? 0.f : ex2(m - m_blk);
+        m = m_blk;
+      }
+      if (kb > 0 && __any_sync(0xffffffffu, need)) {
+#pragma unroll 1
+        for (int c = 0; c < D / 16; ++c) {
+          uint32_t orow[16];
+          tc::tmem_ld16(t_o + c * 16 + lane_off, orow);
+          tc::tmem_wait_ld();
+          tc::reg_fence16(orow);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) orow[e] = __float_as_uint(__uint_as_float(orow[e]) * alpha);
+          tc::tmem_st16(t_o + c * 16 + lane_off, orow);
+        }
+      }
+      const float nmv = (m == -INFINITY) ? -INFINITY : cst - m;  // nothing seen yet: exp2(-inf) = 0
+      const float2 nm = make_float2(nmv, nmv), mul2 = make_float2(mul, mul);
+      float2 rs4[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        uint32_t w[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const int c = hh * 64 + 2 * i;
+          const float2 x = __ffma2_rn(make_float2(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), mul2, nm);
+          const float2 e2 = make_float2(ex2(x.x), ex2(x.y));
+          rs4[i & 3] = __fadd2_rn(rs4[i & 3], e2);
+          w[i] = pack2<BF16>(e2.x, e2.y);
+          if (PREC) {  // what the rounding left, packed over the score
+            const float2 hi = unpack2<BF16>(w[i]);
+            sr[c] = pack2<BF16>(e2.x - hi.x, e2.y - hi.y);
+          }
+        }
+        tc::tmem_st32(t_s + hh * 32 + lane_off, w);
+        if (PREC) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) w[i] = sr[hh * 64 + 2 * i];
+          tc::tmem_st32(t_s + 64 + hh * 32 + lane_off, w);
+        }
+      }
+      const float2 rs2 = __fadd2_rn(__fadd2_rn(rs4[0], rs4[1]), __fadd2_rn(rs4[2], rs4[3]));
+      l = l * alpha + (rs2.x + rs2.y);
+      if (!full && p.mask != nullptr) {
+        // masked keys may hold anything, and 0 * NaN is NaN in the P V product: clear their rows of V
+        if (!tc::mbar_wait(&v_full[t % NS], (uint32_t)((t / NS) & 1), p.err)) { ok = false; break; }
+        if (!((bits[quarter] >> lane) & 1u)) {
+#pragma unroll
+          for (int c = 0; c < C::DCH; ++c) {
+            uint4* row = reinterpret_cast<uint4*>(smem + C::OFF_V + (t % NS) * C::KV_BYTES + c * (C::BK * 128) + r * 128);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) row[i] = make_uint4(0u, 0u, 0u, 0u);
+          }
+        }
+        tc::fence_async_shared();
+        __syncwarp();
+      }
+      tc::tmem_wait_st();
+      tc::tc_fence_before();
+      tc::mbar_arrive(&p_full[g]);
+    }
+    // ---------------- epilogue: join the two groups ----------------
+    if (ok && kb > 0 && !tc::mbar_wait(&o_upd[g], (uint32_t)((kb - 1) & 1), p.err)) ok = false;
+    float2* x0p = reinterpret_cast<float2*>(smem + C::OFF_Q);  // Q is done with once both groups are here
+    float2* x1p = x0p + C::BQ;
+    tc::named_bar_sync(1, 256);
+    (g ? x1p : x0p)[r] = make_float2(m, l);
+    tc::named_bar_sync(1, 256);
+    if (ok && !*abort_flag) {
+      tc::tc_fence_after();
+      const float2 x0 = x0p[r], x1 = x1p[r];
+      const float M = fmaxf(x0.x, x1.x);
+      const float a0 = x0.x == -INFINITY ? 0.f : ex2(x0.x - M);
+      const float a1 = x1.x == -INFINITY ? 0.f : ex2(x1.x - M);
+      const float L = x0.y * a0 + x1.y * a1;
+      const bool split = p.nsplit > 1;
+      const float inv = split ? 1.f : (L > 0.f ? 1.f / L : 0.f);
+      const float s0 = a0 * inv, s1 = a1 * inv;
+      const int qrow = q0 + r;
+      const int64_t row = (int64_t)blockIdx.y * p.Sq + qrow;
+      const int64_t prow = (int64_t)blockIdx.z * p.B * p.H * p.Sq + row;
+      uint8_t* stg = smem + C::OFF_K + (warp - 2) * (D / 64) * 2048;
+#pragma unroll
+      for (int cc = 0; cc < D / 64; ++cc) {
+        const int c = g * (D / 64) + cc;  // this group's 32-column chunks
+        float v[32];
+        {
+          uint32_t o0[32], o1[32];
+          __syncwarp();
+          if (n > 0) tc::tmem_ld32(tbase + C::T_O + c * 32 + lane_off, o0);
+          if (n > 1) tc::tmem_ld32(tbase + C::T_O + 128 + c * 32 + lane_off, o1);
+          tc::tmem_wait_ld();
+          if (n > 0) tc::reg_fence32(o0);
+          if (n > 1) tc::reg_fence32(o1);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            v[e] = n > 0 ? __uint_as_float(o0[e]) * s0 : 0.f;
+            if (n > 1) v[e] = fmaf(__uint_as_float(o1[e]), s1, v[e]);
+          }
+        }
+        if ((split || PREC) && qrow < p.Sq) {
+          float* po = (split ? p.part_o + prow * p.D : p.o32 + row * p.D) + c * 32;
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            if (c * 32 + e < p.D) *reinterpret_cast<float4*>(po + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+        }
+        if (split) continue;
+        // O rows leave through a per-warp staging tile in the idle K ring, one 32 x 32 box per tile store
+        uint32_t w[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) w[e] = pack2<BF16>(v[2 * e], v[2 * e + 1]);
+        uint8_t* buf = stg + cc * 2048;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          *reinterpret_cast<uint4*>(buf + lane * 64 + ((e ^ ((lane >> 1) & 3)) << 4)) =
+              make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+        tc::fence_async_shared();
+        __syncwarp();
+        if (lane == 0 && q0 + quarter * 32 < p.Sq && c * 32 < p.D) {
+          tc::tma_store_4d(&tmO, buf, c * 32, q0 + quarter * 32, h, b);
+          tc::bulk_commit();
+        }
+      }
+      if (lane == 0) tc::bulk_wait0();
+      if (g == 0 && qrow < p.Sq) {
+        if (split) p.part_ml[prow] = make_float2(M, L);
+        else if (p.lse) p.lse[row] = L > 0.f ? (M + __log2f(L)) * kLn2 : -INFINITY;
+      }
+    } else {
+      *abort_flag = 1;
+    }
+  }
+  __syncwarp();  // warps 0 and 1 arrive diverged; the block barrier is an aligned one
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tc::tc_fence_after();
+    tc::tmem_dealloc(tbase, C::TMEM_COLS);
+  }
+}
+
+// ==================================================================================================
+// backward: the same walk with the two sides in either place. The fixed side's two operands X1, X2 (128 rows) stay in
+// shared memory, the walked side's Y1, Y2 come in tiles of NT rows:
+//   KEYS = false  X = Q, dO (a block owns 128 queries), Y = K, V:   dQ += dS K, and the bias gradient
+//   KEYS = true   X = K, V (a block owns 128 keys),    Y = Q, dO:   dK += dS^T Q, dV += P^T dO, over every query head
+//                                                                   that shares the key/value head
+// S = X1 Y1^T and dP = X2 Y2^T are recomputed on both sides (7 products instead of 5), which leaves every gradient one
+// owner: no atomics, no accumulator in memory, the same bits on every run. Two warpgroups take the tiles in turn, each
+// with its own S and dP columns in TMEM; P and dS (16 bits) replace them and are the A operands of the gradient MMAs.
+// ==================================================================================================
+template <int D, bool KEYS>
+struct Bwd {
+  static constexpr int BX = 128, DCH = D / 64;
+  static constexpr int NT = (KEYS && D == 128) ? 64 : 96;  // walked rows per tile: what TMEM holds twice beside the sums
+  static constexpr int X_BYTES = BX * D * 2, Y_BYTES = NT * D * 2;
+  static constexpr int LD_BYTES = KEYS ? NT * 8 : 0;       // (lse log2 e, delta) of the walked queries
+  static constexpr int STAGE = 2 * Y_BYTES + (LD_BYTES + 1023) / 1024 * 1024;
+  static constexpr int NS = D == 64 ? 3 : 2;
+  static constexpr int OFF_X = 0, OFF_Y = 2 * X_BYTES, OFF_BAR = OFF_Y + NS * STAGE, OFF_VEC = OFF_BAR + 256;
+  static constexpr int THREADS = 320;
+  static constexpr uint32_t T_S = 0, T_DP = NT, T_BUF = 2 * NT, T_ACC = 4 * NT, TMEM_COLS = 512;
+  static constexpr uint32_t T_ACC2 = T_ACC + D;  // KEYS: dV at T_ACC, dK behind it
+  static_assert(4 * NT + (KEYS ? 2 * D : D) <= 512, "TMEM columns");
+};
+
+// Adds the diagonal sums of a 32 x 16 block (rows = lanes, v = this lane's 16 columns) to arr[column - row]. Running sums
+// travel up the lanes by one per column: the sum that lane l holds at column e belongs to the diagonal e - l; the one
+// that has passed lane 31 is complete and is put aside. Two blocks run interleaved to hide the shuffle's latency.
+__device__ __forceinline__ void add_diagonals(const float* v, float* arr, float* scratch, int lane) {
+  float a0 = v[0], a1 = v[16];
+  const int from = (lane + 31) & 31;
+#pragma unroll
+  for (int e = 1; e < 16; ++e) {
+    float t0 = __shfl_sync(0xffffffffu, a0, from), t1 = __shfl_sync(0xffffffffu, a1, from);
+    if (lane == 0) {
+      scratch[e - 1] = t0, scratch[16 + e - 1] = t1;
+      t0 = t1 = 0.f;
+    }
+    a0 = t0 + v[e], a1 = t1 + v[16 + e];
+  }
+  __syncwarp();
+  arr[15 - lane] += a0;
+  if (lane < 15) arr[lane - 31] += scratch[lane];
+  __syncwarp();
+  arr[31 - lane] += a1;
+  if (lane < 15) arr[lane - 15] += scratch[16 + lane];
+  __syncwarp();
+}
+
+template <int D, bool BF16, bool KEYS>
+__global__ void __launch_bounds__(320, 1)
+    bias_bwd_tc(const __grid_constant__ CUtensorMap tmX1, const __grid_constant__ CUtensorMap tmX2,
+                const __grid_constant__ CUtensorMap tmY1, const __grid_constant__ CUtensorMap tmY2,
+                const __grid_constant__ CUtensorMap tmG1, const __grid_constant__ CUtensorMap tmG2,
+                const __grid_constant__ Params p, const float2* __restrict__ lsed, int sq_pad) {
+  using C = Bwd<D, KEYS>;
+  constexpr int NS = C::NS, NT = C::NT;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+  uint64_t* x_full = bar;
+  uint64_t* y_full = bar + 1;          // [NS]
+  uint64_t* y_empty = y_full + NS;     // [NS]
+  uint64_t* sd_full = y_empty + NS;    // [2] S and dP of tile t in buffer t & 1
+  uint64_t* pd_full = sd_full + 2;     // [2] P / dS of tile t in TMEM (count 128)
+  uint64_t* acc_full = pd_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(acc_full + 2);
+  const int vlen4 = (vec_len(p) + 3) / 4 * 4;
+  float* vec = reinterpret_cast<float*>(smem + C::OFF_VEC);  // KEYS: one per warpgroup (the head changes along the walk)
+  float* darr = vec + vlen4;                                 // !KEYS: diagonal sums, one array per warp
+  float* dscr = darr + 8 * vlen4;                            // !KEYS: 32 floats per warp
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int heads = KEYS ? p.Hk : p.H, G = p.H / p.Hk;
+  // causal: the query tiles with the most keys come first; the key tiles with the most queries already do
+  const int xt = (!KEYS && p.causal) ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x;
+  const int x0 = xt * C::BX;
+  const int b = (int)blockIdx.y / heads, hx = (int)blockIdx.y % heads;
+
+  if (threadIdx.x == 0) {
+    tc::mbar_init(x_full, 1);
+    for (int i = 0; i < NS; ++i) tc::mbar_init(&y_full[i], 1), tc::mbar_init(&y_empty[i], 1);
+    for (int i = 0; i < 2; ++i) tc::mbar_init(&sd_full[i], 1), tc::mbar_init(&pd_full[i], 128);
+    tc::mbar_init(acc_full, 1);
+    *abort_flag = 0;
+    tc::fence_barrier_init();
+  }
+  tc::pdl_wait();
+  if (warp == 1) {
+    tc::tmem_alloc(tmem_slot, C::TMEM_COLS);
+    tc::tmem_relinquish();
+  }
+  int first = 0, tiles;  // tiles first .. first + tiles of every walked head
+  if (KEYS) {
+    const int any = p.mask == nullptr ||
+                    __syncthreads_or((int)threadIdx.x < C::BX && x0 + (int)threadIdx.x < p.Sk &&
+                                     p.mask[(int64_t)b * p.mask_sb + x0 + threadIdx.x] != 0);
+    const int nt = (p.Sq + NT - 1) / NT;
+    if (p.causal) first = (int)min((int64_t)nt, max((int64_t)0, (int64_t)x0 - p.q_off) / NT);
+    tiles = any ? nt - first : 0;
+  } else {
+    fill_vec(p, hx, vec, threadIdx.x, C::THREADS);
+    if (p.dtab)
+      for (int i = threadIdx.x; i < 8 * vlen4; i += C::THREADS) darr[i] = 0.f;
+    tiles = (trim_end(p, b, key_end(p, min(x0 + C::BX, p.Sq) - 1), C::THREADS) + NT - 1) / NT;
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tbase = *tmem_slot;
+  tc::pdl_trigger();
+  const int n = KEYS ? tiles * G : tiles;
+
+  if (warp == 0) {
+    if (lane == 0 && n > 0) {
+      // ---------------- producer ----------------
+      tc::mbar_arrive_expect_tx(x_full, 2 * C::X_BYTES);
+      for (int c = 0; c < C::DCH; ++c) {
+        tc::tma_load_4d(smem + C::OFF_X + c * (C::BX * 128), &tmX1, x_full, c * 64, x0, hx, b);
+        tc::tma_load_4d(smem + C::OFF_X + C::X_BYTES + c * (C::BX * 128), &tmX2, x_full, c * 64, x0, hx, b);
+      }
+      int issued[NS] = {};
+      bool ok = true;
+      for (int t = 0; t < n; ++t) {
+        const int s = t % NS;
+        const int gi = KEYS ? t / tiles : 0;
+        const int hy = KEYS ? hx * G + gi : hx / G;
+        const int y0 = KEYS ? (first + t - gi * tiles) * NT : t * NT;
+        if (!tc::mbar_wait(&y_empty[s], (uint32_t)((t / NS) & 1) ^ 1, p.err) || *abort_flag) { ok = false; break; }
+        uint8_t* st = smem + C::OFF_Y + s * C::STAGE;
+        tc::mbar_arrive_expect_tx(&y_full[s], 2 * C::Y_BYTES + C::LD_BYTES);
+        for (int c = 0; c < C::DCH; ++c) {
+          tc::tma_load_4d(st + c * (NT * 128), &tmY1, &y_full[s], c * 64, y0, hy, b);
+          tc::tma_load_4d(st + C::Y_BYTES + c * (NT * 128), &tmY2, &y_full[s], c * 64, y0, hy, b);
+        }
+        if (KEYS) tc::bulk_load(st + 2 * C::Y_BYTES, lsed + ((int64_t)b * p.H + hy) * sq_pad + y0, C::LD_BYTES, &y_full[s]);
+        issued[s]++;
+      }
+      if (!ok) {
+        *abort_flag = 1;
+        tc::mbar_wait(x_full, 0, nullptr);
+        for (int s = 0; s < NS; ++s)
+          if (issued[s]) tc::mbar_wait(&y_full[s], (uint32_t)((issued[s] - 1) & 1), nullptr);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && n > 0) {
+      // ---------------- MMA issuer ----------------
+      constexpr uint32_t IDESC_S = tc::idesc_f16(128, NT, BF16, false, false);
+      constexpr uint32_t IDESC_G = tc::idesc_f16(128, D, BF16, false, true);
+      const tc::SDesc x1 = tc::sdesc_parts(tc::smem_u32(smem + C::OFF_X), 16, 1024);
+      const tc::SDesc x2 = tc::sdesc_parts(tc::smem_u32(smem + C::OFF_X + C::X_BYTES), 16, 1024);
+      bool ok = tc::mbar_wait(x_full, 0, p.err);
+      auto issue_sd = [&](int t) -> bool {
+        const int s = t % NS;
+        if (!tc::mbar_wait(&y_full[s], (uint32_t)((t / NS) & 1), p.err)) return false;
+        tc::tc_fence_after();
+        const uint32_t st = tc::smem_u32(smem + C::OFF_Y + s * C::STAGE);
+        const tc::SDesc y1 = tc::sdesc_parts(st, 16, 1024), y2 = tc::sdesc_parts(st + C::Y_BYTES, 16, 1024);
+        const uint32_t buf = tbase + (t & 1) * C::T_BUF;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          tc::mma_f16_ss(buf + C::T_S, tc::sdesc_at(x1, (k >> 2) * (C::BX * 128) + (k & 3) * 32),
+                         tc::sdesc_at(y1, (k >> 2) * (NT * 128) + (k & 3) * 32), IDESC_S, k > 0 ? 1u : 0u);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          tc::mma_f16_ss(buf + C::T_DP, tc::sdesc_at(x2, (k >> 2) * (C::BX * 128) + (k & 3) * 32),
+                         tc::sdesc_at(y2, (k >> 2) * (NT * 128) + (k & 3) * 32), IDESC_S, k > 0 ? 1u : 0u);
+        tc::mma_commit(&sd_full[t & 1]);
+        return true;
+      };
+      if (ok) ok = issue_sd(0);
+      if (ok && n > 1) ok = issue_sd(1);
+      for (int t = 0; t < n && ok; ++t) {
+        const int s = t % NS;
+        if (!tc::mbar_wait(&pd_full[t & 1], (uint32_t)((t >> 1) & 1), p.err)) { ok = false; break; }
+        tc::tc_fence_after();
+        const uint32_t st = tc::smem_u32(smem + C::OFF_Y + s * C::STAGE);
+        const tc::SDesc y1 = tc::sdesc_parts(st, NT * 128, 1024), y2 = tc::sdesc_parts(st + C::Y_BYTES, NT * 128, 1024);
+        const uint32_t buf = tbase + (t & 1) * C::T_BUF;
+        const uint32_t acc0 = t > 0 ? 1u : 0u;
+        if (KEYS) {
+#pragma unroll
+          for (int k = 0; k < NT / 16; ++k)  // dV += P^T dO
+            tc::mma_f16_ts(tbase + C::T_ACC, buf + C::T_S + k * 8, tc::sdesc_at(y2, k * 2048), IDESC_G, k > 0 ? 1u : acc0);
+#pragma unroll
+          for (int k = 0; k < NT / 16; ++k)  // dK += dS^T Q
+            tc::mma_f16_ts(tbase + C::T_ACC2, buf + C::T_DP + k * 8, tc::sdesc_at(y1, k * 2048), IDESC_G, k > 0 ? 1u : acc0);
+        } else {
+#pragma unroll
+          for (int k = 0; k < NT / 16; ++k)  // dQ += dS K
+            tc::mma_f16_ts(tbase + C::T_ACC, buf + C::T_S + k * 8, tc::sdesc_at(y1, k * 2048), IDESC_G, k > 0 ? 1u : acc0);
+        }
+        tc::mma_commit(&y_empty[s]);
+        if (t + 2 < n && !issue_sd(t + 2)) ok = false;
+      }
+      if (ok) tc::mma_commit(acc_full);
+      else *abort_flag = 1;
+    }
+  } else {
+    // ---------------- element-wise warpgroups: thread = row of the fixed side ----------------
+    const int g = (warp - 2) >> 2, quarter = warp & 3;
+    const int r = quarter * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+    const uint32_t buf = tbase + g * C::T_BUF + lane_off;
+    const float sl2 = p.scale * kLog2e;
+    const float2 sl22 = make_float2(sl2, sl2);
+    // f16: P carries a factor of 2^8 so that 1 / Sk stays clear of the subnormals; dS does not
+    constexpr float PUP = BF16 ? 0.f : 8.f;
+    constexpr float PDOWN = BF16 ? 1.f : 1.f / 256.f;
+    float* myvec = KEYS ? vec + g * vlen4 : vec;
+    float* mydarr = darr + (warp - 2) * vlen4;
+    float* myscr = dscr + (warp - 2) * 32;
+    float nL = 0.f, nd = 0.f;  // !KEYS: -(lse log2 e) and -delta of this row
+    bool live = true;          // KEYS: this row's key takes part
+    if (!KEYS) {
+      const float2 ld = lsed[((int64_t)b * p.H + hx) * sq_pad + x0 + r];
+      nL = -ld.x, nd = -ld.y;
+    } else {
+      live = x0 + r < p.Sk && (p.mask == nullptr || p.mask[(int64_t)b * p.mask_sb + x0 + r] != 0);
+    }
+    float far_lo = 0.f, far_hi = 0.f;
+    int cur = -1;  // KEYS: the head whose bias is in myvec
+    bool ok = true;
+    int kb = 0;
+    for (int t = g; t < n; t += 2, ++kb) {
+      const int gi = KEYS ? t / tiles : 0;
+      const int y0 = KEYS ? (first + t - gi * tiles) * NT : t * NT;
+      if (KEYS && gi != cur) {
+        tc::named_bar_sync(2 + g, 128);  // nobody still reads the last head's
+        fill_vec(p, hx * G + gi, myvec, r, 128);
+        tc::named_bar_sync(2 + g, 128);
+        cur = gi;
+      }
+      uint32_t bits[NT / 32];
+      bool full = true;
+      if (!KEYS) {
+#pragma unroll
+        for (int c = 0; c < NT / 32; ++c) {
+          bits[c] = key_bits(p, b, y0 + c * 32);
+          full = full && bits[c] == 0xffffffffu;
+        }
+      }
+      // relative position of column 0 against row 0, and how it moves: -row + column (queries own the rows) or +row - column
+      const int rel0 = KEYS ? x0 - y0 - p.q_off : y0 - x0 - p.q_off;
+      const bool near = KEYS ? (rel0 - (NT - 1) < p.R && rel0 + 127 > -p.R) : (rel0 - 127 < p.R && rel0 + (NT - 1) > -p.R);
+      const float* bv = myvec + (rel0 + (KEYS ? r : -r) + p.R + kPad);
+      const float cst = near ? 0.f : (rel0 > 0 ? myvec[vec_len(p) - 1] : myvec[0]);
+      if (!tc::mbar_wait(&sd_full[g], (uint32_t)(kb & 1), p.err) || *abort_flag) { ok = false; break; }
+      if (KEYS && !tc::mbar_wait(&y_full[t % NS], (uint32_t)((t / NS) & 1), p.err)) { ok = false; break; }
+      tc::tc_fence_after();
+      __syncwarp();
+      const float4* ld4 = reinterpret_cast<const float4*>(smem + C::OFF_Y + (t % NS) * C::STAGE + 2 * C::Y_BYTES);
+#pragma unroll
+      for (int c = 0; c < NT / 32; ++c) {
+        uint32_t sv[32], dp[32];
+        tc::tmem_ld32(buf + C::T_S + c * 32, sv);
+        tc::tmem_ld32(buf + C::T_DP + c * 32, dp);
+        tc::tmem_wait_ld();
+        tc::reg_fence32(sv);
+        tc::reg_fence32(dp);
+        uint32_t wp[16], wd[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int col = c * 32 + 2 * e;
+          float2 off, del;
+          if (KEYS) {
+            const float4 L = ld4[col >> 1];
+            off = make_float2(PUP - L.x, PUP - L.z), del = make_float2(-L.y * PDOWN, -L.w * PDOWN);
+          } else {
+            off = make_float2(nL, nL), del = make_float2(nd, nd);
+          }
+          if (near) off = __fadd2_rn(off, KEYS ? make_float2(bv[-col], bv[-col - 1]) : make_float2(bv[col], bv[col + 1]));
+          else off = __fadd2_rn(off, make_float2(cst, cst));
+          const float2 x = __ffma2_rn(make_float2(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), sl22, off);
+          float2 pr = make_float2(ex2(x.x), ex2(x.y));
+          float2 dd = make_float2(__uint_as_float(dp[2 * e]), __uint_as_float(dp[2 * e + 1]));
+          dd = KEYS ? __ffma2_rn(dd, make_float2(PDOWN, PDOWN), del) : __fadd2_rn(dd, del);
+          float2 ds = __fmul2_rn(pr, dd);
+          if (KEYS) {
+            if (!live) pr = ds = make_float2(0.f, 0.f);
+            wp[e] = pack2<BF16>(pr.x, pr.y);
+          } else if (!full) {
+            if (!((bits[c] >> (2 * e)) & 1u)) ds.x = 0.f;
+            if (!((bits[c] >> (2 * e + 1)) & 1u)) ds.y = 0.f;
+          }
+          wd[e] = pack2<BF16>(ds.x, ds.y);
+          sv[2 * e] = __float_as_uint(ds.x), sv[2 * e + 1] = __float_as_uint(ds.y);
+        }
+        // P over S, dS over dP (KEYS) or over S: columns [16 c, 16 c + 16), whose scores this warp has read
+        if (KEYS) {
+          tc::tmem_st16(buf + C::T_S + c * 16, wp);
+          tc::tmem_st16(buf + C::T_DP + c * 16, wd);
+        } else {
+          tc::tmem_st16(buf + C::T_S + c * 16, wd);
+          if (p.dtab) {
+            const float* dsv = reinterpret_cast<const float*>(sv);
+            if (near) {
+              add_diagonals(dsv, mydarr + (rel0 + c * 32 - quarter * 32 + p.R + kPad), myscr, lane);
+            } else {
+              float s = 0.f;
+#pragma unroll
+              for (int e = 0; e < 32; ++e) s += dsv[e];
+              if (rel0 > 0) far_hi += s;
+              else far_lo += s;
+            }
+          }
+        }
+      }
+      if (!KEYS && !full && p.mask != nullptr) {
+        // masked keys may hold anything, and 0 * NaN is NaN in the dS K product: clear their rows of K
+        if (r < NT && !((bits[quarter < NT / 32 ? quarter : 0] >> lane) & 1u)) {
+#pragma unroll
+          for (int c = 0; c < C::DCH; ++c) {
+            uint4* row = reinterpret_cast<uint4*>(smem + C::OFF_Y + (t % NS) * C::STAGE + c * (NT * 128) + r * 128);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) row[i] = make_uint4(0u, 0u, 0u, 0u);
+          }
+        }
+        tc::fence_async_shared();
+        __syncwarp();
+      }
+      tc::tmem_wait_st();
+      tc::tc_fence_before();
+      tc::mbar_arrive(&pd_full[g]);
+    }
+    if (!KEYS && p.dtab) {
+      // this warp's far tiles join the ends of its array; then the arrays are added and cut into buckets
+      const float lo = warp_sum(far_lo), hi = warp_sum(far_hi);
+      if (lane == 0) mydarr[0] += lo, mydarr[vec_len(p) - 1] += hi;
+      tc::named_bar_sync(1, 256);
+      const int ew = (int)threadIdx.x - 64;
+      for (int i = ew; i < vec_len(p); i += 256) {
+        float s = 0.f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) s += darr[w * vlen4 + i];
+        vec[i] = s;  // the bias itself is no longer needed
+      }
+      tc::named_bar_sync(1, 256);
+      // bucket nb of a side holds the distances [thr[nb - 1], thr[nb]), the last one all beyond
+      for (int bk = warp - 2; bk < p.nb; bk += 8) {
+        const int side = p.bidir ? p.nb / 2 : p.nb;
+        const bool pos = p.bidir && bk >= side;
+        const int i = pos ? bk - side : bk;
+        int d0 = i == 0 ? 0 : (int)p.thr[i - 1], d1 = i == side - 1 ? p.R + kPad + 1 : (int)p.thr[i];
+        float s = 0.f;
+        if (pos) {
+          d0 = max(d0, 1);
+          for (int d = d0 + lane; d < d1; d += 32) s += vec[d + p.R + kPad];
+        } else {
+          for (int d = d0 + lane; d < d1; d += 32) s += vec[p.R + kPad - d];
+          if (!p.bidir && i == 0)  // one-sided: keys after the query share bucket 0
+            for (int d = 1 + lane; d <= p.R + kPad; d += 32) s += vec[d + p.R + kPad];
+        }
+        s = warp_sum(s);
+        if (lane == 0) p.dtab[((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * p.nb + bk] = s;
+      }
+    }
+    // ---------------- epilogue: group g writes its half of the columns ----------------
+    if (ok && n > 0) ok = tc::mbar_wait(acc_full, 0, p.err);
+    if (ok && !*abort_flag) {
+      tc::tc_fence_after();
+      const int rows = KEYS ? p.Sk : p.Sq;
+      // staging in the idle Y ring: every MMA that read it is done
+      uint8_t* stg = smem + C::OFF_Y + (warp - 2) * (KEYS ? 2 : 1) * C::DCH * 2048;
+#pragma unroll
+      for (int which = 0; which < (KEYS ? 2 : 1); ++which) {  // KEYS: dV, then dK
+        const bool wanted = KEYS ? (which ? p.dk != nullptr : p.dv != nullptr) : p.dq != nullptr;
+        if (!wanted) continue;
+        const float mul = KEYS ? (which ? p.scale : PDOWN) : p.scale;
+        const CUtensorMap* tm = which ? &tmG2 : &tmG1;
+#pragma unroll
+        for (int cc = 0; cc < C::DCH; ++cc) {
+          const int c = g * C::DCH + cc;
+          uint32_t v[32], w[16];
+          __syncwarp();
+          if (n > 0) {
+            tc::tmem_ld32(tbase + (which ? C::T_ACC2 : C::T_ACC) + c * 32 + lane_off, v);
+            tc::tmem_wait_ld();
+            tc::reg_fence32(v);
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            w[e] = n > 0 ? pack2<BF16>(__uint_as_float(v[2 * e]) * mul, __uint_as_float(v[2 * e + 1]) * mul) : 0u;
+          uint8_t* sb = stg + (which * C::DCH + cc) * 2048;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            *reinterpret_cast<uint4*>(sb + lane * 64 + ((e ^ ((lane >> 1) & 3)) << 4)) =
+                make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+          tc::fence_async_shared();
+          __syncwarp();
+          if (lane == 0 && x0 + quarter * 32 < rows && c * 32 < p.D) {
+            tc::tma_store_4d(tm, sb, c * 32, x0 + quarter * 32, hx, b);
+            tc::bulk_commit();
+          }
+        }
+      }
+      if (lane == 0) tc::bulk_wait0();
+    } else {
+      *abort_flag = 1;
+    }
+  }
+  __syncwarp();
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tc::tc_fence_after();
+    tc::tmem_dealloc(tbase, C::TMEM_COLS);
+  }
+}
+
+// lsed[bh][q] = (lse log2 e, sum_d dO O) for q < Sq, (+inf, 0) for padding and for rows without a key: exp2(x - inf) = 0.
+// Eight lanes a row, 16-byte loads.
+template <typename T>
+__global__ void __launch_bounds__(256) bias_bwd_prep(const __grid_constant__ Params p, float2* __restrict__ lsed, int sq_pad) {
+  tc::pdl_wait();
+  tc::pdl_trigger();
+  const int64_t idx = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 3;
+  const int part = threadIdx.x & 7;
+  const int64_t bh = idx / sq_pad;
+  const int q = (int)(idx - bh * sq_pad);
+  if (bh >= (int64_t)p.B * p.H) return;  // whole groups of eight lanes; warps of the last block may be partial
+  const int b = (int)(bh / p.H), h = (int)(bh % p.H);
+  float s = 0.f;
+  if (q < p.Sq) {
+    const T* o = row_of<T>((const void*)p.o, p.o_s, b, h, q);
+    const T* g = row_of<T>(p.d_o, p.do_s, b, h, q);
+    for (int d = part * 8; d < p.D; d += 64) {
+      const uint4 b4 = *reinterpret_cast<const uint4*>(g + d);
+      const T* c = reinterpret_cast<const T*>(&b4);
+      float a[8];
+      if (p.o32) {
+        const float4* f = reinterpret_cast<const float4*>(p.o32 + (bh * p.Sq + q) * p.D + d);
+        const float4 lo = f[0], hi = f[1];
+        a[0] = lo.x, a[1] = lo.y, a[2] = lo.z, a[3] = lo.w, a[4] = hi.x, a[5] = hi.y, a[6] = hi.z, a[7] = hi.w;
+      } else {
+        const uint4 a4 = *reinterpret_cast<const uint4*>(o + d);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a[i] = to_f32<T>(reinterpret_cast<const T*>(&a4)[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s = fmaf(a[i], to_f32<T>(c[i]), s);
+    }
+  }
+  const uint32_t m = __activemask();
+  s += __shfl_xor_sync(m, s, 1);
+  s += __shfl_xor_sync(m, s, 2);
+  s += __shfl_xor_sync(m, s, 4);
+  if (part == 0) {
+    const float lse = q < p.Sq ? p.lse[bh * p.Sq + q] : -INFINITY;
+    lsed[idx] = lse == -INFINITY ? make_float2(INFINITY, 0.f) : make_float2(lse * kLog2e, s);
+  }
+}
+
+bool bhsd_map(CUtensorMap* m, const void* base, const int64_t* s3, int64_t B, int64_t H, int64_t S, int64_t D, bool bf16,
+              uint32_t box_rows, uint32_t box_inner = 64, CUtensorMapSwizzle sw = CU_TENSOR_MAP_SWIZZLE_128B) {
+  uint64_t dims[4] = {(uint64_t)D, (uint64_t)S, (uint64_t)H, (uint64_t)B};
+  uint64_t strides[3] = {(uint64_t)s3[2] * 2, (uint64_t)s3[1] * 2, (uint64_t)s3[0] * 2};
+  // dimensions of size 1: any valid stride
+  if (S == 1) strides[0] = (uint64_t)((D + 7) / 8 * 8) * 2;
+  if (H == 1) strides[1] = strides[0] * (uint64_t)S;
+  if (B == 1) strides[2] = strides[1] * (uint64_t)H;
+  uint32_t box[4] = {box_inner, box_rows, 1, 1};
+  return make_tmap(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, base, dims, strides, box, sw);
+}
+bool store_map(CUtensorMap* m, void* base, const int64_t* s3, int64_t B, int64_t H, int64_t S, int64_t D, bool bf16) {
+  memset(m, 0, sizeof(*m));
+  return base == nullptr || bhsd_map(m, base, s3, B, H, S, D, bf16, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
+// 16-byte aligned rows with positive strides below 2^40 bytes
+bool layout_ok(const void* t, const int64_t* s, int64_t B, int64_t H, int64_t S) {
+  auto ok = [](int64_t v) { return v > 0 && v % 8 == 0 && v < (1ll << 38); };
+  return ((uintptr_t)t & 15) == 0 && (S <= 1 || ok(s[2])) && (H <= 1 || ok(s[1])) && (B <= 1 || ok(s[0]));
+}
+
+template <int D, bool BF16, bool PREC>
+int fwd_t(const Params& p, cudaStream_t st) {
+  using C = Fwd<D>;
+  const int smem = C::OFF_VEC + vec_bytes(p) + 1024;
+  auto kern = bias_fwd_tc<D, BF16, PREC>;
+  if (int rc = allow_smem(kern, smem, "bias_attn_fwd_tc")) return rc;
+  CUtensorMap tq, tk, tv, to;
+  if (!bhsd_map(&tq, p.q, p.q_s, p.B, p.H, p.Sq, p.D, BF16, 128) || !bhsd_map(&tk, p.k, p.k_s, p.B, p.Hk, p.Sk, p.D, BF16, 128) ||
+      !bhsd_map(&tv, p.v, p.v_s, p.B, p.Hk, p.Sk, p.D, BF16, 128) || !store_map(&to, p.o, p.o_s, p.B, p.H, p.Sq, p.D, BF16))
+    return fail(B2_ERR_ARG, "bias_attn_fwd: tensor map rejected");
+  dim3 grid((p.Sq + 127) / 128, p.B * p.H, p.nsplit);
+  return launch_pdl("bias_attn_fwd_tc", kern, grid, dim3(C::THREADS), smem, st, tq, tk, tv, to, p);
+}
+
+template <int D, bool KEYS>
+int bwd_smem(const Params& p) {
+  const int vb = vec_bytes(p);
+  return Bwd<D, KEYS>::OFF_VEC + (KEYS ? 2 * vb : vb + (p.dtab ? 8 * vb + 8 * 128 : 0)) + 1024;
+}
+
+template <int D, bool BF16, bool KEYS>
+int bwd_launch(const Params& p, const float2* lsed, int sq_pad, cudaStream_t st) {
+  using C = Bwd<D, KEYS>;
+  auto kern = bias_bwd_tc<D, BF16, KEYS>;
+  const char* name = KEYS ? "bias_attn_dkv_tc" : "bias_attn_dq_tc";
+  const int smem = bwd_smem<D, KEYS>(p);
+  if (int rc = allow_smem(kern, smem, name)) return rc;
+  CUtensorMap q, k, v, g, g1, g2;
+  const uint32_t qrows = KEYS ? C::NT : 128, krows = KEYS ? 128 : C::NT;
+  bool ok = bhsd_map(&q, p.q, p.q_s, p.B, p.H, p.Sq, p.D, BF16, qrows) && bhsd_map(&g, p.d_o, p.do_s, p.B, p.H, p.Sq, p.D, BF16, qrows) &&
+            bhsd_map(&k, p.k, p.k_s, p.B, p.Hk, p.Sk, p.D, BF16, krows) && bhsd_map(&v, p.v, p.v_s, p.B, p.Hk, p.Sk, p.D, BF16, krows);
+  if (KEYS)
+    ok = ok && store_map(&g1, p.dv, p.dv_s, p.B, p.Hk, p.Sk, p.D, BF16) && store_map(&g2, p.dk, p.dk_s, p.B, p.Hk, p.Sk, p.D, BF16);
+  else
+    ok = ok && store_map(&g1, p.dq, p.dq_s, p.B, p.H, p.Sq, p.D, BF16) && store_map(&g2, nullptr, p.dq_s, 1, 1, 1, p.D, BF16);
+  if (!ok) return fail(B2_ERR_ARG, std::string(name) + ": tensor map rejected");
+  dim3 grid(((KEYS ? p.Sk : p.Sq) + 127) / 128, p.B * (KEYS ? p.Hk : p.H));
+  return KEYS ? launch_pdl(name, kern, grid, dim3(C::THREADS), smem, st, k, v, q, g, g1, g2, p, lsed, sq_pad)
+              : launch_pdl(name, kern, grid, dim3(C::THREADS), smem, st, q, g, k, v, g1, g2, p, lsed, sq_pad);
+}
+
+template <int D, bool BF16>
+int bwd_t(const Params& p, float2* lsed, int sq_pad, cudaStream_t st) {
+  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+  const int64_t rows = (int64_t)p.B * p.H * sq_pad;
+  if (int rc = launch_pdl("bias_attn_bwd_prep", bias_bwd_prep<T>, dim3((unsigned)((rows * 8 + 255) / 256)), dim3(256), 0, st, p,
+                          lsed, sq_pad))
+    return rc;
+  if (p.dq || p.dtab)
+    if (int rc = bwd_launch<D, BF16, false>(p, lsed, sq_pad, st)) return rc;
+  if (p.dk || p.dv)
+    if (int rc = bwd_launch<D, BF16, true>(p, lsed, sq_pad, st)) return rc;
+  return 0;
+}
+
+}  // namespace
+
+// What the tensor-core kernels take: 16-bit tensors with D a multiple of 8 (TMA rows are whole 16-byte groups), aligned
+// rows, and a positive scale (the running maximum is taken before scaling). scale * log2 e must be finite.
+bool tc_fwd_eligible(const b2_bias_attn_args* a) {
+  if (a->dtype != B2_BF16 && a->dtype != B2_F16) return false;
+  if (!device_info().tcgen05 || a->Sk < 1 || a->D % 8 || !(a->scale > 0.f) || !(a->scale < 1e30f)) return false;
+  return layout_ok(a->q, a->q_s, a->B, a->H, a->Sq) && layout_ok(a->k, a->k_s, a->B, a->Hk, a->Sk) &&
+         layout_ok(a->v, a->v_s, a->B, a->Hk, a->Sk) && (a->o == nullptr || layout_ok(a->o, a->o_s, a->B, a->H, a->Sq));
+}
+
+bool tc_bwd_eligible(const b2_bias_attn_args* a) {
+  if (!tc_fwd_eligible(a)) return false;
+  if (!layout_ok(a->d_o, a->do_s, a->B, a->H, a->Sq) || (a->dq && !layout_ok(a->dq, a->dq_s, a->B, a->H, a->Sq)) ||
+      (a->dk && !layout_ok(a->dk, a->dk_s, a->B, a->Hk, a->Sk)) || (a->dv && !layout_ok(a->dv, a->dv_s, a->B, a->Hk, a->Sk)))
+    return false;
+  // the bias gradient of a long max_distance at wide heads does not fit beside the tiles
+  Params p{};
+  p.R = a->max_distance, p.dtab = a->dtable;
+  const int need = a->D <= 64 ? bwd_smem<64, false>(p) : bwd_smem<128, false>(p);
+  return need <= device_info().smem_optin;
+}
+
+template <bool BF16>
+int fwd_d(const Params& p, cudaStream_t st) {
+  if (p.D <= 64) return p.o32 ? fwd_t<64, BF16, true>(p, st) : fwd_t<64, BF16, false>(p, st);
+  return p.o32 ? fwd_t<128, BF16, true>(p, st) : fwd_t<128, BF16, false>(p, st);
+}
+int tc_fwd(const Params& p, bool bf16, cudaStream_t st) { return bf16 ? fwd_d<true>(p, st) : fwd_d<false>(p, st); }
+
+int tc_bwd(const Params& p, bool bf16, float2* lsed, int sq_pad, cudaStream_t st) {
+  if (p.D <= 64) return bf16 ? bwd_t<64, true>(p, lsed, sq_pad, st) : bwd_t<64, false>(p, lsed, sq_pad, st);
+  return bf16 ? bwd_t<128, true>(p, lsed, sq_pad, st) : bwd_t<128, false>(p, lsed, sq_pad, st);
+}
+
+}  // namespace bias_attn
+}  // namespace b2

@@ -188,7 +188,17 @@ at::Tensor mx4_lora_dx(const at::Tensor& dy, const at::Tensor& codes, const at::
 at::Tensor bshd(int64_t B, int64_t H, int64_t S, int64_t D, const at::TensorOptions& o) {
   return at::empty({B, S, H, D}, o).permute({0, 2, 1, 3});
 }
-at::Tensor unit_last(const at::Tensor& t) { return t.size(3) == 1 || t.stride(3) == 1 ? t : t.contiguous(); }
+// The tensor as the kernels read it in place, or a copy: unit stride along D always; 16-bit tensors of a head dim that
+// the tensor-core kernels take also want 16-byte aligned rows and no broadcast (zero) strides.
+at::Tensor readable(const at::Tensor& t) {
+  const bool tc = t.scalar_type() != at::kFloat && t.size(3) % 8 == 0;
+  bool ok = t.size(3) == 1 || t.stride(3) == 1;
+  if (tc) {
+    ok = ok && (uintptr_t)t.data_ptr() % 16 == 0;
+    for (int i = 0; i < 3; ++i) ok = ok && (t.size(i) <= 1 || (t.stride(i) > 0 && t.stride(i) % 8 == 0));
+  }
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
 void strides3(int64_t* dst, const at::Tensor& t) { dst[0] = t.stride(0), dst[1] = t.stride(1), dst[2] = t.stride(2); }
 
 struct BiasAttn {
@@ -222,7 +232,7 @@ BiasAttn bias_attn_args(const at::Tensor& q, const at::Tensor& k, const at::Tens
               ": lengths and q_offset must be below 2^30");
   TORCH_CHECK(q.size(0) * q.size(1) <= 65535, name, ": batch * heads must be at most 65535");
   BiasAttn r;
-  r.q = unit_last(q), r.k = unit_last(k), r.v = unit_last(v);
+  r.q = readable(q), r.k = readable(k), r.v = readable(v);
   r.table = table.to(at::kFloat).contiguous();
   b2_bias_attn_args& a = r.a;
   if (key_mask.has_value() && key_mask->defined()) {
@@ -244,24 +254,31 @@ BiasAttn bias_attn_args(const at::Tensor& q, const at::Tensor& k, const at::Tens
   return r;
 }
 
-std::tuple<at::Tensor, at::Tensor> bias_attn_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-                                                 const at::Tensor& table, const std::optional<at::Tensor>& key_mask,
-                                                 int64_t max_distance, bool bidirectional, bool causal, double scale,
-                                                 int64_t q_offset) {
+std::tuple<at::Tensor, at::Tensor, at::Tensor> bias_attn_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                             const at::Tensor& table,
+                                                             const std::optional<at::Tensor>& key_mask,
+                                                             int64_t max_distance, bool bidirectional, bool causal,
+                                                             double scale, int64_t q_offset, bool keep_o32) {
   const char* name = "b2::bias_attn_fwd";
   c10::cuda::OptionalCUDAGuard guard(q.is_cuda() ? std::optional<c10::Device>(q.device()) : std::nullopt);
   BiasAttn r = bias_attn_args(q, k, v, table, key_mask, max_distance, bidirectional, causal, scale, q_offset, name);
   b2_bias_attn_args& a = r.a;
   at::Tensor out = bshd(a.B, a.H, a.Sq, a.D, q.options());
   at::Tensor lse = at::empty({a.B, a.H, a.Sq}, q.options().dtype(at::kFloat));
-  if (out.numel() == 0) return {out, lse};
+  // the unrounded output, for a backward that wants the bias gradient (fp32 outputs are that already)
+  at::Tensor o32;
+  if (keep_o32 && q.scalar_type() != at::kFloat) {
+    o32 = at::empty({a.B, a.H, a.Sq, a.D}, q.options().dtype(at::kFloat));
+    a.o32 = o32.data_ptr<float>();
+  }
+  if (out.numel() == 0) return {out, lse, o32};
   a.o = out.data_ptr(), a.lse = lse.data_ptr<float>();
   strides3(a.o_s, out);
   at::Tensor ws = workspace(b2_bias_attn_workspace_bytes(&a, 0), q);
   a.workspace = ws.defined() ? ws.data_ptr() : nullptr;
   b2_check(b2_bias_attn_fwd(&a, cur_stream()), name);
   count(name);
-  return {out, lse};
+  return {out, lse, o32};
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> bias_attn_bwd(
@@ -272,11 +289,12 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> bias_attn_bwd(
   c10::cuda::OptionalCUDAGuard guard(q.is_cuda() ? std::optional<c10::Device>(q.device()) : std::nullopt);
   BiasAttn r = bias_attn_args(q, k, v, table, key_mask, max_distance, bidirectional, causal, scale, q_offset, name);
   b2_bias_attn_args& a = r.a;
+  const bool wide = o0.scalar_type() == at::kFloat && q.scalar_type() != at::kFloat;  // the forward's unrounded output
   TORCH_CHECK(go0.sizes() == q.sizes() && o0.sizes() == q.sizes() && go0.scalar_type() == q.scalar_type() &&
-                  o0.scalar_type() == q.scalar_type() && lse0.scalar_type() == at::kFloat &&
+                  (wide || o0.scalar_type() == q.scalar_type()) && lse0.scalar_type() == at::kFloat &&
                   lse0.numel() == a.B * a.H * a.Sq,
               name, ": grad, output and lse must match q");
-  at::Tensor go = unit_last(go0), o = unit_last(o0), lse = lse0.contiguous();
+  at::Tensor go = readable(go0), o = wide ? o0.contiguous() : readable(o0), lse = lse0.contiguous();
   at::Tensor dq, dk, dv, dt;
   if (want[0]) dq = bshd(a.B, a.H, a.Sq, a.D, q.options()), a.dq = dq.data_ptr(), strides3(a.dq_s, dq);
   if (want[1]) dk = bshd(a.B, a.Hk, a.Sk, a.D, q.options()), a.dk = dk.data_ptr(), strides3(a.dk_s, dk);
@@ -285,7 +303,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> bias_attn_bwd(
     dt = at::empty({a.num_buckets, a.H}, q.options().dtype(at::kFloat));
     a.dtable = dt.data_ptr<float>();
   }
-  a.o = o.data_ptr(), a.lse = lse.data_ptr<float>(), a.d_o = go.data_ptr();
+  if (wide) a.o32 = o.data_ptr<float>();
+  else a.o = o.data_ptr();
+  a.lse = lse.data_ptr<float>(), a.d_o = go.data_ptr();
   strides3(a.o_s, o), strides3(a.do_s, go);
   at::Tensor ws = workspace(b2_bias_attn_workspace_bytes(&a, 1), q);
   a.workspace = ws.defined() ? ws.data_ptr() : nullptr;
@@ -313,7 +333,7 @@ TORCH_LIBRARY_FRAGMENT(b2, m) {
   m.def("mx4_lora_fwd(Tensor x, Tensor codes, Tensor scales, Tensor? bias, Tensor h, Tensor b) -> Tensor");
   m.def("mx4_lora_dx(Tensor dy, Tensor codes, Tensor scales, int cols, Tensor dh, Tensor a) -> Tensor");
   m.def("bias_attn_fwd(Tensor q, Tensor k, Tensor v, Tensor table, Tensor? key_mask, int max_distance, bool bidirectional, "
-        "bool causal, float scale, int q_offset) -> (Tensor, Tensor)");
+        "bool causal, float scale, int q_offset, bool keep_o32) -> (Tensor, Tensor, Tensor)");
   m.def("bias_attn_bwd(Tensor grad_out, Tensor q, Tensor k, Tensor v, Tensor out, Tensor lse, Tensor table, Tensor? key_mask, "
         "int max_distance, bool bidirectional, bool causal, float scale, int q_offset, bool[4] want) -> "
         "(Tensor, Tensor, Tensor, Tensor)");
