@@ -168,6 +168,30 @@ def test_lora_forward_and_gradients(m, k, n, r):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n,r", [(2100, 288, 2500, 24), (2100, 2500, 288, 16), (4096, 160, 1300, 8)])
+def test_many_tiles(m, k, n, r):
+    """Enough 256 x 256 tiles for CTA pairs, ragged in every direction, several tiles a pair."""
+    import torch_vulkan_b200 as tv
+
+    x, w, bias, gy, a, b = _linear_case(m, k, n, m + k + n, r)
+    xq, wq = ot.mx4_round(x), ot.mx4_round(w)
+    xd = x.cuda().requires_grad_(True)
+    wd = tv.mx4_quantize(w.cuda())
+    X, A, Bm, G = (t.double() for t in (x, a, b, gy))
+    h, dh = X @ A.t(), G @ Bm
+    _close(tv.mx4_linear(xd, wd, bias.cuda()), xq @ wq.t() + bias.double(), xq.abs() @ wq.abs().t() + bias.double().abs())
+    if k % 8 == 0:
+        y = tv.mx4_lora_linear(xd, wd, bias.cuda(), a.cuda(), b.cuda())
+        _close(y, xq @ wq.t() + bias.double() + h @ Bm.t(), xq.abs() @ wq.abs().t() + (X.abs() @ A.abs().t()) @ Bm.abs().t(),
+               h.abs() @ Bm.abs().t())
+        y.backward(gy.cuda())
+        _close(xd.grad, G @ wq + dh @ A, G.abs() @ wq.abs() + (G.abs() @ Bm.abs()) @ A.abs(), dh.abs() @ A.abs())
+    else:
+        tv.mx4_linear(xd, wd).backward(gy.cuda())
+        _close(xd.grad, G @ wq, G.abs() @ wq.abs())
+
+
+@pytest.mark.gpu
 def test_dx_is_the_derivative_along_the_weight():
     """y is linear in the quantised activation, so replacing Q(x) by another quantised x' moves sum(gy * y) by exactly
     (x' - x) . dx: a difference test at inputs that quantisation leaves as they are."""

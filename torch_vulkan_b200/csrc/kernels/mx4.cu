@@ -231,10 +231,14 @@ extern "C" int b2_mx4_dequantize(const b2_mx4_args* a, b2_stream_t stream) {
 }
 
 // ---- product ------------------------------------------------------------------------------------------------------
-// Every MXFP4 value that quantisation makes is a bf16 value, so the product of the bf16 read-backs is the product of
-// the codes. Both operands are expanded into the workspace, the LoRA operands beside them as r more terms of the
-// reduction, and multiplied by the bf16 GEMM, which sums in fp32 and rounds once.
+// The tensor-core kernels of mx4_gemm.cu; dX reads W from the workspace, where it is expanded to bf16 first (exactly:
+// every MXFP4 value that quantisation makes is a bf16 value).
 namespace b2 {
+
+bool mx4_gemm_tc_eligible(const b2_mx4_gemm_args* a);  // mx4_gemm.cu
+int mx4_gemm_fwd(const b2_mx4_gemm_args* a, cudaStream_t st);
+int mx4_gemm_dx(const b2_mx4_gemm_args* a, const void* x, int64_t x_ld, const void* w, int64_t w_ld, cudaStream_t st);
+
 namespace {
 
 int64_t pad_to(int64_t k, int64_t m) { return (k + m - 1) / m * m; }
@@ -246,10 +250,6 @@ int expand(const uint8_t* codes, const uint8_t* scales, void* out, int64_t rows,
   d.rows = rows, d.cols = cols, d.ld = ld, d.dtype = B2_BF16;
   return b2_mx4_dequantize(&d, st);
 }
-int copy2d(void* dst, int64_t dld, const void* src, int64_t sld, int64_t rows, int64_t cols, cudaStream_t st) {
-  return check_cuda(cudaMemcpy2DAsync(dst, dld * 2, src, sld * 2, cols * 2, rows, cudaMemcpyDeviceToDevice, st), "mx4_gemm copy");
-}
-
 int gemm_check(const b2_mx4_gemm_args* a) {
   if (!a) return fail(B2_ERR_ARG, "mx4_gemm: null arguments");
   if (a->M < 0 || a->N < 0 || a->K < 0) return fail(B2_ERR_ARG, "mx4_gemm: negative size");
@@ -268,22 +268,18 @@ int gemm_check(const b2_mx4_gemm_args* a) {
   return 0;
 }
 
-// Operand buffers of the expanded product: A [M][lda], W [wrows][ldw].
-struct Expanded {
-  int64_t kp, lda, ldw, wrows;
-  bool copy_x;
+struct DxPlan {
+  int64_t ldw, ldx;      // row strides of the expanded weight and of the copied dY
+  bool copy_x;           // dY's rows are not whole 16-byte groups: copied into the workspace
+  uint64_t x, bytes;     // offset of that copy; workspace bytes
 };
-Expanded expanded(const b2_mx4_gemm_args* a) {
-  Expanded e;
-  e.kp = pad_to(a->K, 32);
-  if (a->transpose_w) {
-    e.copy_x = a->lora_r != 0;
-    e.lda = pad_to(a->N + a->lora_r, 8), e.ldw = e.kp, e.wrows = a->N + a->lora_r;
-  } else {
-    e.copy_x = true;
-    e.lda = e.ldw = e.kp + a->lora_r, e.wrows = a->N;
-  }
-  return e;
+DxPlan dx_plan(const b2_mx4_gemm_args* a) {
+  DxPlan d;
+  d.ldw = pad_to(a->K, 32), d.ldx = pad_to(a->N, 8);
+  d.copy_x = a->x_ld % 8 || ((uintptr_t)a->x & 15);
+  d.x = up16((uint64_t)a->N * d.ldw * 2);
+  d.bytes = d.x + (d.copy_x ? (uint64_t)a->M * d.ldx * 2 : 0);
+  return d;
 }
 
 }  // namespace
@@ -291,9 +287,8 @@ Expanded expanded(const b2_mx4_gemm_args* a) {
 
 extern "C" uint64_t b2_mx4_gemm_workspace_bytes(const b2_mx4_gemm_args* a) {
   using namespace b2;
-  if (!a || a->M <= 0 || a->N <= 0 || a->K <= 0) return 0;
-  const Expanded e = expanded(a);
-  return up16((uint64_t)e.wrows * e.ldw * 2) + (e.copy_x ? up16((uint64_t)a->M * e.lda * 2) : 0);
+  if (!a || a->M <= 0 || a->N <= 0 || a->K <= 0 || !a->transpose_w) return 0;
+  return dx_plan(a).bytes;
 }
 
 extern "C" int b2_mx4_gemm(const b2_mx4_gemm_args* a, b2_stream_t stream) {
@@ -301,35 +296,20 @@ extern "C" int b2_mx4_gemm(const b2_mx4_gemm_args* a, b2_stream_t stream) {
   if (int rc = gemm_check(a)) return rc;
   if (a->M == 0 || a->N == 0 || a->K == 0) return 0;
   if (int rc = ensure_init()) return rc;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (!mx4_gemm_tc_eligible(a)) return fail(B2_ERR_ARG, "mx4_gemm: sizes beyond 2^30, or no sm_100a device");
+  if (!a->transpose_w) return mx4_gemm_fwd(a, st);
   if (!a->workspace || ((uintptr_t)a->workspace & 15))
     return fail(B2_ERR_ARG, "mx4_gemm: a 16-byte aligned workspace of b2_mx4_gemm_workspace_bytes() is required");
-  cudaStream_t st = (cudaStream_t)stream;
-  const Expanded e = expanded(a);
-  const int r = a->lora_r;
-  uint16_t* w = (uint16_t*)a->workspace;
-  uint16_t* x = (uint16_t*)((char*)a->workspace + up16((uint64_t)e.wrows * e.ldw * 2));
-  if (int rc = expand(a->w_codes, a->w_scales, w, a->N, e.kp, e.ldw, st)) return rc;
-  b2_gemm_args g{};
-  g.b = w, g.c = a->out, g.M = a->M, g.batch = 1, g.alpha = 1.f, g.dtype = B2_BF16;
-  g.c_sm = a->out_ld, g.c_sn = 1;
-  if (a->transpose_w) {
-    g.a = a->x, g.a_sm = a->x_ld, g.a_sk = 1;
-    g.N = a->K, g.K = a->N + r, g.b_sk = e.ldw, g.b_sn = 1;
-    if (r) {
-      if (int rc = copy2d(w + a->N * e.ldw, e.ldw, a->lora_b, a->lora_b_ld, r, a->K, st)) return rc;
-      if (int rc = copy2d(x, e.lda, a->x, a->x_ld, a->M, a->N, st)) return rc;
-      if (int rc = copy2d(x + a->N, e.lda, a->lora_h, a->lora_h_ld, a->M, r, st)) return rc;
-      g.a = x, g.a_sm = e.lda;
-    }
-  } else {
-    if (int rc = expand(a->x_codes, a->x_scales, x, a->M, e.kp, e.lda, st)) return rc;
-    if (r) {
-      if (int rc = copy2d(w + e.kp, e.ldw, a->lora_b, a->lora_b_ld, a->N, r, st)) return rc;
-      if (int rc = copy2d(x + e.kp, e.lda, a->lora_h, a->lora_h_ld, a->M, r, st)) return rc;
-    }
-    g.a = x, g.a_sm = e.lda, g.a_sk = 1;
-    g.N = a->N, g.K = e.kp + r, g.b_sn = e.ldw, g.b_sk = 1;
-    if (a->bias) g.bias = a->bias, g.bias_sn = 1, g.has_bias = 1, g.beta = 1.f;
+  const DxPlan d = dx_plan(a);
+  if (int rc = expand(a->w_codes, a->w_scales, a->workspace, a->N, d.ldw, d.ldw, st)) return rc;
+  const void* x = a->x;
+  if (d.copy_x) {
+    void* xc = (char*)a->workspace + d.x;
+    if (int rc = check_cuda(cudaMemcpy2DAsync(xc, d.ldx * 2, a->x, a->x_ld * 2, a->N * 2, a->M, cudaMemcpyDeviceToDevice, st),
+                            "mx4_gemm copy"))
+      return rc;
+    x = xc;
   }
-  return b2_gemm(&g, st);
+  return mx4_gemm_dx(a, x, d.copy_x ? d.ldx : a->x_ld, a->workspace, d.ldw, st);
 }
