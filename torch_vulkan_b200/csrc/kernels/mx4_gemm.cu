@@ -3,14 +3,16 @@
 //   dX       out[M][K] = dY[M][N] W + h[M][r] a[r][K]         dY bf16, W expanded to bf16 (exact) by a kernel before
 //
 // Forward: tcgen05.mma.kind::mxf4.block_scale multiplies E2M1 codes and applies the two E8M0 scales of every 32 products
-// itself, with fp32 accumulation in TMEM; a K block of 256 columns is 128 bytes a row. The scales reach TMEM through shared
-// memory (tcgen05.cp 32x128b.warpx4: row r of a 128-row block at lane r % 32, column r / 32, one byte per block of 32
-// columns), which is the order the scale array is stored in. dX: W's scales run along its output, not along the
+// itself, with fp32 accumulation in TMEM; a K block of 256 columns is 128 bytes a row. The scale of row r of a 128-row block
+// stands in TMEM at lane r % 32 (of all four lane quarters), column r / 32, one byte per block of 32 columns, which is the
+// order the scale array is stored in: four warps copy each stage's 512-byte pieces with one 16-byte load per lane and
+// tcgen05.st. (tcgen05.cp 32x128b.warpx4 does the same from the MMA thread, but its copies and the MMAs do not overlap:
+// 0.49 us a stage for the six of a 256 x 256 pair tile next to 0.52 us of MMAs, 0.75 us together.) dX: W's scales run along its output, not along the
 // reduction, so the block-scaled MMA cannot apply them: kind::f16 with W as the N-major operand. The LoRA term is one more
 // K block of bf16 operands, zero-filled past r, into the same accumulator: one rounding for the sum.
 //
 // Persistent CTAs, or CTA pairs (CG = 2: each CTA stages its own 128 rows of A and half of the W tile, the leader issues
-// M = 256 MMAs for both; W's scales are needed whole in each). warp 0: TMA producer. warp 1: scales to TMEM, MMAs.
+// M = 256 MMAs for both; W's scales are needed whole in each). warp 0: TMA producer. warp 1: MMAs. warps 10..13: scales.
 // warps 2..9: epilogue, which takes the whole tile into registers as bf16 before it stores anything, so that the next
 // tile's MMAs wait for a few hundred cycles only.
 #include "common.cuh"
@@ -31,7 +33,7 @@ struct P4 {
   int KR;             // reduction: columns padded to 32 (forward), N (dX)
   int tiles_m, tiles_n;
   int lora_r;
-  int tma_out;        // out described by a tensor map, else stored element by element
+  int vec_out;        // rows of out are whole 16-byte groups
   int* err;
 };
 
@@ -42,20 +44,20 @@ struct Cfg4 {
   static constexpr int BC = BN / CG;                   // rows of W (dX: columns) that this CTA stages
   static constexpr int A_BYTES = 128 * 128, B_BYTES = BC * 128;
   static constexpr int SA_BYTES = DX ? 0 : 1024, SB_BYTES = DX ? 0 : 1024 * (BN / 128);
-  static constexpr int TX = A_BYTES + B_BYTES + SA_BYTES + SB_BYTES;
-  static constexpr int STAGE = TX;
-  static constexpr int NS = (BN == 256 && !DX) ? 5 : 6;
+  static constexpr int TX = A_BYTES + B_BYTES;
+  static constexpr int STAGE = TX + SA_BYTES + SB_BYTES;
+  static constexpr int NS = 5;
   static constexpr int NACC = 256 / BN;                // accumulators in TMEM
   static constexpr int SFC = DX ? 0 : 8 + BN / 16;     // TMEM columns of a stage's scales (A: 2 x 4, W: 2 x BN / 32)
   static constexpr uint32_t T_SF = 256, TMEM_COLS = 512;
   static_assert(T_SF + NS * SFC <= 512, "TMEM columns");
-  static constexpr int OFF_STG = NS * STAGE;           // 8 warps x 2 KB
-  static constexpr int OFF_BIAS = OFF_STG + 8 * 2048;  // 2 x BN floats
+  static constexpr int OFF_STG = NS * STAGE;           // 8 warps x a 4 KB box
+  static constexpr int OFF_BIAS = OFF_STG + 8 * 4096;  // 2 x BN floats
   static constexpr int OFF_BAR = OFF_BIAS + 2 * BN * 4;
   static constexpr int SMEM = OFF_BAR + 256 + 1024;
   static_assert(SMEM <= 232448, "shared memory");
   static_assert(STAGE % 1024 == 0, "swizzled tiles start on 1024-byte boundaries");
-  static constexpr int THREADS = 320;
+  static constexpr int THREADS = DX ? 320 : 448;
 };
 
 // Instruction descriptor of kind::mxf4 (PTX ISA, block-scaled kinds): [4,6) scale id of B | [7,10) A format, 1 = E2M1 |
@@ -90,24 +92,12 @@ __device__ __forceinline__ void mma_bf16(uint32_t d, uint64_t a, uint64_t b, uin
   else tc::mma_f16_ss(d, a, b, idesc, acc);
 }
 
-// 512 bytes of shared memory (32 rows of 16 bytes) -> 4 TMEM columns, the same in all four lane quarters (of both CTAs of
-// a pair, each from its own shared memory).
-template <int CG>
-__device__ __forceinline__ void cp_scales(uint32_t taddr, uint64_t sdesc) {
-  if (CG == 2) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
-  else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
-}
-// Descriptor of such a piece: no swizzle, 8-row groups 128 bytes apart.
-__device__ __forceinline__ uint64_t sdesc_scales(uint32_t saddr) {
-  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)8 << 16) | ((uint64_t)8 << 32) | (1ull << 46);
-}
-
 template <int BN, int CG, bool DX>
-__global__ void __launch_bounds__(320, 1)
+__global__ void __launch_bounds__(DX ? 320 : 448, 1)
     mx4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
                     const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSW,
                     const __grid_constant__ CUtensorMap tmH, const __grid_constant__ CUtensorMap tmB,
-                    const __grid_constant__ CUtensorMap tmO, const __grid_constant__ P4 p) {
+                    const __grid_constant__ P4 p) {
   using C = Cfg4<BN, CG, DX>;
   constexpr int NS = C::NS, NACC = C::NACC;
   extern __shared__ uint8_t smem_raw[];
@@ -116,8 +106,10 @@ __global__ void __launch_bounds__(320, 1)
   uint64_t* empty = full + NS;                                      // [NS]
   uint64_t* acc_full = empty + NS;                                  // [2]
   uint64_t* acc_empty = acc_full + 2;                               // [2] one arrival per epilogue warp (of both CTAs)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(acc_empty + 3);
+  uint64_t* sfull = acc_empty + 2;                                  // [NS] this CTA's scales of a stage landed
+  uint64_t* sready = sfull + NS;                                    // [NS] and are in TMEM (pairs: in both CTAs' TMEM)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sready + NS);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(sready + NS + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? tc::cluster_ctarank() : 0u;
   auto leader_bar = [&](uint64_t* bar) -> uint32_t {
@@ -125,7 +117,10 @@ __global__ void __launch_bounds__(320, 1)
   };
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < NS; ++i) tc::mbar_init(&full[i], 1), tc::mbar_init(&empty[i], 1);
+    for (int i = 0; i < NS; ++i) {
+      tc::mbar_init(&full[i], 1), tc::mbar_init(&empty[i], 1);
+      tc::mbar_init(&sfull[i], 1), tc::mbar_init(&sready[i], 4 * CG);
+    }
     for (int i = 0; i < 2; ++i) tc::mbar_init(&acc_full[i], 1), tc::mbar_init(&acc_empty[i], 8 * CG);
     *abort_flag = 0;
     tc::fence_barrier_init();
@@ -170,7 +165,7 @@ __global__ void __launch_bounds__(320, 1)
           uint8_t* sb = st + C::A_BYTES;
           uint8_t* sc = sb + C::B_BYTES;
           const bool lora = kb == nkm;
-          if (rank == 0) tc::mbar_arrive_expect_tx(&full[s], (lora ? C::A_BYTES + C::B_BYTES : C::TX) * CG);
+          if (rank == 0) tc::mbar_arrive_expect_tx(&full[s], C::TX * CG);
           auto load = [&](void* dst, const CUtensorMap* m, int x, int y) {
             if (CG == 2) tc::tma_load_2d_pair(dst, m, leader_bar(&full[s]), x, y);
             else tc::tma_load_2d(dst, m, &full[s], x, y);
@@ -180,13 +175,15 @@ __global__ void __launch_bounds__(320, 1)
             for (int c = 0; c < C::BC / 64; ++c)  // 64 rows x 64 columns per box
               load(sb + c * 8192, lora ? &tmB : &tmW, nb0 + c * 64, lora ? 0 : kb * 64);
           } else if (lora) {
+            tc::mbar_arrive(&sfull[s]);  // no scales
             load(st, &tmH, 0, m0);
             load(sb, &tmB, 0, nb0);
           } else {
+            tc::mbar_arrive_expect_tx(&sfull[s], C::SA_BYTES + C::SB_BYTES);
+            tc::tma_load_2d(sc, &tmSA, &sfull[s], kb * 256, m0 / 128);
+            tc::tma_load_2d(sc + 1024, &tmSW, &sfull[s], kb * 256, n0 / 128);
             load(st, &tmA, kb * 128, m0);
             load(sb, &tmW, kb * 128, nb0);
-            load(sc, &tmSA, kb * 256, m0 / 128);
-            load(sc + 1024, &tmSW, kb * 256, n0 / 128);
           }
           issued[s]++;
         }
@@ -198,9 +195,11 @@ __global__ void __launch_bounds__(320, 1)
       }
       if (!ok) {
         *abort_flag = 1;
-        if (rank == 0)
-          for (int s = 0; s < NS; ++s)
-            if (issued[s]) tc::mbar_wait(&full[s], (uint32_t)((issued[s] - 1) & 1), nullptr);
+        for (int s = 0; s < NS; ++s)
+          if (issued[s]) {
+            if (rank == 0) tc::mbar_wait(&full[s], (uint32_t)((issued[s] - 1) & 1), nullptr);
+            if (!DX) tc::mbar_wait(&sfull[s], (uint32_t)((issued[s] - 1) & 1), nullptr);
+          }
       }
     }
   } else if (warp == 1) {
@@ -217,7 +216,11 @@ __global__ void __launch_bounds__(320, 1)
         const uint32_t acc = tbase + a * BN;
         for (int kb = 0; kb < nk; ++kb, ++it) {
           const int s = it % NS;
-          if (!tc::mbar_wait(&full[s], (uint32_t)((it / NS) & 1), p.err) || *abort_flag) { ok = false; break; }
+          if (!tc::mbar_wait(&full[s], (uint32_t)((it / NS) & 1), p.err) ||
+              (!DX && !tc::mbar_wait(&sready[s], (uint32_t)((it / NS) & 1), p.err)) || *abort_flag) {
+            ok = false;
+            break;
+          }
           tc::tc_fence_after();
           const uint32_t st = tc::smem_u32(smem + s * C::STAGE);
           const tc::SDesc ad = tc::sdesc_parts(st, 16, 1024);
@@ -230,14 +233,7 @@ __global__ void __launch_bounds__(320, 1)
           } else {
             const tc::SDesc bd = tc::sdesc_parts(st + C::A_BYTES, 16, 1024);
             const uint32_t sfa = tbase + C::T_SF + s * C::SFC, sfb = sfa + 8;
-            const uint32_t sc = st + C::A_BYTES + C::B_BYTES;
             const int steps = min(4, (p.KR - kb * C::BK + 63) / 64);
-            for (int c = 0; c < (steps + 1) / 2; ++c) {
-              cp_scales<CG>(sfa + 4 * c, sdesc_scales(sc + 512 * c));
-#pragma unroll
-              for (int j = 0; j < BN / 128; ++j)
-                cp_scales<CG>(sfb + (BN / 32) * c + 4 * j, sdesc_scales(sc + 1024 * (1 + j) + 512 * c));
-            }
             for (int k = 0; k < steps; ++k)
               mma_mxf4<CG>(acc, tc::sdesc_at(ad, k * 32), tc::sdesc_at(bd, k * 32), (k & 1) ? ID2 : ID0, sfa + 4 * (k >> 1),
                            sfb + (BN / 32) * (k >> 1), (kb > 0 || k > 0) ? 1u : 0u);
@@ -252,12 +248,47 @@ __global__ void __launch_bounds__(320, 1)
       }
       if (!ok) *abort_flag = 1;
     }
+  } else if (!DX && warp >= 10) {
+    // ---------------- scales: warp = one lane quarter of TMEM ----------------
+    const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+    int it = 0;
+    bool ok = true;
+    for (int t = unit; t < tiles && ok; t += units)
+      for (int kb = 0; kb < nk; ++kb, ++it) {
+        const int s = it % NS;
+        // its slot in TMEM is free: the loads waited for the MMAs that read the slot before
+        if (!tc::mbar_wait(&sfull[s], (uint32_t)((it / NS) & 1), p.err) || *abort_flag) { ok = false; break; }
+        if (kb < nkm) {
+          const uint8_t* sc = smem + s * C::STAGE + C::A_BYTES + C::B_BYTES + lane * 16;
+          uint32_t va[8], vb[BN / 16];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {  // 128-column pieces
+            *reinterpret_cast<uint4*>(va + 4 * c) = *reinterpret_cast<const uint4*>(sc + 512 * c);
+#pragma unroll
+            for (int j = 0; j < BN / 128; ++j)
+              *reinterpret_cast<uint4*>(vb + (BN / 32) * c + 4 * j) = *reinterpret_cast<const uint4*>(sc + 1024 * (1 + j) + 512 * c);
+          }
+          __syncwarp();
+          const uint32_t sf = tbase + C::T_SF + s * C::SFC + lane_off;
+          tc::tmem_st8(sf, va);
+          if (BN == 256) tc::tmem_st16(sf + 8, vb);
+          else tc::tmem_st8(sf + 8, vb);
+          tc::tmem_wait_st();
+          tc::tc_fence_before();
+        }
+        __syncwarp();
+        if (lane == 0) {
+          if (CG == 2) tc::mbar_arrive_cluster(leader_bar(&sready[s]));
+          else tc::mbar_arrive(&sready[s]);
+        }
+      }
+    if (!ok) *abort_flag = 1;
   } else {
     // ---------------- epilogue: warp = 32 rows (TMEM lane quarter) x half of the columns ----------------
     const int half = (warp - 2) >> 2, quarter = warp & 3;
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
     const int ew = (int)threadIdx.x - 64;
-    uint8_t* stg = smem + C::OFF_STG + (warp - 2) * 2048;
+    uint8_t* stg = smem + C::OFF_STG + (warp - 2) * 4096;
     float* bias_s = reinterpret_cast<float*>(smem + C::OFF_BIAS);
     constexpr int BOX = BN / 64;  // 32-column boxes of this warp
     int ti = 0;
@@ -293,33 +324,43 @@ __global__ void __launch_bounds__(320, 1)
         if (CG == 2) tc::mbar_arrive_cluster(leader_bar(&acc_empty[a]));
         else tc::mbar_arrive(&acc_empty[a]);
       }
-      const int row = m0 + quarter * 32 + lane;
+      if (!ok) continue;
+      const int r0 = m0 + quarter * 32;
 #pragma unroll
-      for (int c = 0; c < BOX; ++c) {
+      for (int c = 0; c < BOX; c += 2) {
+        // 32 rows x 64 columns through a swizzled staging tile, then whole 128-byte lines per row. Plain stores: nothing
+        // waits for them, where a tile store's staging buffer is held until it has been read
         const int col = n0 + half * (BN / 2) + c * 32;
-        if (p.tma_out) {
-          if (lane == 0) tc::bulk_wait_read0();  // the last box has left the staging tile
-          __syncwarp();
+        __syncwarp();
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            *reinterpret_cast<uint4*>(stg + lane * 64 + ((e ^ ((lane >> 1) & 3)) << 4)) =
-                make_uint4(w[c][4 * e], w[c][4 * e + 1], w[c][4 * e + 2], w[c][4 * e + 3]);
-          tc::fence_async_shared();
-          __syncwarp();
-          if (lane == 0 && ok && m0 + quarter * 32 < p.M && col < p.NO) {
-            tc::tma_store_2d(&tmO, stg, col, m0 + quarter * 32);
-            tc::bulk_commit();
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t* v = &w[c + (e >> 2)][4 * (e & 3)];
+          *reinterpret_cast<uint4*>(stg + lane * 128 + ((e ^ (lane & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+        }
+        __syncwarp();
+        if (p.vec_out) {
+          const int cc = col + (lane & 7) * 8;  // NO is a multiple of 8 here: an 8-column group is whole or absent
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int r = i * 4 + (lane >> 3);
+            const uint4 v = *reinterpret_cast<const uint4*>(stg + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+            if (r0 + r < p.M && cc < p.NO) *reinterpret_cast<uint4*>(p.out + (int64_t)(r0 + r) * p.out_ld + cc) = v;
           }
-        } else if (ok && row < p.M) {
-          const __nv_bfloat16* wv = reinterpret_cast<const __nv_bfloat16*>(w[c]);
-          __nv_bfloat16* o = p.out + (int64_t)row * p.out_ld + col;
+        } else {
+#pragma unroll 4
+          for (int r = 0; r < 32; ++r) {
+            if (r0 + r >= p.M) break;
+            __nv_bfloat16* o = p.out + (int64_t)(r0 + r) * p.out_ld;
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (col + e < p.NO) o[e] = wv[e];
+            for (int j = 0; j < 2; ++j) {
+              const int e = lane + 32 * j;
+              const __nv_bfloat16 v = *reinterpret_cast<const __nv_bfloat16*>(stg + r * 128 + (((e >> 3) ^ (r & 7)) << 4) + (e & 7) * 2);
+              if (col + e < p.NO) o[col + e] = v;
+            }
+          }
         }
       }
     }
-    if (lane == 0) tc::bulk_wait0();
   }
   __syncwarp();
   tc::tc_fence_before();
@@ -363,11 +404,11 @@ int launch4(const b2_mx4_gemm_args* a, const Shape& sh, cudaStream_t st) {
   p.tiles_m = (int)((a->M + C::BM - 1) / C::BM), p.tiles_n = (int)((sh.NO + BN - 1) / BN);
   p.lora_r = a->lora_r;
   p.err = device_error_ptr();
-  p.tma_out = a->out_ld % 8 == 0 && ((uintptr_t)a->out & 15) == 0;
-  CUtensorMap ta, tw, tsa, tsw, th, tb, to;
-  for (CUtensorMap* m : {&tsa, &tsw, &th, &tb, &to}) memset(m, 0, sizeof(*m));
+  p.vec_out = a->out_ld % 8 == 0 && sh.NO % 8 == 0 && ((uintptr_t)a->out & 15) == 0;
+  CUtensorMap ta, tw, tsa, tsw, th, tb;
+  for (CUtensorMap* m : {&tsa, &tsw, &th, &tb}) memset(m, 0, sizeof(*m));
   const auto U8 = CU_TENSOR_MAP_DATA_TYPE_UINT8, BF = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, I32 = CU_TENSOR_MAP_DATA_TYPE_INT32;
-  const auto S128 = CU_TENSOR_MAP_SWIZZLE_128B, S64 = CU_TENSOR_MAP_SWIZZLE_64B, S0 = CU_TENSOR_MAP_SWIZZLE_NONE;
+  const auto S128 = CU_TENSOR_MAP_SWIZZLE_128B, S0 = CU_TENSOR_MAP_SWIZZLE_NONE;
   bool ok;
   if (DX) {
     ok = map2d(&ta, BF, sh.x, a->N, a->M, sh.x_ld * 2, 64, 128, S128) && map2d(&tw, BF, sh.w, a->K, a->N, sh.w_ld * 2, 64, 64, S128);
@@ -377,7 +418,6 @@ int launch4(const b2_mx4_gemm_args* a, const Shape& sh, cudaStream_t st) {
          map2d(&tsa, I32, a->x_scales, nkb * 128, (a->M + 127) / 128, nkb * 512, 256, 1, S0) &&
          map2d(&tsw, I32, a->w_scales, nkb * 128, (a->N + 127) / 128, nkb * 512, 256, BN / 128, S0);
   }
-  if (p.tma_out) ok = ok && map2d(&to, BF, a->out, sh.NO, a->M, a->out_ld * 2, 32, 32, S64);
   if (a->lora_r) {
     ok = ok && map2d(&th, BF, a->lora_h, a->lora_r, a->M, a->lora_h_ld * 2, 64, 128, S128);
     ok = ok && (DX ? map2d(&tb, BF, a->lora_b, a->K, a->lora_r, a->lora_b_ld * 2, 64, 64, S128)
@@ -385,7 +425,7 @@ int launch4(const b2_mx4_gemm_args* a, const Shape& sh, cudaStream_t st) {
   }
   if (!ok) return fail(B2_ERR_ARG, std::string(name) + ": tensor map rejected");
   const int units = std::min(p.tiles_m * p.tiles_n, device_info().sm_count / CG);
-  if (CG == 1) return launch_pdl(name, kern, dim3(units), dim3(C::THREADS), C::SMEM, st, ta, tw, tsa, tsw, th, tb, to, p);
+  if (CG == 1) return launch_pdl(name, kern, dim3(units), dim3(C::THREADS), C::SMEM, st, ta, tw, tsa, tsw, th, tb, p);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(units * CG);
   cfg.blockDim = dim3(C::THREADS);
@@ -398,7 +438,7 @@ int launch4(const b2_mx4_gemm_args* a, const Shape& sh, cudaStream_t st) {
   cudaError_t e;
   {
     LaunchScope ls(name, st);
-    e = cudaLaunchKernelEx(&cfg, kern, ta, tw, tsa, tsw, th, tb, to, p);
+    e = cudaLaunchKernelEx(&cfg, kern, ta, tw, tsa, tsw, th, tb, p);
   }
   if (e != cudaSuccess) {
     (void)cudaGetLastError();
