@@ -245,6 +245,37 @@ def test_linear_empty_strides_streams_and_repeatability():
 
 
 @pytest.mark.gpu
+def test_gradients_wanted_one_at_a_time_and_leading_dimensions():
+    import torch_vulkan_b200 as tv
+
+    m, k, n, r = 40, 64, 72, 8
+    x, w, bias, gy, a, b = (t.cuda() for t in _linear_case(m, k, n, 3, r))
+    wd = tv.mx4_quantize(w)
+    for with_bias in (True, False):
+        args = dict(x=x.view(2, 20, k), bias=bias if with_bias else None, a=a, b=b)
+        names = [t for t in args if args[t] is not None]
+
+        def run(wanted):
+            leaf = {t: (args[t].detach().requires_grad_(t in wanted) if args[t] is not None else None) for t in args}
+            y = tv.mx4_lora_linear(leaf["x"], wd, leaf["bias"], leaf["a"], leaf["b"])
+            assert y.shape == (2, 20, n)
+            return dict(zip(wanted, torch.autograd.grad(y, [leaf[t] for t in wanted], gy.view(2, 20, n))))
+
+        every = run(names)
+        for t in names:
+            assert every[t].shape == args[t].shape
+            assert torch.equal(run([t])[t], every[t]), t
+        for t in names[:2]:
+            leaf = {u: args[u].detach().requires_grad_(u == t) if u in names[:2] else None for u in args}
+            y = tv.mx4_linear(leaf["x"], wd, leaf["bias"]) if with_bias else tv.mx4_linear(args["x"].detach().requires_grad_(True), wd)
+            if with_bias:
+                (g,) = torch.autograd.grad(y, leaf[t], gy.view(2, 20, n))
+                assert g.shape == args[t].shape
+    with torch.no_grad():
+        assert not tv.mx4_lora_linear(x, wd, bias, a.requires_grad_(True), b).requires_grad
+
+
+@pytest.mark.gpu
 def test_refusals():
     import torch_vulkan_b200 as tv
 

@@ -16,24 +16,6 @@ def relative_position_bucket(rel: int, num_buckets: int = 32, max_distance: int 
     return int(torch.ops.b2.bias_bucket(int(rel), int(num_buckets), int(max_distance), bool(bidirectional)))
 
 
-class _BucketBiasAttention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, table, key_mask, max_distance, bidirectional, causal, scale, q_offset):
-        args = (max_distance, bidirectional, causal, scale, q_offset)
-        # a backward keeps the unrounded output: its dS cancels over each row
-        o, lse, o32 = torch.ops.b2.bias_attn_fwd(q, k, v, table, key_mask, *args, any(ctx.needs_input_grad[:4]))
-        ctx.save_for_backward(q, k, v, o if o32 is None else o32, lse, table, key_mask)
-        ctx.args = args
-        return o
-
-    @staticmethod
-    def backward(ctx, go):
-        q, k, v, o, lse, table, key_mask = ctx.saved_tensors
-        want = list(ctx.needs_input_grad[:4])
-        grads = torch.ops.b2.bias_attn_bwd(go, q, k, v, o, lse, table, key_mask, *ctx.args, want)
-        return (*(g if w else None for g, w in zip(grads, want)), None, None, None, None, None, None)
-
-
 def bucket_bias_attention(q, k, v, table, key_mask=None, max_distance=128, bidirectional=True, causal=False, scale=None,
                           q_offset=0):
     """softmax(scale * q k^T + table[bucket(j - i - q_offset)]) v.
@@ -46,5 +28,4 @@ def bucket_bias_attention(q, k, v, table, key_mask=None, max_distance=128, bidir
     every sum has a fixed order, so results are the same bits on every call."""
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
-    return _BucketBiasAttention.apply(q, k, v, table, key_mask, int(max_distance), bool(bidirectional), bool(causal),
-                                      float(scale), int(q_offset))
+    return torch.ops.b2.bucket_bias_attention(q, k, v, table, key_mask, max_distance, bidirectional, causal, scale, q_offset)

@@ -90,11 +90,5 @@ int tc_bwd(const Params& p, bool bf16, float2* lsed, int sq_pad, cudaStream_t st
 constexpr int kTcTile = 128;
 constexpr int kTcPad = 384;  // (lse, delta) rows are padded to a multiple of every tile height
 
-// More than the default 48 KB of shared memory, set once per kernel and device.
-template <typename K>
-int allow_smem(K kern, int bytes, const char* what) {
-  return check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), what);
-}
-
 }  // namespace bias_attn
 }  // namespace b2

@@ -372,7 +372,7 @@ int smem_bytes(const Params& p, int tiles, int ps) {
 template <typename T, int DP>
 int fwd_t(const Params& p, cudaStream_t st) {
   const int sm = smem_bytes<DP>(p, 3, 1);
-  if (int rc = allow_smem(fwd_kernel<T, DP>, sm, "bias_attn_fwd_simt")) return rc;
+  if (int rc = allow_smem<fwd_kernel<T, DP>>(sm, "bias_attn_fwd_simt")) return rc;
   {
     LaunchScope ls("bias_attn_fwd_simt", st);
     dim3 grid((p.Sq + T64 - 1) / T64, p.B * p.H, p.nsplit);
@@ -385,7 +385,7 @@ template <typename T, int DP>
 int bwd_t(const Params& p, cudaStream_t st) {
   const int sq = smem_bytes<DP>(p, 4, 1), sk = smem_bytes<DP>(p, 4, 2);
   if (p.dq || p.dtab) {
-    if (int rc = allow_smem(dq_kernel<T, DP>, sq, "bias_attn_dq_simt")) return rc;
+    if (int rc = allow_smem<dq_kernel<T, DP>>(sq, "bias_attn_dq_simt")) return rc;
     {
       LaunchScope ls("bias_attn_dq_simt", st);
       dq_kernel<T, DP><<<dim3((p.Sq + T64 - 1) / T64, p.B * p.H), 256, sq, st>>>(p);
@@ -393,7 +393,7 @@ int bwd_t(const Params& p, cudaStream_t st) {
     if (int rc = after_launch("bias_attn_dq_simt")) return rc;
   }
   if (p.dk || p.dv) {
-    if (int rc = allow_smem(dkv_kernel<T, DP>, sk, "bias_attn_dkv_simt")) return rc;
+    if (int rc = allow_smem<dkv_kernel<T, DP>>(sk, "bias_attn_dkv_simt")) return rc;
     {
       LaunchScope ls("bias_attn_dkv_simt", st);
       dkv_kernel<T, DP><<<dim3((p.Sk + T64 - 1) / T64, p.B * p.Hk), 256, sk, st>>>(p);

@@ -907,7 +907,7 @@ int fwd_t(const Params& p, cudaStream_t st) {
   using C = Fwd<D>;
   const int smem = C::OFF_VEC + vec_bytes(p) + 1024;
   auto kern = bias_fwd_tc<D, BF16, PREC>;
-  if (int rc = allow_smem(kern, smem, "bias_attn_fwd_tc")) return rc;
+  if (int rc = allow_smem<bias_fwd_tc<D, BF16, PREC>>(smem, "bias_attn_fwd_tc")) return rc;
   CUtensorMap tq, tk, tv, to;
   if (!bhsd_map(&tq, p.q, p.q_s, p.B, p.H, p.Sq, p.D, BF16, 128) || !bhsd_map(&tk, p.k, p.k_s, p.B, p.Hk, p.Sk, p.D, BF16, 128) ||
       !bhsd_map(&tv, p.v, p.v_s, p.B, p.Hk, p.Sk, p.D, BF16, 128) || !store_map(&to, p.o, p.o_s, p.B, p.H, p.Sq, p.D, BF16))
@@ -928,7 +928,7 @@ int bwd_launch(const Params& p, const float2* lsed, int sq_pad, cudaStream_t st)
   auto kern = bias_bwd_tc<D, BF16, KEYS>;
   const char* name = KEYS ? "bias_attn_dkv_tc" : "bias_attn_dq_tc";
   const int smem = bwd_smem<D, KEYS>(p);
-  if (int rc = allow_smem(kern, smem, name)) return rc;
+  if (int rc = allow_smem<bias_bwd_tc<D, BF16, KEYS>>(smem, name)) return rc;
   CUtensorMap q, k, v, g, g1, g2;
   const uint32_t qrows = KEYS ? C::NT : 128, krows = KEYS ? 128 : C::NT;
   bool ok = bhsd_map(&q, p.q, p.q_s, p.B, p.H, p.Sq, p.D, BF16, qrows) && bhsd_map(&g, p.d_o, p.do_s, p.B, p.H, p.Sq, p.D, BF16, qrows) &&

@@ -37,23 +37,25 @@ struct P4 {
   int* err;
 };
 
-template <int BN, int CG, bool DX>
+// MS: 128-row sub-tiles of A per CTA that share the stage's W tile.
+template <int BN, int CG, int MS, bool DX>
 struct Cfg4 {
-  static constexpr int BM = 128 * CG;                  // rows of a tile, 128 per CTA
+  static constexpr int BMC = 128 * MS;                 // rows of a tile in this CTA
+  static constexpr int BM = BMC * CG;                  // rows of a tile
   static constexpr int BK = DX ? 64 : 256;             // reduction per K block: 128 bytes a row
   static constexpr int BC = BN / CG;                   // rows of W (dX: columns) that this CTA stages
-  static constexpr int A_BYTES = 128 * 128, B_BYTES = BC * 128;
+  static constexpr int A_BYTES = BMC * 128, B_BYTES = BC * 128;
   static constexpr int SA_BYTES = DX ? 0 : 1024, SB_BYTES = DX ? 0 : 1024 * (BN / 128);
   static constexpr int TX = A_BYTES + B_BYTES;
   static constexpr int STAGE = TX + SA_BYTES + SB_BYTES;
-  static constexpr int NS = 5;
-  static constexpr int NACC = 256 / BN;                // accumulators in TMEM
+  static constexpr int NS = MS == 2 ? 4 : (BN / CG == 64 ? 6 : 5);
+  static constexpr int NACC = MS == 2 ? 1 : 256 / BN;  // accumulators in TMEM, MS * BN columns each
   static constexpr int SFC = DX ? 0 : 8 + BN / 16;     // TMEM columns of a stage's scales (A: 2 x 4, W: 2 x BN / 32)
   static constexpr uint32_t T_SF = 256, TMEM_COLS = 512;
-  static_assert(T_SF + NS * SFC <= 512, "TMEM columns");
+  static_assert((DX || MS == 1) && MS * BN <= 512 && (DX || T_SF + NS * SFC <= 512), "TMEM columns");
   static constexpr int OFF_STG = NS * STAGE;           // 8 warps x a 4 KB box
   static constexpr int OFF_BIAS = OFF_STG + 8 * 4096;  // 2 x BN floats
-  static constexpr int OFF_BAR = OFF_BIAS + 2 * BN * 4;
+  static constexpr int OFF_BAR = OFF_BIAS + (DX ? 0 : 2 * BN * 4);
   static constexpr int SMEM = OFF_BAR + 256 + 1024;
   static_assert(SMEM <= 232448, "shared memory");
   static_assert(STAGE % 1024 == 0, "swizzled tiles start on 1024-byte boundaries");
@@ -92,13 +94,13 @@ __device__ __forceinline__ void mma_bf16(uint32_t d, uint64_t a, uint64_t b, uin
   else tc::mma_f16_ss(d, a, b, idesc, acc);
 }
 
-template <int BN, int CG, bool DX>
+template <int BN, int CG, int MS, bool DX>
 __global__ void __launch_bounds__(DX ? 320 : 448, 1)
     mx4_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
                     const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSW,
                     const __grid_constant__ CUtensorMap tmH, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ P4 p) {
-  using C = Cfg4<BN, CG, DX>;
+  using C = Cfg4<BN, CG, MS, DX>;
   constexpr int NS = C::NS, NACC = C::NACC;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -147,7 +149,7 @@ __global__ void __launch_bounds__(DX ? 320 : 448, 1)
   const int nk = nkm + (p.lora_r ? 1 : 0);
   const int unit = (int)blockIdx.x / CG, units = (int)gridDim.x / CG;
   // consecutive units take consecutive row tiles of one column of tiles, so they share W in L2
-  auto tile_m = [&](int t) { return t % p.tiles_m * C::BM + (int)rank * 128; };  // this CTA's first row
+  auto tile_m = [&](int t) { return t % p.tiles_m * C::BM + (int)rank * C::BMC; };  // this CTA's first row
   auto tile_n = [&](int t) { return t / p.tiles_m * BN; };
 
   if (warp == 0) {
@@ -205,8 +207,8 @@ __global__ void __launch_bounds__(DX ? 320 : 448, 1)
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
       // ---------------- MMA issuer (pairs: the leader) ----------------
-      constexpr uint32_t ID0 = idesc_mxf4(C::BM, BN, 0), ID2 = idesc_mxf4(C::BM, BN, 2);
-      constexpr uint32_t IDF = tc::idesc_f16(C::BM, BN, true, false, DX);
+      constexpr uint32_t ID0 = idesc_mxf4(128 * CG, BN, 0), ID2 = idesc_mxf4(128 * CG, BN, 2);
+      constexpr uint32_t IDF = tc::idesc_f16(128 * CG, BN, true, false, DX);
       int it = 0, ti = 0;
       bool ok = true;
       for (int t = unit; t < tiles && ok; t += units, ++ti) {
@@ -229,7 +231,10 @@ __global__ void __launch_bounds__(DX ? 320 : 448, 1)
             const tc::SDesc bd = tc::sdesc_parts(st + C::A_BYTES, DX ? 8192 : 16, 1024);
             const int steps = min(4, ((lora ? p.lora_r : p.KR - kb * 64) + 15) / 16);
             for (int k = 0; k < steps; ++k)
-              mma_bf16<CG>(acc, tc::sdesc_at(ad, k * 32), tc::sdesc_at(bd, DX ? k * 2048 : k * 32), IDF, (kb > 0 || k > 0) ? 1u : 0u);
+#pragma unroll
+              for (int m = 0; m < MS; ++m)
+                mma_bf16<CG>(acc + m * BN, tc::sdesc_at(ad, m * 16384 + k * 32), tc::sdesc_at(bd, DX ? k * 2048 : k * 32), IDF,
+                             (kb > 0 || k > 0) ? 1u : 0u);
           } else {
             const tc::SDesc bd = tc::sdesc_parts(st + C::A_BYTES, 16, 1024);
             const uint32_t sfa = tbase + C::T_SF + s * C::SFC, sfb = sfa + 8;
@@ -295,67 +300,77 @@ __global__ void __launch_bounds__(DX ? 320 : 448, 1)
     for (int t = unit; t < tiles; t += units, ++ti) {
       const int m0 = tile_m(t), n0 = tile_n(t), a = ti % NACC;
       float* bs = bias_s + (ti & 1) * BN;
-      if (ew < BN) bs[ew] = (p.bias && n0 + ew < p.NO) ? __bfloat162float(p.bias[n0 + ew]) : 0.f;
-      tc::named_bar_sync(1, 256);
+      if (!DX) {
+        if (ew < BN) bs[ew] = (p.bias && n0 + ew < p.NO) ? __bfloat162float(p.bias[n0 + ew]) : 0.f;
+        tc::named_bar_sync(1, 256);
+      }
       // after a wait that ran out, the remaining tiles are walked without waiting or storing: every warp still meets
       // the others at the named barrier
       const bool ok = !*abort_flag && tc::mbar_wait(&acc_full[a], (uint32_t)((ti / NACC) & 1), p.err);
       if (!ok) *abort_flag = 1;
       tc::tc_fence_after();
-      // the whole half tile into registers as bf16 pairs, so that the accumulator is free before anything is stored
-      uint32_t w[BOX][16];
-      __syncwarp();
-#pragma unroll
-      for (int c = 0; c < BOX; ++c) {
-        uint32_t v[32];
-        tc::tmem_ld32(tbase + a * BN + half * (BN / 2) + c * 32 + lane_off, v);
-        tc::tmem_wait_ld();
-        tc::reg_fence32(v);
-        const float* bc = bs + half * (BN / 2) + c * 32;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          __nv_bfloat162 b2v = __floats2bfloat162_rn(__uint_as_float(v[2 * e]) + bc[2 * e], __uint_as_float(v[2 * e + 1]) + bc[2 * e + 1]);
-          w[c][e] = *reinterpret_cast<uint32_t*>(&b2v);
-        }
-      }
-      tc::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if (CG == 2) tc::mbar_arrive_cluster(leader_bar(&acc_empty[a]));
-        else tc::mbar_arrive(&acc_empty[a]);
-      }
-      if (!ok) continue;
-      const int r0 = m0 + quarter * 32;
-#pragma unroll
-      for (int c = 0; c < BOX; c += 2) {
-        // 32 rows x 64 columns through a swizzled staging tile, then whole 128-byte lines per row. Plain stores: nothing
-        // waits for them, where a tile store's staging buffer is held until it has been read
-        const int col = n0 + half * (BN / 2) + c * 32;
+#pragma unroll 1
+      for (int ms = 0; ms < MS; ++ms) {
+        // half a row of the sub-tile into registers as bf16 pairs, so that the accumulator is free before the last
+        // sub-tile is stored
+        uint32_t w[BOX][16];
         __syncwarp();
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint32_t* v = &w[c + (e >> 2)][4 * (e & 3)];
-          *reinterpret_cast<uint4*>(stg + lane * 128 + ((e ^ (lane & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
-        }
-        __syncwarp();
-        if (p.vec_out) {
-          const int cc = col + (lane & 7) * 8;  // NO is a multiple of 8 here: an 8-column group is whole or absent
+        for (int c = 0; c < BOX; ++c) {
+          uint32_t v[32];
+          tc::tmem_ld32(tbase + (a * MS + ms) * BN + half * (BN / 2) + c * 32 + lane_off, v);
+          tc::tmem_wait_ld();
+          tc::reg_fence32(v);
+          const float* bc = bs + half * (BN / 2) + c * 32;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int r = i * 4 + (lane >> 3);
-            const uint4 v = *reinterpret_cast<const uint4*>(stg + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
-            if (r0 + r < p.M && cc < p.NO) *reinterpret_cast<uint4*>(p.out + (int64_t)(r0 + r) * p.out_ld + cc) = v;
+          for (int e = 0; e < 16; ++e) {
+            float lo = __uint_as_float(v[2 * e]), hi = __uint_as_float(v[2 * e + 1]);
+            if (!DX) lo += bc[2 * e], hi += bc[2 * e + 1];
+            __nv_bfloat162 b2v = __floats2bfloat162_rn(lo, hi);
+            w[c][e] = *reinterpret_cast<uint32_t*>(&b2v);
           }
-        } else {
-#pragma unroll 4
-          for (int r = 0; r < 32; ++r) {
-            if (r0 + r >= p.M) break;
-            __nv_bfloat16* o = p.out + (int64_t)(r0 + r) * p.out_ld;
+        }
+        if (ms == MS - 1) {
+          tc::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if (CG == 2) tc::mbar_arrive_cluster(leader_bar(&acc_empty[a]));
+            else tc::mbar_arrive(&acc_empty[a]);
+          }
+        }
+        if (!ok) continue;
+        const int r0 = m0 + ms * 128 + quarter * 32;
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const int e = lane + 32 * j;
-              const __nv_bfloat16 v = *reinterpret_cast<const __nv_bfloat16*>(stg + r * 128 + (((e >> 3) ^ (r & 7)) << 4) + (e & 7) * 2);
-              if (col + e < p.NO) o[col + e] = v;
+        for (int c = 0; c < BOX; c += 2) {
+          // 32 rows x 64 columns through a swizzled staging tile, then whole 128-byte lines per row. Plain stores:
+          // nothing waits for them, where a tile store's staging buffer is held until it has been read
+          const int col = n0 + half * (BN / 2) + c * 32;
+          __syncwarp();
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const uint32_t* v = &w[c + (e >> 2)][4 * (e & 3)];
+            *reinterpret_cast<uint4*>(stg + lane * 128 + ((e ^ (lane & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+          }
+          __syncwarp();
+          if (p.vec_out) {
+            const int cc = col + (lane & 7) * 8;  // NO is a multiple of 8 here: an 8-column group is whole or absent
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int r = i * 4 + (lane >> 3);
+              const uint4 v = *reinterpret_cast<const uint4*>(stg + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+              if (r0 + r < p.M && cc < p.NO) *reinterpret_cast<uint4*>(p.out + (int64_t)(r0 + r) * p.out_ld + cc) = v;
+            }
+          } else {
+#pragma unroll 4
+            for (int r = 0; r < 32; ++r) {
+              if (r0 + r >= p.M) break;
+              __nv_bfloat16* o = p.out + (int64_t)(r0 + r) * p.out_ld;
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                const int e = lane + 32 * j;
+                const __nv_bfloat16 v = *reinterpret_cast<const __nv_bfloat16*>(stg + r * 128 + (((e >> 3) ^ (r & 7)) << 4) + (e & 7) * 2);
+                if (col + e < p.NO) o[col + e] = v;
+              }
             }
           }
         }
@@ -391,12 +406,12 @@ struct Shape {
   int64_t w_ld;
 };
 
-template <int BN, int CG, bool DX>
+template <int BN, int CG, int MS, bool DX>
 int launch4(const b2_mx4_gemm_args* a, const Shape& sh, cudaStream_t st) {
-  using C = Cfg4<BN, CG, DX>;
+  using C = Cfg4<BN, CG, MS, DX>;
   const char* name = DX ? "mx4_gemm_dx" : "mx4_gemm";
-  auto kern = mx4_gemm_kernel<BN, CG, DX>;
-  if (int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM), name)) return rc;
+  auto kern = mx4_gemm_kernel<BN, CG, MS, DX>;
+  if (int rc = allow_smem<mx4_gemm_kernel<BN, CG, MS, DX>>(C::SMEM, name)) return rc;
   P4 p{};
   p.bias = DX ? nullptr : (const __nv_bfloat16*)a->bias;
   p.out = (__nv_bfloat16*)a->out, p.out_ld = a->out_ld;
@@ -411,7 +426,7 @@ int launch4(const b2_mx4_gemm_args* a, const Shape& sh, cudaStream_t st) {
   const auto S128 = CU_TENSOR_MAP_SWIZZLE_128B, S0 = CU_TENSOR_MAP_SWIZZLE_NONE;
   bool ok;
   if (DX) {
-    ok = map2d(&ta, BF, sh.x, a->N, a->M, sh.x_ld * 2, 64, 128, S128) && map2d(&tw, BF, sh.w, a->K, a->N, sh.w_ld * 2, 64, 64, S128);
+    ok = map2d(&ta, BF, sh.x, a->N, a->M, sh.x_ld * 2, 64, C::BMC, S128) && map2d(&tw, BF, sh.w, a->K, a->N, sh.w_ld * 2, 64, 64, S128);
   } else {
     const int64_t cb = b2_mx4_code_bytes(a->K), nkb = (a->K + 127) / 128;
     ok = map2d(&ta, U8, a->x_codes, cb, a->M, cb, 128, 128, S128) && map2d(&tw, U8, a->w_codes, cb, a->N, cb, 128, C::BC, S128) &&
@@ -419,7 +434,7 @@ int launch4(const b2_mx4_gemm_args* a, const Shape& sh, cudaStream_t st) {
          map2d(&tsw, I32, a->w_scales, nkb * 128, (a->N + 127) / 128, nkb * 512, 256, BN / 128, S0);
   }
   if (a->lora_r) {
-    ok = ok && map2d(&th, BF, a->lora_h, a->lora_r, a->M, a->lora_h_ld * 2, 64, 128, S128);
+    ok = ok && map2d(&th, BF, a->lora_h, a->lora_r, a->M, a->lora_h_ld * 2, 64, C::BMC, S128);
     ok = ok && (DX ? map2d(&tb, BF, a->lora_b, a->K, a->lora_r, a->lora_b_ld * 2, 64, 64, S128)
                    : map2d(&tb, BF, a->lora_b, a->lora_r, a->N, a->lora_b_ld * 2, 64, C::BC, S128));
   }
@@ -447,12 +462,41 @@ int launch4(const b2_mx4_gemm_args* a, const Shape& sh, cudaStream_t st) {
   return after_launch(name);
 }
 
-// 256 x 256 tiles on CTA pairs read the fewest operand bytes per product; 128 x 128 ones on single CTAs where the pairs
-// would have less than about one tile each.
+// The tile whose waves cost least. A K block costs a CTA the longer of its MMAs and its operand loads: L2 feeds an SM
+// about 75 KB per microsecond when all of them load (measured: 70 to 87), 256 columns of a 128-row MMA take 0.27 us for 64
+// bf16 products and 0.52 us for 256 4-bit ones (as measured, the latter with the scales in place); each tile adds about
+// 1.5 us of draining, and a pair launch about 1.2 us of cluster set-up. Measured: dX of 4096 x 8192 -> 2048 takes 129 us
+// with 256 x 256 pair tiles (two waves) and 90 us with 512 x 256 ones (one wave); the forward of 1024 x 2048 -> 2048 takes
+// 9.6 us with 256 x 128 pair tiles and 8.5 us with 128 x 128 ones.
+struct Tile {
+  int bn, cg, ms;
+};
+Tile pick_tile(int64_t M, int64_t NO, int64_t KR, bool dx) {
+  static constexpr Tile cand[] = {{128, 1, 1}, {128, 2, 1}, {256, 2, 1}, {256, 2, 2}};
+  Tile best = cand[0];
+  double best_t = 1e30;
+  const int64_t sms = device_info().sm_count;
+  for (const Tile& c : cand) {
+    if (c.ms == 2 && !dx) continue;
+    const int64_t bm = 128 * c.ms * c.cg;
+    const int64_t tiles = (M + bm - 1) / bm * ((NO + c.bn - 1) / c.bn);
+    const int64_t waves = (tiles + sms / c.cg - 1) / (sms / c.cg);
+    const double kb = (double)((KR + (dx ? 63 : 255)) / (dx ? 64 : 256));
+    const double kbytes = 16.0 * c.ms + c.bn / c.cg / 8.0 + (dx ? 0.0 : 1.0 + c.bn / 128.0);
+    const double mma = (dx ? 0.27 : 0.52) * c.ms * c.bn / 256;
+    const double t = waves * (kb * std::max(mma, kbytes / 75.0) + 1.5 * c.ms * c.bn / 256 + 0.5) + (c.cg == 2 ? 1.2 : 0.0);
+    if (t < best_t) best_t = t, best = c;
+  }
+  return best;
+}
+
 template <bool DX>
 int launch_best(const b2_mx4_gemm_args* a, const Shape& sh, cudaStream_t st) {
-  const int64_t pairs = (a->M + 255) / 256 * ((sh.NO + 255) / 256);
-  return pairs >= device_info().sm_count / 2 ? launch4<256, 2, DX>(a, sh, st) : launch4<128, 1, DX>(a, sh, st);
+  const Tile t = pick_tile(a->M, sh.NO, sh.KR, DX);
+  if constexpr (DX)
+    if (t.ms == 2) return launch4<256, 2, 2, true>(a, sh, st);
+  if (t.bn == 256) return launch4<256, 2, 1, DX>(a, sh, st);
+  return t.cg == 2 ? launch4<128, 2, 1, DX>(a, sh, st) : launch4<128, 1, 1, DX>(a, sh, st);
 }
 
 }  // namespace

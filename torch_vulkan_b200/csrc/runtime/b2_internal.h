@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <string>
 
 #include "../../../include/b2rt.h"
@@ -73,6 +74,20 @@ int launch_pdl(const char* name, void (*kernel)(KArgs...), dim3 grid, dim3 block
     return fail_cuda(e, name);
   }
   return after_launch(name);
+}
+
+// Raises a kernel's dynamic shared-memory limit, once per kernel and device (and again only for a larger size): the
+// attribute call costs about as much host time as a launch. KERNEL is a template parameter, so each has its own record.
+template <auto KERNEL>
+int allow_smem(int bytes, const char* what) {
+  static std::atomic<int> have[64];
+  int dev = 0;
+  if (int rc = check_cuda(cudaGetDevice(&dev), what)) return rc;
+  const bool known = dev >= 0 && dev < 64;
+  if (known && have[dev].load(std::memory_order_relaxed) >= bytes) return 0;
+  if (int rc = check_cuda(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), what)) return rc;
+  if (known) have[dev].store(bytes, std::memory_order_relaxed);
+  return 0;
 }
 
 // Device error word (bounded waits that expired write a non-zero code here).

@@ -1,8 +1,11 @@
 // ATen operators of the 4-bit linears and of the relative-position-bias attention (b2::mx4_*, b2::bias_attn_*): the
 // wrappers validate, compute strides, allocate outputs and workspaces on the current allocator and launch on the
-// current stream, as those of ops.cpp do.
+// current stream, as those of ops.cpp do. The differentiable operators (mx4_linear, mx4_lora_linear,
+// bucket_bias_attention) are C++ autograd functions: their smallest calls are bound by the host, and a Python function's
+// forward and backward cost more there than the kernels.
 #include <ATen/Functions.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
 #include <array>
@@ -167,20 +170,88 @@ at::Tensor mx4_dx(const at::Tensor& dy0, const at::Tensor& codes, const at::Tens
   return dx;
 }
 
-at::Tensor mx4_linear_fwd(const at::Tensor& x, const at::Tensor& codes, const at::Tensor& scales,
-                          const std::optional<at::Tensor>& bias) {
+at::Tensor sum_rows(const at::Tensor& gy) { return rows_of(gy).sum(0); }
+
+using torch::autograd::AutogradContext;
+using torch::autograd::Variable;
+using torch::autograd::variable_list;
+
+// y = Q(x) W^T + bias; straight-through dx = dy W.
+at::Tensor mx4_linear(const at::Tensor& x, const at::Tensor& codes, const at::Tensor& scales,
+                      const std::optional<at::Tensor>& bias) {
   return mx4_fwd(x, codes, scales, bias, nullptr, nullptr, "b2::mx4_linear");
 }
-at::Tensor mx4_linear_dx(const at::Tensor& dy, const at::Tensor& codes, const at::Tensor& scales, int64_t cols) {
-  return mx4_dx(dy, codes, scales, cols, nullptr, nullptr, "b2::mx4_linear_dx");
+struct Mx4Linear : torch::autograd::Function<Mx4Linear> {
+  static Variable forward(AutogradContext* ctx, const Variable& x, const Variable& codes, const Variable& scales,
+                          const std::optional<Variable>& bias) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    ctx->save_for_backward({codes, scales});
+    ctx->saved_data["cols"] = x.dim() ? x.size(-1) : 0;
+    ctx->saved_data["bias"] = bias.has_value() && bias->defined();
+    return mx4_linear(x, codes, scales, bias);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const variable_list saved = ctx->get_saved_variables();
+    variable_list out(4);
+    if (ctx->needs_input_grad(0))
+      out[0] = mx4_dx(g[0], saved[0], saved[1], ctx->saved_data["cols"].toInt(), nullptr, nullptr, "b2::mx4_linear_dx");
+    if (ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(3)) out[3] = sum_rows(g[0]);
+    return out;
+  }
+};
+at::Tensor mx4_linear_autograd(const at::Tensor& x, const at::Tensor& codes, const at::Tensor& scales,
+                               const std::optional<at::Tensor>& bias) {
+  return Mx4Linear::apply(x, codes, scales, bias);
 }
-at::Tensor mx4_lora_fwd(const at::Tensor& x, const at::Tensor& codes, const at::Tensor& scales,
-                        const std::optional<at::Tensor>& bias, const at::Tensor& h, const at::Tensor& b) {
-  return mx4_fwd(x, codes, scales, bias, &h, &b, "b2::mx4_lora_fwd");
+
+// y = Q(x) W^T + bias + (x a^T) b^T, with the hidden activation h = x a^T [rows, r] as the second result.
+std::tuple<at::Tensor, at::Tensor> mx4_lora_fwd(const at::Tensor& x, const at::Tensor& codes, const at::Tensor& scales,
+                                                const std::optional<at::Tensor>& bias, const at::Tensor& a,
+                                                const at::Tensor& b) {
+  const char* name = "b2::mx4_lora_linear";
+  TORCH_CHECK(x.is_cuda() && x.scalar_type() == at::kBFloat16 && x.dim() >= 1, name, ": x must be a bfloat16 CUDA tensor");
+  TORCH_CHECK(a.dim() == 2 && b.dim() == 2 && a.is_cuda() && a.scalar_type() == at::kBFloat16 && a.size(1) == x.size(-1), name,
+              ": a must be a bf16 CUDA matrix [r, ", x.size(-1), "], got ", a.scalar_type(), " ", a.sizes());
+  c10::cuda::CUDAGuard guard(x.device());
+  at::Tensor h = at::mm(rows_of(x), a.t());  // of the unquantised activation
+  at::Tensor y = mx4_fwd(x, codes, scales, bias, &h, &b, name);
+  return {y, h};
 }
-at::Tensor mx4_lora_dx(const at::Tensor& dy, const at::Tensor& codes, const at::Tensor& scales, int64_t cols,
-                       const at::Tensor& dh, const at::Tensor& a) {
-  return mx4_dx(dy, codes, scales, cols, &dh, &a, "b2::mx4_lora_dx");
+at::Tensor mx4_lora_linear(const at::Tensor& x, const at::Tensor& codes, const at::Tensor& scales,
+                           const std::optional<at::Tensor>& bias, const at::Tensor& a, const at::Tensor& b) {
+  return std::get<0>(mx4_lora_fwd(x, codes, scales, bias, a, b));
+}
+struct Mx4Lora : torch::autograd::Function<Mx4Lora> {
+  static Variable forward(AutogradContext* ctx, const Variable& x, const Variable& codes, const Variable& scales,
+                          const std::optional<Variable>& bias, const Variable& a, const Variable& b) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    auto [y, h] = mx4_lora_fwd(x, codes, scales, bias, a, b);
+    ctx->save_for_backward({x, codes, scales, a, b, h});
+    ctx->saved_data["bias"] = bias.has_value() && bias->defined();
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const variable_list s = ctx->get_saved_variables();
+    const at::Tensor &x = s[0], &codes = s[1], &scales = s[2], &a = s[3], &b = s[4], &h = s[5];
+    c10::cuda::CUDAGuard guard(x.device());
+    at::Tensor gy = rows_of(g[0]);
+    variable_list out(6);
+    // edges are counted over the tensors that were given: without a bias, a and b move up by one
+    const int e = ctx->saved_data["bias"].toBool() ? 4 : 3;
+    if (ctx->needs_input_grad(0) || ctx->needs_input_grad(e)) {
+      at::Tensor dh = at::mm(gy, b);
+      if (ctx->needs_input_grad(0))
+        out[0] = mx4_dx(gy, codes, scales, x.size(-1), &dh, &a, "b2::mx4_lora_dx").view_as(x);
+      if (ctx->needs_input_grad(e)) out[4] = at::mm(dh.t(), rows_of(x));
+    }
+    if (ctx->needs_input_grad(e + 1)) out[5] = at::mm(gy.t(), h);
+    if (e == 4 && ctx->needs_input_grad(3)) out[3] = sum_rows(gy);
+    return out;
+  }
+};
+at::Tensor mx4_lora_linear_autograd(const at::Tensor& x, const at::Tensor& codes, const at::Tensor& scales,
+                                    const std::optional<at::Tensor>& bias, const at::Tensor& a, const at::Tensor& b) {
+  return Mx4Lora::apply(x, codes, scales, bias, a, b);
 }
 
 // =============================== relative-position-bias attention ====================================
@@ -315,6 +386,51 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> bias_attn_bwd(
   return {dq, dk, dv, dt};
 }
 
+at::Tensor bucket_bias_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& table,
+                                 const std::optional<at::Tensor>& key_mask, int64_t max_distance, bool bidirectional,
+                                 bool causal, double scale, int64_t q_offset) {
+  return std::get<0>(bias_attn_fwd(q, k, v, table, key_mask, max_distance, bidirectional, causal, scale, q_offset, false));
+}
+struct BucketBiasAttention : torch::autograd::Function<BucketBiasAttention> {
+  static Variable forward(AutogradContext* ctx, const Variable& q, const Variable& k, const Variable& v, const Variable& table,
+                          const std::optional<Variable>& key_mask, int64_t max_distance, bool bidirectional, bool causal,
+                          double scale, int64_t q_offset) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    const bool grad = q.requires_grad() || k.requires_grad() || v.requires_grad() || table.requires_grad();
+    // a backward keeps the unrounded output: its dS cancels over each row
+    auto [o, lse, o32] =
+        bias_attn_fwd(q, k, v, table, key_mask, max_distance, bidirectional, causal, scale, q_offset, grad);
+    if (grad) {
+      ctx->save_for_backward({q, k, v, o32.defined() ? o32 : o, lse, table, key_mask.has_value() ? *key_mask : at::Tensor()});
+      ctx->saved_data["max_distance"] = max_distance;
+      ctx->saved_data["bidirectional"] = bidirectional;
+      ctx->saved_data["causal"] = causal;
+      ctx->saved_data["scale"] = scale;
+      ctx->saved_data["q_offset"] = q_offset;
+    }
+    return o;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const variable_list s = ctx->get_saved_variables();
+    auto& d = ctx->saved_data;
+    std::array<bool, 4> want;
+    for (int i = 0; i < 4; ++i) want[i] = ctx->needs_input_grad(i);
+    const std::optional<at::Tensor> mask = s[6].defined() ? std::optional<at::Tensor>(s[6]) : std::nullopt;
+    auto [dq, dk, dv, dt] = bias_attn_bwd(g[0], s[0], s[1], s[2], s[3], s[4], s[5], mask, d["max_distance"].toInt(),
+                                          d["bidirectional"].toBool(), d["causal"].toBool(), d["scale"].toDouble(),
+                                          d["q_offset"].toInt(), want);
+    variable_list out(10);
+    out[0] = dq, out[1] = dk, out[2] = dv, out[3] = dt;
+    return out;
+  }
+};
+at::Tensor bucket_bias_attention_autograd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                          const at::Tensor& table, const std::optional<at::Tensor>& key_mask,
+                                          int64_t max_distance, bool bidirectional, bool causal, double scale,
+                                          int64_t q_offset) {
+  return BucketBiasAttention::apply(q, k, v, table, key_mask, max_distance, bidirectional, causal, scale, q_offset);
+}
+
 int64_t bias_bucket(int64_t rel, int64_t num_buckets, int64_t max_distance, bool bidirectional) {
   TORCH_CHECK(num_buckets >= 0 && num_buckets <= B2_BIAS_MAX_BUCKETS && max_distance >= 0 && max_distance <= B2_BIAS_MAX_DISTANCE,
               "bias_bucket: num_buckets must be at most 128 and max_distance at most 1024");
@@ -328,25 +444,23 @@ int64_t bias_bucket(int64_t rel, int64_t num_buckets, int64_t max_distance, bool
 TORCH_LIBRARY_FRAGMENT(b2, m) {
   m.def("mx4_quantize(Tensor x) -> (Tensor, Tensor)");
   m.def("mx4_dequantize(Tensor codes, Tensor scales, int cols, ScalarType dtype) -> Tensor");
-  m.def("mx4_linear_fwd(Tensor x, Tensor codes, Tensor scales, Tensor? bias) -> Tensor");
-  m.def("mx4_linear_dx(Tensor dy, Tensor codes, Tensor scales, int cols) -> Tensor");
-  m.def("mx4_lora_fwd(Tensor x, Tensor codes, Tensor scales, Tensor? bias, Tensor h, Tensor b) -> Tensor");
-  m.def("mx4_lora_dx(Tensor dy, Tensor codes, Tensor scales, int cols, Tensor dh, Tensor a) -> Tensor");
-  m.def("bias_attn_fwd(Tensor q, Tensor k, Tensor v, Tensor table, Tensor? key_mask, int max_distance, bool bidirectional, "
-        "bool causal, float scale, int q_offset, bool keep_o32) -> (Tensor, Tensor, Tensor)");
-  m.def("bias_attn_bwd(Tensor grad_out, Tensor q, Tensor k, Tensor v, Tensor out, Tensor lse, Tensor table, Tensor? key_mask, "
-        "int max_distance, bool bidirectional, bool causal, float scale, int q_offset, bool[4] want) -> "
-        "(Tensor, Tensor, Tensor, Tensor)");
+  m.def("mx4_linear(Tensor x, Tensor codes, Tensor scales, Tensor? bias) -> Tensor");
+  m.def("mx4_lora_linear(Tensor x, Tensor codes, Tensor scales, Tensor? bias, Tensor a, Tensor b) -> Tensor");
+  m.def("bucket_bias_attention(Tensor q, Tensor k, Tensor v, Tensor table, Tensor? key_mask, int max_distance, "
+        "bool bidirectional, bool causal, float scale, int q_offset) -> Tensor");
   m.def("bias_bucket(int rel, int num_buckets, int max_distance, bool bidirectional) -> int", &bias_bucket);
 }
 
 TORCH_LIBRARY_IMPL(b2, CUDA, m) {
   m.impl("mx4_quantize", &mx4_quantize);
   m.impl("mx4_dequantize", &mx4_dequantize);
-  m.impl("mx4_linear_fwd", &mx4_linear_fwd);
-  m.impl("mx4_linear_dx", &mx4_linear_dx);
-  m.impl("mx4_lora_fwd", &mx4_lora_fwd);
-  m.impl("mx4_lora_dx", &mx4_lora_dx);
-  m.impl("bias_attn_fwd", &bias_attn_fwd);
-  m.impl("bias_attn_bwd", &bias_attn_bwd);
+  m.impl("mx4_linear", &mx4_linear);
+  m.impl("mx4_lora_linear", &mx4_lora_linear);
+  m.impl("bucket_bias_attention", &bucket_bias_attention);
+}
+
+TORCH_LIBRARY_IMPL(b2, AutogradCUDA, m) {
+  m.impl("mx4_linear", &mx4_linear_autograd);
+  m.impl("mx4_lora_linear", &mx4_lora_linear_autograd);
+  m.impl("bucket_bias_attention", &bucket_bias_attention_autograd);
 }

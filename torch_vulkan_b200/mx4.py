@@ -34,7 +34,7 @@ def mx4_quantize(x: torch.Tensor) -> Mx4:
     """Quantise a matrix (fp32, bf16 or f16; rows may be strided). The scale of a block is
     2^(floor(log2(largest magnitude)) - 2); elements round to the nearest code, ties to the even one, and magnitudes
     above 6 scales become 6."""
-    codes, scales = torch.ops.b2.mx4_quantize(x.detach())
+    codes, scales = torch.ops.b2.mx4_quantize(x.detach() if x.requires_grad else x)
     return Mx4(codes, scales, x.shape[1])
 
 
@@ -43,57 +43,10 @@ def mx4_dequantize(w: Mx4, dtype=torch.bfloat16) -> torch.Tensor:
     return torch.ops.b2.mx4_dequantize(w.codes, w.scales, w.cols, dtype)
 
 
-class _Mx4Linear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, codes, scales, cols, bias):
-        if x.shape[-1] != cols:
-            raise RuntimeError(f"mx4_linear: x has {x.shape[-1]} features, the weight {cols}")
-        ctx.save_for_backward(codes, scales)
-        ctx.cols, ctx.has_bias = cols, bias is not None
-        return torch.ops.b2.mx4_linear_fwd(x, codes, scales, bias)
-
-    @staticmethod
-    def backward(ctx, gy):
-        codes, scales = ctx.saved_tensors
-        gx = torch.ops.b2.mx4_linear_dx(gy, codes, scales, ctx.cols) if ctx.needs_input_grad[0] else None
-        gb = gy.reshape(-1, gy.shape[-1]).sum(0) if (ctx.has_bias and ctx.needs_input_grad[4]) else None
-        return gx, None, None, None, gb
-
-
 def mx4_linear(x: torch.Tensor, w: Mx4, bias: torch.Tensor | None = None) -> torch.Tensor:
     """y = Q(x) W^T + bias: x bf16 [..., K] is quantised to MXFP4 in the call, the element products are exact and
     summed in fp32. Differentiable in x (straight-through: dx = dy W) and bias; W is frozen."""
-    return _Mx4Linear.apply(x, w.codes, w.scales, w.cols, bias)
-
-
-class _Mx4LoRA(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, codes, scales, cols, bias, a, b):
-        if x.shape[-1] != cols:
-            raise RuntimeError(f"mx4_lora_linear: x has {x.shape[-1]} features, the weight {cols}")
-        x2 = x.reshape(-1, cols)
-        h = torch.mm(x2, a.t())  # the rank-r down-projection, of the unquantised activation
-        y = torch.ops.b2.mx4_lora_fwd(x2, codes, scales, bias, h, b)
-        ctx.save_for_backward(x2, codes, scales, a, b, h)
-        ctx.cols, ctx.x_shape, ctx.has_bias = cols, x.shape, bias is not None
-        return y.view(*x.shape[:-1], codes.shape[0])
-
-    @staticmethod
-    def backward(ctx, gy):
-        x2, codes, scales, a, b, h = ctx.saved_tensors
-        gy2 = gy.reshape(-1, gy.shape[-1])
-        if not gy2.is_contiguous():
-            gy2 = gy2.contiguous()
-        gx = ga = None
-        if ctx.needs_input_grad[0] or ctx.needs_input_grad[5]:
-            dh = torch.mm(gy2, b)
-            if ctx.needs_input_grad[0]:
-                gx = torch.ops.b2.mx4_lora_dx(gy2, codes, scales, ctx.cols, dh, a).view(ctx.x_shape)
-            if ctx.needs_input_grad[5]:
-                ga = torch.mm(dh.t(), x2)
-        gb = torch.mm(gy2.t(), h) if ctx.needs_input_grad[6] else None
-        gbias = gy2.sum(0) if (ctx.has_bias and ctx.needs_input_grad[4]) else None
-        return gx, None, None, None, gbias, ga, gb
+    return torch.ops.b2.mx4_linear(x, w.codes, w.scales, bias)
 
 
 def mx4_lora_linear(x, w: Mx4, bias, a, b) -> torch.Tensor:
@@ -101,4 +54,4 @@ def mx4_lora_linear(x, w: Mx4, bias, a, b) -> torch.Tensor:
     and b [N, r] the up-projection already multiplied by alpha / r (r a multiple of 8, at most 64). The side path reads
     the unquantised x and is added inside the product; in the backward dX = dY W + (dY b) a is one product too.
     Differentiable in x, a, b (and bias). bf16."""
-    return _Mx4LoRA.apply(x, w.codes, w.scales, w.cols, bias, a, b)
+    return torch.ops.b2.mx4_lora_linear(x, w.codes, w.scales, bias, a, b)
