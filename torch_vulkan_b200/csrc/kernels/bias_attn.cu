@@ -149,17 +149,17 @@ struct Plan {
 
 uint64_t up16(uint64_t v) { return (v + 15) / 16 * 16; }
 
-// Key splits of the forward: the waves of blocks times the key tiles a block walks plus about four tiles' worth of set-up,
+// Key splits of the forward: the waves of blocks times the key tiles a block walks plus 1.6 us of set-up,
 // and for the join its bytes (each split's fp32 output written and read) at the memory's rate, where a tile takes about
-// 0.4 us, and a launch. At least two tiles a split. Measured, 16 heads x 4096 x 4096: 2 splits save a sixth of the walk
+// 0.4 us on the tensor cores and 6 us on the FMA pipe, and a launch. At least two tiles a split. Measured, 16 heads x 4096 x 4096: 2 splits save a sixth of the walk
 // (3.5 waves) and their join takes 47 us of it back.
-int pick_splits(int64_t blocks, int64_t tk, int64_t out_elems) {
+int pick_splits(int64_t blocks, int64_t tk, int64_t out_elems, double tile_us) {
   const int64_t sms = device_info().sm_count > 0 ? device_info().sm_count : 148;
   int best = 1;
   double best_cost = 1e30;
   for (int64_t ns = 1; ns <= std::max<int64_t>(1, std::min<int64_t>(tk / 2, 64)); ++ns) {
-    const double join = ns > 1 ? 8.0 + (double)ns * out_elems * 8.0 / 3e6 / 0.4 : 0.0;
-    const double cost = (double)((blocks * ns + sms - 1) / sms) * ((tk + ns - 1) / ns + 4) + join;
+    const double join = ns > 1 ? (3.0 + (double)ns * out_elems * 8.0 / 3e6) / tile_us : 0.0;
+    const double cost = (double)((blocks * ns + sms - 1) / sms) * ((tk + ns - 1) / ns + 1.6 / tile_us) + join;
     if (cost < best_cost) best_cost = cost, best = (int)ns;
   }
   return best;
@@ -172,7 +172,7 @@ Plan make_plan(const b2_bias_attn_args* a, bool bwd) {
   const int tile = pl.tc ? kTcTile : kSimtTile;
   const int64_t tq = (a->Sq + tile - 1) / tile, tk = (a->Sk + tile - 1) / tile;
   if (!bwd) {
-    pl.nsplit = pick_splits(tq * a->B * a->H, tk, rows * a->D);
+    pl.nsplit = pick_splits(tq * a->B * a->H, tk, rows * a->D, pl.tc ? 0.4 : 6.0);
     if (pl.nsplit > 1) {
       pl.part_o = 0;
       pl.part_ml = up16((uint64_t)pl.nsplit * rows * a->D * 4);

@@ -8,6 +8,8 @@
 #include "bias_attn.cuh"
 #include "tc_ptx.cuh"
 
+#include <type_traits>
+
 namespace b2 {
 
 bool make_tmap(CUtensorMap* m, CUtensorMapDataType dt, int rank, const void* base, const uint64_t* dims,
@@ -78,8 +80,8 @@ template <int D>
 struct Fwd {
   static constexpr int BQ = 128, BK = 128, DCH = D / 64;
   static constexpr int Q_BYTES = BQ * D * 2, KV_BYTES = BK * D * 2;
-  static constexpr int NS = D == 64 ? 4 : 2;  // K / V ring depth
-  static constexpr int OFF_Q = 0, OFF_K = Q_BYTES, OFF_V = OFF_K + NS * KV_BYTES, OFF_BAR = OFF_V + NS * KV_BYTES;
+  static constexpr int NK = D == 64 ? 4 : 3, NV = D == 64 ? 4 : 2;  // K / V ring depths
+  static constexpr int OFF_Q = 0, OFF_K = Q_BYTES, OFF_V = OFF_K + NK * KV_BYTES, OFF_BAR = OFF_V + NV * KV_BYTES;
   static constexpr int OFF_VEC = OFF_BAR + 256;
   static constexpr int THREADS = 320;
   static constexpr uint32_t T_S = 0, T_O = 256, TMEM_COLS = 512;
@@ -94,16 +96,16 @@ __global__ void __launch_bounds__(320, 1)
                 const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO,
                 const __grid_constant__ Params p) {
   using C = Fwd<D>;
-  constexpr int NS = C::NS;
+  constexpr int NK = C::NK, NV = C::NV;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
   uint64_t* q_full = bar;
-  uint64_t* k_full = bar + 1;         // [NS]
-  uint64_t* k_empty = k_full + NS;    // [NS]
-  uint64_t* v_full = k_empty + NS;    // [NS]
-  uint64_t* v_empty = v_full + NS;    // [NS]
-  uint64_t* s_full = v_empty + NS;    // [2] S of tile t in S[t & 1]
+  uint64_t* k_full = bar + 1;         // [NK]
+  uint64_t* k_empty = k_full + NK;    // [NK]
+  uint64_t* v_full = k_empty + NK;    // [NV]
+  uint64_t* v_empty = v_full + NV;    // [NV]
+  uint64_t* s_full = v_empty + NV;    // [2] S of tile t in S[t & 1]
   uint64_t* p_full = s_full + 2;      // [2] P of tile t in TMEM over S[t & 1]
   uint64_t* o_upd = p_full + 2;       // [2] P V of tile t done
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_upd + 2);
@@ -118,10 +120,8 @@ __global__ void __launch_bounds__(320, 1)
 
   if (threadIdx.x == 0) {
     tc::mbar_init(q_full, 1);
-    for (int i = 0; i < NS; ++i) {
-      tc::mbar_init(&k_full[i], 1), tc::mbar_init(&k_empty[i], 1);
-      tc::mbar_init(&v_full[i], 1), tc::mbar_init(&v_empty[i], 1);
-    }
+    for (int i = 0; i < NK; ++i) tc::mbar_init(&k_full[i], 1), tc::mbar_init(&k_empty[i], 1);
+    for (int i = 0; i < NV; ++i) tc::mbar_init(&v_full[i], 1), tc::mbar_init(&v_empty[i], 1);
     for (int i = 0; i < 2; ++i) tc::mbar_init(&s_full[i], 1), tc::mbar_init(&p_full[i], 128), tc::mbar_init(&o_upd[i], 1);
     *abort_flag = 0;
     tc::fence_barrier_init();
@@ -149,28 +149,27 @@ __global__ void __launch_bounds__(320, 1)
       bool ok = true;
       tc::mbar_arrive_expect_tx(q_full, C::Q_BYTES);
       for (int c = 0; c < C::DCH; ++c) tc::tma_load_4d(smem + C::OFF_Q + c * (C::BQ * 128), &tmQ, q_full, c * 64, q0, h, b);
-      int issued_k[NS] = {}, issued_v[NS] = {};
+      int issued_k[NK] = {}, issued_v[NV] = {};
       for (int t = 0; t < n; ++t) {
-        const int s = t % NS, k0 = (t0 + t) * C::BK;
-        const uint32_t ph = (uint32_t)((t / NS) & 1) ^ 1;
-        if (!tc::mbar_wait(&k_empty[s], ph, p.err) || *abort_flag) { ok = false; break; }
+        const int s = t % NK, v = t % NV, k0 = (t0 + t) * C::BK;
+        if (!tc::mbar_wait(&k_empty[s], (uint32_t)((t / NK) & 1) ^ 1, p.err) || *abort_flag) { ok = false; break; }
         tc::mbar_arrive_expect_tx(&k_full[s], C::KV_BYTES);
         for (int c = 0; c < C::DCH; ++c)
           tc::tma_load_4d(smem + C::OFF_K + s * C::KV_BYTES + c * (C::BK * 128), &tmK, &k_full[s], c * 64, k0, hk, b);
         issued_k[s]++;
-        if (!tc::mbar_wait(&v_empty[s], ph, p.err) || *abort_flag) { ok = false; break; }
-        tc::mbar_arrive_expect_tx(&v_full[s], C::KV_BYTES);
+        if (!tc::mbar_wait(&v_empty[v], (uint32_t)((t / NV) & 1) ^ 1, p.err) || *abort_flag) { ok = false; break; }
+        tc::mbar_arrive_expect_tx(&v_full[v], C::KV_BYTES);
         for (int c = 0; c < C::DCH; ++c)
-          tc::tma_load_4d(smem + C::OFF_V + s * C::KV_BYTES + c * (C::BK * 128), &tmV, &v_full[s], c * 64, k0, hk, b);
-        issued_v[s]++;
+          tc::tma_load_4d(smem + C::OFF_V + v * C::KV_BYTES + c * (C::BK * 128), &tmV, &v_full[v], c * 64, k0, hk, b);
+        issued_v[v]++;
       }
       if (!ok) {
         *abort_flag = 1;
         tc::mbar_wait(q_full, 0, nullptr);
-        for (int s = 0; s < NS; ++s) {
+        for (int s = 0; s < NK; ++s)
           if (issued_k[s]) tc::mbar_wait(&k_full[s], (uint32_t)((issued_k[s] - 1) & 1), nullptr);
+        for (int s = 0; s < NV; ++s)
           if (issued_v[s]) tc::mbar_wait(&v_full[s], (uint32_t)((issued_v[s] - 1) & 1), nullptr);
-        }
       }
     }
   } else if (warp == 1) {
@@ -182,8 +181,8 @@ __global__ void __launch_bounds__(320, 1)
       const tc::SDesc qd = tc::sdesc_parts(tc::smem_u32(smem + C::OFF_Q), 16, 1024);
       bool ok = tc::mbar_wait(q_full, 0, p.err);
       auto issue_s = [&](int t) -> bool {
-        const int ks = t % NS;
-        if (!tc::mbar_wait(&k_full[ks], (uint32_t)((t / NS) & 1), p.err)) return false;
+        const int ks = t % NK;
+        if (!tc::mbar_wait(&k_full[ks], (uint32_t)((t / NK) & 1), p.err)) return false;
         tc::tc_fence_after();
         const tc::SDesc kd = tc::sdesc_parts(tc::smem_u32(smem + C::OFF_K + ks * C::KV_BYTES), 16, 1024);
 #pragma unroll
@@ -198,9 +197,9 @@ __global__ void __launch_bounds__(320, 1)
       if (ok) ok = issue_s(0);
       if (ok && n > 1) ok = issue_s(1);
       for (int t = 0; t < n && ok; ++t) {
-        const int s = t & 1, vs = t % NS;
+        const int s = t & 1, vs = t % NV;
         if (!tc::mbar_wait(&p_full[s], (uint32_t)((t >> 1) & 1), p.err) ||
-            !tc::mbar_wait(&v_full[vs], (uint32_t)((t / NS) & 1), p.err)) {
+            !tc::mbar_wait(&v_full[vs], (uint32_t)((t / NV) & 1), p.err)) {
           ok = false;
           break;
         }
@@ -327,11 +326,11 @@ __global__ void __launch_bounds__(320, 1)
       l = l * alpha + (rs2.x + rs2.y);
       if (!full && p.mask != nullptr) {
         // masked keys may hold anything, and 0 * NaN is NaN in the P V product: clear their rows of V
-        if (!tc::mbar_wait(&v_full[t % NS], (uint32_t)((t / NS) & 1), p.err)) { ok = false; break; }
+        if (!tc::mbar_wait(&v_full[t % NV], (uint32_t)((t / NV) & 1), p.err)) { ok = false; break; }
         if (!((bits[quarter] >> lane) & 1u)) {
 #pragma unroll
           for (int c = 0; c < C::DCH; ++c) {
-            uint4* row = reinterpret_cast<uint4*>(smem + C::OFF_V + (t % NS) * C::KV_BYTES + c * (C::BK * 128) + r * 128);
+            uint4* row = reinterpret_cast<uint4*>(smem + C::OFF_V + (t % NV) * C::KV_BYTES + c * (C::BK * 128) + r * 128);
 #pragma unroll
             for (int i = 0; i < 8; ++i) row[i] = make_uint4(0u, 0u, 0u, 0u);
           }
@@ -431,56 +430,71 @@ __global__ void __launch_bounds__(320, 1)
 //   KEYS = true   X = K, V (a block owns 128 keys),    Y = Q, dO:   dK += dS^T Q, dV += P^T dO, over every query head
 //                                                                   that shares the key/value head
 // S = X1 Y1^T and dP = X2 Y2^T are recomputed on both sides (7 products instead of 5), which leaves every gradient one
-// owner: no atomics, no accumulator in memory, the same bits on every run. Two warpgroups take the tiles in turn, each
-// with its own S and dP columns in TMEM; P and dS (16 bits) replace them and are the A operands of the gradient MMAs.
+// owner: no atomics, no accumulator in memory, the same bits on every run. Two teams of eight warps take the tiles in turn,
+// each with its own S and dP columns in TMEM; in a team, two warps share a lane quarter and split its columns. P and dS
+// (16 bits) replace the scores a warp has read and are the A operands of the gradient MMAs, 8 columns per 16 of the
+// reduction at any place. (Eight warps in all, half as many, left the MMAs waiting for them: 357 us instead of 285 for the
+// key side at 16 heads x 4096 x 4096 x 64.)
 // ==================================================================================================
 template <int D, bool KEYS>
 struct Bwd {
   static constexpr int BX = 128, DCH = D / 64;
-  static constexpr int NT = (KEYS && D == 128) ? 64 : 96;  // walked rows per tile: what TMEM holds twice beside the sums
+  static constexpr int NT = D == 128 ? 64 : 96;  // walked rows per tile: what TMEM holds twice beside the sums
+  static constexpr int HC = NT / 2;                        // columns of a tile per warp
   static constexpr int X_BYTES = BX * D * 2, Y_BYTES = NT * D * 2;
-  static constexpr int LD_BYTES = KEYS ? NT * 8 : 0;       // (lse log2 e, delta) of the walked queries
+  static constexpr int LD_BYTES = KEYS ? NT * 8 : 0;       // (-lse log2 e, -delta) of the walked queries
   static constexpr int STAGE = 2 * Y_BYTES + (LD_BYTES + 1023) / 1024 * 1024;
-  static constexpr int NS = D == 64 ? 3 : 2;
+  // ring depth: a stage is freed by the gradient MMAs of its tile, and its next load takes about a microsecond from there.
+  // Two stages at D = 128 put that latency into every tile (612 us for the key side at 16 heads x 4096 x 4096 x 128)
+  static constexpr int NS = D == 64 ? 5 : (KEYS ? 4 : 3);
   static constexpr int OFF_X = 0, OFF_Y = 2 * X_BYTES, OFF_BAR = OFF_Y + NS * STAGE, OFF_VEC = OFF_BAR + 256;
-  static constexpr int THREADS = 320;
+  static constexpr int EW = 512, THREADS = 64 + EW;        // element-wise threads
   static constexpr uint32_t T_S = 0, T_DP = NT, T_BUF = 2 * NT, T_ACC = 4 * NT, TMEM_COLS = 512;
   static constexpr uint32_t T_ACC2 = T_ACC + D;  // KEYS: dV at T_ACC, dK behind it
   static_assert(4 * NT + (KEYS ? 2 * D : D) <= 512, "TMEM columns");
+  // columns of the A operand's 16-deep step k, counted from the scores' first column
+  static __device__ __forceinline__ constexpr uint32_t a_col(int k) { return k < HC / 16 ? k * 8 : HC + (k - HC / 16) * 8; }
 };
 
-// Adds the diagonal sums of a 32 x 16 block (rows = lanes, v = this lane's 16 columns) to arr[column - row]. Running sums
-// travel up the lanes by one per column: the sum that lane l holds at column e belongs to the diagonal e - l; the one
-// that has passed lane 31 is complete and is put aside. Two blocks run interleaved to hide the shuffle's latency.
-__device__ __forceinline__ void add_diagonals(const float* v, float* arr, float* scratch, int lane) {
-  float a0 = v[0], a1 = v[16];
+// Adds the diagonal sums of a 32 x 16 block (rows = lanes, v = this lane's 16 columns) to arr[clamp(rel + column - row)],
+// where arr is centred on relative position 0 and spans -R .. R. Running sums travel up the lanes by one per column: the
+// sum that lane l holds at column e belongs to the diagonal e - l; the one that has passed lane 31 is complete and is put
+// aside. Positions beyond +-R share a slot: those lanes are added up first.
+__device__ __forceinline__ void add_at(float* arr, int pos, float x, bool on, int R, int lane) {
+  const bool hi = on && pos > R, lo = on && pos < -R;
+  if (__any_sync(0xffffffffu, hi || lo)) {
+    const float sh = warp_sum(hi ? x : 0.f), sl = warp_sum(lo ? x : 0.f);
+    if (lane == 0) arr[R] += sh, arr[-R] += sl;
+    __syncwarp();
+  }
+  if (on && !hi && !lo) arr[pos] += x;
+  __syncwarp();
+}
+__device__ __forceinline__ void add_diagonals(const float* v, float* arr, int rel, int R, float* scratch, int lane) {
+  float a = v[0];
   const int from = (lane + 31) & 31;
 #pragma unroll
   for (int e = 1; e < 16; ++e) {
-    float t0 = __shfl_sync(0xffffffffu, a0, from), t1 = __shfl_sync(0xffffffffu, a1, from);
+    float t = __shfl_sync(0xffffffffu, a, from);
     if (lane == 0) {
-      scratch[e - 1] = t0, scratch[16 + e - 1] = t1;
-      t0 = t1 = 0.f;
+      scratch[e - 1] = t;
+      t = 0.f;
     }
-    a0 = t0 + v[e], a1 = t1 + v[16 + e];
+    a = t + v[e];
   }
   __syncwarp();
-  arr[15 - lane] += a0;
-  if (lane < 15) arr[lane - 31] += scratch[lane];
-  __syncwarp();
-  arr[31 - lane] += a1;
-  if (lane < 15) arr[lane - 15] += scratch[16 + lane];
-  __syncwarp();
+  add_at(arr, rel + 15 - lane, a, true, R, lane);
+  add_at(arr, rel + lane - 31, lane < 15 ? scratch[lane] : 0.f, lane < 15, R, lane);
 }
 
 template <int D, bool BF16, bool KEYS>
-__global__ void __launch_bounds__(320, 1)
+__global__ void __launch_bounds__(576, 1)
     bias_bwd_tc(const __grid_constant__ CUtensorMap tmX1, const __grid_constant__ CUtensorMap tmX2,
                 const __grid_constant__ CUtensorMap tmY1, const __grid_constant__ CUtensorMap tmY2,
                 const __grid_constant__ CUtensorMap tmG1, const __grid_constant__ CUtensorMap tmG2,
                 const __grid_constant__ Params p, const float2* __restrict__ lsed, int sq_pad) {
   using C = Bwd<D, KEYS>;
-  constexpr int NS = C::NS, NT = C::NT;
+  constexpr int NS = C::NS, NT = C::NT, HC = C::HC;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
@@ -488,14 +502,14 @@ __global__ void __launch_bounds__(320, 1)
   uint64_t* y_full = bar + 1;          // [NS]
   uint64_t* y_empty = y_full + NS;     // [NS]
   uint64_t* sd_full = y_empty + NS;    // [2] S and dP of tile t in buffer t & 1
-  uint64_t* pd_full = sd_full + 2;     // [2] P / dS of tile t in TMEM (count 128)
+  uint64_t* pd_full = sd_full + 2;     // [2] P / dS of tile t in TMEM (one arrival per warp of the team)
   uint64_t* acc_full = pd_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(acc_full + 2);
-  const int vlen4 = (vec_len(p) + 3) / 4 * 4;
-  float* vec = reinterpret_cast<float*>(smem + C::OFF_VEC);  // KEYS: one per warpgroup (the head changes along the walk)
+  const int vlen4 = (vec_len(p) + 3) / 4 * 4, dlen = (2 * p.R + 1 + 3) / 4 * 4;
+  float* vec = reinterpret_cast<float*>(smem + C::OFF_VEC);  // KEYS: one per team (the head changes along the walk)
   float* darr = vec + vlen4;                                 // !KEYS: diagonal sums, one array per warp
-  float* dscr = darr + 8 * vlen4;                            // !KEYS: 32 floats per warp
+  float* dscr = darr + 16 * dlen;                            // !KEYS: 16 floats per warp
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int heads = KEYS ? p.Hk : p.H, G = p.H / p.Hk;
@@ -507,7 +521,7 @@ __global__ void __launch_bounds__(320, 1)
   if (threadIdx.x == 0) {
     tc::mbar_init(x_full, 1);
     for (int i = 0; i < NS; ++i) tc::mbar_init(&y_full[i], 1), tc::mbar_init(&y_empty[i], 1);
-    for (int i = 0; i < 2; ++i) tc::mbar_init(&sd_full[i], 1), tc::mbar_init(&pd_full[i], 128);
+    for (int i = 0; i < 2; ++i) tc::mbar_init(&sd_full[i], 1), tc::mbar_init(&pd_full[i], 8);
     tc::mbar_init(acc_full, 1);
     *abort_flag = 0;
     tc::fence_barrier_init();
@@ -528,7 +542,7 @@ __global__ void __launch_bounds__(320, 1)
   } else {
     fill_vec(p, hx, vec, threadIdx.x, C::THREADS);
     if (p.dtab)
-      for (int i = threadIdx.x; i < 8 * vlen4; i += C::THREADS) darr[i] = 0.f;
+      for (int i = threadIdx.x; i < 16 * dlen; i += C::THREADS) darr[i] = 0.f;
     tiles = (trim_end(p, b, key_end(p, min(x0 + C::BX, p.Sq) - 1), C::THREADS) + NT - 1) / NT;
   }
   tc::tc_fence_before();
@@ -609,14 +623,14 @@ __global__ void __launch_bounds__(320, 1)
         if (KEYS) {
 #pragma unroll
           for (int k = 0; k < NT / 16; ++k)  // dV += P^T dO
-            tc::mma_f16_ts(tbase + C::T_ACC, buf + C::T_S + k * 8, tc::sdesc_at(y2, k * 2048), IDESC_G, k > 0 ? 1u : acc0);
+            tc::mma_f16_ts(tbase + C::T_ACC, buf + C::T_S + C::a_col(k), tc::sdesc_at(y2, k * 2048), IDESC_G, k > 0 ? 1u : acc0);
 #pragma unroll
           for (int k = 0; k < NT / 16; ++k)  // dK += dS^T Q
-            tc::mma_f16_ts(tbase + C::T_ACC2, buf + C::T_DP + k * 8, tc::sdesc_at(y1, k * 2048), IDESC_G, k > 0 ? 1u : acc0);
+            tc::mma_f16_ts(tbase + C::T_ACC2, buf + C::T_DP + C::a_col(k), tc::sdesc_at(y1, k * 2048), IDESC_G, k > 0 ? 1u : acc0);
         } else {
 #pragma unroll
           for (int k = 0; k < NT / 16; ++k)  // dQ += dS K
-            tc::mma_f16_ts(tbase + C::T_ACC, buf + C::T_S + k * 8, tc::sdesc_at(y1, k * 2048), IDESC_G, k > 0 ? 1u : acc0);
+            tc::mma_f16_ts(tbase + C::T_ACC, buf + C::T_S + C::a_col(k), tc::sdesc_at(y1, k * 2048), IDESC_G, k > 0 ? 1u : acc0);
         }
         tc::mma_commit(&y_empty[s]);
         if (t + 2 < n && !issue_sd(t + 2)) ok = false;
@@ -625,26 +639,25 @@ __global__ void __launch_bounds__(320, 1)
       else *abort_flag = 1;
     }
   } else {
-    // ---------------- element-wise warpgroups: thread = row of the fixed side ----------------
-    const int g = (warp - 2) >> 2, quarter = warp & 3;
+    // ---------------- element-wise warps: thread = row of the fixed side, half of the tile's columns ----------------
+    const int w16 = warp - 2;                        // 0..15
+    const int g = w16 >> 3, hh = (w16 >> 2) & 1, quarter = warp & 3;
     const int r = quarter * 32 + lane;
+    const int tt = hh * 128 + r;                     // thread of the team, 0..255
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
-    const uint32_t buf = tbase + g * C::T_BUF + lane_off;
+    const uint32_t buf = tbase + g * C::T_BUF + hh * HC + lane_off;  // this warp's columns of S (and, + T_DP, of dP)
     const float sl2 = p.scale * kLog2e;
     const float2 sl22 = make_float2(sl2, sl2);
-    // f16: P carries a factor of 2^8 so that 1 / Sk stays clear of the subnormals; dS does not
+    // f16: P carries a factor of 2^8 (in its bias) so that 1 / Sk stays clear of the subnormals; dS does not
     constexpr float PUP = BF16 ? 0.f : 8.f;
     constexpr float PDOWN = BF16 ? 1.f : 1.f / 256.f;
     float* myvec = KEYS ? vec + g * vlen4 : vec;
-    float* mydarr = darr + (warp - 2) * vlen4;
-    float* myscr = dscr + (warp - 2) * 32;
+    float* mydarr = darr + w16 * dlen + p.R;         // centred on relative position 0
+    float* myscr = dscr + w16 * 16;
     float nL = 0.f, nd = 0.f;  // !KEYS: -(lse log2 e) and -delta of this row
-    bool live = true;          // KEYS: this row's key takes part
     if (!KEYS) {
       const float2 ld = lsed[((int64_t)b * p.H + hx) * sq_pad + x0 + r];
-      nL = -ld.x, nd = -ld.y;
-    } else {
-      live = x0 + r < p.Sk && (p.mask == nullptr || p.mask[(int64_t)b * p.mask_sb + x0 + r] != 0);
+      nL = ld.x, nd = ld.y;
     }
     float far_lo = 0.f, far_hi = 0.f;
     int cur = -1;  // KEYS: the head whose bias is in myvec
@@ -654,172 +667,186 @@ __global__ void __launch_bounds__(320, 1)
       const int gi = KEYS ? t / tiles : 0;
       const int y0 = KEYS ? (first + t - gi * tiles) * NT : t * NT;
       if (KEYS && gi != cur) {
-        tc::named_bar_sync(2 + g, 128);  // nobody still reads the last head's
-        fill_vec(p, hx * G + gi, myvec, r, 128);
-        tc::named_bar_sync(2 + g, 128);
+        tc::named_bar_sync(2 + g, 256);  // nobody still reads the last head's
+        for (int i = tt; i < vec_len(p); i += 256) myvec[i] = bias_at(p, hx * G + gi, i - p.R - kPad) + PUP;
+        tc::named_bar_sync(2 + g, 256);
         cur = gi;
       }
-      uint32_t bits[NT / 32];
+      // after a wait that ran out the tiles are still counted off, so that the team meets at the barriers above
+      if (!ok) continue;
+      uint64_t bits = ~0ull;  // !KEYS: one bit per column of this warp
       bool full = true;
       if (!KEYS) {
-#pragma unroll
-        for (int c = 0; c < NT / 32; ++c) {
-          bits[c] = key_bits(p, b, y0 + c * 32);
-          full = full && bits[c] == 0xffffffffu;
-        }
+        const uint32_t b0 = key_bits(p, b, y0 + hh * HC), b1 = key_bits(p, b, y0 + hh * HC + 32);
+        bits = (uint64_t)b0 | ((uint64_t)b1 << 32);
+        full = (~bits & ((1ull << HC) - 1)) == 0;
       }
       // relative position of column 0 against row 0, and how it moves: -row + column (queries own the rows) or +row - column
       const int rel0 = KEYS ? x0 - y0 - p.q_off : y0 - x0 - p.q_off;
       const bool near = KEYS ? (rel0 - (NT - 1) < p.R && rel0 + 127 > -p.R) : (rel0 - 127 < p.R && rel0 + (NT - 1) > -p.R);
-      const float* bv = myvec + (rel0 + (KEYS ? r : -r) + p.R + kPad);
+      const float* bv = myvec + (rel0 + (KEYS ? r - hh * HC : hh * HC - r) + p.R + kPad);
       const float cst = near ? 0.f : (rel0 > 0 ? myvec[vec_len(p) - 1] : myvec[0]);
-      if (!tc::mbar_wait(&sd_full[g], (uint32_t)(kb & 1), p.err) || *abort_flag) { ok = false; break; }
-      if (KEYS && !tc::mbar_wait(&y_full[t % NS], (uint32_t)((t / NS) & 1), p.err)) { ok = false; break; }
+      if (!tc::mbar_wait(&sd_full[g], (uint32_t)(kb & 1), p.err) || *abort_flag ||
+          (KEYS && !tc::mbar_wait(&y_full[t % NS], (uint32_t)((t / NS) & 1), p.err))) {
+        ok = false;
+        continue;
+      }
       tc::tc_fence_after();
       __syncwarp();
-      const float4* ld4 = reinterpret_cast<const float4*>(smem + C::OFF_Y + (t % NS) * C::STAGE + 2 * C::Y_BYTES);
+      const float4* ld4 = reinterpret_cast<const float4*>(smem + C::OFF_Y + (t % NS) * C::STAGE + 2 * C::Y_BYTES) + hh * (HC / 2);
+      // one straight piece of code for each kind of tile
+      auto walk = [&](auto near_c, auto mask_c) {
+        constexpr bool NEAR = decltype(near_c)::value, MASK = decltype(mask_c)::value;
+        const float2 row_off = make_float2(nL + cst, nL + cst), row_del = make_float2(nd, nd);
 #pragma unroll
-      for (int c = 0; c < NT / 32; ++c) {
-        uint32_t sv[32], dp[32];
-        tc::tmem_ld32(buf + C::T_S + c * 32, sv);
-        tc::tmem_ld32(buf + C::T_DP + c * 32, dp);
-        tc::tmem_wait_ld();
-        tc::reg_fence32(sv);
-        tc::reg_fence32(dp);
-        uint32_t wp[16], wd[16];
+        for (int c = 0; c < HC / 16; ++c) {
+          uint32_t sv[16], dp[16];
+          tc::tmem_ld16(buf + C::T_S + c * 16, sv);
+          tc::tmem_ld16(buf + C::T_DP + c * 16, dp);
+          tc::tmem_wait_ld();
+          tc::reg_fence16(sv);
+          tc::reg_fence16(dp);
+          uint32_t wp[8], wd[8];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int col = c * 32 + 2 * e;
-          float2 off, del;
+          for (int e = 0; e < 8; ++e) {
+            const int col = c * 16 + 2 * e;
+            float2 off = row_off, del = row_del;
+            if (KEYS) {
+              const float4 L = ld4[col >> 1];
+              off = make_float2(L.x, L.z), del = make_float2(L.y, L.w);
+              off = __fadd2_rn(off, NEAR ? make_float2(bv[-col], bv[-col - 1]) : make_float2(cst, cst));
+            } else if (NEAR) {
+              off = __fadd2_rn(off, make_float2(bv[col], bv[col + 1]));
+            }
+            const float2 x = __ffma2_rn(make_float2(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), sl22, off);
+            const float2 pr = make_float2(ex2(x.x), ex2(x.y));
+            float2 dd = __fadd2_rn(make_float2(__uint_as_float(dp[2 * e]), __uint_as_float(dp[2 * e + 1])), del);
+            if (KEYS && !BF16) dd = __fmul2_rn(dd, make_float2(PDOWN, PDOWN));
+            float2 ds = __fmul2_rn(pr, dd);
+            if (MASK) {
+              if (!((bits >> col) & 1ull)) ds.x = 0.f;
+              if (!((bits >> (col + 1)) & 1ull)) ds.y = 0.f;
+            }
+            if (KEYS) wp[e] = pack2<BF16>(pr.x, pr.y);
+            wd[e] = pack2<BF16>(ds.x, ds.y);
+            if (!KEYS) sv[2 * e] = __float_as_uint(ds.x), sv[2 * e + 1] = __float_as_uint(ds.y);
+          }
+          // P over S, dS over dP (KEYS) or over S: 8 columns whose scores this warp has read
           if (KEYS) {
-            const float4 L = ld4[col >> 1];
-            off = make_float2(PUP - L.x, PUP - L.z), del = make_float2(-L.y * PDOWN, -L.w * PDOWN);
+            tc::tmem_st8(buf + C::T_S + c * 8, wp);
+            tc::tmem_st8(buf + C::T_DP + c * 8, wd);
           } else {
-            off = make_float2(nL, nL), del = make_float2(nd, nd);
-          }
-          if (near) off = __fadd2_rn(off, KEYS ? make_float2(bv[-col], bv[-col - 1]) : make_float2(bv[col], bv[col + 1]));
-          else off = __fadd2_rn(off, make_float2(cst, cst));
-          const float2 x = __ffma2_rn(make_float2(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), sl22, off);
-          float2 pr = make_float2(ex2(x.x), ex2(x.y));
-          float2 dd = make_float2(__uint_as_float(dp[2 * e]), __uint_as_float(dp[2 * e + 1]));
-          dd = KEYS ? __ffma2_rn(dd, make_float2(PDOWN, PDOWN), del) : __fadd2_rn(dd, del);
-          float2 ds = __fmul2_rn(pr, dd);
-          if (KEYS) {
-            if (!live) pr = ds = make_float2(0.f, 0.f);
-            wp[e] = pack2<BF16>(pr.x, pr.y);
-          } else if (!full) {
-            if (!((bits[c] >> (2 * e)) & 1u)) ds.x = 0.f;
-            if (!((bits[c] >> (2 * e + 1)) & 1u)) ds.y = 0.f;
-          }
-          wd[e] = pack2<BF16>(ds.x, ds.y);
-          sv[2 * e] = __float_as_uint(ds.x), sv[2 * e + 1] = __float_as_uint(ds.y);
-        }
-        // P over S, dS over dP (KEYS) or over S: columns [16 c, 16 c + 16), whose scores this warp has read
-        if (KEYS) {
-          tc::tmem_st16(buf + C::T_S + c * 16, wp);
-          tc::tmem_st16(buf + C::T_DP + c * 16, wd);
-        } else {
-          tc::tmem_st16(buf + C::T_S + c * 16, wd);
-          if (p.dtab) {
-            const float* dsv = reinterpret_cast<const float*>(sv);
-            if (near) {
-              add_diagonals(dsv, mydarr + (rel0 + c * 32 - quarter * 32 + p.R + kPad), myscr, lane);
-            } else {
-              float s = 0.f;
+            tc::tmem_st8(buf + C::T_S + c * 8, wd);
+            if (p.dtab) {
+              const float* dsv = reinterpret_cast<const float*>(sv);
+              if (NEAR) {
+                add_diagonals(dsv, mydarr, rel0 + hh * HC + c * 16 - quarter * 32, p.R, myscr, lane);
+              } else {
+                float s = 0.f;
 #pragma unroll
-              for (int e = 0; e < 32; ++e) s += dsv[e];
-              if (rel0 > 0) far_hi += s;
-              else far_lo += s;
+                for (int e = 0; e < 16; ++e) s += dsv[e];
+                if (rel0 > 0) far_hi += s;
+                else far_lo += s;
+              }
             }
           }
         }
+      };
+      using yes = std::true_type;
+      using no = std::false_type;
+      if (near) {
+        if (KEYS || full) walk(yes{}, no{});
+        else walk(yes{}, std::integral_constant<bool, !KEYS>{});
+      } else {
+        if (KEYS || full) walk(no{}, no{});
+        else walk(no{}, std::integral_constant<bool, !KEYS>{});
       }
       if (!KEYS && !full && p.mask != nullptr) {
         // masked keys may hold anything, and 0 * NaN is NaN in the dS K product: clear their rows of K
-        if (r < NT && !((bits[quarter < NT / 32 ? quarter : 0] >> lane) & 1u)) {
+        for (int i = lane; i < HC; i += 32)
+          if (!((bits >> i) & 1ull) && quarter < 2 * C::DCH) {
+            // the four warps of this column half share the work: 64 bytes of a row each
+            uint4* row = reinterpret_cast<uint4*>(smem + C::OFF_Y + (t % NS) * C::STAGE + (quarter >> 1) * (NT * 128) +
+                                                  (hh * HC + i) * 128 + (quarter & 1) * 64);
 #pragma unroll
-          for (int c = 0; c < C::DCH; ++c) {
-            uint4* row = reinterpret_cast<uint4*>(smem + C::OFF_Y + (t % NS) * C::STAGE + c * (NT * 128) + r * 128);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) row[i] = make_uint4(0u, 0u, 0u, 0u);
+            for (int j = 0; j < 4; ++j) row[j] = make_uint4(0u, 0u, 0u, 0u);
           }
-        }
         tc::fence_async_shared();
-        __syncwarp();
       }
       tc::tmem_wait_st();
       tc::tc_fence_before();
-      tc::mbar_arrive(&pd_full[g]);
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&pd_full[g]);
     }
     if (!KEYS && p.dtab) {
       // this warp's far tiles join the ends of its array; then the arrays are added and cut into buckets
       const float lo = warp_sum(far_lo), hi = warp_sum(far_hi);
-      if (lane == 0) mydarr[0] += lo, mydarr[vec_len(p) - 1] += hi;
-      tc::named_bar_sync(1, 256);
-      const int ew = (int)threadIdx.x - 64;
-      for (int i = ew; i < vec_len(p); i += 256) {
+      if (lane == 0) mydarr[-p.R] += lo, mydarr[p.R] += hi;
+      tc::named_bar_sync(1, C::EW);
+      for (int i = (int)threadIdx.x - 64; i < 2 * p.R + 1; i += C::EW) {
         float s = 0.f;
 #pragma unroll
-        for (int w = 0; w < 8; ++w) s += darr[w * vlen4 + i];
+        for (int w = 0; w < 16; ++w) s += darr[w * dlen + i];
         vec[i] = s;  // the bias itself is no longer needed
       }
-      tc::named_bar_sync(1, 256);
-      // bucket nb of a side holds the distances [thr[nb - 1], thr[nb]), the last one all beyond
-      for (int bk = warp - 2; bk < p.nb; bk += 8) {
+      tc::named_bar_sync(1, C::EW);
+      // bucket i of a side holds the distances [thr[i - 1], thr[i]), the last one all beyond
+      for (int bk = w16; bk < p.nb; bk += 16) {
         const int side = p.bidir ? p.nb / 2 : p.nb;
         const bool pos = p.bidir && bk >= side;
         const int i = pos ? bk - side : bk;
-        int d0 = i == 0 ? 0 : (int)p.thr[i - 1], d1 = i == side - 1 ? p.R + kPad + 1 : (int)p.thr[i];
+        int d0 = i == 0 ? 0 : (int)p.thr[i - 1];
+        const int d1 = i == side - 1 ? p.R + 1 : (int)p.thr[i];
         float s = 0.f;
         if (pos) {
           d0 = max(d0, 1);
-          for (int d = d0 + lane; d < d1; d += 32) s += vec[d + p.R + kPad];
+          for (int d = d0 + lane; d < d1; d += 32) s += vec[p.R + d];
         } else {
-          for (int d = d0 + lane; d < d1; d += 32) s += vec[p.R + kPad - d];
+          for (int d = d0 + lane; d < d1; d += 32) s += vec[p.R - d];
           if (!p.bidir && i == 0)  // one-sided: keys after the query share bucket 0
-            for (int d = 1 + lane; d <= p.R + kPad; d += 32) s += vec[d + p.R + kPad];
+            for (int d = 1 + lane; d <= p.R; d += 32) s += vec[p.R + d];
         }
         s = warp_sum(s);
         if (lane == 0) p.dtab[((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * p.nb + bk] = s;
       }
     }
-    // ---------------- epilogue: group g writes its half of the columns ----------------
+    // ---------------- epilogue: a warp writes 32 rows x 32 columns of a gradient at a time ----------------
     if (ok && n > 0) ok = tc::mbar_wait(acc_full, 0, p.err);
     if (ok && !*abort_flag) {
       tc::tc_fence_after();
       const int rows = KEYS ? p.Sk : p.Sq;
+      // a masked key's row of the sums holds whatever its K and V gave: its gradient is zero
+      const bool live = !KEYS || (x0 + r < p.Sk && (p.mask == nullptr || p.mask[(int64_t)b * p.mask_sb + x0 + r] != 0));
+      constexpr int CH = D / 32, JOBS = (KEYS ? 2 : 1) * CH;
       // staging in the idle Y ring: every MMA that read it is done
-      uint8_t* stg = smem + C::OFF_Y + (warp - 2) * (KEYS ? 2 : 1) * C::DCH * 2048;
-#pragma unroll
-      for (int which = 0; which < (KEYS ? 2 : 1); ++which) {  // KEYS: dV, then dK
+      uint8_t* stg = smem + C::OFF_Y + w16 * 4096;
+      int use = 0;
+      for (int job = w16 >> 2; job < JOBS; job += 4, ++use) {
+        const int which = job / CH, c = job % CH;  // KEYS: dV, then dK
         const bool wanted = KEYS ? (which ? p.dk != nullptr : p.dv != nullptr) : p.dq != nullptr;
         if (!wanted) continue;
         const float mul = KEYS ? (which ? p.scale : PDOWN) : p.scale;
         const CUtensorMap* tm = which ? &tmG2 : &tmG1;
+        uint32_t v[32], w[16];
+        __syncwarp();
+        if (n > 0) {
+          tc::tmem_ld32(tbase + (which ? C::T_ACC2 : C::T_ACC) + c * 32 + lane_off, v);
+          tc::tmem_wait_ld();
+          tc::reg_fence32(v);
+        }
 #pragma unroll
-        for (int cc = 0; cc < C::DCH; ++cc) {
-          const int c = g * C::DCH + cc;
-          uint32_t v[32], w[16];
-          __syncwarp();
-          if (n > 0) {
-            tc::tmem_ld32(tbase + (which ? C::T_ACC2 : C::T_ACC) + c * 32 + lane_off, v);
-            tc::tmem_wait_ld();
-            tc::reg_fence32(v);
-          }
+        for (int e = 0; e < 16; ++e)
+          w[e] = n > 0 && live ? pack2<BF16>(__uint_as_float(v[2 * e]) * mul, __uint_as_float(v[2 * e + 1]) * mul) : 0u;
+        uint8_t* sb = stg + (use & 1) * 2048;  // at most two jobs a warp
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            w[e] = n > 0 ? pack2<BF16>(__uint_as_float(v[2 * e]) * mul, __uint_as_float(v[2 * e + 1]) * mul) : 0u;
-          uint8_t* sb = stg + (which * C::DCH + cc) * 2048;
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            *reinterpret_cast<uint4*>(sb + lane * 64 + ((e ^ ((lane >> 1) & 3)) << 4)) =
-                make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
-          tc::fence_async_shared();
-          __syncwarp();
-          if (lane == 0 && x0 + quarter * 32 < rows && c * 32 < p.D) {
-            tc::tma_store_4d(tm, sb, c * 32, x0 + quarter * 32, hx, b);
-            tc::bulk_commit();
-          }
+        for (int e = 0; e < 4; ++e)
+          *reinterpret_cast<uint4*>(sb + lane * 64 + ((e ^ ((lane >> 1) & 3)) << 4)) =
+              make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+        tc::fence_async_shared();
+        __syncwarp();
+        if (lane == 0 && x0 + quarter * 32 < rows && c * 32 < p.D) {
+          tc::tma_store_4d(tm, sb, c * 32, x0 + quarter * 32, hx, b);
+          tc::bulk_commit();
         }
       }
       if (lane == 0) tc::bulk_wait0();
@@ -837,7 +864,7 @@ __global__ void __launch_bounds__(320, 1)
   }
 }
 
-// lsed[bh][q] = (lse log2 e, sum_d dO O) for q < Sq, (+inf, 0) for padding and for rows without a key: exp2(x - inf) = 0.
+// lsed[bh][q] = (-lse log2 e, -sum_d dO O) for q < Sq, (-inf, 0) for padding and for rows without a key: exp2(x - inf) = 0.
 // Eight lanes a row, 16-byte loads.
 template <typename T>
 __global__ void __launch_bounds__(256) bias_bwd_prep(const __grid_constant__ Params p, float2* __restrict__ lsed, int sq_pad) {
@@ -876,7 +903,7 @@ __global__ void __launch_bounds__(256) bias_bwd_prep(const __grid_constant__ Par
   s += __shfl_xor_sync(m, s, 4);
   if (part == 0) {
     const float lse = q < p.Sq ? p.lse[bh * p.Sq + q] : -INFINITY;
-    lsed[idx] = lse == -INFINITY ? make_float2(INFINITY, 0.f) : make_float2(lse * kLog2e, s);
+    lsed[idx] = lse == -INFINITY ? make_float2(-INFINITY, 0.f) : make_float2(-lse * kLog2e, -s);
   }
 }
 
@@ -919,7 +946,8 @@ int fwd_t(const Params& p, cudaStream_t st) {
 template <int D, bool KEYS>
 int bwd_smem(const Params& p) {
   const int vb = vec_bytes(p);
-  return Bwd<D, KEYS>::OFF_VEC + (KEYS ? 2 * vb : vb + (p.dtab ? 8 * vb + 8 * 128 : 0)) + 1024;
+  const int db = (2 * p.R + 1 + 3) / 4 * 16;
+  return Bwd<D, KEYS>::OFF_VEC + (KEYS ? 2 * vb : vb + (p.dtab ? 16 * db + 16 * 64 : 0)) + 1024;
 }
 
 template <int D, bool BF16, bool KEYS>
