@@ -3,6 +3,7 @@
 #include <cmath>
 
 #include "bias_attn.cuh"
+#include "tc_ptx.cuh"
 
 namespace b2 {
 namespace bias_attn {
@@ -31,38 +32,46 @@ bool bucket_args_ok(int32_t nb, int32_t max_distance, int32_t bidir) {
          max_distance <= B2_BIAS_MAX_DISTANCE;
 }
 
-// O = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s over the key splits, one warp per query row.
+// O = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s over the key splits, one block of four warps per query row: each warp
+// adds up every fourth split, four of them in flight, and the four sums are added in order.
 template <typename T>
-__global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ Params p) {
+  __shared__ float so[4][128], sl[4];
   const int64_t nrow = (int64_t)p.B * p.H * p.Sq;
-  const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (row >= nrow) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = blockIdx.x;
+  tc::pdl_wait();
   float M = -INFINITY;
   for (int s = lane; s < p.nsplit; s += 32) M = fmaxf(M, p.part_ml[s * nrow + row].x);
   M = warp_max(M);
   const float ref = M == -INFINITY ? 0.f : M;
   float acc[4] = {}, l = 0.f;
-  for (int s = 0; s < p.nsplit; ++s) {
+#pragma unroll 4
+  for (int s = warp; s < p.nsplit; s += 4) {
     const float2 ml = p.part_ml[s * nrow + row];
     const float w = exp2f(ml.x - ref);
-    if (w == 0.f) continue;
     l = fmaf(ml.y, w, l);
     const float* po = p.part_o + (s * nrow + row) * p.D;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (lane + 32 * i < p.D) acc[i] = fmaf(po[lane + 32 * i], w, acc[i]);
-  }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  const int64_t i = row % p.Sq, bh = row / p.Sq;
-  T* o = row_of<T>(p.o, p.o_s, (int)(bh / p.H), (int)(bh % p.H), i);
-#pragma unroll
-  for (int c = 0; c < 4; ++c)
-    if (lane + 32 * c < p.D) {
-      o[lane + 32 * c] = from_f32<T>(acc[c] * inv);
-      if (p.o32) p.o32[row * p.D + lane + 32 * c] = acc[c] * inv;
+    for (int i = 0; i < 4; ++i) {
+      const float o = lane + 32 * i < p.D ? po[lane + 32 * i] : 0.f;
+      acc[i] = fmaf(o, w, acc[i]);
     }
-  if (lane == 0 && p.lse) p.lse[row] = l > 0.f ? (M + log2f(l)) * kLn2 : -INFINITY;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) so[warp][lane + 32 * i] = acc[i];
+  if (lane == 0) sl[warp] = l;
+  __syncthreads();
+  const float L = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+  const float inv = L > 0.f ? 1.f / L : 0.f;
+  const int64_t i = row % p.Sq, bh = row / p.Sq;
+  const int d = threadIdx.x;
+  if (d < p.D) {
+    const float o = ((so[0][d] + so[1][d]) + (so[2][d] + so[3][d])) * inv;
+    row_of<T>(p.o, p.o_s, (int)(bh / p.H), (int)(bh % p.H), i)[d] = from_f32<T>(o);
+    if (p.o32) p.o32[row * p.D + d] = o;
+  }
+  if (d == 0 && p.lse) p.lse[row] = L > 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
 }
 
 // delta[row] = sum_d dO * O, one warp per row.
@@ -140,7 +149,7 @@ int check(const b2_bias_attn_args* a, bool bwd) {
 }
 
 struct Plan {
-  bool tc = false;
+  bool tc = false, rows = false;
   int nsplit = 1;
   int ntq = 0;               // query tiles of the bias-gradient partial sums
   int sq_pad = 0;            // tensor-core backward: rows of (lse, delta) per head
@@ -171,19 +180,28 @@ Plan make_plan(const b2_bias_attn_args* a, bool bwd) {
   pl.tc = bwd ? tc_bwd_eligible(a) : tc_fwd_eligible(a);
   const int tile = pl.tc ? kTcTile : kSimtTile;
   const int64_t tq = (a->Sq + tile - 1) / tile, tk = (a->Sk + tile - 1) / tile;
-  if (!bwd) {
-    pl.nsplit = pick_splits(tq * a->B * a->H, tk, rows * a->D, pl.tc ? 0.4 : 6.0);
-    if (pl.nsplit > 1) {
-      pl.part_o = 0;
-      pl.part_ml = up16((uint64_t)pl.nsplit * rows * a->D * 4);
-      pl.bytes = pl.part_ml + up16((uint64_t)pl.nsplit * rows * 8);
+  if (!bwd && rows_eligible(a)) {
+    // few query rows: blocks of 128 threads, about six to an SM; a block costs its keys and about 96 keys' worth of set-up
+    pl.rows = true;
+    const int64_t blocks = a->B * a->Hk, sms = device_info().sm_count > 0 ? device_info().sm_count : 148;
+    int64_t best = INT64_MAX;
+    for (int64_t ns = 1; ns <= std::max<int64_t>(1, std::min<int64_t>(a->Sk / 64, 128)); ++ns) {
+      const int64_t cost = (blocks * ns + sms * 6 - 1) / (sms * 6) * ((a->Sk + ns - 1) / ns + 96) + (ns > 1 ? 64 + 4 * ns : 0);
+      if (cost < best) best = cost, pl.nsplit = (int)ns;
     }
+  } else if (!bwd) {
+    pl.nsplit = pick_splits(tq * a->B * a->H, tk, rows * a->D, pl.tc ? 0.4 : 6.0);
   } else {
     pl.ntq = (int)tq;
     pl.delta = 0;
     pl.sq_pad = (int)((a->Sq + kTcPad - 1) / kTcPad * kTcPad);
     pl.dtab = pl.tc ? (uint64_t)(a->B * a->H) * pl.sq_pad * 8 : up16((uint64_t)rows * 4);
     pl.bytes = pl.dtab + (a->dtable ? up16((uint64_t)(a->B * a->H * tq) * a->num_buckets * 4) : 0);
+  }
+  if (pl.nsplit > 1) {
+    pl.part_o = 0;
+    pl.part_ml = up16((uint64_t)pl.nsplit * rows * a->D * 4);
+    pl.bytes = pl.part_ml + up16((uint64_t)pl.nsplit * rows * 8);
   }
   return pl;
 }
@@ -221,12 +239,7 @@ int by_dtype(int dt, A&&... args) {
 template <typename T>
 struct Combine {
   static int run(const Params& p, cudaStream_t st) {
-    const int64_t rows = (int64_t)p.B * p.H * p.Sq;
-    {
-      LaunchScope ls("bias_attn_combine", st);
-      combine_kernel<T><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(p);
-    }
-    return after_launch("bias_attn_combine");
+    return launch_pdl("bias_attn_combine", combine_kernel<T>, dim3((unsigned)(p.B * p.H * (int64_t)p.Sq)), dim3(128), 0, st, p);
   }
 };
 template <typename T>
@@ -284,7 +297,8 @@ extern "C" int b2_bias_attn_fwd(const b2_bias_attn_args* a, b2_stream_t stream) 
   p.nsplit = pl.nsplit;
   p.part_o = (float*)((char*)a->workspace + pl.part_o);
   p.part_ml = (float2*)((char*)a->workspace + pl.part_ml);
-  if (int rc = pl.tc ? tc_fwd(p, a->dtype == B2_BF16, st) : simt_fwd(p, a->dtype, st)) return rc;
+  if (int rc = pl.rows ? rows_fwd(p, a->dtype, st) : pl.tc ? tc_fwd(p, a->dtype == B2_BF16, st) : simt_fwd(p, a->dtype, st))
+    return rc;
   return p.nsplit > 1 ? by_dtype<Combine>(a->dtype, p, st) : 0;
 }
 
