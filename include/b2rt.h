@@ -435,7 +435,8 @@ int64_t b2_mx4_scale_bytes(int64_t rows, int64_t cols);
 
 /* Linear over a frozen MXFP4 weight W [N][K], with the LoRA side path as one more term of the same product.
  *   transpose_w == 0 (forward): out[M][N] = A W^T + bias[N] + lora_h[M][r] lora_b[N][r]^T, A an MXFP4 matrix [M][K]
- *                               (x_codes, x_scales); the element products are exact, the sums fp32;
+ *                               (x_codes, x_scales), or, where b2_mx4_takes_x(M, N, K) says so (few rows), x bf16 [M][K],
+ *                               quantised in the same launch; the element products are exact, the sums fp32;
  *   transpose_w == 1 (dX):      out[M][K] = x[M][N] W + lora_h[M][r] lora_b[r][K], x bf16 (the straight-through
  *                               gradient of the quantised activation).
  * out is bf16 with row stride out_ld, bias bf16. lora_r = 0: no side path; else 8..64, a multiple of 8, bf16 rows
@@ -444,7 +445,7 @@ int64_t b2_mx4_scale_bytes(int64_t rows, int64_t cols);
 typedef struct b2_mx4_gemm_args {
   const uint8_t* x_codes; /* forward */
   const uint8_t* x_scales;
-  const void* x;          /* dX */
+  const void* x;          /* dX; forward of few rows (then x_codes and x_scales are not read) */
   const uint8_t* w_codes;
   const uint8_t* w_scales;
   const void* bias;       /* NULL: none (forward only) */
@@ -458,6 +459,7 @@ typedef struct b2_mx4_gemm_args {
   int32_t transpose_w;
 } b2_mx4_gemm_args;
 int b2_mx4_gemm(const b2_mx4_gemm_args* args, b2_stream_t stream);
+int b2_mx4_takes_x(int64_t M, int64_t N, int64_t K);
 uint64_t b2_mx4_gemm_workspace_bytes(const b2_mx4_gemm_args* args);
 
 /* ------------------------------------------------------------------------------------------ */

@@ -168,6 +168,44 @@ def test_lora_forward_and_gradients(m, k, n, r):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 7, 8, 9])
+@pytest.mark.parametrize("k,n", [(2048, 700), (40, 33), (4096, 130), (9000, 64)])
+def test_few_rows(m, k, n):
+    """One to nine rows (the weight-stream kernel and the first size past it), with bias, LoRA and strided rows."""
+    import torch_vulkan_b200 as tv
+
+    x, w, bias, _, a, b = _linear_case(m, k, n, m * 7 + k + n, 16)
+    xq, wq = ot.mx4_round(x), ot.mx4_round(w)
+    wd = tv.mx4_quantize(w.cuda())
+    h = x.double() @ a.double().t()
+    ref = xq @ wq.t() + bias.double()
+    _close(tv.mx4_linear(x.cuda(), wd, bias.cuda()), ref, xq.abs() @ wq.abs().t() + bias.double().abs())
+    _close(tv.mx4_lora_linear(x.cuda(), wd, bias.cuda(), a.cuda(), b.cuda()), ref + h @ b.double().t(),
+           xq.abs() @ wq.abs().t() + (x.double().abs() @ a.double().abs().t()) @ b.double().abs().t(), h.abs() @ b.double().abs().t())
+    wide = torch.randn(m, k + 3).to(BF).cuda()
+    assert torch.equal(tv.mx4_linear(wide[:, 3:], wd), tv.mx4_linear(wide[:, 3:].contiguous(), wd))
+
+
+@pytest.mark.gpu
+def test_few_rows_extreme_scales():
+    """Blocks with scales from 2^-120 to 2^100, zero blocks and a NaN row."""
+    import torch_vulkan_b200 as tv
+
+    g = torch.Generator().manual_seed(1)
+    x, w = torch.randn(3, 256, generator=g), torch.randn(50, 256, generator=g)
+    e = torch.randint(-60, 50, (1, 8), generator=g).float()
+    x *= torch.exp2(e).repeat_interleave(32, 1)
+    w *= torch.exp2(-e - 3).repeat_interleave(32, 1)
+    w[:, 64:96] = 0
+    x, w = x.to(BF), w.to(BF)
+    x[1, 7] = float("nan")
+    y = tv.mx4_linear(x.cuda(), tv.mx4_quantize(w.cuda()))
+    assert torch.isnan(y[1]).all()
+    xq, wq = ot.mx4_round(x)[[0, 2]], ot.mx4_round(w)
+    _close(y[[0, 2]], xq @ wq.t(), xq.abs() @ wq.abs().t())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("m,k,n,r", [(2100, 288, 2500, 24), (2100, 2500, 288, 16), (4096, 160, 1300, 8)])
 def test_many_tiles(m, k, n, r):
     """Enough 256 x 256 tiles for CTA pairs, ragged in every direction, several tiles a pair."""

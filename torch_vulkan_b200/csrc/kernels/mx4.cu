@@ -4,51 +4,12 @@
 // A block's scale is 2^(floor(log2(amax)) - 2): with the fp32 exponent field e of amax that is the E8M0 code
 // max(e - 2, 0), and multiplying by 2^(127 - code) divides exactly. The E2M1 rounding (nearest, ties to even,
 // saturating) is the cvt.rn.satfinite.e2m1x2 instruction; reading back is one exact product per element.
-#include "common.cuh"
+#include "mx4.cuh"
 
 namespace b2 {
 namespace {
 
-constexpr int kBlk = 32;  // columns per scale
-
-// Byte of the scale of (row, block of 32 columns) in the tiled scale array (see b2_mx4_args).
-__host__ __device__ __forceinline__ int64_t scale_at(int64_t row, int64_t blk, int64_t nkb) {
-  return ((row >> 7) * nkb + (blk >> 2)) * 512 + (row & 31) * 16 + ((row & 127) >> 5) * 4 + (blk & 3);
-}
-
-__device__ __forceinline__ float e8m0_to_f32(uint32_t code) {
-  if (code == 255u) return __uint_as_float(0x7FC00000u);
-  return code ? __uint_as_float(code << 23) : __uint_as_float(0x00400000u);  // code 0: 2^-127
-}
-
-// Eight floats -> eight E2M1 codes, element 0 in the lowest nibble.
-__device__ __forceinline__ uint32_t e2m1x8(const float* v) {
-  uint32_t r;
-  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
-      "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
-      : "=r"(r)
-      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
-  return r;
-}
-
-// Eight codes -> four half2 (exact: every E2M1 value is a half).
-__device__ __forceinline__ void e2m1x8_to_half2(uint32_t c, __half2* h) {
-  uint32_t o[4];
-  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
-      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
-      : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3])
-      : "r"(c));
-#pragma unroll
-  for (int i = 0; i < 4; ++i) h[i] = *reinterpret_cast<__half2*>(&o[i]);
-}
+using namespace mx4;
 
 // Eight consecutive elements at p as floats; `n` (< 8 at a ragged end) of them exist.
 template <typename T, bool VEC>
@@ -104,10 +65,9 @@ __global__ void __launch_bounds__(256) mx4_quantize_k(const T* __restrict__ x, u
     uint32_t b = bad ? 1u : 0u;
     b |= __shfl_xor_sync(0xffffffffu, b, 1);
     b |= __shfl_xor_sync(0xffffffffu, b, 2);
-    const int e = (int)(__float_as_uint(am) >> 23);
-    const uint32_t code = b ? 255u : (uint32_t)max(e - 2, 0);
+    const uint32_t code = scale_code(am, b != 0);
     if (row < rows && c0 < cb * 2) {
-      const float inv = b ? 0.f : __uint_as_float((254u - code) << 23);
+      const float inv = inverse_scale(code);
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[k] = b ? 0.f : v[k] * inv;
       *reinterpret_cast<uint32_t*>(codes + row * cb + g * 4) = e2m1x8(v);
@@ -237,6 +197,8 @@ namespace b2 {
 
 bool mx4_gemm_tc_eligible(const b2_mx4_gemm_args* a);  // mx4_gemm.cu
 int mx4_gemm_fwd(const b2_mx4_gemm_args* a, cudaStream_t st);
+bool mx4_rows_eligible(const b2_mx4_gemm_args* a);     // mx4_rows.cu
+int mx4_rows(const b2_mx4_gemm_args* a, cudaStream_t st);
 int mx4_gemm_dx(const b2_mx4_gemm_args* a, const void* x, int64_t x_ld, const void* w, int64_t w_ld, cudaStream_t st);
 
 namespace {
@@ -254,12 +216,14 @@ int gemm_check(const b2_mx4_gemm_args* a) {
   if (!a) return fail(B2_ERR_ARG, "mx4_gemm: null arguments");
   if (a->M < 0 || a->N < 0 || a->K < 0) return fail(B2_ERR_ARG, "mx4_gemm: negative size");
   if (a->M == 0 || a->N == 0 || a->K == 0) return 0;
-  if (!a->w_codes || !a->w_scales || !a->out || (a->transpose_w ? !a->x : (!a->x_codes || !a->x_scales)))
+  if (!a->w_codes || !a->w_scales || !a->out || (a->transpose_w ? !a->x : !a->x && (!a->x_codes || !a->x_scales)))
     return fail(B2_ERR_ARG, "mx4_gemm: null pointer");
   if (((uintptr_t)a->w_codes | (uintptr_t)a->w_scales | (uintptr_t)a->x_codes | (uintptr_t)a->x_scales) & 15)
     return fail(B2_ERR_ARG, "mx4_gemm: codes and scales must be 16-byte aligned");
   if (a->out_ld < (a->transpose_w ? a->K : a->N)) return fail(B2_ERR_ARG, "mx4_gemm: out_ld smaller than a row");
-  if (a->transpose_w && a->x_ld < a->N) return fail(B2_ERR_ARG, "mx4_gemm: x_ld smaller than a row");
+  if (a->x && a->x_ld < (a->transpose_w ? a->N : a->K)) return fail(B2_ERR_ARG, "mx4_gemm: x_ld smaller than a row");
+  if (!a->transpose_w && a->x && !mx4_rows_eligible(a))
+    return fail(B2_ERR_ARG, "mx4_gemm: a forward with this many values of x takes them quantised");
   if (a->lora_r) {
     if (a->lora_r < 8 || a->lora_r > 64 || a->lora_r % 8 || !a->lora_h || !a->lora_b || a->lora_h_ld % 8 || a->lora_b_ld % 8 ||
         (((uintptr_t)a->lora_h | (uintptr_t)a->lora_b) & 15))
@@ -285,6 +249,12 @@ DxPlan dx_plan(const b2_mx4_gemm_args* a) {
 }  // namespace
 }  // namespace b2
 
+extern "C" int b2_mx4_takes_x(int64_t M, int64_t N, int64_t K) {
+  b2_mx4_gemm_args a{};
+  a.M = M, a.N = N, a.K = K, a.x = &a;
+  return b2::mx4_rows_eligible(&a) ? 1 : 0;
+}
+
 extern "C" uint64_t b2_mx4_gemm_workspace_bytes(const b2_mx4_gemm_args* a) {
   using namespace b2;
   if (!a || a->M <= 0 || a->N <= 0 || a->K <= 0 || !a->transpose_w) return 0;
@@ -298,7 +268,7 @@ extern "C" int b2_mx4_gemm(const b2_mx4_gemm_args* a, b2_stream_t stream) {
   if (int rc = ensure_init()) return rc;
   cudaStream_t st = (cudaStream_t)stream;
   if (!mx4_gemm_tc_eligible(a)) return fail(B2_ERR_ARG, "mx4_gemm: sizes beyond 2^30, or no sm_100a device");
-  if (!a->transpose_w) return mx4_gemm_fwd(a, st);
+  if (!a->transpose_w) return a->x ? mx4_rows(a, st) : mx4_gemm_fwd(a, st);
   if (!a->workspace || ((uintptr_t)a->workspace & 15))
     return fail(B2_ERR_ARG, "mx4_gemm: a 16-byte aligned workspace of b2_mx4_gemm_workspace_bytes() is required");
   const DxPlan d = dx_plan(a);

@@ -126,9 +126,14 @@ at::Tensor mx4_fwd(const at::Tensor& x0, const at::Tensor& codes, const at::Tens
   if (out.numel() == 0) return out;
   TORCH_CHECK(K > 0, name, ": no input features");
   at::Tensor x = rows_of(x0);
-  auto [xc, xs] = mx4_quantize(x);
   b2_mx4_gemm_args g{};
-  g.x_codes = xc.data_ptr<uint8_t>(), g.x_scales = xs.data_ptr<uint8_t>();
+  at::Tensor xc, xs;
+  if (b2_mx4_takes_x(x.size(0), N, K)) {
+    g.x = x.data_ptr(), g.x_ld = K;
+  } else {
+    std::tie(xc, xs) = mx4_quantize(x);
+    g.x_codes = xc.data_ptr<uint8_t>(), g.x_scales = xs.data_ptr<uint8_t>();
+  }
   g.w_codes = codes.data_ptr<uint8_t>(), g.w_scales = scales.data_ptr<uint8_t>();
   g.bias = bias.defined() ? bias.data_ptr() : nullptr;
   g.out = out.data_ptr();
