@@ -30,71 +30,89 @@ __device__ __forceinline__ void load8(const T* p, int n, float* v) {
   }
 }
 
+// Both kernels walk a grid of (8-column groups) x (rows): a block is TX groups wide and 256 / TX rows high, and each thread
+// takes kU rows of its column, whose loads are in flight together. No division per element, and no two threads of a
+// warp further apart than its columns.
+constexpr int kU = 4;
+
 // Four lanes own a block of 32 columns, eight columns each. The grid covers the padded scale array (rows to a
 // multiple of 128, blocks to a multiple of 4), whose padding is written as zeros here.
 // VEC: every 8-column group that exists is whole and 16-byte aligned.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) mx4_quantize_k(const T* __restrict__ x, uint8_t* __restrict__ codes,
                                                       uint8_t* __restrict__ scales, int64_t rows, int64_t cols,
-                                                      int64_t x_ld, int64_t nkb) {
-  const int64_t groups = nkb * 16;  // 8-column groups per padded row
-  const int64_t total = (rows + 127) / 128 * 128 * groups;
+                                                      int64_t ld, int64_t nkb, int txl) {
+  const int64_t groups = nkb * 16;  // 8-column groups per padded row, a multiple of 16: quads of lanes are whole
+  const int64_t g = ((int64_t)blockIdx.y << txl) + (threadIdx.x & ((1 << txl) - 1));
   const int64_t cb = (cols + kBlk - 1) / kBlk * 16;  // code bytes per row
-  // total is a multiple of 32, so whole warps leave the loop together
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / groups, g = i - row * groups;
-    const int64_t c0 = g * 8;
-    float v[8];
-    float am = 0.f;
-    bool bad = false;
-    const bool in = row < rows && c0 < cols;
-    if (in) {
-      load8<T, VEC>(x + row * x_ld + c0, (int)min((int64_t)8, cols - c0), v);
+  const int64_t c0 = g * 8;
+  const int64_t row0 = ((int64_t)blockIdx.x * (256 >> txl) + (threadIdx.x >> txl)) * kU;
+  const int n = (int)max((int64_t)0, min((int64_t)8, cols - c0));
+  float v[kU][8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float a = fabsf(v[k]);
-        bad |= !(a <= 3.402823466e38f);
-        am = fmaxf(am, a);
-      }
+  for (int u = 0; u < kU; ++u) {
+    if (row0 + u < rows && n > 0) {
+      load8<T, VEC>(x + (row0 + u) * ld + c0, n, v[u]);
     } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = 0.f;
+      for (int k = 0; k < 8; ++k) v[u][k] = 0.f;
     }
+  }
+#pragma unroll
+  for (int u = 0; u < kU; ++u) {
+    const int64_t row = row0 + u;
+    float am = 0.f;
+    bool bad = false;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float a = fabsf(v[u][k]);
+      bad |= !(a <= 3.402823466e38f);
+      am = fmaxf(am, a);
+    }
+    am = bad ? INFINITY : am;  // the block's maximum carries the mark
     am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 1));
     am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 2));
-    uint32_t b = bad ? 1u : 0u;
-    b |= __shfl_xor_sync(0xffffffffu, b, 1);
-    b |= __shfl_xor_sync(0xffffffffu, b, 2);
-    const uint32_t code = scale_code(am, b != 0);
+    const uint32_t code = scale_code(am, am == INFINITY);
     if (row < rows && c0 < cb * 2) {
       const float inv = inverse_scale(code);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = b ? 0.f : v[k] * inv;
-      *reinterpret_cast<uint32_t*>(codes + row * cb + g * 4) = e2m1x8(v);
+      for (int k = 0; k < 8; ++k) v[u][k] = code == 255u ? 0.f : v[u][k] * inv;
+      *reinterpret_cast<uint32_t*>(codes + row * cb + g * 4) = e2m1x8(v[u]);
     }
-    if ((g & 3) == 0) scales[scale_at(row, g >> 2, nkb)] = (row < rows && c0 < cols) ? (uint8_t)code : (uint8_t)0;
+    if ((g & 3) == 0 && g < groups && row < (rows + 127) / 128 * 128)
+      scales[scale_at(row, g >> 2, nkb)] = (row < rows && c0 < cols) ? (uint8_t)code : (uint8_t)0;
   }
 }
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) mx4_dequantize_k(const uint8_t* __restrict__ codes,
                                                         const uint8_t* __restrict__ scales, T* __restrict__ out,
-                                                        int64_t rows, int64_t cols, int64_t ld, int64_t nkb) {
-  const int64_t groups = (cols + 7) / 8;
+                                                        int64_t rows, int64_t cols, int64_t ld, int64_t nkb, int txl) {
+  const int64_t g = ((int64_t)blockIdx.y << txl) + (threadIdx.x & ((1 << txl) - 1));
   const int64_t cb = (cols + kBlk - 1) / kBlk * 16;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * groups; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / groups, g = i - row * groups;
-    const uint32_t c = *reinterpret_cast<const uint32_t*>(codes + row * cb + g * 4);
-    const float s = e8m0_to_f32(scales[scale_at(row, g >> 2, nkb)]);
+  const int64_t row0 = ((int64_t)blockIdx.x * (256 >> txl) + (threadIdx.x >> txl)) * kU;
+  const int n = (int)max((int64_t)0, min((int64_t)8, cols - g * 8));
+  if (n == 0) return;
+  uint32_t c[kU], sc[kU];
+#pragma unroll
+  for (int u = 0; u < kU; ++u) {
+    const int64_t row = min(row0 + u, rows - 1);
+    c[u] = *reinterpret_cast<const uint32_t*>(codes + row * cb + g * 4);
+    sc[u] = scales[scale_at(row, g >> 2, nkb)];
+  }
+#pragma unroll
+  for (int u = 0; u < kU; ++u) {
+    if (row0 + u >= rows) break;
+    const float s = e8m0_to_f32(sc[u]);
     __half2 h[4];
-    e2m1x8_to_half2(c, h);
+    e2m1x8_to_half2(c[u], h);
     float v[8];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const float2 f = __half22float2(h[k]);
       v[2 * k] = f.x * s, v[2 * k + 1] = f.y * s;
     }
-    T* o = out + row * ld + g * 8;
+    T* o = out + (row0 + u) * ld + g * 8;
     if (VEC) {
       if constexpr (sizeof(T) == 4) {
         *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
@@ -107,24 +125,37 @@ __global__ void __launch_bounds__(256) mx4_dequantize_k(const uint8_t* __restric
         *reinterpret_cast<uint4*>(o) = raw;
       }
     } else {
-      const int n = (int)min((int64_t)8, cols - g * 8);
       for (int k = 0; k < n; ++k) o[k] = from_f32<T>(v[k]);
     }
   }
 }
 
+// Block width (log2 of the 8-column groups, 16 to 256) and grid for `rows` x `groups`.
+struct Walk {
+  int txl;
+  dim3 grid;
+};
+bool make_walk(int64_t rows, int64_t groups, Walk& w) {
+  w.txl = 4;
+  while (w.txl < 8 && (1ll << w.txl) < groups) ++w.txl;
+  const int64_t gx = (rows + (256 >> w.txl) * kU - 1) / ((256 >> w.txl) * kU), gy = (groups + (1ll << w.txl) - 1) >> w.txl;
+  if (gx >= (1ll << 31) || gy > 65535) return false;
+  w.grid = dim3((unsigned)gx, (unsigned)gy);
+  return true;
+}
+
 template <typename T>
 int quantize_t(const b2_mx4_args* a, cudaStream_t st) {
   const int64_t nkb = (a->cols + 127) / 128;
-  const int64_t work = (a->rows + 127) / 128 * 128 * nkb * 16;
   const bool vec = a->cols % 8 == 0 && ((uintptr_t)a->x & 15) == 0 && (a->ld * (int64_t)sizeof(T)) % 16 == 0;
-  const int grid = grid_for(work, 256, 16);
+  Walk w;
+  if (!make_walk((a->rows + 127) / 128 * 128, nkb * 16, w)) return fail(B2_ERR_ARG, "mx4_quantize: matrix too large");
   {
     LaunchScope ls("mx4_quantize", st);
     if (vec)
-      mx4_quantize_k<T, true><<<grid, 256, 0, st>>>((const T*)a->x, a->codes, a->scales, a->rows, a->cols, a->ld, nkb);
+      mx4_quantize_k<T, true><<<w.grid, 256, 0, st>>>((const T*)a->x, a->codes, a->scales, a->rows, a->cols, a->ld, nkb, w.txl);
     else
-      mx4_quantize_k<T, false><<<grid, 256, 0, st>>>((const T*)a->x, a->codes, a->scales, a->rows, a->cols, a->ld, nkb);
+      mx4_quantize_k<T, false><<<w.grid, 256, 0, st>>>((const T*)a->x, a->codes, a->scales, a->rows, a->cols, a->ld, nkb, w.txl);
   }
   return after_launch("mx4_quantize");
 }
@@ -132,14 +163,15 @@ int quantize_t(const b2_mx4_args* a, cudaStream_t st) {
 template <typename T>
 int dequantize_t(const b2_mx4_args* a, cudaStream_t st) {
   const int64_t nkb = (a->cols + 127) / 128;
-  const int grid = grid_for(a->rows * ((a->cols + 7) / 8), 256, 16);
   const bool vec = a->cols % 8 == 0 && ((uintptr_t)a->out & 15) == 0 && (a->ld * (int64_t)sizeof(T)) % 16 == 0;
+  Walk w;
+  if (!make_walk(a->rows, (a->cols + 7) / 8, w)) return fail(B2_ERR_ARG, "mx4_dequantize: matrix too large");
   {
     LaunchScope ls("mx4_dequantize", st);
     if (vec)
-      mx4_dequantize_k<T, true><<<grid, 256, 0, st>>>(a->codes, a->scales, (T*)a->out, a->rows, a->cols, a->ld, nkb);
+      mx4_dequantize_k<T, true><<<w.grid, 256, 0, st>>>(a->codes, a->scales, (T*)a->out, a->rows, a->cols, a->ld, nkb, w.txl);
     else
-      mx4_dequantize_k<T, false><<<grid, 256, 0, st>>>(a->codes, a->scales, (T*)a->out, a->rows, a->cols, a->ld, nkb);
+      mx4_dequantize_k<T, false><<<w.grid, 256, 0, st>>>(a->codes, a->scales, (T*)a->out, a->rows, a->cols, a->ld, nkb, w.txl);
   }
   return after_launch("mx4_dequantize");
 }
