@@ -226,6 +226,11 @@ at::Tensor mx4_lora_linear(const at::Tensor& x, const at::Tensor& codes, const a
                            const std::optional<at::Tensor>& bias, const at::Tensor& a, const at::Tensor& b) {
   return std::get<0>(mx4_lora_fwd(x, codes, scales, bias, a, b));
 }
+// dx = dy W + dh a, for callers that keep h themselves (several LoRA modules on one stacked weight).
+at::Tensor mx4_lora_dx(const at::Tensor& dy, const at::Tensor& codes, const at::Tensor& scales, int64_t cols,
+                       const at::Tensor& dh, const at::Tensor& a) {
+  return mx4_dx(dy, codes, scales, cols, &dh, &a, "b2::mx4_lora_dx");
+}
 struct Mx4Lora : torch::autograd::Function<Mx4Lora> {
   static Variable forward(AutogradContext* ctx, const Variable& x, const Variable& codes, const Variable& scales,
                           const std::optional<Variable>& bias, const Variable& a, const Variable& b) {
@@ -451,6 +456,8 @@ TORCH_LIBRARY_FRAGMENT(b2, m) {
   m.def("mx4_dequantize(Tensor codes, Tensor scales, int cols, ScalarType dtype) -> Tensor");
   m.def("mx4_linear(Tensor x, Tensor codes, Tensor scales, Tensor? bias) -> Tensor");
   m.def("mx4_lora_linear(Tensor x, Tensor codes, Tensor scales, Tensor? bias, Tensor a, Tensor b) -> Tensor");
+  m.def("mx4_lora_fwd(Tensor x, Tensor codes, Tensor scales, Tensor? bias, Tensor a, Tensor b) -> (Tensor, Tensor)");
+  m.def("mx4_lora_dx(Tensor dy, Tensor codes, Tensor scales, int cols, Tensor dh, Tensor a) -> Tensor");
   m.def("bucket_bias_attention(Tensor q, Tensor k, Tensor v, Tensor table, Tensor? key_mask, int max_distance, "
         "bool bidirectional, bool causal, float scale, int q_offset) -> Tensor");
   m.def("bias_bucket(int rel, int num_buckets, int max_distance, bool bidirectional) -> int", &bias_bucket);
@@ -461,6 +468,8 @@ TORCH_LIBRARY_IMPL(b2, CUDA, m) {
   m.impl("mx4_dequantize", &mx4_dequantize);
   m.impl("mx4_linear", &mx4_linear);
   m.impl("mx4_lora_linear", &mx4_lora_linear);
+  m.impl("mx4_lora_fwd", &mx4_lora_fwd);
+  m.impl("mx4_lora_dx", &mx4_lora_dx);
   m.impl("bucket_bias_attention", &bucket_bias_attention);
 }
 

@@ -5,7 +5,7 @@ Built from the BASELINE description (the Anima model code of the reference's sd-
 the reference repository): hidden 2048, 16 heads x 128, self-attention + cross-attention to 512 text tokens
 of width 1024, GELU MLP 2048 -> 8192 -> 2048, adaLN-modulated (affine-free) LayerNorm, LoRA rank 16 /
 alpha 16 on the q/k/v/o linears of both attentions (the module layout of tests/anima_on_vk.py:43-48 of the
-reference), every base linear frozen as int8 with a per-output-row fp32 scale. The hot operators run on
+reference), every base linear frozen as int8 with a per-output-row fp32 scale (or, with base="mx4", in 4 bits). The hot operators run on
 this package's kernels: int8 linears on the fused dequant GEMM (`b2::int8_linear_fwd/dx`) with the LoRA
 up-projection as one more reduction block of it (`tv.int8_lora_linear`; the rank-r down-projection and the
 LoRA weight gradients on `mm`), the MLP with GELU and its derivative in the int8 GEMM epilogues
@@ -61,6 +61,42 @@ class LoRAInt8Linear(nn.Module):
         # the up-projection (h B^T) * alpha / r is one more reduction block of the int8 GEMM
         b = self.lora_up if self.scale == 1.0 else self.lora_up * self.scale
         return tv.int8_lora_linear(x, self.base.q, self.base.scale, self.base.bias, self.lora_down, b)
+
+
+class Mx4Linear(nn.Module):
+    """Frozen 4-bit weight (MXFP4, 4.25 bits a value) [out, in]; y = Q(x) W^T + b with x quantised in the call."""
+
+    def __init__(self, in_f, out_f, bias=True, std=0.02, generator=None, device="cuda"):
+        super().__init__()
+        w = torch.randn(out_f, in_f, generator=generator, device=generator.device if generator else device) * std
+        packed = tv.mx4_quantize(w.to(device))
+        self.in_f = in_f
+        self.register_buffer("codes", packed.codes)
+        self.register_buffer("scales", packed.scales)
+        self.register_buffer("bias", torch.zeros(out_f, dtype=torch.bfloat16, device=device) if bias else None)
+
+    @property
+    def weight(self) -> tv.Mx4:
+        return tv.Mx4(self.codes, self.scales, self.in_f)
+
+    def forward(self, x):
+        return tv.mx4_linear(x, self.weight, self.bias)
+
+
+class LoRAMx4Linear(nn.Module):
+    """Frozen 4-bit base + trainable LoRA: y = base(x) + (x A^T) B^T * alpha / r, the LoRA term in the same product."""
+
+    def __init__(self, in_f, out_f, rank=16, alpha=16.0, generator=None, device="cuda", dtype=torch.bfloat16):
+        super().__init__()
+        self.base = Mx4Linear(in_f, out_f, bias=True, generator=generator, device=device)
+        gdev = generator.device if generator else device
+        self.lora_down = nn.Parameter((torch.randn(rank, in_f, generator=generator, device=gdev) / math.sqrt(in_f)).to(dtype).to(device))
+        self.lora_up = nn.Parameter((torch.randn(out_f, rank, generator=generator, device=gdev) * 0.02).to(dtype).to(device))
+        self.scale = alpha / rank
+
+    def forward(self, x):
+        b = self.lora_up if self.scale == 1.0 else self.lora_up * self.scale
+        return tv.mx4_lora_linear(x, self.base.weight, self.base.bias, self.lora_down, b)
 
 
 class LoRAGroup:
@@ -151,6 +187,49 @@ def stacked_lora_forward(x, q, scale, bias, grp: LoRAGroup, whole=False):
     return out.split([m.base.q.shape[0] for m in grp.mods], dim=-1)
 
 
+class _StackedMx4LoRA(torch.autograd.Function):
+    """_StackedInt8LoRA over a stacked 4-bit base: y = Q(x) W^T + bias + (x A^T) B_bd^T, straight-through in x."""
+
+    @staticmethod
+    def forward(ctx, x, codes, scales, bias, grp, *params):
+        x2 = x.reshape(-1, x.shape[-1])
+        if not x2.is_contiguous():
+            x2 = x2.contiguous()
+        y, h = torch.ops.b2.mx4_lora_fwd(x2, codes, scales, bias, grp.a, grp.b_bd)
+        ctx.save_for_backward(x2, codes, scales, h)
+        ctx.grp, ctx.x_shape = grp, x.shape
+        return y.view(*x.shape[:-1], codes.shape[0])
+
+    @staticmethod
+    def backward(ctx, gy):
+        x2, codes, scales, h = ctx.saved_tensors
+        grp = ctx.grp
+        gy2 = gy.reshape(-1, gy.shape[-1])
+        if not gy2.is_contiguous():
+            gy2 = gy2.contiguous()
+        dh = torch.mm(gy2, grp.b_bd)
+        gx = None
+        if ctx.needs_input_grad[0]:
+            gx = torch.ops.b2.mx4_lora_dx(gy2, codes, scales, x2.shape[1], dh, grp.a).view(ctx.x_shape)
+        ga = torch.mm(dh.t(), x2)
+        gb = grp.diag_blocks(torch.mm(gy2.t(), h))
+        if grp.scale != 1.0:
+            gb.mul_(grp.scale)
+        gdown = [ga[i * grp.r:(i + 1) * grp.r] for i in range(grp.g)]
+        gup = [gb[i * grp.n:(i + 1) * grp.n] for i in range(grp.g)]
+        return (gx, None, None, None, None, *gdown, *gup)
+
+
+def stacked_mx4_lora_forward(x, codes, scales, bias, grp: LoRAGroup, whole=False):
+    """stacked_lora_forward for LoRAMx4Linear modules whose 4-bit bases are stacked in (codes, scales, bias)."""
+    grp.refresh()
+    params = [m.lora_down for m in grp.mods] + [m.lora_up for m in grp.mods]
+    out = _StackedMx4LoRA.apply(x, codes, scales, bias, grp, *params)
+    if whole:
+        return out
+    return out.split([m.lora_up.shape[0] for m in grp.mods], dim=-1)
+
+
 class _StackedSDPA(torch.autograd.Function):
     """softmax(q k^T / sqrt(d)) v with q, k, v taken as hd-wide column blocks (at q_off, k_off, v_off) of
     projection outputs [B, S, *] (the stacked q/k/v output for self-attention; the q output and the stacked
@@ -186,18 +265,28 @@ class _StackedSDPA(torch.autograd.Function):
 
 
 class DiTBlock(nn.Module):
-    def __init__(self, hidden=2048, heads=16, text_dim=1024, mlp=8192, rank=16, alpha=16.0, seed=0, device="cuda"):
+    """base="int8": frozen int8 weights (the default); base="mx4": frozen 4-bit weights, half the memory, whose products
+    run on the block-scaled tensor cores with the activations quantised per call (hidden a multiple of 128)."""
+
+    def __init__(self, hidden=2048, heads=16, text_dim=1024, mlp=8192, rank=16, alpha=16.0, seed=0, device="cuda", base="int8"):
         super().__init__()
+        if base not in ("int8", "mx4"):
+            raise ValueError(f"DiTBlock: base must be 'int8' or 'mx4', got {base!r}")
+        if base == "mx4" and hidden % 128:
+            raise ValueError(f"DiTBlock: a 4-bit base stacks its projections by 128 rows; hidden {hidden} is no multiple")
+        self.base = base
+        frozen = Int8Linear if base == "int8" else Mx4Linear
+        lora = LoRAInt8Linear if base == "int8" else LoRAMx4Linear
         g = torch.Generator(device=device).manual_seed(seed)
         self.h, self.heads, self.d = hidden, heads, hidden // heads
-        mk = lambda i, o: LoRAInt8Linear(i, o, rank, alpha, generator=g, device=device)  # noqa: E731
+        mk = lambda i, o: lora(i, o, rank, alpha, generator=g, device=device)  # noqa: E731
         self.q, self.k, self.v, self.o = mk(hidden, hidden), mk(hidden, hidden), mk(hidden, hidden), mk(hidden, hidden)
         self.cq, self.ck, self.cv, self.co = mk(hidden, hidden), mk(text_dim, hidden), mk(text_dim, hidden), mk(hidden, hidden)
-        self.fc1 = Int8Linear(hidden, mlp, generator=g, device=device)
-        self.fc2 = Int8Linear(mlp, hidden, generator=g, device=device)
+        self.fc1 = frozen(hidden, mlp, generator=g, device=device)
+        self.fc2 = frozen(mlp, hidden, generator=g, device=device)
         # adaLN modulation: (shift, scale, gate) for self-attn, cross-attn and MLP from the conditioning vector
-        self.ada = Int8Linear(hidden, 9 * hidden, generator=g, device=device)
-        # projections that read the same input keep their frozen int8 bases in one stacked weight
+        self.ada = frozen(hidden, 9 * hidden, generator=g, device=device)
+        # projections that read the same input keep their frozen bases in one stacked weight
         # (each module's base buffers are views of it): one GEMM forward and one dX GEMM backward
         self._stack_bases("qkv", (self.q, self.k, self.v))
         self._stack_bases("ckv", (self.ck, self.cv))
@@ -205,7 +294,7 @@ class DiTBlock(nn.Module):
         self._lora_groups = {"qkv": LoRAGroup((self.q, self.k, self.v)), "ckv": LoRAGroup((self.ck, self.cv))}
 
     def _stack_bases(self, name, mods):
-        for part in ("q", "scale", "bias"):
+        for part in ("q", "scale", "bias") if self.base == "int8" else ("codes", "scales", "bias"):
             full = torch.cat([getattr(m.base, part) for m in mods], 0)
             self.register_buffer(f"{name}_{part}", full)
             o = 0
@@ -217,6 +306,9 @@ class DiTBlock(nn.Module):
     def _stacked(self, name, x, mods, whole=False):
         grp = self._lora_groups[name]
         assert all(a is b for a, b in zip(grp.mods, mods))
+        if self.base == "mx4":
+            return stacked_mx4_lora_forward(x, getattr(self, f"{name}_codes"), getattr(self, f"{name}_scales"),
+                                            getattr(self, f"{name}_bias"), grp, whole=whole)
         return stacked_lora_forward(x, getattr(self, f"{name}_q"), getattr(self, f"{name}_scale"),
                                     getattr(self, f"{name}_bias"), grp, whole=whole)
 
@@ -281,8 +373,11 @@ class DiTBlock(nn.Module):
         h = modln(x, sh2, sc2, 1)
         x = torch.addcmul(x, g2, self._attn(h, text, text, self.cq, self.ck, self.cv, self.co, kv=kv))
         h = modln(x, sh3, sc3, 2)
-        # MLP fc2(gelu(fc1(h))) with the GELU (and its backward) in the int8 GEMM epilogues
-        mlp = tv.int8_mlp(h, self.fc1.q, self.fc1.scale, self.fc1.bias, self.fc2.q, self.fc2.scale, self.fc2.bias)
+        if self.base == "mx4":
+            mlp = self.fc2(F.gelu(self.fc1(h), approximate="tanh"))
+        else:
+            # MLP fc2(gelu(fc1(h))) with the GELU (and its backward) in the int8 GEMM epilogues
+            mlp = tv.int8_mlp(h, self.fc1.q, self.fc1.scale, self.fc1.bias, self.fc2.q, self.fc2.scale, self.fc2.bias)
         x = torch.addcmul(x, g3, mlp)
         return x
 
