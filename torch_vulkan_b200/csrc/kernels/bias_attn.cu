@@ -160,7 +160,7 @@ uint64_t up16(uint64_t v) { return (v + 15) / 16 * 16; }
 
 // Key splits of the forward: the waves of blocks times the key tiles a block walks plus 1.6 us of set-up,
 // and for the join its bytes (each split's fp32 output written and read) at the memory's rate, where a tile takes about
-// 0.4 us on the tensor cores and 6 us on the FMA pipe, and a launch. At least two tiles a split. Measured, 16 heads x 4096 x 4096: 2 splits save a sixth of the walk
+// 0.4 us on the tensor cores and 3 us on the FMA pipe, and a launch. At least two tiles a split. Measured, 16 heads x 4096 x 4096: 2 splits save a sixth of the walk
 // (3.5 waves) and their join takes 47 us of it back.
 int pick_splits(int64_t blocks, int64_t tk, int64_t out_elems, double tile_us) {
   const int64_t sms = device_info().sm_count > 0 ? device_info().sm_count : 148;
@@ -179,7 +179,8 @@ Plan make_plan(const b2_bias_attn_args* a, bool bwd) {
   const int64_t rows = a->B * a->H * a->Sq;
   pl.tc = bwd ? tc_bwd_eligible(a) : tc_fwd_eligible(a);
   const int tile = pl.tc ? kTcTile : kSimtTile;
-  const int64_t tq = (a->Sq + tile - 1) / tile, tk = (a->Sk + tile - 1) / tile;
+  const int64_t walk = pl.tc ? kTcTile : kSimtWalk;
+  const int64_t tq = (a->Sq + tile - 1) / tile, tk = (a->Sk + walk - 1) / walk;
   if (!bwd && rows_eligible(a)) {
     // few query rows: blocks of 128 threads, about six to an SM; a block costs its keys and about 96 keys' worth of set-up
     pl.rows = true;
@@ -190,7 +191,7 @@ Plan make_plan(const b2_bias_attn_args* a, bool bwd) {
       if (cost < best) best = cost, pl.nsplit = (int)ns;
     }
   } else if (!bwd) {
-    pl.nsplit = pick_splits(tq * a->B * a->H, tk, rows * a->D, pl.tc ? 0.4 : 6.0);
+    pl.nsplit = pick_splits(tq * a->B * a->H, tk, rows * a->D, pl.tc ? 0.4 : 3.0);
   } else {
     pl.ntq = (int)tq;
     pl.delta = 0;

@@ -82,7 +82,7 @@ __device__ __forceinline__ int key_end(const Params& p, int64_t last_row) {
 
 int simt_fwd(const Params& p, int dtype, cudaStream_t st);   // bias_attn_simt.cu
 int simt_bwd(const Params& p, int dtype, cudaStream_t st);
-constexpr int kSimtTile = 64;
+constexpr int kSimtTile = 32, kSimtWalk = 64;
 bool tc_fwd_eligible(const b2_bias_attn_args* a);            // bias_attn_tc.cu
 bool tc_bwd_eligible(const b2_bias_attn_args* a);
 int tc_fwd(const Params& p, bool bf16, cudaStream_t st);

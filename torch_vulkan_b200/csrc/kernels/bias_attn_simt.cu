@@ -1,6 +1,6 @@
 // Relative-position-bias attention on the FMA pipe: fp32 inputs, and 16-bit inputs whose layout the tensor-core
-// kernels do not take. A block of 256 threads works on 64 x 64 tiles held in shared memory as fp32, each thread on
-// 4 x 4 scores and on 4 rows x DP / 16 columns of the outputs; every operand read is a 16-byte shared-memory load
+// kernels do not take. A block of 128 threads owns 32 rows and walks the other side in tiles of 64, held in shared memory
+// as fp32, each thread on 4 x 4 scores and on 4 rows x DP / 16 columns of the outputs; every operand read is a 16-byte shared-memory load
 // whose bank pattern is conflict-free (rows padded by 4 floats). Forward: one pass with the running maximum and sum,
 // the key axis split over blockIdx.z when there are few query tiles. Backward: one kernel owns query tiles (dQ and the
 // bias gradient), one owns key tiles (dK, dV, summed over the query heads that share them), so every sum has one owner
@@ -11,23 +11,39 @@ namespace b2 {
 namespace bias_attn {
 namespace {
 
-constexpr int T64 = kSimtTile;
+constexpr int OWN = kSimtTile, T64 = 64;  // rows a block owns, rows of a walked tile
+constexpr int NTH = OWN / 4 * 16;         // threads
 constexpr int PS = T64 + 4;
 
 template <int DP>
 struct Smem {
   static constexpr int LD = DP + 4;
-  static constexpr int TILE = T64 * LD;  // floats of a 64-row operand tile
+  static constexpr int TILE = T64 * LD, OTILE = OWN * LD;  // floats of a walked and of an owned operand tile
 };
 
-// 64 rows of an operand -> fp32 tile, zeros past the end of the rows, past D, and (keep != NULL) in masked rows.
-template <typename T, int DP>
+// ROWS rows of an operand -> fp32 tile, zeros past the end of the rows, past D, and (keep != NULL) in masked rows. Rows of
+// whole aligned 16-byte groups are read so.
+template <typename T, int DP, int ROWS>
 __device__ __forceinline__ void load_tile(float* dst, const void* base, const int64_t* s, int b, int h, int r0, int rows,
                                           int D, float mul, const uint8_t* keep) {
-  for (int e = threadIdx.x; e < T64 * DP; e += 256) {
+  constexpr int V = 16 / (int)sizeof(T);
+  const T* origin = row_of<T>(base, s, b, h, r0);
+  if (D % V == 0 && s[2] % V == 0 && ((uintptr_t)origin & 15) == 0) {
+#pragma unroll 4
+    for (int e = threadIdx.x; e < ROWS * (DP / V); e += NTH) {
+      const int r = e / (DP / V), d = e % (DP / V) * V;
+      uint4 raw = make_uint4(0u, 0u, 0u, 0u);
+      if (r0 + r < rows && d < D && (keep == nullptr || keep[r])) raw = *reinterpret_cast<const uint4*>(origin + r * s[2] + d);
+      const T* t = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+      for (int i = 0; i < V; ++i) dst[r * Smem<DP>::LD + d + i] = to_f32<T>(t[i]) * mul;
+    }
+    return;
+  }
+  for (int e = threadIdx.x; e < ROWS * DP; e += NTH) {
     const int r = e / DP, d = e % DP;
     float v = 0.f;
-    if (r0 + r < rows && d < D && (keep == nullptr || keep[r])) v = to_f32<T>(row_of<T>(base, s, b, h, r0 + r)[d]) * mul;
+    if (r0 + r < rows && d < D && (keep == nullptr || keep[r])) v = to_f32<T>(origin[r * s[2] + d]) * mul;
     dst[r * Smem<DP>::LD + d] = v;
   }
 }
@@ -92,10 +108,10 @@ __device__ __forceinline__ float sum16(float v) {
   return v;
 }
 
-// keep[j] for the 64 keys from k0; returns whether any is left.
-__device__ __forceinline__ bool load_keep(const Params& p, int b, int k0, uint8_t* keep) {
+// keep[j] for the n keys from k0; returns whether any is left.
+__device__ __forceinline__ bool load_keep(const Params& p, int b, int k0, int n, uint8_t* keep) {
   bool any = false;
-  if (threadIdx.x < T64) {
+  if ((int)threadIdx.x < n) {
     const int j = k0 + threadIdx.x;
     const bool ok = j < p.Sk && (p.mask == nullptr || p.mask[(int64_t)b * p.mask_sb + j] != 0);
     keep[threadIdx.x] = ok;
@@ -105,7 +121,7 @@ __device__ __forceinline__ bool load_keep(const Params& p, int b, int k0, uint8_
 }
 
 __device__ __forceinline__ void fill_bias(const Params& p, int h, float* bias) {
-  for (int i = threadIdx.x; i <= 2 * p.R; i += 256) bias[i] = bias_at(p, h, i - p.R);
+  for (int i = threadIdx.x; i <= 2 * p.R; i += NTH) bias[i] = bias_at(p, h, i - p.R);
 }
 __device__ __forceinline__ float bias_get(const Params& p, const float* bias, int rel) {
   if (p.causal && rel > 0) return -INFINITY;
@@ -113,19 +129,19 @@ __device__ __forceinline__ float bias_get(const Params& p, const float* bias, in
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(256) fwd_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(NTH) fwd_kernel(const __grid_constant__ Params p) {
   extern __shared__ float4 sm4[];
   float* Qs = reinterpret_cast<float*>(sm4);
-  float* Ks = Qs + Smem<DP>::TILE;
+  float* Ks = Qs + Smem<DP>::OTILE;
   float* Vs = Ks + Smem<DP>::TILE;
   float* Ps = Vs + Smem<DP>::TILE;
-  float* bias = Ps + T64 * PS;
+  float* bias = Ps + OWN * PS;
   uint8_t* keep = reinterpret_cast<uint8_t*>(bias + 2 * p.R + 1);
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int q0 = blockIdx.x * T64;
+  const int q0 = blockIdx.x * OWN;
   const int b = blockIdx.y / p.H, h = blockIdx.y % p.H, hk = h / (p.H / p.Hk);
   fill_bias(p, h, bias);
-  load_tile<T, DP>(Qs, p.q, p.q_s, b, h, q0, p.Sq, p.D, p.scale * kLog2e, nullptr);
+  load_tile<T, DP, OWN>(Qs, p.q, p.q_s, b, h, q0, p.Sq, p.D, p.scale * kLog2e, nullptr);
   float m[4], l[4], acc[4][DP / 16];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -133,15 +149,15 @@ __global__ void __launch_bounds__(256) fwd_kernel(const __grid_constant__ Params
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) acc[i][c] = 0.f;
   }
-  const int nt = (key_end(p, min(q0 + T64, p.Sq) - 1) + T64 - 1) / T64;
+  const int nt = (key_end(p, min(q0 + OWN, p.Sq) - 1) + T64 - 1) / T64;
   const int per = (nt + p.nsplit - 1) / p.nsplit;
   const int t1 = min(nt, ((int)blockIdx.z + 1) * per);
   for (int t = blockIdx.z * per; t < t1; ++t) {
     const int k0 = t * T64;
     __syncthreads();
-    if (!load_keep(p, b, k0, keep)) continue;
-    load_tile<T, DP>(Ks, p.k, p.k_s, b, hk, k0, p.Sk, p.D, 1.f, keep);
-    load_tile<T, DP>(Vs, p.v, p.v_s, b, hk, k0, p.Sk, p.D, 1.f, keep);
+    if (!load_keep(p, b, k0, T64, keep)) continue;
+    load_tile<T, DP, T64>(Ks, p.k, p.k_s, b, hk, k0, p.Sk, p.D, 1.f, keep);
+    load_tile<T, DP, T64>(Vs, p.v, p.v_s, b, hk, k0, p.Sk, p.D, 1.f, keep);
     __syncthreads();
     float s[4][4] = {};
     dot_tile<DP>(Qs, Ks, ty, tx, s);
@@ -203,25 +219,25 @@ __global__ void __launch_bounds__(256) fwd_kernel(const __grid_constant__ Params
   }
 }
 
-// dQ and the bias gradient: a block owns 64 query rows of one head and walks the keys.
+// dQ and the bias gradient: a block owns 32 query rows of one head and walks the keys.
 template <typename T, int DP>
-__global__ void __launch_bounds__(256) dq_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(NTH) dq_kernel(const __grid_constant__ Params p) {
   extern __shared__ float4 sm4[];
   float* Qs = reinterpret_cast<float*>(sm4);
-  float* Gs = Qs + Smem<DP>::TILE;  // dO
-  float* Ks = Gs + Smem<DP>::TILE;
+  float* Gs = Qs + Smem<DP>::OTILE;  // dO
+  float* Ks = Gs + Smem<DP>::OTILE;
   float* Vs = Ks + Smem<DP>::TILE;
   float* Ps = Vs + Smem<DP>::TILE;  // dS
-  float* bias = Ps + T64 * PS;
-  float* diag = bias + 2 * p.R + 1;                       // 127 diagonal sums of a tile
+  float* bias = Ps + OWN * PS;
+  float* diag = bias + 2 * p.R + 1;                       // 95 diagonal sums of a tile
   int* dbk = reinterpret_cast<int*>(diag + 2 * T64);      // and their buckets
   uint8_t* keep = reinterpret_cast<uint8_t*>(dbk + 2 * T64);
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int q0 = blockIdx.x * T64;
+  const int q0 = blockIdx.x * OWN;
   const int b = blockIdx.y / p.H, h = blockIdx.y % p.H, hk = h / (p.H / p.Hk);
   fill_bias(p, h, bias);
-  load_tile<T, DP>(Qs, p.q, p.q_s, b, h, q0, p.Sq, p.D, p.scale * kLog2e, nullptr);
-  load_tile<T, DP>(Gs, p.d_o, p.do_s, b, h, q0, p.Sq, p.D, 1.f, nullptr);
+  load_tile<T, DP, OWN>(Qs, p.q, p.q_s, b, h, q0, p.Sq, p.D, p.scale * kLog2e, nullptr);
+  load_tile<T, DP, OWN>(Gs, p.d_o, p.do_s, b, h, q0, p.Sq, p.D, 1.f, nullptr);
   float L[4], dl[4], acc[4][DP / 16];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -235,13 +251,13 @@ __global__ void __launch_bounds__(256) dq_kernel(const __grid_constant__ Params 
     for (int c = 0; c < DP / 16; ++c) acc[i][c] = 0.f;
   }
   float db = 0.f;  // thread n: sum of dS over bucket n
-  const int nt = (key_end(p, min(q0 + T64, p.Sq) - 1) + T64 - 1) / T64;
+  const int nt = (key_end(p, min(q0 + OWN, p.Sq) - 1) + T64 - 1) / T64;
   for (int t = 0; t < nt; ++t) {
     const int k0 = t * T64;
     __syncthreads();
-    if (!load_keep(p, b, k0, keep)) continue;
-    load_tile<T, DP>(Ks, p.k, p.k_s, b, hk, k0, p.Sk, p.D, 1.f, keep);
-    load_tile<T, DP>(Vs, p.v, p.v_s, b, hk, k0, p.Sk, p.D, 1.f, keep);
+    if (!load_keep(p, b, k0, T64, keep)) continue;
+    load_tile<T, DP, T64>(Ks, p.k, p.k_s, b, hk, k0, p.Sk, p.D, 1.f, keep);
+    load_tile<T, DP, T64>(Vs, p.v, p.v_s, b, hk, k0, p.Sk, p.D, 1.f, keep);
     __syncthreads();
     float s[4][4] = {}, dp[4][4] = {};
     dot_tile<DP>(Qs, Ks, ty, tx, s);
@@ -258,16 +274,16 @@ __global__ void __launch_bounds__(256) dq_kernel(const __grid_constant__ Params 
     }
     if (p.dtab) {
       __syncthreads();
-      if (threadIdx.x < 2 * T64 - 1) {
-        const int d = (int)threadIdx.x - (T64 - 1);  // key - query inside the tile
+      if (threadIdx.x < OWN + T64 - 1) {
+        const int d = (int)threadIdx.x - (OWN - 1);  // key - query inside the tile
         float a = 0.f;
-        for (int r = max(0, -d); r < min(T64, T64 - d); ++r) a += Ps[r * PS + r + d];
+        for (int r = max(0, -d); r < min(OWN, T64 - d); ++r) a += Ps[r * PS + r + d];
         diag[threadIdx.x] = a;
         dbk[threadIdx.x] = bucket_of(p, max(-p.R, min(p.R, k0 + d - q0 - p.q_off)));
       }
       __syncthreads();
       if ((int)threadIdx.x < p.nb)
-        for (int i = 0; i < 2 * T64 - 1; ++i) db += dbk[i] == (int)threadIdx.x ? diag[i] : 0.f;
+        for (int i = 0; i < OWN + T64 - 1; ++i) db += dbk[i] == (int)threadIdx.x ? diag[i] : 0.f;
     } else {
       __syncwarp();
     }
@@ -288,26 +304,26 @@ __global__ void __launch_bounds__(256) dq_kernel(const __grid_constant__ Params 
     p.dtab[((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * p.nb + threadIdx.x] = db;
 }
 
-// dK, dV: a block owns 64 keys of one key/value head and walks the queries of every head that shares it.
+// dK, dV: a block owns 32 keys of one key/value head and walks the queries of every head that shares it.
 template <typename T, int DP>
-__global__ void __launch_bounds__(256) dkv_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(NTH) dkv_kernel(const __grid_constant__ Params p) {
   extern __shared__ float4 sm4[];
   float* Ks = reinterpret_cast<float*>(sm4);
-  float* Vs = Ks + Smem<DP>::TILE;
-  float* Qs = Vs + Smem<DP>::TILE;
+  float* Vs = Ks + Smem<DP>::OTILE;
+  float* Qs = Vs + Smem<DP>::OTILE;
   float* Gs = Qs + Smem<DP>::TILE;  // dO
   float* Pt = Gs + Smem<DP>::TILE;  // P^T
-  float* St = Pt + T64 * PS;        // dS^T
-  float* bias = St + T64 * PS;
+  float* St = Pt + OWN * PS;        // dS^T
+  float* bias = St + OWN * PS;
   float* Lq = bias + 2 * p.R + 1;
   float* Dq = Lq + T64;
   uint8_t* keep = reinterpret_cast<uint8_t*>(Dq + T64);
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int k0 = blockIdx.x * T64;
+  const int k0 = blockIdx.x * OWN;
   const int b = blockIdx.y / p.Hk, hk = blockIdx.y % p.Hk, G = p.H / p.Hk;
-  const bool some = load_keep(p, b, k0, keep);
-  load_tile<T, DP>(Ks, p.k, p.k_s, b, hk, k0, p.Sk, p.D, 1.f, keep);
-  load_tile<T, DP>(Vs, p.v, p.v_s, b, hk, k0, p.Sk, p.D, 1.f, keep);
+  const bool some = load_keep(p, b, k0, OWN, keep);
+  load_tile<T, DP, OWN>(Ks, p.k, p.k_s, b, hk, k0, p.Sk, p.D, 1.f, keep);
+  load_tile<T, DP, OWN>(Vs, p.v, p.v_s, b, hk, k0, p.Sk, p.D, 1.f, keep);
   float dk[4][DP / 16] = {}, dv[4][DP / 16] = {};
   // causal: the first query row that sees key k0
   const int64_t first = p.causal ? max((int64_t)0, (int64_t)k0 - p.q_off) : 0;
@@ -319,8 +335,8 @@ __global__ void __launch_bounds__(256) dkv_kernel(const __grid_constant__ Params
     for (int t = (int)min((int64_t)nt, first / T64); t < nt; ++t) {
       const int q0 = t * T64;
       __syncthreads();
-      load_tile<T, DP>(Qs, p.q, p.q_s, b, h, q0, p.Sq, p.D, 1.f, nullptr);
-      load_tile<T, DP>(Gs, p.d_o, p.do_s, b, h, q0, p.Sq, p.D, 1.f, nullptr);
+      load_tile<T, DP, T64>(Qs, p.q, p.q_s, b, h, q0, p.Sq, p.D, 1.f, nullptr);
+      load_tile<T, DP, T64>(Gs, p.d_o, p.do_s, b, h, q0, p.Sq, p.D, 1.f, nullptr);
       if (threadIdx.x < T64) {
         const int qi = q0 + threadIdx.x;
         const int64_t row = ((int64_t)b * p.H + h) * p.Sq + qi;
@@ -365,30 +381,30 @@ __global__ void __launch_bounds__(256) dkv_kernel(const __grid_constant__ Params
 }
 
 template <int DP>
-int smem_bytes(const Params& p, int tiles, int ps) {
-  return (tiles * Smem<DP>::TILE + ps * T64 * PS + 2 * p.R + 1 + 4 * T64 + 4) * 4 + T64;
+int smem_bytes(const Params& p, int own, int walked, int ps) {
+  return (own * Smem<DP>::OTILE + walked * Smem<DP>::TILE + ps * OWN * PS + 2 * p.R + 1 + 4 * T64 + 4) * 4 + T64;
 }
 
 template <typename T, int DP>
 int fwd_t(const Params& p, cudaStream_t st) {
-  const int sm = smem_bytes<DP>(p, 3, 1);
+  const int sm = smem_bytes<DP>(p, 1, 2, 1);
   if (int rc = allow_smem<fwd_kernel<T, DP>>(sm, "bias_attn_fwd_simt")) return rc;
   {
     LaunchScope ls("bias_attn_fwd_simt", st);
-    dim3 grid((p.Sq + T64 - 1) / T64, p.B * p.H, p.nsplit);
-    fwd_kernel<T, DP><<<grid, 256, sm, st>>>(p);
+    dim3 grid((p.Sq + OWN - 1) / OWN, p.B * p.H, p.nsplit);
+    fwd_kernel<T, DP><<<grid, NTH, sm, st>>>(p);
   }
   return after_launch("bias_attn_fwd_simt");
 }
 
 template <typename T, int DP>
 int bwd_t(const Params& p, cudaStream_t st) {
-  const int sq = smem_bytes<DP>(p, 4, 1), sk = smem_bytes<DP>(p, 4, 2);
+  const int sq = smem_bytes<DP>(p, 2, 2, 1), sk = smem_bytes<DP>(p, 2, 2, 2);
   if (p.dq || p.dtab) {
     if (int rc = allow_smem<dq_kernel<T, DP>>(sq, "bias_attn_dq_simt")) return rc;
     {
       LaunchScope ls("bias_attn_dq_simt", st);
-      dq_kernel<T, DP><<<dim3((p.Sq + T64 - 1) / T64, p.B * p.H), 256, sq, st>>>(p);
+      dq_kernel<T, DP><<<dim3((p.Sq + OWN - 1) / OWN, p.B * p.H), NTH, sq, st>>>(p);
     }
     if (int rc = after_launch("bias_attn_dq_simt")) return rc;
   }
@@ -396,7 +412,7 @@ int bwd_t(const Params& p, cudaStream_t st) {
     if (int rc = allow_smem<dkv_kernel<T, DP>>(sk, "bias_attn_dkv_simt")) return rc;
     {
       LaunchScope ls("bias_attn_dkv_simt", st);
-      dkv_kernel<T, DP><<<dim3((p.Sk + T64 - 1) / T64, p.B * p.Hk), 256, sk, st>>>(p);
+      dkv_kernel<T, DP><<<dim3((p.Sk + OWN - 1) / OWN, p.B * p.Hk), NTH, sk, st>>>(p);
     }
     if (int rc = after_launch("bias_attn_dkv_simt")) return rc;
   }
