@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(NTH) fwd_kernel(const __grid_constant__ Params
 
 // dQ and the bias gradient: a block owns 32 query rows of one head and walks the keys.
 template <typename T, int DP>
-__global__ void __launch_bounds__(NTH) dq_kernel(const __grid_constant__ Params p) {
+__device__ __forceinline__ void dq_side(const Params& p, int block, int xtiles) {
   extern __shared__ float4 sm4[];
   float* Qs = reinterpret_cast<float*>(sm4);
   float* Gs = Qs + Smem<DP>::OTILE;  // dO
@@ -233,8 +233,8 @@ __global__ void __launch_bounds__(NTH) dq_kernel(const __grid_constant__ Params 
   int* dbk = reinterpret_cast<int*>(diag + 2 * T64);      // and their buckets
   uint8_t* keep = reinterpret_cast<uint8_t*>(dbk + 2 * T64);
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int q0 = blockIdx.x * OWN;
-  const int b = blockIdx.y / p.H, h = blockIdx.y % p.H, hk = h / (p.H / p.Hk);
+  const int bh = block / xtiles, q0 = (block - bh * xtiles) * OWN;
+  const int b = bh / p.H, h = bh % p.H, hk = h / (p.H / p.Hk);
   fill_bias(p, h, bias);
   load_tile<T, DP, OWN>(Qs, p.q, p.q_s, b, h, q0, p.Sq, p.D, p.scale * kLog2e, nullptr);
   load_tile<T, DP, OWN>(Gs, p.d_o, p.do_s, b, h, q0, p.Sq, p.D, 1.f, nullptr);
@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(NTH) dq_kernel(const __grid_constant__ Params 
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int qi = q0 + ty * 4 + i;
-    const int64_t row = (int64_t)blockIdx.y * p.Sq + qi;
+    const int64_t row = (int64_t)bh * p.Sq + qi;
     // rows past the end and rows with no key: exp2(x - inf) = 0
     L[i] = qi < p.Sq ? p.lse[row] * kLog2e : INFINITY;
     if (L[i] == -INFINITY) L[i] = INFINITY;
@@ -301,12 +301,12 @@ __global__ void __launch_bounds__(NTH) dq_kernel(const __grid_constant__ Params 
     }
   }
   if (p.dtab && (int)threadIdx.x < p.nb)
-    p.dtab[((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * p.nb + threadIdx.x] = db;
+    p.dtab[(int64_t)block * p.nb + threadIdx.x] = db;
 }
 
 // dK, dV: a block owns 32 keys of one key/value head and walks the queries of every head that shares it.
 template <typename T, int DP>
-__global__ void __launch_bounds__(NTH) dkv_kernel(const __grid_constant__ Params p) {
+__device__ __forceinline__ void dkv_side(const Params& p, int block, int xtiles) {
   extern __shared__ float4 sm4[];
   float* Ks = reinterpret_cast<float*>(sm4);
   float* Vs = Ks + Smem<DP>::OTILE;
@@ -319,8 +319,8 @@ __global__ void __launch_bounds__(NTH) dkv_kernel(const __grid_constant__ Params
   float* Dq = Lq + T64;
   uint8_t* keep = reinterpret_cast<uint8_t*>(Dq + T64);
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int k0 = blockIdx.x * OWN;
-  const int b = blockIdx.y / p.Hk, hk = blockIdx.y % p.Hk, G = p.H / p.Hk;
+  const int bh = block / xtiles, k0 = (block - bh * xtiles) * OWN;
+  const int b = bh / p.Hk, hk = bh % p.Hk, G = p.H / p.Hk;
   const bool some = load_keep(p, b, k0, OWN, keep);
   load_tile<T, DP, OWN>(Ks, p.k, p.k_s, b, hk, k0, p.Sk, p.D, 1.f, keep);
   load_tile<T, DP, OWN>(Vs, p.v, p.v_s, b, hk, k0, p.Sk, p.D, 1.f, keep);
@@ -380,6 +380,13 @@ __global__ void __launch_bounds__(NTH) dkv_kernel(const __grid_constant__ Params
   }
 }
 
+// Both sides in one launch, the key blocks (the longer walks) first: either alone leaves SMs idle at these sizes.
+template <typename T, int DP>
+__global__ void __launch_bounds__(NTH) bwd_kernel(const __grid_constant__ Params p, int key_blocks, int key_tiles, int query_tiles) {
+  if ((int)blockIdx.x < key_blocks) dkv_side<T, DP>(p, blockIdx.x, key_tiles);
+  else dq_side<T, DP>(p, (int)blockIdx.x - key_blocks, query_tiles);
+}
+
 template <int DP>
 int smem_bytes(const Params& p, int own, int walked, int ps) {
   return (own * Smem<DP>::OTILE + walked * Smem<DP>::TILE + ps * OWN * PS + 2 * p.R + 1 + 4 * T64 + 4) * 4 + T64;
@@ -399,24 +406,18 @@ int fwd_t(const Params& p, cudaStream_t st) {
 
 template <typename T, int DP>
 int bwd_t(const Params& p, cudaStream_t st) {
-  const int sq = smem_bytes<DP>(p, 2, 2, 1), sk = smem_bytes<DP>(p, 2, 2, 2);
-  if (p.dq || p.dtab) {
-    if (int rc = allow_smem<dq_kernel<T, DP>>(sq, "bias_attn_dq_simt")) return rc;
-    {
-      LaunchScope ls("bias_attn_dq_simt", st);
-      dq_kernel<T, DP><<<dim3((p.Sq + OWN - 1) / OWN, p.B * p.H), NTH, sq, st>>>(p);
-    }
-    if (int rc = after_launch("bias_attn_dq_simt")) return rc;
+  const int ktiles = (p.Sk + OWN - 1) / OWN, qtiles = (p.Sq + OWN - 1) / OWN;
+  const int64_t kblocks = p.dk || p.dv ? (int64_t)p.B * p.Hk * ktiles : 0;
+  const int64_t qblocks = p.dq || p.dtab ? (int64_t)p.B * p.H * qtiles : 0;
+  if (kblocks + qblocks == 0) return 0;
+  if (kblocks + qblocks >= (1ll << 31)) return fail(B2_ERR_ARG, "bias_attn_bwd: too many tiles");
+  const int sm = kblocks ? smem_bytes<DP>(p, 2, 2, 2) : smem_bytes<DP>(p, 2, 2, 1);
+  if (int rc = allow_smem<bwd_kernel<T, DP>>(sm, "bias_attn_bwd_simt")) return rc;
+  {
+    LaunchScope ls("bias_attn_bwd_simt", st);
+    bwd_kernel<T, DP><<<(unsigned)(kblocks + qblocks), NTH, sm, st>>>(p, (int)kblocks, ktiles, qtiles);
   }
-  if (p.dk || p.dv) {
-    if (int rc = allow_smem<dkv_kernel<T, DP>>(sk, "bias_attn_dkv_simt")) return rc;
-    {
-      LaunchScope ls("bias_attn_dkv_simt", st);
-      dkv_kernel<T, DP><<<dim3((p.Sk + OWN - 1) / OWN, p.B * p.Hk), NTH, sk, st>>>(p);
-    }
-    if (int rc = after_launch("bias_attn_dkv_simt")) return rc;
-  }
-  return 0;
+  return after_launch("bias_attn_bwd_simt");
 }
 
 template <typename T>

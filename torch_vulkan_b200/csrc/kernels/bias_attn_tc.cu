@@ -487,12 +487,11 @@ __device__ __forceinline__ void add_diagonals(const float* v, float* arr, int re
   add_at(arr, rel + lane - 31, lane < 15 ? scratch[lane] : 0.f, lane < 15, R, lane);
 }
 
+// block: index among the blocks of this side, xtiles of them per head.
 template <int D, bool BF16, bool KEYS>
-__global__ void __launch_bounds__(576, 1)
-    bias_bwd_tc(const __grid_constant__ CUtensorMap tmX1, const __grid_constant__ CUtensorMap tmX2,
-                const __grid_constant__ CUtensorMap tmY1, const __grid_constant__ CUtensorMap tmY2,
-                const __grid_constant__ CUtensorMap tmG1, const __grid_constant__ CUtensorMap tmG2,
-                const __grid_constant__ Params p, const float2* __restrict__ lsed, int sq_pad) {
+__device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensorMap& tmX2, const CUtensorMap& tmY1,
+                                         const CUtensorMap& tmY2, const CUtensorMap& tmG1, const CUtensorMap& tmG2,
+                                         const Params& p, const float2* __restrict__ lsed, int sq_pad, int block, int xtiles) {
   using C = Bwd<D, KEYS>;
   constexpr int NS = C::NS, NT = C::NT, HC = C::HC;
   extern __shared__ uint8_t smem_raw[];
@@ -514,9 +513,10 @@ __global__ void __launch_bounds__(576, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int heads = KEYS ? p.Hk : p.H, G = p.H / p.Hk;
   // causal: the query tiles with the most keys come first; the key tiles with the most queries already do
-  const int xt = (!KEYS && p.causal) ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x;
+  const int bh = block / xtiles, xi = block - bh * xtiles;
+  const int xt = (!KEYS && p.causal) ? xtiles - 1 - xi : xi;
   const int x0 = xt * C::BX;
-  const int b = (int)blockIdx.y / heads, hx = (int)blockIdx.y % heads;
+  const int b = bh / heads, hx = bh % heads;
 
   if (threadIdx.x == 0) {
     tc::mbar_init(x_full, 1);
@@ -807,7 +807,7 @@ __global__ void __launch_bounds__(576, 1)
             for (int d = 1 + lane; d <= p.R; d += 32) s += vec[p.R + d];
         }
         s = warp_sum(s);
-        if (lane == 0) p.dtab[((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * p.nb + bk] = s;
+        if (lane == 0) p.dtab[(int64_t)block * p.nb + bk] = s;
       }
     }
     // ---------------- epilogue: a warp writes 32 rows x 32 columns of a gradient at a time ----------------
@@ -862,6 +862,22 @@ __global__ void __launch_bounds__(576, 1)
     tc::tc_fence_after();
     tc::tmem_dealloc(tbase, C::TMEM_COLS);
   }
+}
+
+// Both sides in one launch: the key blocks, whose walks are the longer ones, start first and the query blocks fill the SMs
+// that they leave.
+struct BwdMaps {
+  CUtensorMap qx, gx, ky, vy, dq;  // query side: boxes of Q, dO it owns, of K, V it walks, and dQ
+  CUtensorMap kx, vx, qy, gy, dv, dk;
+};
+template <int D, bool BF16>
+__global__ void __launch_bounds__(576, 1)
+    bias_bwd_tc(const __grid_constant__ BwdMaps m, const __grid_constant__ Params p, const float2* __restrict__ lsed, int sq_pad,
+                int key_blocks, int key_tiles, int query_tiles) {
+  if ((int)blockIdx.x < key_blocks)
+    bwd_side<D, BF16, true>(m.kx, m.vx, m.qy, m.gy, m.dv, m.dk, p, lsed, sq_pad, blockIdx.x, key_tiles);
+  else
+    bwd_side<D, BF16, false>(m.qx, m.gx, m.ky, m.vy, m.dq, m.dq, p, lsed, sq_pad, (int)blockIdx.x - key_blocks, query_tiles);
 }
 
 // lsed[bh][q] = (-lse log2 e, -sum_d dO O) for q < Sq, (-inf, 0) for padding and for rows without a key: exp2(x - inf) = 0.
@@ -950,27 +966,6 @@ int bwd_smem(const Params& p) {
   return Bwd<D, KEYS>::OFF_VEC + (KEYS ? 2 * vb : vb + (p.dtab ? 16 * db + 16 * 64 : 0)) + 1024;
 }
 
-template <int D, bool BF16, bool KEYS>
-int bwd_launch(const Params& p, const float2* lsed, int sq_pad, cudaStream_t st) {
-  using C = Bwd<D, KEYS>;
-  auto kern = bias_bwd_tc<D, BF16, KEYS>;
-  const char* name = KEYS ? "bias_attn_dkv_tc" : "bias_attn_dq_tc";
-  const int smem = bwd_smem<D, KEYS>(p);
-  if (int rc = allow_smem<bias_bwd_tc<D, BF16, KEYS>>(smem, name)) return rc;
-  CUtensorMap q, k, v, g, g1, g2;
-  const uint32_t qrows = KEYS ? C::NT : 128, krows = KEYS ? 128 : C::NT;
-  bool ok = bhsd_map(&q, p.q, p.q_s, p.B, p.H, p.Sq, p.D, BF16, qrows) && bhsd_map(&g, p.d_o, p.do_s, p.B, p.H, p.Sq, p.D, BF16, qrows) &&
-            bhsd_map(&k, p.k, p.k_s, p.B, p.Hk, p.Sk, p.D, BF16, krows) && bhsd_map(&v, p.v, p.v_s, p.B, p.Hk, p.Sk, p.D, BF16, krows);
-  if (KEYS)
-    ok = ok && store_map(&g1, p.dv, p.dv_s, p.B, p.Hk, p.Sk, p.D, BF16) && store_map(&g2, p.dk, p.dk_s, p.B, p.Hk, p.Sk, p.D, BF16);
-  else
-    ok = ok && store_map(&g1, p.dq, p.dq_s, p.B, p.H, p.Sq, p.D, BF16) && store_map(&g2, nullptr, p.dq_s, 1, 1, 1, p.D, BF16);
-  if (!ok) return fail(B2_ERR_ARG, std::string(name) + ": tensor map rejected");
-  dim3 grid(((KEYS ? p.Sk : p.Sq) + 127) / 128, p.B * (KEYS ? p.Hk : p.H));
-  return KEYS ? launch_pdl(name, kern, grid, dim3(C::THREADS), smem, st, k, v, q, g, g1, g2, p, lsed, sq_pad)
-              : launch_pdl(name, kern, grid, dim3(C::THREADS), smem, st, q, g, k, v, g1, g2, p, lsed, sq_pad);
-}
-
 template <int D, bool BF16>
 int bwd_t(const Params& p, float2* lsed, int sq_pad, cudaStream_t st) {
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
@@ -978,11 +973,29 @@ int bwd_t(const Params& p, float2* lsed, int sq_pad, cudaStream_t st) {
   if (int rc = launch_pdl("bias_attn_bwd_prep", bias_bwd_prep<T>, dim3((unsigned)((rows * 8 + 255) / 256)), dim3(256), 0, st, p,
                           lsed, sq_pad))
     return rc;
-  if (p.dq || p.dtab)
-    if (int rc = bwd_launch<D, BF16, false>(p, lsed, sq_pad, st)) return rc;
-  if (p.dk || p.dv)
-    if (int rc = bwd_launch<D, BF16, true>(p, lsed, sq_pad, st)) return rc;
-  return 0;
+  using Q = Bwd<D, false>;
+  using K = Bwd<D, true>;
+  static_assert(Q::THREADS == K::THREADS, "one launch for both sides");
+  const int ktiles = (p.Sk + 127) / 128, qtiles = (p.Sq + 127) / 128;
+  const int64_t kblocks = p.dk || p.dv ? (int64_t)p.B * p.Hk * ktiles : 0;
+  const int64_t qblocks = p.dq || p.dtab ? (int64_t)p.B * p.H * qtiles : 0;
+  if (kblocks + qblocks == 0) return 0;
+  if (kblocks + qblocks >= (1ll << 31)) return fail(B2_ERR_ARG, "bias_attn_bwd: too many tiles");
+  const int smem = std::max(kblocks ? bwd_smem<D, true>(p) : 0, qblocks ? bwd_smem<D, false>(p) : 0);
+  if (int rc = allow_smem<bias_bwd_tc<D, BF16>>(smem, "bias_attn_bwd_tc")) return rc;
+  BwdMaps m;
+  auto in = [&](CUtensorMap* t, const void* base, const int64_t* s, int heads, int len, uint32_t box) {
+    return bhsd_map(t, base, s, p.B, heads, len, p.D, BF16, box);
+  };
+  if (!in(&m.qx, p.q, p.q_s, p.H, p.Sq, 128) || !in(&m.gx, p.d_o, p.do_s, p.H, p.Sq, 128) ||
+      !in(&m.ky, p.k, p.k_s, p.Hk, p.Sk, Q::NT) || !in(&m.vy, p.v, p.v_s, p.Hk, p.Sk, Q::NT) ||
+      !in(&m.kx, p.k, p.k_s, p.Hk, p.Sk, 128) || !in(&m.vx, p.v, p.v_s, p.Hk, p.Sk, 128) ||
+      !in(&m.qy, p.q, p.q_s, p.H, p.Sq, K::NT) || !in(&m.gy, p.d_o, p.do_s, p.H, p.Sq, K::NT) ||
+      !store_map(&m.dq, p.dq, p.dq_s, p.B, p.H, p.Sq, p.D, BF16) || !store_map(&m.dk, p.dk, p.dk_s, p.B, p.Hk, p.Sk, p.D, BF16) ||
+      !store_map(&m.dv, p.dv, p.dv_s, p.B, p.Hk, p.Sk, p.D, BF16))
+    return fail(B2_ERR_ARG, "bias_attn_bwd: tensor map rejected");
+  return launch_pdl("bias_attn_bwd_tc", bias_bwd_tc<D, BF16>, dim3((unsigned)(kblocks + qblocks)), dim3(K::THREADS), smem, st, m, p,
+                    (const float2*)lsed, sq_pad, (int)kblocks, ktiles, qtiles);
 }
 
 }  // namespace
