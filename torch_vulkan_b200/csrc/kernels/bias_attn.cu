@@ -222,7 +222,15 @@ Params make_params(const b2_bias_attn_args* a) {
   p.nb = a->num_buckets;
   p.bidir = a->bidirectional ? 1 : 0, p.causal = a->causal ? 1 : 0;
   p.nsplit = 1;
-  p.nthr = thresholds(p.bidir ? p.nb / 2 : p.nb, p.R, p.thr);
+  {
+    // a function of the two numbers alone, remembered per thread: its logarithms cost more than a launch
+    thread_local int nb = 0, dist = 0, n = 0;
+    thread_local uint16_t thr[B2_BIAS_MAX_BUCKETS];
+    const int side = p.bidir ? p.nb / 2 : p.nb;
+    if (nb != side || dist != p.R) n = thresholds(side, p.R, thr), nb = side, dist = p.R;
+    p.nthr = n;
+    std::copy(thr, thr + n, p.thr);
+  }
   p.scale = a->scale;
   p.err = device_error_ptr();
   return p;

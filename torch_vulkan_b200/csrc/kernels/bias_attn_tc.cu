@@ -57,20 +57,20 @@ __device__ __forceinline__ uint32_t key_bits(const Params& p, int b, int k) {
   return __ballot_sync(0xffffffffu, ok);
 }
 
-// One past the last key below `end` that the mask leaves (whole block of nthreads; contains block barriers).
-__device__ __forceinline__ int trim_end(const Params& p, int b, int end, int nthreads) {
+// One past the last key below `end` that the mask leaves (every thread of the block; contains block barriers). The whole
+// row of the mask is read at once: one trip to memory. slot: shared memory, not in use otherwise.
+__device__ __forceinline__ int trim_end(const Params& p, int b, int end, int nthreads, int* slot) {
   if (p.mask == nullptr) return end;
   const uint8_t* m = p.mask + (int64_t)b * p.mask_sb;
-  while (end > 0) {
-    const int j = end - 1 - (int)threadIdx.x;
-    const bool any = (int)threadIdx.x < nthreads && j >= 0 && m[j] != 0;
-    if (__syncthreads_or(any)) {
-      // a key among the last nthreads: the exact end does not matter, tiles are dropped whole
-      return end;
-    }
-    end -= nthreads;
-  }
-  return 0;
+  if (threadIdx.x == 0) *slot = 0;
+  int last = 0;
+#pragma unroll 8
+  for (int j = (int)threadIdx.x; j < end; j += nthreads) last = m[j] != 0 ? j + 1 : last;
+  __syncthreads();
+  last = __reduce_max_sync(0xffffffffu, last);
+  if ((threadIdx.x & 31) == 0 && last > 0) atomicMax(slot, last);
+  __syncthreads();
+  return *slot;
 }
 
 // ==================================================================================================
@@ -131,8 +131,7 @@ __global__ void __launch_bounds__(320, 1)
     tc::tmem_alloc(tmem_slot, C::TMEM_COLS);
     tc::tmem_relinquish();
   }
-  fill_vec(p, h, vec, threadIdx.x, C::THREADS);
-  const int end = trim_end(p, b, key_end(p, min(q0 + C::BQ, p.Sq) - 1), C::THREADS);
+  const int end = trim_end(p, b, key_end(p, min(q0 + C::BQ, p.Sq) - 1), C::THREADS, reinterpret_cast<int*>(vec));
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
@@ -231,6 +230,8 @@ __global__ void __launch_bounds__(320, 1)
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     int kb = 0;
+    fill_vec(p, h, vec, (int)threadIdx.x - 64, 256);  // while the first tiles are loaded and multiplied
+    tc::named_bar_sync(1, 256);
     for (int t = g; t < n; t += 2, ++kb) {
       const int k0 = (t0 + t) * C::BK;
       uint32_t bits[4];
@@ -540,10 +541,7 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
     if (p.causal) first = (int)min((int64_t)nt, max((int64_t)0, (int64_t)x0 - p.q_off) / NT);
     tiles = any ? nt - first : 0;
   } else {
-    fill_vec(p, hx, vec, threadIdx.x, C::THREADS);
-    if (p.dtab)
-      for (int i = threadIdx.x; i < 16 * dlen; i += C::THREADS) darr[i] = 0.f;
-    tiles = (trim_end(p, b, key_end(p, min(x0 + C::BX, p.Sq) - 1), C::THREADS) + NT - 1) / NT;
+    tiles = (trim_end(p, b, key_end(p, min(x0 + C::BX, p.Sq) - 1), C::THREADS, reinterpret_cast<int*>(vec)) + NT - 1) / NT;
   }
   tc::tc_fence_before();
   __syncthreads();
@@ -655,9 +653,13 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
     float* mydarr = darr + w16 * dlen + p.R;         // centred on relative position 0
     float* myscr = dscr + w16 * 16;
     float nL = 0.f, nd = 0.f;  // !KEYS: -(lse log2 e) and -delta of this row
-    if (!KEYS) {
+    if (!KEYS) {  // while the first tiles are loaded and multiplied
       const float2 ld = lsed[((int64_t)b * p.H + hx) * sq_pad + x0 + r];
       nL = ld.x, nd = ld.y;
+      fill_vec(p, hx, vec, (int)threadIdx.x - 64, C::EW);
+      if (p.dtab)
+        for (int i = (int)threadIdx.x - 64; i < 16 * dlen; i += C::EW) darr[i] = 0.f;
+      tc::named_bar_sync(1, C::EW);
     }
     float far_lo = 0.f, far_hi = 0.f;
     int cur = -1;  // KEYS: the head whose bias is in myvec
