@@ -163,7 +163,7 @@ uint64_t up16(uint64_t v) { return (v + 15) / 16 * 16; }
 // 0.4 us on the tensor cores and 3 us on the FMA pipe, and a launch. At least two tiles a split. Measured, 16 heads x 4096 x 4096: 2 splits save a sixth of the walk
 // (3.5 waves) and their join takes 47 us of it back.
 int pick_splits(int64_t blocks, int64_t tk, int64_t out_elems, double tile_us) {
-  const int64_t sms = device_info().sm_count > 0 ? device_info().sm_count : 148;
+  const int64_t sms = 2 * (device_info().sm_count > 0 ? device_info().sm_count : 148);  // two blocks to an SM
   int best = 1;
   double best_cost = 1e30;
   for (int64_t ns = 1; ns <= std::max<int64_t>(1, std::min<int64_t>(tk / 2, 64)); ++ns) {
