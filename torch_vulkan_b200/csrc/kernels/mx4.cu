@@ -6,6 +6,8 @@
 // saturating) is the cvt.rn.satfinite.e2m1x2 instruction; reading back is one exact product per element.
 #include "mx4.cuh"
 
+#include <type_traits>
+
 namespace b2 {
 namespace {
 
@@ -49,38 +51,49 @@ __global__ void __launch_bounds__(256) mx4_quantize_k(const T* __restrict__ x, u
   const int64_t row0 = ((int64_t)blockIdx.x * (256 >> txl) + (threadIdx.x >> txl)) * kU;
   const int n = (int)max((int64_t)0, min((int64_t)8, cols - c0));
   float v[kU][8];
+  const T* px = x + row0 * ld + c0;
 #pragma unroll
-  for (int u = 0; u < kU; ++u) {
+  for (int u = 0; u < kU; ++u, px += ld) {
     if (row0 + u < rows && n > 0) {
-      load8<T, VEC>(x + (row0 + u) * ld + c0, n, v[u]);
+      load8<T, VEC>(px, n, v[u]);
     } else {
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[u][k] = 0.f;
     }
   }
+  const bool write_codes = c0 < cb * 2, write_scale = (g & 3) == 0 && g < groups;
+  const int64_t padded = (rows + 127) / 128 * 128;
+  uint8_t* pc = codes + row0 * cb + g * 4;
+  uint8_t* ps = scales + scale_at(row0, g >> 2, nkb);  // kU rows share a group of 32: 16 bytes apart
 #pragma unroll
-  for (int u = 0; u < kU; ++u) {
-    const int64_t row = row0 + u;
-    float am = 0.f;
-    bool bad = false;
+  for (int u = 0; u < kU; ++u, pc += cb, ps += 16) {
+    const bool in = row0 + u < rows;
+    uint32_t top = 0;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float a = fabsf(v[u][k]);
-      bad |= !(a <= 3.402823466e38f);
-      am = fmaxf(am, a);
-    }
-    am = bad ? INFINITY : am;  // the block's maximum carries the mark
-    am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 1));
-    am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 2));
-    const uint32_t code = scale_code(am, am == INFINITY);
-    if (row < rows && c0 < cb * 2) {
+    for (int k = 0; k < 8; ++k) top = max(top, magnitude_bits(v[u][k]));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const uint32_t code = scale_code(top);
+    if (in && write_codes) {
       const float inv = inverse_scale(code);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[u][k] = code == 255u ? 0.f : v[u][k] * inv;
-      *reinterpret_cast<uint32_t*>(codes + row * cb + g * 4) = e2m1x8(v[u]);
+      for (int k = 0; k < 8; ++k) v[u][k] *= inv;
+      const uint32_t c = e2m1x8(v[u]);
+      *reinterpret_cast<uint32_t*>(pc) = code == 255u ? 0u : c;
     }
-    if ((g & 3) == 0 && g < groups && row < (rows + 127) / 128 * 128)
-      scales[scale_at(row, g >> 2, nkb)] = (row < rows && c0 < cols) ? (uint8_t)code : (uint8_t)0;
+    if (write_scale && row0 + u < padded) *ps = (in && n > 0) ? (uint8_t)code : (uint8_t)0;
+  }
+}
+
+// Two floats -> two T, rounded to nearest.
+template <typename T>
+__device__ __forceinline__ uint32_t pack_pair(float a, float b) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
   }
 }
 
@@ -94,14 +107,18 @@ __global__ void __launch_bounds__(256) mx4_dequantize_k(const uint8_t* __restric
   const int n = (int)max((int64_t)0, min((int64_t)8, cols - g * 8));
   if (n == 0) return;
   uint32_t c[kU], sc[kU];
+  const uint8_t* pc = codes + row0 * cb + g * 4;
+  const uint8_t* ps = scales + scale_at(row0, g >> 2, nkb);  // kU rows share a group of 32: 16 bytes apart
 #pragma unroll
   for (int u = 0; u < kU; ++u) {
-    const int64_t row = min(row0 + u, rows - 1);
-    c[u] = *reinterpret_cast<const uint32_t*>(codes + row * cb + g * 4);
-    sc[u] = scales[scale_at(row, g >> 2, nkb)];
+    if (row0 + u < rows) {
+      c[u] = *reinterpret_cast<const uint32_t*>(pc + u * cb);
+      sc[u] = ps[16 * u];
+    }
   }
+  T* o = out + row0 * ld + g * 8;
 #pragma unroll
-  for (int u = 0; u < kU; ++u) {
+  for (int u = 0; u < kU; ++u, o += ld) {
     if (row0 + u >= rows) break;
     const float s = e8m0_to_f32(sc[u]);
     __half2 h[4];
@@ -112,17 +129,13 @@ __global__ void __launch_bounds__(256) mx4_dequantize_k(const uint8_t* __restric
       const float2 f = __half22float2(h[k]);
       v[2 * k] = f.x * s, v[2 * k + 1] = f.y * s;
     }
-    T* o = out + (row0 + u) * ld + g * 8;
     if (VEC) {
       if constexpr (sizeof(T) == 4) {
         *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
         *(reinterpret_cast<float4*>(o) + 1) = make_float4(v[4], v[5], v[6], v[7]);
       } else {
-        uint4 raw;
-        T* t = reinterpret_cast<T*>(&raw);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) t[k] = from_f32<T>(v[k]);
-        *reinterpret_cast<uint4*>(o) = raw;
+        *reinterpret_cast<uint4*>(o) = make_uint4(pack_pair<T>(v[0], v[1]), pack_pair<T>(v[2], v[3]), pack_pair<T>(v[4], v[5]),
+                                                  pack_pair<T>(v[6], v[7]));
       }
     } else {
       for (int k = 0; k < n; ++k) o[k] = from_f32<T>(v[k]);

@@ -13,10 +13,11 @@ __host__ __device__ __forceinline__ int64_t scale_at(int64_t row, int64_t blk, i
   return ((row >> 7) * nkb + (blk >> 2)) * 512 + (row & 31) * 16 + ((row & 127) >> 5) * 4 + (blk & 3);
 }
 
-// The E8M0 code of a block whose largest magnitude is am: 2^(floor(log2 am) - 2) is the fp32 exponent field less two; a
-// block that holds an infinity or a NaN gets the NaN scale.
-__device__ __forceinline__ uint32_t scale_code(float am, bool bad) {
-  return bad ? 255u : (uint32_t)max((int)(__float_as_uint(am) >> 23) - 2, 0);
+// The E8M0 code of a block, from the largest of its elements' bits without the sign (NaN and infinity are the largest):
+// 2^(floor(log2 amax) - 2) is the fp32 exponent field less two; a block with an infinity or a NaN gets the NaN scale.
+__device__ __forceinline__ uint32_t magnitude_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+__device__ __forceinline__ uint32_t scale_code(uint32_t top) {
+  return top >= 0x7f800000u ? 255u : (uint32_t)max((int)(top >> 23) - 2, 0);
 }
 // 2^(127 - code), by which the elements are divided (exactly).
 __device__ __forceinline__ float inverse_scale(uint32_t code) {

@@ -68,8 +68,7 @@ __global__ void __launch_bounds__(NWARP * 32, 2) mx4_rows_kernel(const __grid_co
   for (int i = threadIdx.x; i < M * p.nblk; i += NWARP * 32) {
     const int m = i / p.nblk, blk = i - m * p.nblk;
     float v[32];
-    float am = 0.f;
-    bool bad = false;
+    uint32_t top = 0;
     const int n = m < p.M ? min(32, p.K - blk * 32) : 0;
     const __nv_bfloat16* px = p.x + (int64_t)m * p.x_ld + blk * 32;
 #pragma unroll
@@ -85,18 +84,14 @@ __global__ void __launch_bounds__(NWARP * 32, 2) mx4_rows_kernel(const __grid_co
       }
     }
 #pragma unroll
-    for (int k = 0; k < 32; ++k) {
-      const float a = fabsf(v[k]);
-      bad |= !(a <= 3.402823466e38f);
-      am = fmaxf(am, a);
-    }
-    const uint32_t code = mx4::scale_code(am, bad);
+    for (int k = 0; k < 32; ++k) top = max(top, mx4::magnitude_bits(v[k]));
+    const uint32_t code = mx4::scale_code(top);
     const float inv = mx4::inverse_scale(code);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       float w[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) w[k] = bad ? 0.f : v[q * 8 + k] * inv;
+      for (int k = 0; k < 8; ++k) w[k] = code == 255u ? 0.f : v[q * 8 + k] * inv;
       const uint32_t c = mx4::e2m1x8(w);
 #pragma unroll
       for (int hlf = 0; hlf < 2; ++hlf) {
