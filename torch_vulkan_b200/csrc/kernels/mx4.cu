@@ -5,6 +5,7 @@
 // max(e - 2, 0), and multiplying by 2^(127 - code) divides exactly. The E2M1 rounding (nearest, ties to even,
 // saturating) is the cvt.rn.satfinite.e2m1x2 instruction; reading back is one exact product per element.
 #include "mx4.cuh"
+#include "tc_ptx.cuh"
 
 #include <type_traits>
 
@@ -50,6 +51,8 @@ __global__ void __launch_bounds__(256) mx4_quantize_k(const T* __restrict__ x, u
   const int64_t c0 = g * 8;
   const int64_t row0 = ((int64_t)blockIdx.x * (256 >> txl) + (threadIdx.x >> txl)) * kU;
   const int n = (int)max((int64_t)0, min((int64_t)8, cols - c0));
+  tc::pdl_wait();
+  tc::pdl_trigger();
   float v[kU][8];
   const T* px = x + row0 * ld + c0;
 #pragma unroll
@@ -105,6 +108,8 @@ __global__ void __launch_bounds__(256) mx4_dequantize_k(const uint8_t* __restric
   const int64_t cb = (cols + kBlk - 1) / kBlk * 16;
   const int64_t row0 = ((int64_t)blockIdx.x * (256 >> txl) + (threadIdx.x >> txl)) * kU;
   const int n = (int)max((int64_t)0, min((int64_t)8, cols - g * 8));
+  tc::pdl_wait();
+  tc::pdl_trigger();
   if (n == 0) return;
   uint32_t c[kU], sc[kU];
   const uint8_t* pc = codes + row0 * cb + g * 4;
@@ -163,14 +168,8 @@ int quantize_t(const b2_mx4_args* a, cudaStream_t st) {
   const bool vec = a->cols % 8 == 0 && ((uintptr_t)a->x & 15) == 0 && (a->ld * (int64_t)sizeof(T)) % 16 == 0;
   Walk w;
   if (!make_walk((a->rows + 127) / 128 * 128, nkb * 16, w)) return fail(B2_ERR_ARG, "mx4_quantize: matrix too large");
-  {
-    LaunchScope ls("mx4_quantize", st);
-    if (vec)
-      mx4_quantize_k<T, true><<<w.grid, 256, 0, st>>>((const T*)a->x, a->codes, a->scales, a->rows, a->cols, a->ld, nkb, w.txl);
-    else
-      mx4_quantize_k<T, false><<<w.grid, 256, 0, st>>>((const T*)a->x, a->codes, a->scales, a->rows, a->cols, a->ld, nkb, w.txl);
-  }
-  return after_launch("mx4_quantize");
+  return launch_pdl("mx4_quantize", vec ? mx4_quantize_k<T, true> : mx4_quantize_k<T, false>, w.grid, dim3(256), 0, st,
+                    (const T*)a->x, a->codes, a->scales, a->rows, a->cols, a->ld, nkb, w.txl);
 }
 
 template <typename T>
@@ -179,14 +178,8 @@ int dequantize_t(const b2_mx4_args* a, cudaStream_t st) {
   const bool vec = a->cols % 8 == 0 && ((uintptr_t)a->out & 15) == 0 && (a->ld * (int64_t)sizeof(T)) % 16 == 0;
   Walk w;
   if (!make_walk(a->rows, (a->cols + 7) / 8, w)) return fail(B2_ERR_ARG, "mx4_dequantize: matrix too large");
-  {
-    LaunchScope ls("mx4_dequantize", st);
-    if (vec)
-      mx4_dequantize_k<T, true><<<w.grid, 256, 0, st>>>(a->codes, a->scales, (T*)a->out, a->rows, a->cols, a->ld, nkb, w.txl);
-    else
-      mx4_dequantize_k<T, false><<<w.grid, 256, 0, st>>>(a->codes, a->scales, (T*)a->out, a->rows, a->cols, a->ld, nkb, w.txl);
-  }
-  return after_launch("mx4_dequantize");
+  return launch_pdl("mx4_dequantize", vec ? mx4_dequantize_k<T, true> : mx4_dequantize_k<T, false>, w.grid, dim3(256), 0, st,
+                    (const uint8_t*)a->codes, (const uint8_t*)a->scales, (T*)a->out, a->rows, a->cols, a->ld, nkb, w.txl);
 }
 
 int check(const b2_mx4_args* a, const void* data, const char* what) {

@@ -321,13 +321,17 @@ __global__ void __launch_bounds__(DX ? 320 : 448, 1)
           tc::tmem_ld32(tbase + (a * MS + ms) * BN + half * (BN / 2) + c * 32 + lane_off, v);
           tc::tmem_wait_ld();
           tc::reg_fence32(v);
-          const float* bc = bs + half * (BN / 2) + c * 32;
+          const float4* bc = reinterpret_cast<const float4*>(bs + half * (BN / 2) + c * 32);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            float lo = __uint_as_float(v[2 * e]), hi = __uint_as_float(v[2 * e + 1]);
-            if (!DX) lo += bc[2 * e], hi += bc[2 * e + 1];
-            __nv_bfloat162 b2v = __floats2bfloat162_rn(lo, hi);
-            w[c][e] = *reinterpret_cast<uint32_t*>(&b2v);
+          for (int e = 0; e < 8; ++e) {
+            float2 lo = make_float2(__uint_as_float(v[4 * e]), __uint_as_float(v[4 * e + 1]));
+            float2 hi = make_float2(__uint_as_float(v[4 * e + 2]), __uint_as_float(v[4 * e + 3]));
+            if (!DX) {
+              const float4 bq = bc[e];
+              lo = __fadd2_rn(lo, make_float2(bq.x, bq.y)), hi = __fadd2_rn(hi, make_float2(bq.z, bq.w));
+            }
+            __nv_bfloat162 p0 = __floats2bfloat162_rn(lo.x, lo.y), p1 = __floats2bfloat162_rn(hi.x, hi.y);
+            w[c][2 * e] = *reinterpret_cast<uint32_t*>(&p0), w[c][2 * e + 1] = *reinterpret_cast<uint32_t*>(&p1);
           }
         }
         if (ms == MS - 1) {
@@ -441,15 +445,24 @@ int launch4(const b2_mx4_gemm_args* a, const Shape& sh, cudaStream_t st) {
   if (!ok) return fail(B2_ERR_ARG, std::string(name) + ": tensor map rejected");
   const int units = std::min(p.tiles_m * p.tiles_n, device_info().sm_count / CG);
   if (CG == 1) return launch_pdl(name, kern, dim3(units), dim3(C::THREADS), C::SMEM, st, ta, tw, tsa, tsw, th, tb, p);
+  // clusters of two; programmatic dependent launch as for single CTAs (outside stream capture)
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(units * CG);
   cfg.blockDim = dim3(C::THREADS);
   cfg.dynamicSmemBytes = C::SMEM;
   cfg.stream = st;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = CG, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
-  cfg.attrs = at, cfg.numAttrs = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(st, &cs) != cudaSuccess) {
+    (void)cudaGetLastError();
+    cs = cudaStreamCaptureStatusActive;
+  }
+  cfg.attrs = at;
+  cfg.numAttrs = (pdl_enabled() && cs == cudaStreamCaptureStatusNone) ? 2 : 1;
   cudaError_t e;
   {
     LaunchScope ls(name, st);
