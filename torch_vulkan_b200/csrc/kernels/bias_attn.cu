@@ -80,6 +80,8 @@ __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ Para
   const int64_t nrow = (int64_t)p.B * p.H * p.Sq;
   const int lane = threadIdx.x & 31;
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  tc::pdl_wait();
+  tc::pdl_trigger();
   if (row >= nrow) return;
   const int64_t i = row % p.Sq, bh = row / p.Sq;
   const T* o = row_of<T>((const void*)p.o, p.o_s, (int)(bh / p.H), (int)(bh % p.H), i);
@@ -96,6 +98,8 @@ __global__ void __launch_bounds__(256) dtable_kernel(const float* __restrict__ p
                                                      int H, int nt, int nb) {
   const int lane = threadIdx.x & 31;
   const int w = blockIdx.x * 8 + (threadIdx.x >> 5);
+  tc::pdl_wait();
+  tc::pdl_trigger();
   if (w >= nb * H) return;
   const int n = w / H, h = w % H;
   float s = 0.f;
@@ -255,11 +259,7 @@ template <typename T>
 struct Delta {
   static int run(const Params& p, float* delta, cudaStream_t st) {
     const int64_t rows = (int64_t)p.B * p.H * p.Sq;
-    {
-      LaunchScope ls("bias_attn_delta", st);
-      delta_kernel<T><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(p, delta);
-    }
-    return after_launch("bias_attn_delta");
+    return launch_pdl("bias_attn_delta", delta_kernel<T>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, p, delta);
   }
 };
 
@@ -341,11 +341,8 @@ extern "C" int b2_bias_attn_bwd(const b2_bias_attn_args* a, b2_stream_t stream) 
     if (int rc = simt_bwd(p, a->dtype, st)) return rc;
   }
   if (a->dtable) {
-    {
-      LaunchScope ls("bias_attn_dtable", st);
-      dtable_kernel<<<(unsigned)((p.nb * p.H + 7) / 8), 256, 0, st>>>(p.dtab, a->dtable, p.B, p.H, pl.ntq, p.nb);
-    }
-    return after_launch("bias_attn_dtable");
+    return launch_pdl("bias_attn_dtable", dtable_kernel, dim3((unsigned)((p.nb * p.H + 7) / 8)), dim3(256), 0, st,
+                      (const float*)p.dtab, a->dtable, p.B, p.H, pl.ntq, p.nb);
   }
   return 0;
 }

@@ -5,9 +5,10 @@
 // head, at most 8). A key's row of K is spread over LPK lanes, 16 bytes each, so a warp takes 32 / LPK keys at a time and
 // U such groups of K and V are loaded before the first is used. Every group of lanes keeps its own running maximum, sum
 // and output in fp32; they are joined through shared memory at the end, and the blocks of a head by the combine kernel.
-// A tensor-core tile would spend 128 rows of exponentials on these few: 74 us against ROWSUS for one row of 8 x 16 heads over 8192
+// A tensor-core tile would spend 128 rows of exponentials on these few: 74 us against 54 for one row of 8 x 16 heads over 8192
 // keys of 64 (268 MB of K and V, 41 us at the measured memory rate).
 #include "bias_attn.cuh"
+#include "tc_ptx.cuh"
 
 namespace b2 {
 namespace bias_attn {
@@ -34,6 +35,8 @@ __global__ void __launch_bounds__(NW * 32) rows_kernel(const __grid_constant__ P
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int sub = lane / LPK, part = lane % LPK;
   const int b = (int)blockIdx.x / p.Hk, hk = (int)blockIdx.x % p.Hk, G = p.H / p.Hk;
+  tc::pdl_wait();
+  tc::pdl_trigger();
   const int vl = 2 * p.R + 1;
   const int end = key_end(p, p.Sq - 1);
   const int per = ((end + p.nsplit - 1) / p.nsplit + NW * KPW * U - 1) / (NW * KPW * U) * (NW * KPW * U);
@@ -172,11 +175,7 @@ int launch(const Params& p, int rows, cudaStream_t st) {
   const int G = p.H / p.Hk;
   const int smem = std::max(G * (2 * p.R + 1), GRP * (LPK * N + 2)) * 4;
   if (int rc = allow_smem<rows_kernel<T, R, LPK>>(smem, "bias_attn_rows")) return rc;
-  {
-    LaunchScope ls("bias_attn_rows", st);
-    rows_kernel<T, R, LPK><<<dim3(p.B * p.Hk, p.nsplit), NW * 32, smem, st>>>(p, rows);
-  }
-  return after_launch("bias_attn_rows");
+  return launch_pdl("bias_attn_rows", rows_kernel<T, R, LPK>, dim3(p.B * p.Hk, p.nsplit), dim3(NW * 32), smem, st, p, rows);
 }
 
 template <typename T, int R>

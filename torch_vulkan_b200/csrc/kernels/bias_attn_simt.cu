@@ -392,6 +392,8 @@ int smem_bytes(const Params& p, int own, int walked, int ps) {
   return (own * Smem<DP>::OTILE + walked * Smem<DP>::TILE + ps * OWN * PS + 2 * p.R + 1 + 4 * T64 + 4) * 4 + T64;
 }
 
+// Plain launches: these blocks are far fewer than the SMs could hold, and blocks that start early, beside a kernel that is
+// still draining, are packed onto the SMs that are free (157 us a step instead of 113 at 203 x 331 x 40, 6 heads).
 template <typename T, int DP>
 int fwd_t(const Params& p, cudaStream_t st) {
   const int sm = smem_bytes<DP>(p, 1, 2, 1);

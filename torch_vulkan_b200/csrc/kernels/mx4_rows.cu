@@ -6,6 +6,7 @@
 // one byte permutation as the table lookup, positive and negative ones apart. Every block of threads quantises x itself
 // (it is a few KB), so the call is one launch.
 #include "mx4.cuh"
+#include "tc_ptx.cuh"
 
 namespace b2 {
 namespace {
@@ -61,6 +62,8 @@ __global__ void __launch_bounds__(NWARP * 32, 2) mx4_rows_kernel(const __grid_co
       sc[r] = p.scales[mx4::scale_at(n, blk, p.nkb)];
     }
   };
+  tc::pdl_wait();
+  tc::pdl_trigger();
   fetch(n0, lane);
   // x as bytes (twice the E2M1 values) in 32-byte blocks, [M][nblk], and a quarter of its scales
   int* xs = reinterpret_cast<int*>(sm16);
@@ -176,11 +179,7 @@ int launch_rows(const RowsP& p, cudaStream_t st) {
   const int64_t unit = NWARP * rows_per_warp(M), need = ((int64_t)p.N + unit - 1) / unit;
   const int64_t turns = (need + device_info().sm_count * 2 - 1) / (device_info().sm_count * 2);
   const int grid = (int)((need + turns - 1) / turns);
-  {
-    LaunchScope ls("mx4_rows", st);
-    mx4_rows_kernel<M><<<grid, NWARP * 32, smem, st>>>(p);
-  }
-  return after_launch("mx4_rows");
+  return launch_pdl("mx4_rows", mx4_rows_kernel<M>, dim3(grid), dim3(NWARP * 32), smem, st, p);
 }
 
 }  // namespace
