@@ -3,8 +3,8 @@
 Importing this package loads two native libraries built for sm_100a (see ``_build.py``):
 
 * ``libb2rt.so`` — the C ABI (``include/b2rt.h``): slab allocator, stream/launch layer, stats, and
-  every kernel (tcgen05 GEMM and int8-dequant GEMM, fused attention, softmax/LayerNorm row kernels,
-  optimizer ternaries);
+  every kernel (tcgen05 GEMM, int8-dequant GEMM and 4-bit block-scaled GEMM, fused attention without and
+  with a relative position bias, softmax/LayerNorm row kernels, optimizer ternaries);
 * ``_b2ops.so`` — the ATen shim that registers ``mm/bmm/addmm/baddbmm``, the SDPA
   ``_fused_attention_overrideable`` pair, ``_softmax``/``_safe_softmax``/``_softmax_backward_data``,
   ``native_layer_norm[_backward]`` and ``addcmul(_)/addcdiv(_)/lerp(_).Scalar`` for the CUDA key.
