@@ -89,6 +89,7 @@ int tc_fwd(const Params& p, bool bf16, cudaStream_t st);
 int tc_bwd(const Params& p, bool bf16, float2* lsed, int sq_pad, cudaStream_t st);
 constexpr int kTcTile = 128;
 bool rows_eligible(const b2_bias_attn_args* a);              // bias_attn_rows.cu
+int rows_blocks_per_sm(const b2_bias_attn_args* a);
 int rows_fwd(const Params& p, int dtype, cudaStream_t st);
 constexpr int kTcPad = 384;  // (lse, delta) rows are padded to a multiple of every tile height
 
