@@ -323,3 +323,50 @@ def test_c_entry_points_refuse_bad_arguments():
     lib = ctypes.CDLL(tv._LIB_PATH)
     assert lib.b2_bias_attn_fwd(None, None) < 0 and lib.b2_bias_attn_bwd(None, None) < 0
     assert lib.b2_bias_bucket(ctypes.c_int64(3), 31, 128, 1) == -1 and lib.b2_bias_bucket(ctypes.c_int64(3), 32, 2000, 1) == -1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("B,H,Hk,Sq,Sk,D", [(2, 16, 2, 1, 700, 128), (1, 12, 1, 1, 130, 40), (1, 10, 2, 3, 515, 96), (2, 8, 1, 7, 1000, 64),
+                                            (1, 40, 1, 1, 65, 8), (1, 6, 2, 8, 2049, 80), (3, 3, 3, 5, 17, 64)])
+def test_few_queries_of_heads_that_share_their_keys(dt, B, H, Hk, Sq, Sk, D):
+    """Rows of several heads and queries side by side, causal and not, with one sample that sees no key."""
+    import torch_vulkan_b200 as tv
+
+    q, k, v, _, table, m = _case(B, H, Hk, Sq, Sk, D, dt, H + Sk, "random")
+    for mask, kw in ((m, {}), (None, dict(causal=True, bidirectional=False, q_offset=Sk - Sq)),
+                     (m, dict(causal=True, q_offset=2))):  # most keys lie past the last query
+        o = tv.bucket_bias_attention(q.cuda(), k.cuda(), v.cuda(), table.cuda(), key_mask=None if mask is None else mask.cuda(), **kw)
+        _near(o, ot.bias_attention(q, k, v, table, key_mask=mask, **kw), OUT[dt], "o")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTS)
+def test_a_masked_key_of_a_cache_may_hold_anything(dt):
+    import torch_vulkan_b200 as tv
+
+    q, k, v, _, table, m = _case(2, 8, 2, 2, 300, 64, dt, 21, "tail")
+    ref = ot.bias_attention(q, k, v, table, key_mask=m)
+    k, v = k.clone(), v.clone()
+    k.masked_fill_(~m[:, None, :, None], float("nan"))
+    v.masked_fill_(~m[:, None, :, None], float("inf"))
+    o = tv.bucket_bias_attention(q.cuda(), k.cuda(), v.cuda(), table.cuda(), key_mask=m.cuda())
+    _near(o, ref, OUT[dt], "o")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Sq", [1, 100])
+def test_in_a_graph(Sq):
+    """Captured once, replayed on new values: the same bits as the call itself."""
+    import torch_vulkan_b200 as tv
+
+    q, k, v, _, table, _ = (t.cuda() if t is not None else None for t in _case(2, 4, 2, Sq, 1500, 64, torch.bfloat16, 3))
+    kw = dict(causal=True, bidirectional=False, q_offset=1500 - Sq)
+    tv.bucket_bias_attention(q, k, v, table, **kw)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        o = tv.bucket_bias_attention(q, k, v, table, **kw)
+    q.copy_(torch.randn_like(q))
+    table.add_(1.0).mul_(0.5)
+    g.replay()
+    assert torch.equal(o, tv.bucket_bias_attention(q, k, v, table, **kw))

@@ -190,7 +190,8 @@ Plan make_plan(const b2_bias_attn_args* a, bool bwd) {
     // partly filled round counts as that many; a block costs its keys and about 75 keys' worth of set-up, the join 64 + 4 ns.
     // 8 x 16 heads over 8192 keys: 50.2, 52.2, 48.0, 49.8 and 51.8 us with 6, 7, 11, 13 and 24 splits.
     pl.rows = true;
-    const int64_t blocks = a->B * a->Hk, sms = device_info().sm_count > 0 ? device_info().sm_count : 148;
+    const int64_t groups = (a->Sq * (a->H / a->Hk) + 7) / 8;
+    const int64_t blocks = a->B * a->Hk * groups, sms = device_info().sm_count > 0 ? device_info().sm_count : 148;
     const int64_t res = rows_blocks_per_sm(a), least = (2 * res + 2) / 3;
     int64_t best = INT64_MAX;
     for (int64_t ns = 1; ns <= std::max<int64_t>(1, std::min<int64_t>(a->Sk / 64, 128)); ++ns) {

@@ -1,13 +1,14 @@
 // Relative-position-bias attention for a few query rows (a decoder's new tokens against its cache): forward, bound by
 // reading K and V once.
 //
-// A block owns one key/value head and a range of keys, for all query rows that read them (Sq x the heads that share the
-// head, at most 8). The blocks of a head are joined by the combine kernel.
+// A block owns one key/value head, a range of keys, and up to 8 of the query rows that read them (Sq x the heads that share
+// the head). Blocks of the same keys are neighbours, so that the keys come from memory once and from L2 after that. The
+// ranges of a row are joined by the combine kernel.
 //
 // 16-bit types: rows_mma_kernel. The keys are the 16 rows of an m16n8k16 product and the query rows its 8 columns,
 // S^T = K Q^T and O^T = V^T P^T, so that 8 query rows cost what one does and nothing is computed for rows that are not
 // there. (A tcgen05 tile has 128 rows of keys or of queries: with the queries as its rows it spends 128 rows of
-// exponentials on these few, 74 us for the case below.) Each warp copies its own tiles of 16 keys through a ring in shared
+// exponentials on these few, 79 us for the case below.) Each warp copies its own tiles of 16 keys through a ring in shared
 // memory, without a barrier of the block, and keeps its own reference, sum and O^T in fp32 until the end. P enters the second
 // product as its rounded value plus the rounded rest, so that P is good to 2^-17 and the sums are fp32.
 // One row of 8 x 16 heads over 8192 keys of 64 (268 MB of K and V, 41 us at the measured memory rate): 48 us with the join;
@@ -79,13 +80,15 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
 
 // KD: 16-wide steps of the head dimension.
 template <typename T, int KD>
-__global__ void __launch_bounds__(NW * 32) rows_mma_kernel(const __grid_constant__ Params p, int rows) {
+__global__ void __launch_bounds__(NW * 32) rows_mma_kernel(const __grid_constant__ Params p, int groups) {
   constexpr int CH = 2 * KD, RB = CH * 16, DP = KD * 16, TILE = KT * RB, PASS = 32 / CH, STEP = NW * KT;
   extern __shared__ __align__(128) uint8_t smem[];
-  float* bias = reinterpret_cast<float*>(smem + NW * ST * 2 * TILE);  // [G][2R + 1] of the block's heads
+  float* bias = reinterpret_cast<float*>(smem + NW * ST * 2 * TILE);  // [heads][2R + 1] of the heads of the block's rows
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
-  const int b = (int)blockIdx.x / p.Hk, hk = (int)blockIdx.x % p.Hk, G = p.H / p.Hk;
+  const int bh = (int)blockIdx.x / groups, b = bh / p.Hk, hk = bh % p.Hk, G = p.H / p.Hk;
+  const int first = (int)blockIdx.x % groups * 8, rows = min(8, p.Sq * G - first);
+  const int h0 = first / p.Sq, nh = (first + rows - 1) / p.Sq - h0 + 1;  // the heads of these rows, after hk * G
   tc::pdl_wait();
   tc::pdl_trigger();
   const int vl = 2 * p.R + 1;
@@ -129,15 +132,16 @@ __global__ void __launch_bounds__(NW * 32) rows_mma_kernel(const __grid_constant
 
   // the part of the bias that these keys reach: a single entry for keys wholly beyond max_distance
   const int lo = max(-p.R, min(p.R, j0 - (p.Sq - 1) - p.q_off)), span = max(-p.R, min(p.R, j1 - 1 - p.q_off)) - lo + 1;
-  for (int i = threadIdx.x; i < G * span; i += NW * 32) {
+  for (int i = threadIdx.x; i < nh * span; i += NW * 32) {
     const int h = i / span, rel = lo + i - h * span;
-    bias[h * vl + rel + p.R] = bias_at(p, hk * G + h, rel);
+    bias[h * vl + rel + p.R] = bias_at(p, hk * G + h0 + h, rel);
   }
-  // Q^T as the second operand: this lane holds dims 16 k + 2 t (+ 1, + 8, + 9) of row g; row r is query r % Sq of head
-  // hk * G + r / Sq
+  // Q^T as the second operand: this lane holds dims 16 k + 2 t (+ 1, + 8, + 9) of row g; row r is query (first + r) % Sq
+  // of head hk * G + (first + r) / Sq
   uint32_t q[KD][2];
   {
-    const T* qr = row_of<T>(p.q, p.q_s, b, hk * G + min(g, rows - 1) / p.Sq, min(g, rows - 1) % p.Sq);
+    const int r = first + min(g, rows - 1);
+    const T* qr = row_of<T>(p.q, p.q_s, b, hk * G + r / p.Sq, r % p.Sq);
 #pragma unroll
     for (int k = 0; k < KD; ++k)
 #pragma unroll
@@ -148,9 +152,9 @@ __global__ void __launch_bounds__(NW * 32) rows_mma_kernel(const __grid_constant
   }
   const int r0 = 2 * t, r1 = 2 * t + 1;  // the two rows whose scores this lane holds
   const bool ok0 = r0 < rows, ok1 = r1 < rows;
-  const float* b0 = bias + min(r0 / p.Sq, G - 1) * vl + p.R;
-  const float* b1 = bias + min(r1 / p.Sq, G - 1) * vl + p.R;
-  const int e0 = r0 % p.Sq + p.q_off, e1 = r1 % p.Sq + p.q_off;
+  const float* b0 = bias + min((first + r0) / p.Sq - h0, nh - 1) * vl + p.R;
+  const float* b1 = bias + min((first + r1) / p.Sq - h0, nh - 1) * vl + p.R;
+  const int e0 = (first + r0) % p.Sq + p.q_off, e1 = (first + r1) % p.Sq + p.q_off;
   const float sc = p.scale * kLog2e;
   __syncthreads();
 
@@ -251,7 +255,7 @@ __global__ void __launch_bounds__(NW * 32) rows_mma_kernel(const __grid_constant
       L = fmaf(sml[2 * (w * 8 + r) + 1], c, L);
       acc = fmaf(so[(w * 8 + r) * LD + d], c, acc);
     }
-    const int h = hk * G + r / p.Sq, i = r % p.Sq;
+    const int h = hk * G + (first + r) / p.Sq, i = (first + r) % p.Sq;
     const int64_t row = ((int64_t)b * p.H + h) * p.Sq + i;
     const int64_t prow = (int64_t)blockIdx.y * p.B * p.H * p.Sq + row;
     if (p.nsplit > 1) {
@@ -267,13 +271,15 @@ __global__ void __launch_bounds__(NW * 32) rows_mma_kernel(const __grid_constant
 }
 
 int mma_smem(int kd, int G, int R) {
-  return std::max(NW * ST * 2 * KT * kd * 32 + G * (2 * R + 1) * 4, NW * 8 * (kd * 16 + 6) * 4);
+  return std::max(NW * ST * 2 * KT * kd * 32 + std::min(G, 8) * (2 * R + 1) * 4, NW * 8 * (kd * 16 + 6) * 4);
 }
 template <typename T, int KD>
 int launch_mma(const Params& p, int rows, cudaStream_t st) {
   const int smem = mma_smem(KD, p.H / p.Hk, p.R);
   if (int rc = allow_smem<rows_mma_kernel<T, KD>>(smem, "bias_attn_rows")) return rc;
-  return launch_pdl("bias_attn_rows", rows_mma_kernel<T, KD>, dim3(p.B * p.Hk, p.nsplit), dim3(NW * 32), smem, st, p, rows);
+  const int groups = (rows + 7) / 8;
+  return launch_pdl("bias_attn_rows", rows_mma_kernel<T, KD>, dim3(p.B * p.Hk * groups, p.nsplit), dim3(NW * 32), smem, st, p,
+                    groups);
 }
 template <typename T>
 int mma_by_width(const Params& p, int rows, cudaStream_t st) {
@@ -448,13 +454,15 @@ int by_rows(const Params& p, int rows, cudaStream_t st) {
 
 }  // namespace
 
-// At most 8 query rows per key/value head, and rows that are whole aligned 16-byte groups.
+// At most 8 queries (fp32: at most 8 query rows per key/value head), and rows that are whole aligned 16-byte groups. With
+// more queries the 128-row tiles win: 8 x 16 heads over 8192 keys of 64 take 90 us here with 16 queries and 127 with 24, 82
+// there; with 2 and 4 queries of 4 x 4 key/value heads shared by 8 over 16384 keys of 128, 42 and 75 us here, 160 there.
 bool rows_eligible(const b2_bias_attn_args* a) {
   const int64_t es = (int64_t)dtype_size(a->dtype), n = 16 / es;
   auto ok = [&](const void* t, const int64_t* s) {
     return ((uintptr_t)t & 15) == 0 && s[0] % n == 0 && s[1] % n == 0 && s[2] % n == 0;
   };
-  return a->Sk >= 1 && a->Sq * (a->H / a->Hk) <= 8 && a->D % n == 0 && ok(a->q, a->q_s) && ok(a->k, a->k_s) && ok(a->v, a->v_s);
+  return a->Sk >= 1 && a->Sq * (a->dtype == B2_F32 ? a->H / a->Hk : 1) <= 8 && a->D % n == 0 && ok(a->q, a->q_s) && ok(a->k, a->k_s) && ok(a->v, a->v_s);
 }
 
 int rows_blocks_per_sm(const b2_bias_attn_args* a) {
