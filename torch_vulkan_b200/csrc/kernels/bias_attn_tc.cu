@@ -81,9 +81,9 @@ __device__ __forceinline__ int trim_end(const Params& p, int b, int end, int nth
 // ==================================================================================================
 template <int D>
 struct Fwd {
-  static constexpr int BQ = 128, BK = 128, DCH = D / 64;
+  static constexpr int BQ = 128, BK = 64, DCH = D / 64;
   static constexpr int Q_BYTES = BQ * D * 2, KV_BYTES = BK * D * 2;
-  static constexpr int NK = D == 64 ? 2 : 1, NV = NK;  // K / V ring depths: what two blocks fit
+  static constexpr int NK = D == 64 ? 4 : 2, NV = NK;  // K / V ring depths: what two blocks fit
   static constexpr int OFF_Q = 0, OFF_K = Q_BYTES, OFF_V = OFF_K + NK * KV_BYTES, OFF_BAR = OFF_V + NV * KV_BYTES;
   static constexpr int OFF_VEC = OFF_BAR + 256;
   static constexpr int THREADS = 192;
@@ -108,9 +108,9 @@ __global__ void __launch_bounds__(192, 2)
   uint64_t* k_empty = k_full + NK;    // [NK]
   uint64_t* v_full = k_empty + NK;    // [NV]
   uint64_t* v_empty = v_full + NV;    // [NV]
-  uint64_t* s_full = v_empty + NV;    // S of tile t in TMEM
-  uint64_t* p_full = s_full + 1;      // P of tile t in TMEM over S
-  uint64_t* o_upd = p_full + 1;       // P V of tile t done
+  uint64_t* s_full = v_empty + NV;    // [2] S of tile t in buffer t & 1 of TMEM
+  uint64_t* p_full = s_full + 2;      // [2] P of tile t in TMEM over S
+  uint64_t* o_upd = p_full + 2;       // P V of tile t done
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_upd + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(o_upd + 2);
   float* vec = reinterpret_cast<float*>(smem + C::OFF_VEC);
@@ -125,7 +125,8 @@ __global__ void __launch_bounds__(192, 2)
     tc::mbar_init(q_full, 1);
     for (int i = 0; i < NK; ++i) tc::mbar_init(&k_full[i], 1), tc::mbar_init(&k_empty[i], 1);
     for (int i = 0; i < NV; ++i) tc::mbar_init(&v_full[i], 1), tc::mbar_init(&v_empty[i], 1);
-    tc::mbar_init(s_full, 1), tc::mbar_init(p_full, 128), tc::mbar_init(o_upd, 1);
+    for (int i = 0; i < 2; ++i) tc::mbar_init(&s_full[i], 1), tc::mbar_init(&p_full[i], 128);
+    tc::mbar_init(o_upd, 1);
     *abort_flag = 0;
     tc::fence_barrier_init();
   }
@@ -176,8 +177,8 @@ __global__ void __launch_bounds__(192, 2)
     }
   } else if (warp == 1) {
     if (lane == 0 && n > 0) {
-      // ---------------- MMA issuer: S_t = Q K_t^T; O += P_t V_t with P_t read from TMEM; then S_t+1 over P_t's columns
-      // (MMAs of one thread execute in order) ----------------
+      // ---------------- MMA issuer: S_t = Q K_t^T; O += P_t V_t with P_t read from TMEM; then S_t+2 over P_t's columns
+      // (MMAs of one thread execute in order), while the softmax warps are at S_t+1 ----------------
       constexpr uint32_t IDESC_S = tc::idesc_f16(128, C::BK, BF16, false, false);
       constexpr uint32_t IDESC_O = tc::idesc_f16(128, D, BF16, false, true);
       const tc::SDesc qd = tc::sdesc_parts(tc::smem_u32(smem + C::OFF_Q), 16, 1024);
@@ -189,17 +190,18 @@ __global__ void __launch_bounds__(192, 2)
         const tc::SDesc kd = tc::sdesc_parts(tc::smem_u32(smem + C::OFF_K + ks * C::KV_BYTES), 16, 1024);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = (k >> 2) * (C::BK * 128) + (k & 3) * 32;
-          tc::mma_f16_ss(tbase + C::T_S, tc::sdesc_at(qd, off), tc::sdesc_at(kd, off), IDESC_S, k > 0 ? 1u : 0u);
+          tc::mma_f16_ss(tbase + C::T_S + (t & 1) * C::BK, tc::sdesc_at(qd, (k >> 2) * (C::BQ * 128) + (k & 3) * 32),
+                         tc::sdesc_at(kd, (k >> 2) * (C::BK * 128) + (k & 3) * 32), IDESC_S, k > 0 ? 1u : 0u);
         }
-        tc::mma_commit(s_full);
+        tc::mma_commit(&s_full[t & 1]);
         tc::mma_commit(&k_empty[ks]);
         return true;
       };
       if (ok) ok = issue_s(0);
+      if (ok && n > 1) ok = issue_s(1);
       for (int t = 0; t < n && ok; ++t) {
         const int vs = t % NV;
-        if (!tc::mbar_wait(p_full, (uint32_t)(t & 1), p.err) ||
+        if (!tc::mbar_wait(&p_full[t & 1], (uint32_t)((t >> 1) & 1), p.err) ||
             !tc::mbar_wait(&v_full[vs], (uint32_t)((t / NV) & 1), p.err)) {
           ok = false;
           break;
@@ -208,15 +210,15 @@ __global__ void __launch_bounds__(192, 2)
         const tc::SDesc vd = tc::sdesc_parts(tc::smem_u32(smem + C::OFF_V + vs * C::KV_BYTES), C::BK * 128, 1024);
 #pragma unroll
         for (int k = 0; k < C::BK / 16; ++k)
-          tc::mma_f16_ts(tbase + C::T_O, tbase + C::T_S + k * 8, tc::sdesc_at(vd, k * 2048), IDESC_O, (k > 0 || t > 0) ? 1u : 0u);
+          tc::mma_f16_ts(tbase + C::T_O, tbase + C::T_S + (t & 1) * C::BK + k * 8, tc::sdesc_at(vd, k * 2048), IDESC_O, (k > 0 || t > 0) ? 1u : 0u);
         if (PREC) {
 #pragma unroll
           for (int k = 0; k < C::BK / 16; ++k)
-            tc::mma_f16_ts(tbase + C::T_O, tbase + C::T_S + 64 + k * 8, tc::sdesc_at(vd, k * 2048), IDESC_O, 1u);
+            tc::mma_f16_ts(tbase + C::T_O, tbase + C::T_S + (t & 1) * C::BK + 32 + k * 8, tc::sdesc_at(vd, k * 2048), IDESC_O, 1u);
         }
         tc::mma_commit(o_upd);
         tc::mma_commit(&v_empty[vs]);
-        if (t + 1 < n && !issue_s(t + 1)) ok = false;
+        if (t + 2 < n && !issue_s(t + 2)) ok = false;
       }
       if (!ok) *abort_flag = 1;
     }
@@ -225,7 +227,7 @@ __global__ void __launch_bounds__(192, 2)
     const int quarter = warp & 3;
     const int r = quarter * 32 + lane;
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
-    const uint32_t t_s = tbase + C::T_S, t_o = tbase + C::T_O;
+    const uint32_t t_o = tbase + C::T_O;
     const float sl2 = p.scale * kLog2e;
     const float2 sl22 = make_float2(sl2, sl2);
     float m = -INFINITY, l = 0.f;
@@ -234,30 +236,29 @@ __global__ void __launch_bounds__(192, 2)
     tc::named_bar_sync(1, 128);
     for (int t = 0; t < n; ++t) {
       const int k0 = (t0 + t) * C::BK;
-      uint32_t bits[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) bits[c] = key_bits(p, b, k0 + c * 32);
-      const bool full = (bits[0] & bits[1] & bits[2] & bits[3]) == 0xffffffffu;
-      if (!tc::mbar_wait(s_full, (uint32_t)(t & 1), p.err) || *abort_flag) {
+      const uint32_t t_s = tbase + C::T_S + (t & 1) * C::BK;
+      const uint32_t bits[2] = {key_bits(p, b, k0), key_bits(p, b, k0 + 32)};
+      const bool full = (bits[0] & bits[1]) == 0xffffffffu;
+      if (!tc::mbar_wait(&s_full[t & 1], (uint32_t)((t >> 1) & 1), p.err) || *abort_flag) {
         ok = false;
         break;
       }
       tc::tc_fence_after();
-      uint32_t sr[128];
+      uint32_t sr[C::BK];
       __syncwarp();
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tc::tmem_ld32(t_s + c * 32 + lane_off, sr + 32 * c);
+      for (int c = 0; c < C::BK / 32; ++c) tc::tmem_ld32(t_s + c * 32 + lane_off, sr + 32 * c);
       tc::tmem_wait_ld();
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tc::reg_fence32(sr + 32 * c);
+      for (int c = 0; c < C::BK / 32; ++c) tc::reg_fence32(sr + 32 * c);
       // bias: x = s * scale_log2 + bias. rel of column 0 against this tile's first row
       const int rel0 = k0 - q0 - p.q_off;
-      const bool near = rel0 - 127 < p.R && rel0 + 127 > -p.R;
+      const bool near = rel0 - 127 < p.R && rel0 + (C::BK - 1) > -p.R;
       float cst = 0.f;
       if (near) {
         const float* bv = vec + (rel0 - r + p.R + kPad);
 #pragma unroll
-        for (int e = 0; e < 128; e += 2) {
+        for (int e = 0; e < C::BK; e += 2) {
           const float2 x = __ffma2_rn(make_float2(__uint_as_float(sr[e]), __uint_as_float(sr[e + 1])), sl22,
                                       make_float2(bv[e], bv[e + 1]));
           sr[e] = __float_as_uint(x.x), sr[e + 1] = __float_as_uint(x.y);
@@ -267,14 +268,14 @@ __global__ void __launch_bounds__(192, 2)
       }
       if (!full) {
 #pragma unroll
-        for (int e = 0; e < 128; ++e)
+        for (int e = 0; e < C::BK; ++e)
           if (!((bits[e >> 5] >> (e & 31)) & 1u)) sr[e] = __float_as_uint(-INFINITY);
       }
       float mx8[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) mx8[e] = __uint_as_float(sr[e]);
 #pragma unroll
-      for (int e = 8; e < 128; ++e) mx8[e & 7] = fmaxf(mx8[e & 7], __uint_as_float(sr[e]));
+      for (int e = 8; e < C::BK; ++e) mx8[e & 7] = fmaxf(mx8[e & 7], __uint_as_float(sr[e]));
       const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])),
                              fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
       const float mul = near ? 1.f : sl2;  // scale > 0
@@ -286,7 +287,12 @@ __global__ void __launch_bounds__(192, 2)
         alpha = (m == -INFINITY) ? 0.f : ex2(m - m_blk);
         m = m_blk;
       }
-      if (t > 0 && __any_sync(0xffffffffu, need)) {
+      // every tile waits once for the last one's P V, so that no phase of the barrier is missed: here when O has to move to
+      // the new maximum, else when this tile's P is ready
+      const bool move = t > 0 && __any_sync(0xffffffffu, need);
+      if (move) {
+        if (!__all_sync(0xffffffffu, tc::mbar_wait(o_upd, (uint32_t)((t - 1) & 1), p.err))) { ok = false; break; }
+        tc::tc_fence_after();
 #pragma unroll 1
         for (int c = 0; c < D / 16; ++c) {
           uint32_t orow[16];
@@ -301,26 +307,24 @@ __global__ void __launch_bounds__(192, 2)
       const float nmv = (m == -INFINITY) ? -INFINITY : cst - m;  // nothing seen yet: exp2(-inf) = 0
       const float2 nm = make_float2(nmv, nmv), mul2 = make_float2(mul, mul);
       float2 rs4[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      {
+        uint32_t w[C::BK / 2];
 #pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {
-        uint32_t w[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const int c = hh * 64 + 2 * i;
-          const float2 x = __ffma2_rn(make_float2(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), mul2, nm);
+        for (int i = 0; i < C::BK / 2; ++i) {
+          const float2 x = __ffma2_rn(make_float2(__uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1])), mul2, nm);
           const float2 e2 = make_float2(ex2(x.x), ex2(x.y));
           rs4[i & 3] = __fadd2_rn(rs4[i & 3], e2);
           w[i] = pack2<BF16>(e2.x, e2.y);
-          if (PREC) {  // what the rounding left, packed over the score
+          if (PREC) {  // what the rounding left
             const float2 hi = unpack2<BF16>(w[i]);
-            sr[c] = pack2<BF16>(e2.x - hi.x, e2.y - hi.y);
+            sr[2 * i] = pack2<BF16>(e2.x - hi.x, e2.y - hi.y);
           }
         }
-        tc::tmem_st32(t_s + hh * 32 + lane_off, w);
+        tc::tmem_st32(t_s + lane_off, w);
         if (PREC) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) w[i] = sr[hh * 64 + 2 * i];
-          tc::tmem_st32(t_s + 64 + hh * 32 + lane_off, w);
+          for (int i = 0; i < C::BK / 2; ++i) w[i] = sr[2 * i];
+          tc::tmem_st32(t_s + 32 + lane_off, w);
         }
       }
       const float2 rs2 = __fadd2_rn(__fadd2_rn(rs4[0], rs4[1]), __fadd2_rn(rs4[2], rs4[3]));
@@ -328,20 +332,22 @@ __global__ void __launch_bounds__(192, 2)
       if (!full && p.mask != nullptr) {
         // masked keys may hold anything, and 0 * NaN is NaN in the P V product: clear their rows of V
         if (!tc::mbar_wait(&v_full[t % NV], (uint32_t)((t / NV) & 1), p.err)) { ok = false; break; }
-        if (!((bits[quarter] >> lane) & 1u)) {
+        if (!((bits[quarter & 1] >> lane) & 1u)) {  // warps 0 and 1 clear one half of a row, 2 and 3 the other
 #pragma unroll
           for (int c = 0; c < C::DCH; ++c) {
-            uint4* row = reinterpret_cast<uint4*>(smem + C::OFF_V + (t % NV) * C::KV_BYTES + c * (C::BK * 128) + r * 128);
+            uint4* row = reinterpret_cast<uint4*>(smem + C::OFF_V + (t % NV) * C::KV_BYTES + c * (C::BK * 128) + (r & 63) * 128 +
+                                                  (quarter >> 1) * 64);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) row[i] = make_uint4(0u, 0u, 0u, 0u);
+            for (int i = 0; i < 4; ++i) row[i] = make_uint4(0u, 0u, 0u, 0u);
           }
         }
         tc::fence_async_shared();
         __syncwarp();
       }
+      if (t > 0 && !move && !__all_sync(0xffffffffu, tc::mbar_wait(o_upd, (uint32_t)((t - 1) & 1), p.err))) { ok = false; break; }
       tc::tmem_wait_st();
       tc::tc_fence_before();
-      tc::mbar_arrive(p_full);
+      tc::mbar_arrive(&p_full[t & 1]);
     }
     // ---------------- epilogue ----------------
     if (ok && n > 0 && !tc::mbar_wait(o_upd, (uint32_t)((n - 1) & 1), p.err)) ok = false;
@@ -940,8 +946,8 @@ int fwd_t(const Params& p, cudaStream_t st) {
   auto kern = bias_fwd_tc<D, BF16, PREC>;
   if (int rc = allow_smem<bias_fwd_tc<D, BF16, PREC>>(smem, "bias_attn_fwd_tc")) return rc;
   CUtensorMap tq, tk, tv, to;
-  if (!bhsd_map(&tq, p.q, p.q_s, p.B, p.H, p.Sq, p.D, BF16, 128) || !bhsd_map(&tk, p.k, p.k_s, p.B, p.Hk, p.Sk, p.D, BF16, 128) ||
-      !bhsd_map(&tv, p.v, p.v_s, p.B, p.Hk, p.Sk, p.D, BF16, 128) || !store_map(&to, p.o, p.o_s, p.B, p.H, p.Sq, p.D, BF16))
+  if (!bhsd_map(&tq, p.q, p.q_s, p.B, p.H, p.Sq, p.D, BF16, 128) || !bhsd_map(&tk, p.k, p.k_s, p.B, p.Hk, p.Sk, p.D, BF16, C::BK) ||
+      !bhsd_map(&tv, p.v, p.v_s, p.B, p.Hk, p.Sk, p.D, BF16, C::BK) || !store_map(&to, p.o, p.o_s, p.B, p.H, p.Sq, p.D, BF16))
     return fail(B2_ERR_ARG, "bias_attn_fwd: tensor map rejected");
   dim3 grid((p.Sq + 127) / 128, p.B * p.H, p.nsplit);
   return launch_pdl("bias_attn_fwd_tc", kern, grid, dim3(C::THREADS), smem, st, tq, tk, tv, to, p);
