@@ -57,6 +57,16 @@ __device__ __forceinline__ uint32_t key_bits(const Params& p, int b, int k) {
   return __ballot_sync(0xffffffffu, ok);
 }
 
+// Whether keys k + lane and k + 32 + lane are there and seen, for a ballot later.
+struct KeyBytes {
+  bool a, b;
+};
+__device__ __forceinline__ KeyBytes key_bytes(const Params& p, int b, int k) {
+  const int j = k + (threadIdx.x & 31);
+  const uint8_t* m = p.mask ? p.mask + (int64_t)b * p.mask_sb : nullptr;
+  return {j < p.Sk && (m == nullptr || m[j] != 0), j + 32 < p.Sk && (m == nullptr || m[j + 32] != 0)};
+}
+
 // One past the last key below `end` that the mask leaves (every thread of the block; contains block barriers). The whole
 // row of the mask is read at once: one trip to memory. slot: shared memory, not in use otherwise.
 __device__ __forceinline__ int trim_end(const Params& p, int b, int end, int nthreads, int* slot) {
@@ -110,9 +120,9 @@ __global__ void __launch_bounds__(192, 2)
   uint64_t* v_empty = v_full + NV;    // [NV]
   uint64_t* s_full = v_empty + NV;    // [2] S of tile t in buffer t & 1 of TMEM
   uint64_t* p_full = s_full + 2;      // [2] P of tile t in TMEM over S
-  uint64_t* o_upd = p_full + 2;       // P V of tile t done
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_upd + 1);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(o_upd + 2);
+  uint64_t* o_upd = p_full + 2;       // [2] P V of the last tile but one, of the last
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_upd + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(o_upd + 3);
   float* vec = reinterpret_cast<float*>(smem + C::OFF_VEC);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -125,8 +135,7 @@ __global__ void __launch_bounds__(192, 2)
     tc::mbar_init(q_full, 1);
     for (int i = 0; i < NK; ++i) tc::mbar_init(&k_full[i], 1), tc::mbar_init(&k_empty[i], 1);
     for (int i = 0; i < NV; ++i) tc::mbar_init(&v_full[i], 1), tc::mbar_init(&v_empty[i], 1);
-    for (int i = 0; i < 2; ++i) tc::mbar_init(&s_full[i], 1), tc::mbar_init(&p_full[i], 128);
-    tc::mbar_init(o_upd, 1);
+    for (int i = 0; i < 2; ++i) tc::mbar_init(&s_full[i], 1), tc::mbar_init(&p_full[i], 4), tc::mbar_init(&o_upd[i], 1);
     *abort_flag = 0;
     tc::fence_barrier_init();
   }
@@ -216,7 +225,7 @@ __global__ void __launch_bounds__(192, 2)
           for (int k = 0; k < C::BK / 16; ++k)
             tc::mma_f16_ts(tbase + C::T_O, tbase + C::T_S + (t & 1) * C::BK + 32 + k * 8, tc::sdesc_at(vd, k * 2048), IDESC_O, 1u);
         }
-        tc::mma_commit(o_upd);
+        if (t >= n - 2) tc::mma_commit(&o_upd[t - (n - 2)]);
         tc::mma_commit(&v_empty[vs]);
         if (t + 2 < n && !issue_s(t + 2)) ok = false;
       }
@@ -234,11 +243,15 @@ __global__ void __launch_bounds__(192, 2)
     bool ok = true;
     fill_vec(p, h, vec, (int)threadIdx.x - 64, 128);  // while the first tiles are loaded and multiplied
     tc::named_bar_sync(1, 128);
+    const float far_lo = vec[0], far_hi = vec[vec_len(p) - 1];  // the bias beyond max_distance
+    KeyBytes kb = key_bytes(p, b, t0 * C::BK);
     for (int t = 0; t < n; ++t) {
       const int k0 = (t0 + t) * C::BK;
       const uint32_t t_s = tbase + C::T_S + (t & 1) * C::BK;
-      const uint32_t bits[2] = {key_bits(p, b, k0), key_bits(p, b, k0 + 32)};
+      const bool whole = p.mask == nullptr && k0 + C::BK <= p.Sk;
+      const uint32_t bits[2] = {whole ? 0xffffffffu : __ballot_sync(0xffffffffu, kb.a), whole ? 0xffffffffu : __ballot_sync(0xffffffffu, kb.b)};
       const bool full = (bits[0] & bits[1]) == 0xffffffffu;
+      kb = key_bytes(p, b, k0 + C::BK);  // the next tile's, on their way during this one
       if (!tc::mbar_wait(&s_full[t & 1], (uint32_t)((t >> 1) & 1), p.err) || *abort_flag) {
         ok = false;
         break;
@@ -264,7 +277,7 @@ __global__ void __launch_bounds__(192, 2)
           sr[e] = __float_as_uint(x.x), sr[e + 1] = __float_as_uint(x.y);
         }
       } else {
-        cst = rel0 > 0 ? vec[vec_len(p) - 1] : vec[0];
+        cst = rel0 > 0 ? far_hi : far_lo;
       }
       if (!full) {
 #pragma unroll
@@ -275,33 +288,42 @@ __global__ void __launch_bounds__(192, 2)
 #pragma unroll
       for (int e = 0; e < 8; ++e) mx8[e] = __uint_as_float(sr[e]);
 #pragma unroll
-      for (int e = 8; e < C::BK; ++e) mx8[e & 7] = fmaxf(mx8[e & 7], __uint_as_float(sr[e]));
+      for (int e = 8; e < C::BK; e += 16)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          mx8[i] = e + 8 < C::BK ? fmaxf(fmaxf(mx8[i], __uint_as_float(sr[e + i])), __uint_as_float(sr[(e + 8 + i) % C::BK]))
+                                 : fmaxf(mx8[i], __uint_as_float(sr[e + i]));
       const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])),
                              fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
       const float mul = near ? 1.f : sl2;  // scale > 0
       const float m_blk = fmaf(mx, mul, cst);
       // keep the old maximum unless the new one is more than 2^8 larger
       const bool need = m_blk > m + 8.f || (m == -INFINITY && m_blk > -INFINITY);
-      float alpha = 1.f;
-      if (need) {
-        alpha = (m == -INFINITY) ? 0.f : ex2(m - m_blk);
-        m = m_blk;
-      }
-      // every tile waits once for the last one's P V, so that no phase of the barrier is missed: here when O has to move to
-      // the new maximum, else when this tile's P is ready
-      const bool move = t > 0 && __any_sync(0xffffffffu, need);
-      if (move) {
-        if (!__all_sync(0xffffffffu, tc::mbar_wait(o_upd, (uint32_t)((t - 1) & 1), p.err))) { ok = false; break; }
-        tc::tc_fence_after();
+      if (__any_sync(0xffffffffu, need)) {
+        float alpha = 1.f;
+        if (need) {
+          alpha = (m == -INFINITY) ? 0.f : ex2(m - m_blk);
+          m = m_blk;
+        }
+        l *= alpha;
+        if (t > 0) {
+          // O moves to the new maximum. The last tile's P V is in it once the next scores are there (MMAs execute in order)
+          if (!__all_sync(0xffffffffu, t + 1 < n ? tc::mbar_wait(&s_full[(t + 1) & 1], (uint32_t)(((t + 1) >> 1) & 1), p.err)
+                                                 : tc::mbar_wait(&o_upd[0], 0, p.err))) {
+            ok = false;
+            break;
+          }
+          tc::tc_fence_after();
 #pragma unroll 1
-        for (int c = 0; c < D / 16; ++c) {
-          uint32_t orow[16];
-          tc::tmem_ld16(t_o + c * 16 + lane_off, orow);
-          tc::tmem_wait_ld();
-          tc::reg_fence16(orow);
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t orow[16];
+            tc::tmem_ld16(t_o + c * 16 + lane_off, orow);
+            tc::tmem_wait_ld();
+            tc::reg_fence16(orow);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) orow[e] = __float_as_uint(__uint_as_float(orow[e]) * alpha);
-          tc::tmem_st16(t_o + c * 16 + lane_off, orow);
+            for (int e = 0; e < 16; ++e) orow[e] = __float_as_uint(__uint_as_float(orow[e]) * alpha);
+            tc::tmem_st16(t_o + c * 16 + lane_off, orow);
+          }
         }
       }
       const float nmv = (m == -INFINITY) ? -INFINITY : cst - m;  // nothing seen yet: exp2(-inf) = 0
@@ -328,7 +350,7 @@ __global__ void __launch_bounds__(192, 2)
         }
       }
       const float2 rs2 = __fadd2_rn(__fadd2_rn(rs4[0], rs4[1]), __fadd2_rn(rs4[2], rs4[3]));
-      l = l * alpha + (rs2.x + rs2.y);
+      l += rs2.x + rs2.y;
       if (!full && p.mask != nullptr) {
         // masked keys may hold anything, and 0 * NaN is NaN in the P V product: clear their rows of V
         if (!tc::mbar_wait(&v_full[t % NV], (uint32_t)((t / NV) & 1), p.err)) { ok = false; break; }
@@ -344,13 +366,13 @@ __global__ void __launch_bounds__(192, 2)
         tc::fence_async_shared();
         __syncwarp();
       }
-      if (t > 0 && !move && !__all_sync(0xffffffffu, tc::mbar_wait(o_upd, (uint32_t)((t - 1) & 1), p.err))) { ok = false; break; }
       tc::tmem_wait_st();
       tc::tc_fence_before();
-      tc::mbar_arrive(&p_full[t & 1]);
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&p_full[t & 1]);
     }
     // ---------------- epilogue ----------------
-    if (ok && n > 0 && !tc::mbar_wait(o_upd, (uint32_t)((n - 1) & 1), p.err)) ok = false;
+    if (ok && n > 0 && !tc::mbar_wait(&o_upd[1], 0, p.err)) ok = false;
     if (ok && !*abort_flag) {
       tc::tc_fence_after();
       const bool split = p.nsplit > 1;
