@@ -57,6 +57,12 @@ __device__ __forceinline__ uint32_t key_bits(const Params& p, int b, int k) {
   return __ballot_sync(0xffffffffu, ok);
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // Whether keys k + lane and k + 32 + lane are there and seen, for a ballot later.
 struct KeyBytes {
   bool a, b;
@@ -244,14 +250,19 @@ __global__ void __launch_bounds__(192, 2)
     fill_vec(p, h, vec, (int)threadIdx.x - 64, 128);  // while the first tiles are loaded and multiplied
     tc::named_bar_sync(1, 128);
     const float far_lo = vec[0], far_hi = vec[vec_len(p) - 1];  // the bias beyond max_distance
+    const int wholes = p.mask == nullptr ? p.Sk / C::BK - t0 : 0;  // tiles without a key to leave out
     KeyBytes kb = key_bytes(p, b, t0 * C::BK);
     for (int t = 0; t < n; ++t) {
       const int k0 = (t0 + t) * C::BK;
       const uint32_t t_s = tbase + C::T_S + (t & 1) * C::BK;
-      const bool whole = p.mask == nullptr && k0 + C::BK <= p.Sk;
-      const uint32_t bits[2] = {whole ? 0xffffffffu : __ballot_sync(0xffffffffu, kb.a), whole ? 0xffffffffu : __ballot_sync(0xffffffffu, kb.b)};
+      uint32_t bits[2] = {0xffffffffu, 0xffffffffu};
+      if (t >= wholes) {
+        bits[0] = __ballot_sync(0xffffffffu, kb.a), bits[1] = __ballot_sync(0xffffffffu, kb.b);
+        kb = key_bytes(p, b, k0 + C::BK);  // the next tile's, on their way during this one
+      } else if (t + 1 == wholes) {
+        kb = key_bytes(p, b, k0 + C::BK);
+      }
       const bool full = (bits[0] & bits[1]) == 0xffffffffu;
-      kb = key_bytes(p, b, k0 + C::BK);  // the next tile's, on their way during this one
       if (!tc::mbar_wait(&s_full[t & 1], (uint32_t)((t >> 1) & 1), p.err) || *abort_flag) {
         ok = false;
         break;
@@ -288,13 +299,12 @@ __global__ void __launch_bounds__(192, 2)
 #pragma unroll
       for (int e = 0; e < 8; ++e) mx8[e] = __uint_as_float(sr[e]);
 #pragma unroll
-      for (int e = 8; e < C::BK; e += 16)
+      for (int e = 8; e < C::BK - 8; e += 16)
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          mx8[i] = e + 8 < C::BK ? fmaxf(fmaxf(mx8[i], __uint_as_float(sr[e + i])), __uint_as_float(sr[(e + 8 + i) % C::BK]))
-                                 : fmaxf(mx8[i], __uint_as_float(sr[e + i]));
-      const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])),
-                             fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
+        for (int i = 0; i < 8; ++i) mx8[i] = max3(mx8[i], __uint_as_float(sr[e + i]), __uint_as_float(sr[e + 8 + i]));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mx8[i] = fmaxf(mx8[i], __uint_as_float(sr[C::BK - 8 + i]));
+      const float mx = fmaxf(max3(mx8[0], mx8[1], mx8[2]), max3(max3(mx8[3], mx8[4], mx8[5]), mx8[6], mx8[7]));
       const float mul = near ? 1.f : sl2;  // scale > 0
       const float m_blk = fmaf(mx, mul, cst);
       // keep the old maximum unless the new one is more than 2^8 larger
