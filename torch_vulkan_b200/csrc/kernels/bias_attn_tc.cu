@@ -473,7 +473,7 @@ struct Bwd {
   // Two stages at D = 128 put that latency into every tile (612 us for the key side at 16 heads x 4096 x 4096 x 128)
   static constexpr int NS = D == 64 ? 5 : (KEYS ? 4 : 3);
   static constexpr int OFF_X = 0, OFF_Y = 2 * X_BYTES, OFF_BAR = OFF_Y + NS * STAGE, OFF_VEC = OFF_BAR + 256;
-  static constexpr int EW = 512, THREADS = 64 + EW;        // element-wise threads
+  static constexpr int EW = 512, THREADS = 64 + EW + 32;   // element-wise threads; producer, two MMA issuers
   static constexpr uint32_t T_S = 0, T_DP = NT, T_BUF = 2 * NT, T_ACC = 4 * NT, TMEM_COLS = 512;
   static constexpr uint32_t T_ACC2 = T_ACC + D;  // KEYS: dV at T_ACC, dK behind it
   static_assert(4 * NT + (KEYS ? 2 * D : D) <= 512, "TMEM columns");
@@ -545,9 +545,9 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
 
   if (threadIdx.x == 0) {
     tc::mbar_init(x_full, 1);
-    for (int i = 0; i < NS; ++i) tc::mbar_init(&y_full[i], 1), tc::mbar_init(&y_empty[i], 1);
-    for (int i = 0; i < 2; ++i) tc::mbar_init(&sd_full[i], 1), tc::mbar_init(&pd_full[i], 8);
-    tc::mbar_init(acc_full, 1);
+    for (int i = 0; i < NS; ++i) tc::mbar_init(&y_full[i], 1), tc::mbar_init(&y_empty[i], 2);
+    for (int i = 0; i < 2; ++i) tc::mbar_init(&sd_full[i], 2), tc::mbar_init(&pd_full[i], 8);
+    tc::mbar_init(acc_full, 2);
     *abort_flag = 0;
     tc::fence_barrier_init();
   }
@@ -606,29 +606,29 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
           if (issued[s]) tc::mbar_wait(&y_full[s], (uint32_t)((issued[s] - 1) & 1), nullptr);
       }
     }
-  } else if (warp == 1) {
+  } else if (warp == 1 || warp == C::THREADS / 32 - 1) {
     if (lane == 0 && n > 0) {
-      // ---------------- MMA issuer ----------------
+      // ---------------- MMA issuers: one for S and what is made of the columns it leaves (dV or dQ), one for dP and dK.
+      // The MMAs of one thread execute in order, so a tile's gradient has read its P or dS before the next scores land there.
+      // An issuing thread shares its scheduler with four element-wise warps and gets few of its slots: a single one took 100
+      // cycles for each product of 56 (backward of 16 heads x 4096 x 4096 x 64: 373 us; two of them on two schedulers: 373) ----
       constexpr uint32_t IDESC_S = tc::idesc_f16(128, NT, BF16, false, false);
       constexpr uint32_t IDESC_G = tc::idesc_f16(128, D, BF16, false, true);
-      const tc::SDesc x1 = tc::sdesc_parts(tc::smem_u32(smem + C::OFF_X), 16, 1024);
-      const tc::SDesc x2 = tc::sdesc_parts(tc::smem_u32(smem + C::OFF_X + C::X_BYTES), 16, 1024);
+      const bool second = warp != 1;
+      const tc::SDesc x = tc::sdesc_parts(tc::smem_u32(smem + C::OFF_X + (second ? C::X_BYTES : 0)), 16, 1024);
+      const uint32_t y_of = second ? C::Y_BYTES : 0, g_of = second ? 0 : (KEYS ? C::Y_BYTES : 0);
+      const uint32_t t_sd = tbase + (second ? C::T_DP : C::T_S), t_acc = tbase + (second ? C::T_ACC2 : C::T_ACC);
       bool ok = tc::mbar_wait(x_full, 0, p.err);
       auto issue_sd = [&](int t) -> bool {
         const int s = t % NS;
         if (!tc::mbar_wait(&y_full[s], (uint32_t)((t / NS) & 1), p.err)) return false;
         tc::tc_fence_after();
-        const uint32_t st = tc::smem_u32(smem + C::OFF_Y + s * C::STAGE);
-        const tc::SDesc y1 = tc::sdesc_parts(st, 16, 1024), y2 = tc::sdesc_parts(st + C::Y_BYTES, 16, 1024);
-        const uint32_t buf = tbase + (t & 1) * C::T_BUF;
+        const tc::SDesc y = tc::sdesc_parts(tc::smem_u32(smem + C::OFF_Y + s * C::STAGE) + y_of, 16, 1024);
+        const uint32_t dst = t_sd + (t & 1) * C::T_BUF;
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
-          tc::mma_f16_ss(buf + C::T_S, tc::sdesc_at(x1, (k >> 2) * (C::BX * 128) + (k & 3) * 32),
-                         tc::sdesc_at(y1, (k >> 2) * (NT * 128) + (k & 3) * 32), IDESC_S, k > 0 ? 1u : 0u);
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k)
-          tc::mma_f16_ss(buf + C::T_DP, tc::sdesc_at(x2, (k >> 2) * (C::BX * 128) + (k & 3) * 32),
-                         tc::sdesc_at(y2, (k >> 2) * (NT * 128) + (k & 3) * 32), IDESC_S, k > 0 ? 1u : 0u);
+          tc::mma_f16_ss(dst, tc::sdesc_at(x, (k >> 2) * (C::BX * 128) + (k & 3) * 32),
+                         tc::sdesc_at(y, (k >> 2) * (NT * 128) + (k & 3) * 32), IDESC_S, k > 0 ? 1u : 0u);
         tc::mma_commit(&sd_full[t & 1]);
         return true;
       };
@@ -638,21 +638,12 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
         const int s = t % NS;
         if (!tc::mbar_wait(&pd_full[t & 1], (uint32_t)((t >> 1) & 1), p.err)) { ok = false; break; }
         tc::tc_fence_after();
-        const uint32_t st = tc::smem_u32(smem + C::OFF_Y + s * C::STAGE);
-        const tc::SDesc y1 = tc::sdesc_parts(st, NT * 128, 1024), y2 = tc::sdesc_parts(st + C::Y_BYTES, NT * 128, 1024);
-        const uint32_t buf = tbase + (t & 1) * C::T_BUF;
-        const uint32_t acc0 = t > 0 ? 1u : 0u;
-        if (KEYS) {
+        if (KEYS || !second) {  // KEYS: dV += P^T dO and dK += dS^T Q; else dQ += dS K
+          const tc::SDesc y = tc::sdesc_parts(tc::smem_u32(smem + C::OFF_Y + s * C::STAGE) + g_of, NT * 128, 1024);
+          const uint32_t src = t_sd + (t & 1) * C::T_BUF;
 #pragma unroll
-          for (int k = 0; k < NT / 16; ++k)  // dV += P^T dO
-            tc::mma_f16_ts(tbase + C::T_ACC, buf + C::T_S + C::a_col(k), tc::sdesc_at(y2, k * 2048), IDESC_G, k > 0 ? 1u : acc0);
-#pragma unroll
-          for (int k = 0; k < NT / 16; ++k)  // dK += dS^T Q
-            tc::mma_f16_ts(tbase + C::T_ACC2, buf + C::T_DP + C::a_col(k), tc::sdesc_at(y1, k * 2048), IDESC_G, k > 0 ? 1u : acc0);
-        } else {
-#pragma unroll
-          for (int k = 0; k < NT / 16; ++k)  // dQ += dS K
-            tc::mma_f16_ts(tbase + C::T_ACC, buf + C::T_S + C::a_col(k), tc::sdesc_at(y1, k * 2048), IDESC_G, k > 0 ? 1u : acc0);
+          for (int k = 0; k < NT / 16; ++k)
+            tc::mma_f16_ts(t_acc, src + C::a_col(k), tc::sdesc_at(y, k * 2048), IDESC_G, k > 0 || t > 0 ? 1u : 0u);
         }
         tc::mma_commit(&y_empty[s]);
         if (t + 2 < n && !issue_sd(t + 2)) ok = false;
@@ -897,7 +888,7 @@ struct BwdMaps {
   CUtensorMap kx, vx, qy, gy, dv, dk;
 };
 template <int D, bool BF16>
-__global__ void __launch_bounds__(576, 1)
+__global__ void __launch_bounds__(608, 1)
     bias_bwd_tc(const __grid_constant__ BwdMaps m, const __grid_constant__ Params p, const float2* __restrict__ lsed, int sq_pad,
                 int key_blocks, int key_tiles, int query_tiles) {
   if ((int)blockIdx.x < key_blocks)
