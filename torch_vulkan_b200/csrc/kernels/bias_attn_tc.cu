@@ -50,13 +50,6 @@ __device__ __forceinline__ void fill_vec(const Params& p, int h, float* vec, int
   for (int i = tid; i < vec_len(p); i += n) vec[i] = bias_at(p, h, i - p.R - kPad);
 }
 
-// One bit per key of the 32 keys from k: inside [0, Sk) and not masked. Whole warp.
-__device__ __forceinline__ uint32_t key_bits(const Params& p, int b, int k) {
-  const int j = k + (threadIdx.x & 31);
-  const bool ok = j < p.Sk && (p.mask == nullptr || p.mask[(int64_t)b * p.mask_sb + j] != 0);
-  return __ballot_sync(0xffffffffu, ok);
-}
-
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -679,30 +672,38 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
     float far_lo = 0.f, far_hi = 0.f;
     int cur = -1;  // KEYS: the head whose bias is in myvec
     bool ok = true;
-    int kb = 0;
-    for (int t = g; t < n; t += 2, ++kb) {
-      const int gi = KEYS ? t / tiles : 0;
-      const int y0 = KEYS ? (first + t - gi * tiles) * NT : t * NT;
+    float b_lo = 0.f, b_hi = 0.f;  // the bias beyond max_distance
+    if (!KEYS) b_lo = vec[0], b_hi = vec[vec_len(p) - 1];
+    const int wholes = KEYS || p.mask != nullptr ? 0 : p.Sk / NT;  // !KEYS: tiles without a key to leave out
+    KeyBytes keys = {true, true};
+    if (!KEYS) keys = key_bytes(p, b, g * NT + hh * HC);
+    int kb = 0, gi = 0, yi = g;  // tile t is tile yi of the walked head gi
+    for (int t = g; t < n; t += 2, ++kb, yi += 2) {
+      if (KEYS)
+        while (yi >= tiles) yi -= tiles, ++gi;
+      const int y0 = (KEYS ? first + yi : t) * NT;
       if (KEYS && gi != cur) {
         tc::named_bar_sync(2 + g, 256);  // nobody still reads the last head's
         for (int i = tt; i < vec_len(p); i += 256) myvec[i] = bias_at(p, hx * G + gi, i - p.R - kPad) + PUP;
         tc::named_bar_sync(2 + g, 256);
         cur = gi;
+        b_lo = myvec[0], b_hi = myvec[vec_len(p) - 1];
       }
       // after a wait that ran out the tiles are still counted off, so that the team meets at the barriers above
       if (!ok) continue;
       uint64_t bits = ~0ull;  // !KEYS: one bit per column of this warp
       bool full = true;
-      if (!KEYS) {
-        const uint32_t b0 = key_bits(p, b, y0 + hh * HC), b1 = key_bits(p, b, y0 + hh * HC + 32);
+      if (!KEYS && t >= wholes) {
+        const uint32_t b0 = __ballot_sync(0xffffffffu, keys.a), b1 = __ballot_sync(0xffffffffu, keys.b);
         bits = (uint64_t)b0 | ((uint64_t)b1 << 32);
         full = (~bits & ((1ull << HC) - 1)) == 0;
       }
+      if (!KEYS && t + 2 >= wholes) keys = key_bytes(p, b, y0 + 2 * NT + hh * HC);  // this team's next tile's, on their way
       // relative position of column 0 against row 0, and how it moves: -row + column (queries own the rows) or +row - column
       const int rel0 = KEYS ? x0 - y0 - p.q_off : y0 - x0 - p.q_off;
       const bool near = KEYS ? (rel0 - (NT - 1) < p.R && rel0 + 127 > -p.R) : (rel0 - 127 < p.R && rel0 + (NT - 1) > -p.R);
       const float* bv = myvec + (rel0 + (KEYS ? r - hh * HC : hh * HC - r) + p.R + kPad);
-      const float cst = near ? 0.f : (rel0 > 0 ? myvec[vec_len(p) - 1] : myvec[0]);
+      const float cst = near ? 0.f : (rel0 > 0 ? b_hi : b_lo);
       if (!tc::mbar_wait(&sd_full[g], (uint32_t)(kb & 1), p.err) || *abort_flag ||
           (KEYS && !tc::mbar_wait(&y_full[t % NS], (uint32_t)((t / NS) & 1), p.err))) {
         ok = false;
