@@ -457,19 +457,20 @@ __global__ void __launch_bounds__(192, 2)
 template <int D, bool KEYS>
 struct Bwd {
   static constexpr int BX = 128, DCH = D / 64;
-  static constexpr int NT = D == 128 ? 64 : 96;  // walked rows per tile: what TMEM holds twice beside the sums
+  static constexpr int NT = 64;                  // walked rows per tile
+  static constexpr int NB = D == 64 ? 3 : 2;     // tiles of scores in TMEM: what it holds beside the sums
   static constexpr int HC = NT / 2;                        // columns of a tile per warp
   static constexpr int X_BYTES = BX * D * 2, Y_BYTES = NT * D * 2;
   static constexpr int LD_BYTES = KEYS ? NT * 8 : 0;       // (-lse log2 e, -delta) of the walked queries
   static constexpr int STAGE = 2 * Y_BYTES + (LD_BYTES + 1023) / 1024 * 1024;
   // ring depth: a stage is freed by the gradient MMAs of its tile, and its next load takes about a microsecond from there.
   // Two stages at D = 128 put that latency into every tile (612 us for the key side at 16 heads x 4096 x 4096 x 128)
-  static constexpr int NS = D == 64 ? 5 : (KEYS ? 4 : 3);
+  static constexpr int NS = D == 64 ? 7 : (KEYS ? 4 : 3);
   static constexpr int OFF_X = 0, OFF_Y = 2 * X_BYTES, OFF_BAR = OFF_Y + NS * STAGE, OFF_VEC = OFF_BAR + 256;
   static constexpr int EW = 512, THREADS = 64 + EW + 32;   // element-wise threads; producer, two MMA issuers
-  static constexpr uint32_t T_S = 0, T_DP = NT, T_BUF = 2 * NT, T_ACC = 4 * NT, TMEM_COLS = 512;
+  static constexpr uint32_t T_S = 0, T_DP = NT, T_BUF = 2 * NT, T_ACC = NB * T_BUF, TMEM_COLS = 512;
   static constexpr uint32_t T_ACC2 = T_ACC + D;  // KEYS: dV at T_ACC, dK behind it
-  static_assert(4 * NT + (KEYS ? 2 * D : D) <= 512, "TMEM columns");
+  static_assert(NB * T_BUF + (KEYS ? 2 * D : D) <= 512, "TMEM columns");
   // columns of the A operand's 16-deep step k, counted from the scores' first column
   static __device__ __forceinline__ constexpr uint32_t a_col(int k) { return k < HC / 16 ? k * 8 : HC + (k - HC / 16) * 8; }
 };
@@ -511,16 +512,16 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
                                          const CUtensorMap& tmY2, const CUtensorMap& tmG1, const CUtensorMap& tmG2,
                                          const Params& p, const float2* __restrict__ lsed, int sq_pad, int block, int xtiles) {
   using C = Bwd<D, KEYS>;
-  constexpr int NS = C::NS, NT = C::NT, HC = C::HC;
+  constexpr int NS = C::NS, NT = C::NT, HC = C::HC, NB = C::NB;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
   uint64_t* x_full = bar;
   uint64_t* y_full = bar + 1;          // [NS]
   uint64_t* y_empty = y_full + NS;     // [NS]
-  uint64_t* sd_full = y_empty + NS;    // [2] S and dP of tile t in buffer t & 1
-  uint64_t* pd_full = sd_full + 2;     // [2] P / dS of tile t in TMEM (one arrival per warp of the team)
-  uint64_t* acc_full = pd_full + 2;
+  uint64_t* sd_full = y_empty + NS;    // [NB] S and dP of tile t in buffer t % NB
+  uint64_t* pd_full = sd_full + NB;     // [NB] P / dS of tile t in TMEM (one arrival per warp of the team)
+  uint64_t* acc_full = pd_full + NB;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(acc_full + 2);
   const int vlen4 = (vec_len(p) + 3) / 4 * 4, dlen = (2 * p.R + 1 + 3) / 4 * 4;
@@ -539,7 +540,7 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
   if (threadIdx.x == 0) {
     tc::mbar_init(x_full, 1);
     for (int i = 0; i < NS; ++i) tc::mbar_init(&y_full[i], 1), tc::mbar_init(&y_empty[i], 2);
-    for (int i = 0; i < 2; ++i) tc::mbar_init(&sd_full[i], 2), tc::mbar_init(&pd_full[i], 8);
+    for (int i = 0; i < NB; ++i) tc::mbar_init(&sd_full[i], 2), tc::mbar_init(&pd_full[i], 8);
     tc::mbar_init(acc_full, 2);
     *abort_flag = 0;
     tc::fence_barrier_init();
@@ -617,29 +618,28 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
         if (!tc::mbar_wait(&y_full[s], (uint32_t)((t / NS) & 1), p.err)) return false;
         tc::tc_fence_after();
         const tc::SDesc y = tc::sdesc_parts(tc::smem_u32(smem + C::OFF_Y + s * C::STAGE) + y_of, 16, 1024);
-        const uint32_t dst = t_sd + (t & 1) * C::T_BUF;
+        const uint32_t dst = t_sd + (t % NB) * C::T_BUF;
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
           tc::mma_f16_ss(dst, tc::sdesc_at(x, (k >> 2) * (C::BX * 128) + (k & 3) * 32),
                          tc::sdesc_at(y, (k >> 2) * (NT * 128) + (k & 3) * 32), IDESC_S, k > 0 ? 1u : 0u);
-        tc::mma_commit(&sd_full[t & 1]);
+        tc::mma_commit(&sd_full[t % NB]);
         return true;
       };
-      if (ok) ok = issue_sd(0);
-      if (ok && n > 1) ok = issue_sd(1);
+      for (int t = 0; t < NB && t < n && ok; ++t) ok = issue_sd(t);
       for (int t = 0; t < n && ok; ++t) {
         const int s = t % NS;
-        if (!tc::mbar_wait(&pd_full[t & 1], (uint32_t)((t >> 1) & 1), p.err)) { ok = false; break; }
+        if (!tc::mbar_wait(&pd_full[t % NB], (uint32_t)((t / NB) & 1), p.err)) { ok = false; break; }
         tc::tc_fence_after();
         if (KEYS || !second) {  // KEYS: dV += P^T dO and dK += dS^T Q; else dQ += dS K
           const tc::SDesc y = tc::sdesc_parts(tc::smem_u32(smem + C::OFF_Y + s * C::STAGE) + g_of, NT * 128, 1024);
-          const uint32_t src = t_sd + (t & 1) * C::T_BUF;
+          const uint32_t src = t_sd + (t % NB) * C::T_BUF;
 #pragma unroll
           for (int k = 0; k < NT / 16; ++k)
             tc::mma_f16_ts(t_acc, src + C::a_col(k), tc::sdesc_at(y, k * 2048), IDESC_G, k > 0 || t > 0 ? 1u : 0u);
         }
         tc::mma_commit(&y_empty[s]);
-        if (t + 2 < n && !issue_sd(t + 2)) ok = false;
+        if (t + NB < n && !issue_sd(t + NB)) ok = false;
       }
       if (ok) tc::mma_commit(acc_full);
       else *abort_flag = 1;
@@ -651,7 +651,7 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
     const int r = quarter * 32 + lane;
     const int tt = hh * 128 + r;                     // thread of the team, 0..255
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
-    const uint32_t buf = tbase + g * C::T_BUF + hh * HC + lane_off;  // this warp's columns of S (and, + T_DP, of dP)
+    const uint32_t buf0 = tbase + hh * HC + lane_off;  // this warp's columns of S (and, + T_DP, of dP) in the first buffer
     const float sl2 = p.scale * kLog2e;
     const float2 sl22 = make_float2(sl2, sl2);
     // f16: P carries a factor of 2^8 (in its bias) so that 1 / Sk stays clear of the subnormals; dS does not
@@ -677,8 +677,8 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
     const int wholes = KEYS || p.mask != nullptr ? 0 : p.Sk / NT;  // !KEYS: tiles without a key to leave out
     KeyBytes keys = {true, true};
     if (!KEYS) keys = key_bytes(p, b, g * NT + hh * HC);
-    int kb = 0, gi = 0, yi = g;  // tile t is tile yi of the walked head gi
-    for (int t = g; t < n; t += 2, ++kb, yi += 2) {
+    int gi = 0, yi = g;  // tile t is tile yi of the walked head gi
+    for (int t = g; t < n; t += 2, yi += 2) {
       if (KEYS)
         while (yi >= tiles) yi -= tiles, ++gi;
       const int y0 = (KEYS ? first + yi : t) * NT;
@@ -704,7 +704,9 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
       const bool near = KEYS ? (rel0 - (NT - 1) < p.R && rel0 + 127 > -p.R) : (rel0 - 127 < p.R && rel0 + (NT - 1) > -p.R);
       const float* bv = myvec + (rel0 + (KEYS ? r - hh * HC : hh * HC - r) + p.R + kPad);
       const float cst = near ? 0.f : (rel0 > 0 ? b_hi : b_lo);
-      if (!tc::mbar_wait(&sd_full[g], (uint32_t)(kb & 1), p.err) || *abort_flag ||
+      const int bi = t % NB;
+      const uint32_t buf = buf0 + bi * C::T_BUF;
+      if (!tc::mbar_wait(&sd_full[bi], (uint32_t)((t / NB) & 1), p.err) || *abort_flag ||
           (KEYS && !tc::mbar_wait(&y_full[t % NS], (uint32_t)((t / NS) & 1), p.err))) {
         ok = false;
         continue;
@@ -794,7 +796,7 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
       tc::tmem_wait_st();
       tc::tc_fence_before();
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&pd_full[g]);
+      if (lane == 0) tc::mbar_arrive(&pd_full[bi]);
     }
     if (!KEYS && p.dtab) {
       // this warp's far tiles join the ends of its array; then the arrays are added and cut into buckets
