@@ -164,8 +164,8 @@ uint64_t up16(uint64_t v) { return (v + 15) / 16 * 16; }
 
 // Key splits of the forward: the waves of blocks times the key tiles a block walks plus 1.6 us of set-up,
 // and for the join its bytes (each split's fp32 output written and read) at the memory's rate, where a tile takes about
-// 0.4 us on the tensor cores and 3 us on the FMA pipe, and a launch. At least two tiles a split. Measured, 16 heads x 4096 x 4096: 2 splits save a sixth of the walk
-// (3.5 waves) and their join takes 47 us of it back.
+// 0.4 us on the tensor cores and 3 us on the FMA pipe, and a launch. At least two tiles a split. Measured, 16 heads x 4096 x
+// 4096: 2 splits save a sixth of the walk (3.5 waves) and their join takes 47 us of it back.
 int pick_splits(int64_t blocks, int64_t tk, int64_t out_elems, double tile_us) {
   const int64_t sms = 2 * (device_info().sm_count > 0 ? device_info().sm_count : 148);  // two blocks to an SM
   int best = 1;

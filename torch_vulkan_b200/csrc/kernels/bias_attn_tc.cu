@@ -82,11 +82,50 @@ __device__ __forceinline__ int trim_end(const Params& p, int b, int end, int nth
   return *slot;
 }
 
+// A warp's 32 rows of O (TMEM, relative to the maximum m) and their earlier part (relative to run_m): in TMEM columns of its own
+// at D = 64, else in memory, column by column, `rows` floats each (the rows that exist), in the place that the finished rows will
+// take. OUT: the sum joins the earlier part; else it goes back to O.
+template <int D, bool OUT>
+__device__ __forceinline__ void add_run(uint32_t t_o, uint32_t t_sum, float* part, bool first, float run_m, float m, int rows,
+                                        int dims) {
+  const int lane = threadIdx.x & 31;
+  const bool on = lane < rows;
+  const float w = first ? 0.f : run_m == m ? 1.f : ex2(run_m - m);
+#pragma unroll 1
+  for (int c = 0; c < D / 16; ++c) {
+    uint32_t o[16], y[16];
+    float* at = part + c * 16 * rows + lane;
+    __syncwarp();
+    if (D == 64) {
+      if (!first) tc::tmem_ld16(t_sum + c * 16, y);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) y[e] = !first && on && c * 16 + e < dims ? __float_as_uint(at[e * rows]) : 0u;
+    }
+    tc::tmem_ld16(t_o + c * 16, o);
+    tc::tmem_wait_ld();
+    tc::reg_fence16(o);
+    if (D == 64) tc::reg_fence16(y);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float x = first ? __uint_as_float(o[e]) : fmaf(__uint_as_float(y[e]), w, __uint_as_float(o[e]));
+      o[e] = __float_as_uint(x);
+      if (OUT && D != 64 && on && c * 16 + e < dims) at[e * rows] = x;
+    }
+    if (!OUT || D == 64) tc::tmem_st16((OUT ? t_sum : t_o) + c * 16, o);
+  }
+  tc::tmem_wait_st();
+  __syncwarp();
+}
+
 // ==================================================================================================
-// forward: a block owns 128 queries of a head, and two blocks share an SM (256 TMEM columns, half of the shared memory
-// each), so that one's set-up, softmax and output run beside the other's MMAs. One block to an SM with two softmax groups
-// took 24.5 us against 20.8 at B4 H16 S512 D64 and 110 against 94 at B8 H16 S1024 D128 (padded): with a few tiles per
-// block the set-up and the output, about 8 us, were not overlapped by anything.
+// forward: a block owns 128 queries of a head and walks the keys in tiles of 64 with two score buffers, so that the next
+// scores are multiplied while a softmax runs. Two blocks share an SM (256 TMEM columns, half of the shared memory each), so
+// that one's set-up, softmax and output run beside the other's. The softmax bounds it: 1800 cycles a tile, 800 of them
+// exponentials of two warps on one scheduler (scores are always ready when they are asked for). 16 heads x 4096 x 4096 x 64:
+// 134 us, for a backward (below) 177. One block to an SM with two softmax groups took 24.5 us against 20.8 at B4 H16 S512
+// D64 and 110 against 94 at B8 H16 S1024 D128 (padded); tiles of 128 with one score buffer 165 us against 151; two threads
+// to a row, 32 columns each, 213 against 174 (for a backward).
 // ==================================================================================================
 template <int D>
 struct Fwd {
@@ -96,12 +135,19 @@ struct Fwd {
   static constexpr int OFF_Q = 0, OFF_K = Q_BYTES, OFF_V = OFF_K + NK * KV_BYTES, OFF_BAR = OFF_V + NV * KV_BYTES;
   static constexpr int OFF_VEC = OFF_BAR + 256;
   static constexpr int THREADS = 192;
-  static constexpr uint32_t T_S = 0, T_O = 128, TMEM_COLS = 256;
+  // PREC: tiles whose P V is summed before the sum leaves the accumulator, to columns of its own where TMEM has them; through
+  // memory a move takes 3 us, so fewer are made (every 8 tiles: 256 us, every 16: 220)
+  static constexpr int RUN = D == 64 ? 8 : 16;
+  static constexpr uint32_t T_S = 0, T_O = 128, T_SUM = 192, TMEM_COLS = 256;  // T_SUM: D = 64
 };
 
 // PREC (o32 wanted, for a backward): P enters the product as two 16-bit numbers, P = hi + lo, so that O is good to about
 // 2^-17 before its rounding. delta = rowsum(dO O) is made from it, and dS = P (dP - delta) cancels over a row: with P
-// rounded once, the bias gradient (a sum of dS over many rows) keeps errors of a few 1e-3 of itself.
+// rounded once, the bias gradient (a sum of dS over many rows) keeps errors of a few 1e-3 of itself. The tensor core also
+// truncates each of its sums towards zero: after 4096 keys (512 of them) O is 8.3e-6 of itself short, and the gradient of a far
+// bucket adds that up over all rows (1e-5 of it). So every RUN tiles the sum joins a sum kept in fp32 elsewhere and the next one
+// starts from zero: 1.1e-6 short at D = 64 (2.0e-6 at D = 128), gradient 2e-6 to 4e-6 off; 163 -> 177 us and, through memory,
+// 183 -> 224 us (16 heads x 4096 x 4096).
 template <int D, bool BF16, bool PREC>
 __global__ void __launch_bounds__(192, 2)
     bias_fwd_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -218,7 +264,7 @@ __global__ void __launch_bounds__(192, 2)
         const tc::SDesc vd = tc::sdesc_parts(tc::smem_u32(smem + C::OFF_V + vs * C::KV_BYTES), C::BK * 128, 1024);
 #pragma unroll
         for (int k = 0; k < C::BK / 16; ++k)
-          tc::mma_f16_ts(tbase + C::T_O, tbase + C::T_S + (t & 1) * C::BK + k * 8, tc::sdesc_at(vd, k * 2048), IDESC_O, (k > 0 || t > 0) ? 1u : 0u);
+          tc::mma_f16_ts(tbase + C::T_O, tbase + C::T_S + (t & 1) * C::BK + k * 8, tc::sdesc_at(vd, k * 2048), IDESC_O, (k > 0 || (PREC ? t % C::RUN != 0 : t > 0)) ? 1u : 0u);
         if (PREC) {
 #pragma unroll
           for (int k = 0; k < C::BK / 16; ++k)
@@ -242,6 +288,14 @@ __global__ void __launch_bounds__(192, 2)
     bool ok = true;
     fill_vec(p, h, vec, (int)threadIdx.x - 64, 128);  // while the first tiles are loaded and multiplied
     tc::named_bar_sync(1, 128);
+    // PREC: this warp's rows of o32 (of the split's partial output), and the maximum that what lies there is relative to
+    const int run_rows = max(0, min(32, p.Sq - q0 - quarter * 32));
+    float* run_o = nullptr;
+    float run_m = 0.f;
+    if (PREC) {
+      const int64_t row = (int64_t)blockIdx.y * p.Sq + q0 + quarter * 32;
+      run_o = p.nsplit > 1 ? p.part_o + ((int64_t)blockIdx.z * p.B * p.H * p.Sq + row) * p.D : p.o32 + row * p.D;
+    }
     const float far_lo = vec[0], far_hi = vec[vec_len(p) - 1];  // the bias beyond max_distance
     const int wholes = p.mask == nullptr ? p.Sk / C::BK - t0 : 0;  // tiles without a key to leave out
     KeyBytes kb = key_bytes(p, b, t0 * C::BK);
@@ -302,21 +356,29 @@ __global__ void __launch_bounds__(192, 2)
       const float m_blk = fmaf(mx, mul, cst);
       // keep the old maximum unless the new one is more than 2^8 larger
       const bool need = m_blk > m + 8.f || (m == -INFINITY && m_blk > -INFINITY);
-      if (__any_sync(0xffffffffu, need)) {
+      const bool fresh = PREC && t % C::RUN == 0;  // this tile's P V starts a new sum
+      const bool moves = __any_sync(0xffffffffu, need);
+      if (t > 0 && (moves || fresh)) {
+        // O is read: the last tile's P V is in it once the next scores are there (MMAs execute in order)
+        if (!__all_sync(0xffffffffu, t + 1 < n ? tc::mbar_wait(&s_full[(t + 1) & 1], (uint32_t)(((t + 1) >> 1) & 1), p.err)
+                                               : tc::mbar_wait(&o_upd[0], 0, p.err))) {
+          ok = false;
+          break;
+        }
+        tc::tc_fence_after();
+      }
+      if (PREC && fresh && t > 0) {
+        add_run<D, true>(t_o + lane_off, tbase + C::T_SUM + lane_off, run_o, t == C::RUN, run_m, m, run_rows, p.D);
+        run_m = m;
+      }
+      if (moves) {
         float alpha = 1.f;
         if (need) {
           alpha = (m == -INFINITY) ? 0.f : ex2(m - m_blk);
           m = m_blk;
         }
         l *= alpha;
-        if (t > 0) {
-          // O moves to the new maximum. The last tile's P V is in it once the next scores are there (MMAs execute in order)
-          if (!__all_sync(0xffffffffu, t + 1 < n ? tc::mbar_wait(&s_full[(t + 1) & 1], (uint32_t)(((t + 1) >> 1) & 1), p.err)
-                                                 : tc::mbar_wait(&o_upd[0], 0, p.err))) {
-            ok = false;
-            break;
-          }
-          tc::tc_fence_after();
+        if (t > 0 && !fresh) {  // O moves to the new maximum
 #pragma unroll 1
           for (int c = 0; c < D / 16; ++c) {
             uint32_t orow[16];
@@ -383,6 +445,7 @@ __global__ void __launch_bounds__(192, 2)
       const int qrow = q0 + r;
       const int64_t row = (int64_t)blockIdx.y * p.Sq + qrow;
       const int64_t prow = (int64_t)blockIdx.z * p.B * p.H * p.Sq + row;
+      if (PREC && n > C::RUN) add_run<D, false>(t_o + lane_off, tbase + C::T_SUM + lane_off, run_o, false, run_m, m, run_rows, p.D);
       uint8_t* stg = smem + C::OFF_K + (warp - 2) * (D / 32) * 2048;  // every MMA that read K is done
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
@@ -448,11 +511,12 @@ __global__ void __launch_bounds__(192, 2)
 //   KEYS = true   X = K, V (a block owns 128 keys),    Y = Q, dO:   dK += dS^T Q, dV += P^T dO, over every query head
 //                                                                   that shares the key/value head
 // S = X1 Y1^T and dP = X2 Y2^T are recomputed on both sides (7 products instead of 5), which leaves every gradient one
-// owner: no atomics, no accumulator in memory, the same bits on every run. Two teams of eight warps take the tiles in turn,
-// each with its own S and dP columns in TMEM; in a team, two warps share a lane quarter and split its columns. P and dS
-// (16 bits) replace the scores a warp has read and are the A operands of the gradient MMAs, 8 columns per 16 of the
-// reduction at any place. (Eight warps in all, half as many, left the MMAs waiting for them: 357 us instead of 285 for the
-// key side at 16 heads x 4096 x 4096 x 64.)
+// owner: no atomics, no accumulator in memory, the same bits on every run. Two teams of eight warps take the tiles in turn;
+// in a team, two warps share a lane quarter and split its columns. P and dS (16 bits) replace the scores a warp has read and
+// are the A operands of the gradient MMAs, 8 columns per 16 of the reduction at any place. At D = 64 TMEM holds three tiles,
+// so that the MMAs of one run while both teams work (4 x 16 heads x 512 x 512: 60 us, with two tiles of 96 columns 67). Issue
+// slots bound it: an issuing thread among element-wise warps takes 80 to 140 cycles for a product of 48 (16 heads x 4096 x
+// 4096: 366 us at D = 64, 464 at 128). Eight element-wise warps, half as many, took 357 us instead of 285 for the key side alone.
 // ==================================================================================================
 template <int D, bool KEYS>
 struct Bwd {
@@ -464,7 +528,7 @@ struct Bwd {
   static constexpr int LD_BYTES = KEYS ? NT * 8 : 0;       // (-lse log2 e, -delta) of the walked queries
   static constexpr int STAGE = 2 * Y_BYTES + (LD_BYTES + 1023) / 1024 * 1024;
   // ring depth: a stage is freed by the gradient MMAs of its tile, and its next load takes about a microsecond from there.
-  // Two stages at D = 128 put that latency into every tile (612 us for the key side at 16 heads x 4096 x 4096 x 128)
+  // Two stages at D = 128 put that latency into every tile (612 us for the key side alone at 16 heads x 4096 x 4096 x 128)
   static constexpr int NS = D == 64 ? 7 : (KEYS ? 4 : 3);
   static constexpr int OFF_X = 0, OFF_Y = 2 * X_BYTES, OFF_BAR = OFF_Y + NS * STAGE, OFF_VEC = OFF_BAR + 256;
   static constexpr int EW = 512, THREADS = 64 + EW + 32;   // element-wise threads; producer, two MMA issuers
@@ -604,8 +668,9 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
     if (lane == 0 && n > 0) {
       // ---------------- MMA issuers: one for S and what is made of the columns it leaves (dV or dQ), one for dP and dK.
       // The MMAs of one thread execute in order, so a tile's gradient has read its P or dS before the next scores land there.
-      // An issuing thread shares its scheduler with four element-wise warps and gets few of its slots: a single one took 100
-      // cycles for each product of 56 (backward of 16 heads x 4096 x 4096 x 64: 373 us; two of them on two schedulers: 373) ----
+      // An issuing thread shares its scheduler with four element-wise warps and gets few of its slots: with a single one the
+      // backward of 16 heads x 4096 x 4096 x 128 took 560 us instead of 473. Loads by one of the two instead of their own warp:
+      // 620 us ----------------
       constexpr uint32_t IDESC_S = tc::idesc_f16(128, NT, BF16, false, false);
       constexpr uint32_t IDESC_G = tc::idesc_f16(128, D, BF16, false, true);
       const bool second = warp != 1;
