@@ -370,3 +370,20 @@ def test_in_a_graph(Sq):
     table.add_(1.0).mul_(0.5)
     g.replay()
     assert torch.equal(o, tv.bucket_bias_attention(q, k, v, table, **kw))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [40, 64, 128])
+def test_long_rows_keep_their_sum(dt, D):
+    """Long rows in one piece (enough blocks that the keys are not split), with values of one sign: a sum that is cut short at every
+    step would show. A 16-wide step of the product may lose 2^-23 of the sum; 1024 keys are 64 steps of P's two halves, 2^-16,
+    and P is good to 2^-17."""
+    q, k, v, go, table, m = _case(4, 70, 70, 40, 2048, D, dt, D, "tail")
+    v = v.abs()
+    ref = ot.bias_attention(q, k, v, table, key_mask=m, go=go)
+    got = _run(q, k, v, table, m, go)
+    _near(got["o"], ref["o"], OUT[dt], "o")
+    err = (got["dtable"].cpu().double() - ref["dtable"]).abs()
+    bound = (2.0 ** -16 + 2.0 ** -17) * ref["dtable_abs"] + 2.0 ** -14 * ref["ds_abs"] + 1e-7
+    assert bool((err <= bound).all()), f"dtable: {(err / bound).max().item():.3g} of the bound"

@@ -139,8 +139,8 @@ int check(const b2_bias_attn_args* a, bool bwd) {
   if (a->H > 0 && (a->Hk < 1 || a->H % a->Hk))
     return fail(B2_ERR_ARG, std::string(w) + ": the query heads must be a multiple of the key/value heads");
   if (a->B * a->H > 65535) return fail(B2_ERR_ARG, std::string(w) + ": batch * heads must be at most 65535");
-  if (a->Sq >= (1ll << 30) || a->Sk >= (1ll << 30) || a->q_offset >= (1ll << 30) || a->q_offset <= -(1ll << 30))
-    return fail(B2_ERR_ARG, std::string(w) + ": lengths and q_offset must be below 2^30");
+  if (a->Sq >= (1ll << 29) || a->Sk >= (1ll << 29) || a->q_offset >= (1ll << 29) || a->q_offset <= -(1ll << 29))
+    return fail(B2_ERR_ARG, std::string(w) + ": lengths and q_offset must be below 2^29");
   if (!bucket_args_ok(a->num_buckets, a->max_distance, a->bidirectional))
     return fail(B2_ERR_ARG, std::string(w) + ": num_buckets must be 2..128 (two-sided: even, 4..128) and max_distance "
                                              "above half a side's buckets and at most 1024");

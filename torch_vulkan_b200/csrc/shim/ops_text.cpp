@@ -308,9 +308,9 @@ BiasAttn bias_attn_args(const at::Tensor& q, const at::Tensor& k, const at::Tens
               " buckets; 2 to 128 are supported, an even number from 4 where both directions are told apart");
   TORCH_CHECK(max_distance > side / 2 && max_distance <= B2_BIAS_MAX_DISTANCE, name, ": max_distance must be above ", side / 2,
               " (half a direction's buckets) and at most ", B2_BIAS_MAX_DISTANCE, ", got ", max_distance);
-  const int64_t lim = int64_t(1) << 30;
+  const int64_t lim = int64_t(1) << 29;
   TORCH_CHECK(q.size(2) < lim && k.size(2) < lim && q_offset < lim && q_offset > -lim, name,
-              ": lengths and q_offset must be below 2^30");
+              ": lengths and q_offset must be below 2^29");
   TORCH_CHECK(q.size(0) * q.size(1) <= 65535, name, ": batch * heads must be at most 65535");
   BiasAttn r;
   r.q = readable(q), r.k = readable(k), r.v = readable(v);
