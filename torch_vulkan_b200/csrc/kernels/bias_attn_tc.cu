@@ -591,7 +591,7 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
   const int vlen4 = (vec_len(p) + 3) / 4 * 4, dlen = (2 * p.R + 1 + 3) / 4 * 4;
   float* vec = reinterpret_cast<float*>(smem + C::OFF_VEC);  // KEYS: one per team (the head changes along the walk)
   float* darr = vec + vlen4;                                 // !KEYS: diagonal sums, one array per warp
-  float* dscr = darr + 16 * dlen;                            // !KEYS: 16 floats per warp
+  float* dscr = darr + 16 * dlen;                            // !KEYS: 16 floats per warp; at the end the buckets' sums
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int heads = KEYS ? p.Hk : p.H, G = p.H / p.Hk;
@@ -892,7 +892,20 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
             for (int d = 1 + lane; d <= p.R; d += 32) s += vec[p.R + d];
         }
         s = warp_sum(s);
-        if (lane == 0) p.dtab[(int64_t)block * p.nb + bk] = s;
+        if (lane == 0) dscr[bk] = s;
+      }
+      tc::named_bar_sync(1, C::EW);
+      // A row of dS adds up to zero over its keys. Where most keys of the block lie in one bucket (beyond the last threshold on one
+      // side) that bucket's sum is minus the others': what an error of delta leaves in a bucket goes with the share of P there
+      if (w16 == 0) {
+        const int side = p.bidir ? p.nb / 2 : p.nb, beyond = p.thr[side - 2];
+        const int keys = min(tiles * NT, p.Sk), mid = x0 + min(C::BX, p.Sq - x0) / 2 + p.q_off;
+        const int past = max(0, min(keys, mid - beyond)), ahead = max(0, min(keys, keys - mid - (p.bidir ? beyond : 0)));
+        const int big = 2 * past > keys ? side - 1 : 2 * ahead > keys ? (p.bidir ? p.nb - 1 : 0) : -1;
+        float rest = 0.f;
+        for (int i = lane; i < p.nb; i += 32) rest += i == big ? 0.f : dscr[i];
+        rest = warp_sum(rest);
+        for (int i = lane; i < p.nb; i += 32) p.dtab[(int64_t)block * p.nb + i] = i == big ? -rest : dscr[i];
       }
     }
     // ---------------- epilogue: a warp writes 32 rows x 32 columns of a gradient at a time ----------------
