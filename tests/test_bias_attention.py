@@ -387,3 +387,17 @@ def test_long_rows_keep_their_sum(dt, D):
     err = (got["dtable"].cpu().double() - ref["dtable"]).abs()
     bound = (2.0 ** -16 + 2.0 ** -17) * ref["dtable_abs"] + 2.0 ** -14 * ref["ds_abs"] + 1e-7
     assert bool((err <= bound).all()), f"dtable: {(err / bound).max().item():.3g} of the bound"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("Sq,Sk,causal", [(1500, 14, False), (300, 1, False), (7, 1200, True), (260, 700, False)])
+def test_bias_gradient_where_one_bucket_has_most_keys(dt, Sq, Sk, causal):
+    """Many rows have all their keys in the bucket beyond max_distance, where the row's dS cancels: the bound of every bucket still
+    holds, and a single key, whose P is 1, gives no gradient at all."""
+    q, k, v, go, table, m = _case(2, 4, 2, Sq, Sk, 64, dt, Sq + Sk, "tail")
+    for bidirectional in (True, False):
+        kw = dict(causal=causal, bidirectional=bidirectional, q_offset=Sk - Sq if causal else 0)
+        got = _check(q, k, v, go, table, m, **kw)
+        if Sk == 1:
+            assert not got["dtable"].any()
