@@ -479,8 +479,9 @@ int b2_bias_bucket(int64_t rel, int32_t num_buckets, int32_t max_distance, int32
 
 /* O = softmax(scale * Q K^T + bias) V with bias[h][i][j] = table[bucket(j - i - q_offset)][h], keys masked by
  * key_mask (bytes [B][Sk], 0 = masked; row stride mask_sb) and, when causal, keys j > i + q_offset. A row whose keys
- * are all masked gives zeros (lse -inf) and zero gradients; K and V at masked positions are never used, whatever they
- * hold. Query head h reads key/value head h / (H / Hk). Tensors are [B, heads, S, D] with (batch, head, seq) strides
+ * are all masked gives zeros (lse -inf) and zero gradients; K and V of keys that key_mask masks, or that causal hides
+ * from every query, are never used, whatever they hold. Query head h reads key/value head h / (H / Hk). Tensors are
+ * [B, heads, S, D] with (batch, head, seq) strides
  * in elements and unit stride along D; lse and delta are fp32 [B, H, Sq].
  * Backward: dQ, dK, dV, and (dtable != NULL) dtable[n][h] = sum of dS over the pairs in bucket n, fp32
  * [num_buckets][H], every sum in a fixed order.

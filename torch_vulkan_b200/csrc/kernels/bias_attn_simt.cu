@@ -108,12 +108,13 @@ __device__ __forceinline__ float sum16(float v) {
   return v;
 }
 
-// keep[j] for the n keys from k0; returns whether any is left.
-__device__ __forceinline__ bool load_keep(const Params& p, int b, int k0, int n, uint8_t* keep) {
+// keep[j] for the n keys from k0, of which those from `end` on are hidden from every query that is asked about; returns
+// whether any is left.
+__device__ __forceinline__ bool load_keep(const Params& p, int b, int k0, int n, int end, uint8_t* keep) {
   bool any = false;
   if ((int)threadIdx.x < n) {
     const int j = k0 + threadIdx.x;
-    const bool ok = j < p.Sk && (p.mask == nullptr || p.mask[(int64_t)b * p.mask_sb + j] != 0);
+    const bool ok = j < end && (p.mask == nullptr || p.mask[(int64_t)b * p.mask_sb + j] != 0);
     keep[threadIdx.x] = ok;
     any = ok;
   }
@@ -149,13 +150,13 @@ __global__ void __launch_bounds__(NTH) fwd_kernel(const __grid_constant__ Params
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) acc[i][c] = 0.f;
   }
-  const int nt = (key_end(p, min(q0 + OWN, p.Sq) - 1) + T64 - 1) / T64;
+  const int end = key_end(p, min(q0 + OWN, p.Sq) - 1), nt = (end + T64 - 1) / T64;
   const int per = (nt + p.nsplit - 1) / p.nsplit;
   const int t1 = min(nt, ((int)blockIdx.z + 1) * per);
   for (int t = blockIdx.z * per; t < t1; ++t) {
     const int k0 = t * T64;
     __syncthreads();
-    if (!load_keep(p, b, k0, T64, keep)) continue;
+    if (!load_keep(p, b, k0, T64, end, keep)) continue;
     load_tile<T, DP, T64>(Ks, p.k, p.k_s, b, hk, k0, p.Sk, p.D, 1.f, keep);
     load_tile<T, DP, T64>(Vs, p.v, p.v_s, b, hk, k0, p.Sk, p.D, 1.f, keep);
     __syncthreads();
@@ -251,11 +252,11 @@ __device__ __forceinline__ void dq_side(const Params& p, int block, int xtiles) 
     for (int c = 0; c < DP / 16; ++c) acc[i][c] = 0.f;
   }
   float db = 0.f;  // thread n: sum of dS over bucket n
-  const int nt = (key_end(p, min(q0 + OWN, p.Sq) - 1) + T64 - 1) / T64;
+  const int end = key_end(p, min(q0 + OWN, p.Sq) - 1), nt = (end + T64 - 1) / T64;
   for (int t = 0; t < nt; ++t) {
     const int k0 = t * T64;
     __syncthreads();
-    if (!load_keep(p, b, k0, T64, keep)) continue;
+    if (!load_keep(p, b, k0, T64, end, keep)) continue;
     load_tile<T, DP, T64>(Ks, p.k, p.k_s, b, hk, k0, p.Sk, p.D, 1.f, keep);
     load_tile<T, DP, T64>(Vs, p.v, p.v_s, b, hk, k0, p.Sk, p.D, 1.f, keep);
     __syncthreads();
@@ -321,7 +322,7 @@ __device__ __forceinline__ void dkv_side(const Params& p, int block, int xtiles)
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int bh = block / xtiles, k0 = (block - bh * xtiles) * OWN;
   const int b = bh / p.Hk, hk = bh % p.Hk, G = p.H / p.Hk;
-  const bool some = load_keep(p, b, k0, OWN, keep);
+  const bool some = load_keep(p, b, k0, OWN, key_end(p, p.Sq - 1), keep);
   load_tile<T, DP, OWN>(Ks, p.k, p.k_s, b, hk, k0, p.Sk, p.D, 1.f, keep);
   load_tile<T, DP, OWN>(Vs, p.v, p.v_s, b, hk, k0, p.Sk, p.D, 1.f, keep);
   float dk[4][DP / 16] = {}, dv[4][DP / 16] = {};

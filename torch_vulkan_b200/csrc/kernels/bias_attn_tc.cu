@@ -56,14 +56,14 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-// Whether keys k + lane and k + 32 + lane are there and seen, for a ballot later.
+// Whether keys k + lane and k + 32 + lane lie below `end` and are seen, for a ballot later.
 struct KeyBytes {
   bool a, b;
 };
-__device__ __forceinline__ KeyBytes key_bytes(const Params& p, int b, int k) {
+__device__ __forceinline__ KeyBytes key_bytes(const Params& p, int b, int k, int end) {
   const int j = k + (threadIdx.x & 31);
   const uint8_t* m = p.mask ? p.mask + (int64_t)b * p.mask_sb : nullptr;
-  return {j < p.Sk && (m == nullptr || m[j] != 0), j + 32 < p.Sk && (m == nullptr || m[j + 32] != 0)};
+  return {j < end && (m == nullptr || m[j] != 0), j + 32 < end && (m == nullptr || m[j + 32] != 0)};
 }
 
 // One past the last key below `end` that the mask leaves (every thread of the block; contains block barriers). The whole
@@ -297,17 +297,17 @@ __global__ void __launch_bounds__(192, 2)
       run_o = p.nsplit > 1 ? p.part_o + ((int64_t)blockIdx.z * p.B * p.H * p.Sq + row) * p.D : p.o32 + row * p.D;
     }
     const float far_lo = vec[0], far_hi = vec[vec_len(p) - 1];  // the bias beyond max_distance
-    const int wholes = p.mask == nullptr ? p.Sk / C::BK - t0 : 0;  // tiles without a key to leave out
-    KeyBytes kb = key_bytes(p, b, t0 * C::BK);
+    const int wholes = p.mask == nullptr ? end / C::BK - t0 : 0;  // tiles without a key to leave out
+    KeyBytes kb = key_bytes(p, b, t0 * C::BK, end);
     for (int t = 0; t < n; ++t) {
       const int k0 = (t0 + t) * C::BK;
       const uint32_t t_s = tbase + C::T_S + (t & 1) * C::BK;
       uint32_t bits[2] = {0xffffffffu, 0xffffffffu};
       if (t >= wholes) {
         bits[0] = __ballot_sync(0xffffffffu, kb.a), bits[1] = __ballot_sync(0xffffffffu, kb.b);
-        kb = key_bytes(p, b, k0 + C::BK);  // the next tile's, on their way during this one
+        kb = key_bytes(p, b, k0 + C::BK, end);  // the next tile's, on their way during this one
       } else if (t + 1 == wholes) {
-        kb = key_bytes(p, b, k0 + C::BK);
+        kb = key_bytes(p, b, k0 + C::BK, end);
       }
       const bool full = (bits[0] & bits[1]) == 0xffffffffu;
       if (!tc::mbar_wait(&s_full[t & 1], (uint32_t)((t >> 1) & 1), p.err) || *abort_flag) {
@@ -416,8 +416,9 @@ __global__ void __launch_bounds__(192, 2)
       }
       const float2 rs2 = __fadd2_rn(__fadd2_rn(rs4[0], rs4[1]), __fadd2_rn(rs4[2], rs4[3]));
       l += rs2.x + rs2.y;
-      if (!full && p.mask != nullptr) {
-        // masked keys may hold anything, and 0 * NaN is NaN in the P V product: clear their rows of V
+      if (!full && (p.mask != nullptr || end < p.Sk)) {
+        // keys that the mask or the causal rule hides may hold anything, and 0 * NaN is NaN in the P V product: clear their
+        // rows of V (past Sk the load has put zeros)
         if (!tc::mbar_wait(&v_full[t % NV], (uint32_t)((t / NV) & 1), p.err)) { ok = false; break; }
         if (!((bits[quarter & 1] >> lane) & 1u)) {  // warps 0 and 1 clear one half of a row, 2 and 3 the other
 #pragma unroll
@@ -614,7 +615,7 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
     tc::tmem_alloc(tmem_slot, C::TMEM_COLS);
     tc::tmem_relinquish();
   }
-  int first = 0, tiles;  // tiles first .. first + tiles of every walked head
+  int first = 0, tiles, end = p.Sk;  // tiles first .. first + tiles of every walked head; !KEYS: one past the last key
   if (KEYS) {
     const int any = p.mask == nullptr ||
                     __syncthreads_or((int)threadIdx.x < C::BX && x0 + (int)threadIdx.x < p.Sk &&
@@ -623,7 +624,8 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
     if (p.causal) first = (int)min((int64_t)nt, max((int64_t)0, (int64_t)x0 - p.q_off) / NT);
     tiles = any ? nt - first : 0;
   } else {
-    tiles = (trim_end(p, b, key_end(p, min(x0 + C::BX, p.Sq) - 1), C::THREADS, reinterpret_cast<int*>(vec)) + NT - 1) / NT;
+    end = trim_end(p, b, key_end(p, min(x0 + C::BX, p.Sq) - 1), C::THREADS, reinterpret_cast<int*>(vec));
+    tiles = (end + NT - 1) / NT;
   }
   tc::tc_fence_before();
   __syncthreads();
@@ -739,9 +741,9 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
     bool ok = true;
     float b_lo = 0.f, b_hi = 0.f;  // the bias beyond max_distance
     if (!KEYS) b_lo = vec[0], b_hi = vec[vec_len(p) - 1];
-    const int wholes = KEYS || p.mask != nullptr ? 0 : p.Sk / NT;  // !KEYS: tiles without a key to leave out
+    const int wholes = KEYS || p.mask != nullptr ? 0 : end / NT;  // !KEYS: tiles without a key to leave out
     KeyBytes keys = {true, true};
-    if (!KEYS) keys = key_bytes(p, b, g * NT + hh * HC);
+    if (!KEYS) keys = key_bytes(p, b, g * NT + hh * HC, end);
     int gi = 0, yi = g;  // tile t is tile yi of the walked head gi
     for (int t = g; t < n; t += 2, yi += 2) {
       if (KEYS)
@@ -763,7 +765,7 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
         bits = (uint64_t)b0 | ((uint64_t)b1 << 32);
         full = (~bits & ((1ull << HC) - 1)) == 0;
       }
-      if (!KEYS && t + 2 >= wholes) keys = key_bytes(p, b, y0 + 2 * NT + hh * HC);  // this team's next tile's, on their way
+      if (!KEYS && t + 2 >= wholes) keys = key_bytes(p, b, y0 + 2 * NT + hh * HC, end);  // this team's next tile's, on their way
       // relative position of column 0 against row 0, and how it moves: -row + column (queries own the rows) or +row - column
       const int rel0 = KEYS ? x0 - y0 - p.q_off : y0 - x0 - p.q_off;
       const bool near = KEYS ? (rel0 - (NT - 1) < p.R && rel0 + 127 > -p.R) : (rel0 - 127 < p.R && rel0 + (NT - 1) > -p.R);
@@ -846,8 +848,8 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
         if (KEYS || full) walk(no{}, no{});
         else walk(no{}, std::integral_constant<bool, !KEYS>{});
       }
-      if (!KEYS && !full && p.mask != nullptr) {
-        // masked keys may hold anything, and 0 * NaN is NaN in the dS K product: clear their rows of K
+      if (!KEYS && !full && (p.mask != nullptr || end < p.Sk)) {
+        // hidden keys may hold anything, and 0 * NaN is NaN in the dS K product: clear their rows of K
         for (int i = lane; i < HC; i += 32)
           if (!((bits >> i) & 1ull) && quarter < 2 * C::DCH) {
             // the four warps of this column half share the work: 64 bytes of a row each
@@ -913,8 +915,8 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
     if (ok && !*abort_flag) {
       tc::tc_fence_after();
       const int rows = KEYS ? p.Sk : p.Sq;
-      // a masked key's row of the sums holds whatever its K and V gave: its gradient is zero
-      const bool live = !KEYS || (x0 + r < p.Sk && (p.mask == nullptr || p.mask[(int64_t)b * p.mask_sb + x0 + r] != 0));
+      // a hidden key's row of the sums holds whatever its K and V gave: its gradient is zero
+      const bool live = !KEYS || (x0 + r < key_end(p, p.Sq - 1) && (p.mask == nullptr || p.mask[(int64_t)b * p.mask_sb + x0 + r] != 0));
       constexpr int CH = D / 32, JOBS = (KEYS ? 2 : 1) * CH;
       // staging in the idle Y ring: every MMA that read it is done
       uint8_t* stg = smem + C::OFF_Y + w16 * 4096;
