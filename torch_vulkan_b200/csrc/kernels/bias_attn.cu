@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ Pa
   if (lane == 0) sl[warp] = l;
   __syncthreads();
   const float L = (sl[0] + sl[1]) + (sl[2] + sl[3]);
-  const float inv = L > 0.f ? 1.f / L : 0.f;
+  const float inv = inverse_sum(L);
   const int64_t i = row % p.Sq, bh = row / p.Sq;
   const int d = threadIdx.x;
   if (d < p.D) {
@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ Pa
     row_of<T>(p.o, p.o_s, (int)(bh / p.H), (int)(bh % p.H), i)[d] = from_f32<T>(o);
     if (p.o32) p.o32[row * p.D + d] = o;
   }
-  if (d == 0 && p.lse) p.lse[row] = L > 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
+  if (d == 0 && p.lse) p.lse[row] = log_sum(M, L);
 }
 
 // delta[row] = sum_d dO * O, one warp per row.

@@ -64,6 +64,11 @@ __device__ __forceinline__ float bias_at(const Params& p, int h, int rel) {
   return p.table[(int64_t)bucket_of(p, r) * p.H + h] * kLog2e;
 }
 
+// What a row's unnormalised output is multiplied by, and its log-sum, from the running maximum m (log2 units) and sum l. A sum of
+// zero is a row without a key: zeros, and a log-sum of -inf. A NaN sum (a NaN or infinite score) stays one.
+__device__ __forceinline__ float inverse_sum(float l) { return l == 0.f ? 0.f : 1.f / l; }
+__device__ __forceinline__ float log_sum(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2; }
+
 template <typename T>
 __device__ __forceinline__ const T* row_of(const void* base, const int64_t* s, int b, int h, int64_t i) {
   return (const T*)base + b * s[0] + h * s[1] + i * s[2];

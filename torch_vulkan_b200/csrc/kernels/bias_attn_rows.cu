@@ -262,10 +262,10 @@ __global__ void __launch_bounds__(NW * 32) rows_mma_kernel(const __grid_constant
       p.part_o[prow * p.D + d] = acc;
       if (d == 0) p.part_ml[prow] = make_float2(M, L);
     } else {
-      acc = L > 0.f ? acc / L : 0.f;
+      acc = L == 0.f ? 0.f : acc / L;
       row_of<T>(p.o, p.o_s, b, h, i)[d] = from_f32<T>(acc);
       if (p.o32) p.o32[row * p.D + d] = acc;
-      if (d == 0 && p.lse) p.lse[row] = L > 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
+      if (d == 0 && p.lse) p.lse[row] = log_sum(M, L);
     }
   }
 }
@@ -415,14 +415,14 @@ __global__ void __launch_bounds__(NW * 32) rows_kernel(const __grid_constant__ P
       if (p.nsplit > 1) {
         p.part_o[prow * p.D + d] = o;
       } else {
-        o = L > 0.f ? o / L : 0.f;
+        o = L == 0.f ? 0.f : o / L;
         row_of<T>(p.o, p.o_s, b, h, i)[d] = o;
         if (p.o32) p.o32[row * p.D + d] = o;
       }
     }
     if (threadIdx.x == 0) {
       if (p.nsplit > 1) p.part_ml[prow] = make_float2(M, L);
-      else if (p.lse) p.lse[row] = L > 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
+      else if (p.lse) p.lse[row] = log_sum(M, L);
     }
     __syncthreads();
   }

@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(NTH) fwd_kernel(const __grid_constant__ Params
         if (d < p.D) p.part_o[pr * p.D + d] = acc[i][c];
       }
     } else {
-      const float inv = l[i] > 0.f ? 1.f / l[i] : 0.f;
+      const float inv = inverse_sum(l[i]);
       T* o = row_of<T>(p.o, p.o_s, b, h, qi);
 #pragma unroll
       for (int c = 0; c < DP / 16; ++c) {
@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(NTH) fwd_kernel(const __grid_constant__ Params
           if (p.o32) p.o32[row * p.D + d] = acc[i][c] * inv;
         }
       }
-      if (tx == 0 && p.lse) p.lse[row] = l[i] > 0.f ? (m[i] + log2f(l[i])) * kLn2 : -INFINITY;
+      if (tx == 0 && p.lse) p.lse[row] = log_sum(m[i], l[i]);
     }
   }
 }

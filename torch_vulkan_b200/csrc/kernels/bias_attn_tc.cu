@@ -442,7 +442,7 @@ __global__ void __launch_bounds__(192, 2)
     if (ok && !*abort_flag) {
       tc::tc_fence_after();
       const bool split = p.nsplit > 1;
-      const float inv = split ? 1.f : (l > 0.f ? 1.f / l : 0.f);
+      const float inv = split ? 1.f : inverse_sum(l);
       const int qrow = q0 + r;
       const int64_t row = (int64_t)blockIdx.y * p.Sq + qrow;
       const int64_t prow = (int64_t)blockIdx.z * p.B * p.H * p.Sq + row;
@@ -488,7 +488,7 @@ __global__ void __launch_bounds__(192, 2)
       }
       if (qrow < p.Sq) {
         if (split) p.part_ml[prow] = make_float2(m, l);
-        else if (p.lse) p.lse[row] = l > 0.f ? (m + __log2f(l)) * kLn2 : -INFINITY;
+        else if (p.lse) p.lse[row] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
       }
       if (lane == 0) tc::bulk_wait0();
     } else {
