@@ -80,3 +80,80 @@ def test_an_infinite_score_is_nan_and_rows_without_keys_stay_zero(dt, Sq):
     m[1] = False
     for o in (_run(q, k, v, table, m, go)["o"], _infer(q, k, v, table, m)):
         assert torch.isnan(o[0, 1]).all() and torch.isfinite(o[0, 0]).all() and not o[1].any()
+
+
+def _pairs(table, keep, max_distance, bidirectional, q_offset):
+    """Visible pairs of each bucket, keep [B, Sq, Sk]."""
+    Sq, Sk = keep.shape[1:]
+    rel = torch.arange(Sk)[None, :] - torch.arange(Sq)[:, None] - q_offset
+    lo = int(rel.min())
+    lut = torch.tensor([ot.bucket(r, table.shape[0], max_distance, bidirectional) for r in range(lo, int(rel.max()) + 1)])
+    return torch.bincount(lut[rel - lo].flatten(), weights=keep.sum(0).flatten().double(), minlength=table.shape[0])
+
+
+def _tight(got, ref, far):
+    """The bias gradient is a sum of fp32 dS. delta comes from an output good to 2^-16 + 2^-17 of itself (1024 keys are 64
+    truncating steps of P's two halves; P is good to 2^-17), the two exponentials and dP move dS by 2^-16 of itself. A far bucket
+    may be taken as minus the sum of the others, and then has their errors."""
+    own = (2.0 ** -16 + 2.0 ** -17) * ref["dtable_abs"] + 2.0 ** -16 * ref["ds_abs"] + 1e-9
+    bound = own.clone()
+    bound[far] = own.sum(0)
+    err = (got["dtable"].cpu().double() - ref["dtable"]).abs()
+    assert bool((err <= bound).all()), f"dtable: {(err / bound).max().item():.3g} of the bound"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("case", ["left", "left_causal", "far", "all_far", "before_the_keys", "none"])
+def test_a_bucket_without_a_pair_has_no_gradient(dt, D, case):
+    """Padding and the causal rule leave some buckets without a pair: their gradient is exactly zero, the others' is right."""
+    Sq, Sk, dist, kw = 1024, 1024, 128, {}
+    keep = torch.ones(1, Sk, dtype=torch.bool)
+    if case.startswith("left"):  # left padding: no two of the keys that are left are far apart
+        keep[:, :941] = False
+        if case == "left_causal":
+            kw = dict(causal=True, bidirectional=False)
+    elif case == "far":  # every key well after the queries is masked, and most before
+        Sq, kw = 300, dict(q_offset=724)
+        keep[:, :700] = keep[:, 760:] = False
+    elif case == "all_far":
+        Sq, Sk, kw = 200, 40, dict(q_offset=700)
+        keep = keep[:, :Sk]
+    elif case == "before_the_keys":  # the first queries see nothing, and no query sees a key after it
+        Sq, Sk, dist, kw = 140, 100, 4, dict(causal=True, bidirectional=True, q_offset=-100)
+        keep = keep[:, :Sk]
+    q, k, v, go, table, _ = _case(1, 2, 2, Sq, Sk, D, dt, D + Sq, nb=4 if dist == 4 else 32)
+    kw["max_distance"] = dist
+    m = None if bool(keep.all()) else keep
+    ref = ot.bias_attention(q, k, v, table, key_mask=m, go=go, **kw)
+    got = _run(q, k, v, table, m, go, **kw)
+    rel = torch.arange(Sk)[None, :] - torch.arange(Sq)[:, None] - kw.get("q_offset", 0)
+    seen = keep[:, None, :] & ((rel <= 0) if kw.get("causal") else torch.ones_like(rel, dtype=torch.bool))
+    bidir = kw.get("bidirectional", True)
+    pairs = _pairs(table, seen, dist, bidir, kw.get("q_offset", 0))
+    assert int((pairs == 0).sum()) >= (1 if case == "none" else 2)  # two-sided: the place of distance 0 after the query
+    assert not got["dtable"].cpu()[pairs == 0].any()
+    side = table.shape[0] // (2 if bidir else 1)
+    _tight(got, ref, [side - 1, table.shape[0] - 1, 0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTS)
+def test_a_nan_in_a_block_of_one_far_bucket_reaches_the_bias_gradient(dt):
+    q, k, v, go, table, _ = _case(1, 2, 2, 130, 40, 64, dt, 3)
+    v = v.clone()
+    v[0, 1, 5, 6] = NAN
+    got = _run(q, k, v, table, None, go, q_offset=900)
+    assert torch.isnan(got["dtable"][15, 1]) and torch.isfinite(got["dtable"][:, 0]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Sq,Sk,D,mask,causal", [(150, 290, 64, "tail", False), (150, 290, 128, "head", True), (700, 700, 128, "random", False),
+                                                 (700, 700, 64, "none", True), (33, 1000, 40, "tail", True), (1000, 60, 96, "none", False)])
+def test_bias_gradient_is_as_good_as_its_output(dt, Sq, Sk, D, mask, causal):
+    q, k, v, go, table, m = _case(2, 4, 2, Sq, Sk, D, dt, Sq + D, mask)
+    kw = dict(causal=causal, bidirectional=not causal, q_offset=Sk - Sq if causal else 0)
+    ref = ot.bias_attention(q, k, v, table, key_mask=m, go=go, **kw)
+    _tight(_run(q, k, v, table, m, go, **kw), ref, [31] if causal else [15, 31])
