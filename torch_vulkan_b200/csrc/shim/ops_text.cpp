@@ -406,18 +406,15 @@ struct BucketBiasAttention : torch::autograd::Function<BucketBiasAttention> {
                           const std::optional<Variable>& key_mask, int64_t max_distance, bool bidirectional, bool causal,
                           double scale, int64_t q_offset) {
     at::AutoDispatchBelowADInplaceOrView guard;
-    const bool grad = q.requires_grad() || k.requires_grad() || v.requires_grad() || table.requires_grad();
     // a backward keeps the unrounded output: its dS cancels over each row
     auto [o, lse, o32] =
-        bias_attn_fwd(q, k, v, table, key_mask, max_distance, bidirectional, causal, scale, q_offset, grad);
-    if (grad) {
-      ctx->save_for_backward({q, k, v, o32.defined() ? o32 : o, lse, table, key_mask.has_value() ? *key_mask : at::Tensor()});
-      ctx->saved_data["max_distance"] = max_distance;
-      ctx->saved_data["bidirectional"] = bidirectional;
-      ctx->saved_data["causal"] = causal;
-      ctx->saved_data["scale"] = scale;
-      ctx->saved_data["q_offset"] = q_offset;
-    }
+        bias_attn_fwd(q, k, v, table, key_mask, max_distance, bidirectional, causal, scale, q_offset, true);
+    ctx->save_for_backward({q, k, v, o32.defined() ? o32 : o, lse, table, key_mask.has_value() ? *key_mask : at::Tensor()});
+    ctx->saved_data["max_distance"] = max_distance;
+    ctx->saved_data["bidirectional"] = bidirectional;
+    ctx->saved_data["causal"] = causal;
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["q_offset"] = q_offset;
     return o;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
@@ -438,6 +435,15 @@ at::Tensor bucket_bias_attention_autograd(const at::Tensor& q, const at::Tensor&
                                           const at::Tensor& table, const std::optional<at::Tensor>& key_mask,
                                           int64_t max_distance, bool bidirectional, bool causal, double scale,
                                           int64_t q_offset) {
+  // Without a backward to come (inputs that want no gradient, or no_grad around a trainable table) the forward that keeps no
+  // unrounded output. Decided here: apply() has gradients switched off inside.
+  bool grad = false;
+  for (const at::Tensor* t : {&q, &k, &v, &table})
+    grad = grad || (at::GradMode::is_enabled() && t->requires_grad()) || t->_fw_grad(0).defined();
+  if (!grad) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return bucket_bias_attention(q, k, v, table, key_mask, max_distance, bidirectional, causal, scale, q_offset);
+  }
   return BucketBiasAttention::apply(q, k, v, table, key_mask, max_distance, bidirectional, causal, scale, q_offset);
 }
 
