@@ -25,7 +25,7 @@ def bucket_bias_attention(q, k, v, table, key_mask=None, max_distance=128, bidir
     key may be attended to; causal hides keys after the query's position i + q_offset (a decoder's new token against a
     cache of Sk keys has q_offset = Sk - Sq). scale defaults to 1 / sqrt(D). A query whose keys are all masked gets
     zeros and zero gradients; what k and v hold at masked positions, or (causal) past the last query's, is never used.
-    Differentiable in q, k, v and table; every sum has a fixed order, so results are the same bits on every call."""
+    Differentiable (once) in q, k, v and table; every sum has a fixed order, so results are the same bits on every call."""
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
     return torch.ops.b2.bucket_bias_attention(q, k, v, table, key_mask, max_distance, bidirectional, causal, scale, q_offset)

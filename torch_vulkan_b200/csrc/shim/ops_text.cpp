@@ -181,6 +181,31 @@ using torch::autograd::AutogradContext;
 using torch::autograd::Variable;
 using torch::autograd::variable_list;
 
+// Gradients of a backward that is itself recorded (create_graph): the same values, whose differentiation along `sources`, what they
+// depend on, raises an error. Derivatives of these gradients are not implemented, and unrecorded they would count as constants.
+struct Refuse : torch::autograd::Function<Refuse> {
+  static variable_list forward(AutogradContext* ctx, const std::string& name, const at::TensorList& grads, const at::TensorList&) {
+    ctx->saved_data["name"] = name;
+    variable_list out;
+    for (const at::Tensor& g : grads) out.push_back(g.detach());
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list&) {
+    TORCH_CHECK(false, ctx->saved_data["name"].toStringRef(), " cannot be differentiated twice");
+  }
+};
+void refuse_second(variable_list& grads, const variable_list& sources, const char* name) {
+  if (!at::GradMode::is_enabled()) return;
+  variable_list defined;
+  for (const Variable& g : grads)
+    if (g.defined()) defined.push_back(g);
+  if (defined.empty()) return;
+  defined = Refuse::apply(std::string(name), at::TensorList(defined), at::TensorList(sources));
+  size_t i = 0;
+  for (Variable& g : grads)
+    if (g.defined()) g = defined[i++];
+}
+
 // y = Q(x) W^T + bias; straight-through dx = dy W.
 at::Tensor mx4_linear(const at::Tensor& x, const at::Tensor& codes, const at::Tensor& scales,
                       const std::optional<at::Tensor>& bias) {
@@ -196,10 +221,15 @@ struct Mx4Linear : torch::autograd::Function<Mx4Linear> {
     return mx4_linear(x, codes, scales, bias);
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    const variable_list saved = ctx->get_saved_variables();
     variable_list out(4);
-    if (ctx->needs_input_grad(0))
-      out[0] = mx4_dx(g[0], saved[0], saved[1], ctx->saved_data["cols"].toInt(), nullptr, nullptr, "b2::mx4_linear_dx");
+    if (ctx->needs_input_grad(0)) {
+      const variable_list saved = ctx->get_saved_variables();
+      {
+        at::NoGradGuard plain;
+        out[0] = mx4_dx(g[0], saved[0], saved[1], ctx->saved_data["cols"].toInt(), nullptr, nullptr, "b2::mx4_linear_dx");
+      }
+      refuse_second(out, {g[0]}, "mx4_linear");
+    }
     if (ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(3)) out[3] = sum_rows(g[0]);
     return out;
   }
@@ -244,18 +274,22 @@ struct Mx4Lora : torch::autograd::Function<Mx4Lora> {
     const variable_list s = ctx->get_saved_variables();
     const at::Tensor &x = s[0], &codes = s[1], &scales = s[2], &a = s[3], &b = s[4], &h = s[5];
     c10::cuda::CUDAGuard guard(x.device());
-    at::Tensor gy = rows_of(g[0]);
     variable_list out(6);
     // edges are counted over the tensors that were given: without a bias, a and b move up by one
     const int e = ctx->saved_data["bias"].toBool() ? 4 : 3;
-    if (ctx->needs_input_grad(0) || ctx->needs_input_grad(e)) {
-      at::Tensor dh = at::mm(gy, b);
-      if (ctx->needs_input_grad(0))
-        out[0] = mx4_dx(gy, codes, scales, x.size(-1), &dh, &a, "b2::mx4_lora_dx").view_as(x);
-      if (ctx->needs_input_grad(e)) out[4] = at::mm(dh.t(), rows_of(x));
+    {
+      at::NoGradGuard plain;
+      at::Tensor gy = rows_of(g[0]);
+      if (ctx->needs_input_grad(0) || ctx->needs_input_grad(e)) {
+        at::Tensor dh = at::mm(gy, b);
+        if (ctx->needs_input_grad(0))
+          out[0] = mx4_dx(gy, codes, scales, x.size(-1), &dh, &a, "b2::mx4_lora_dx").view_as(x);
+        if (ctx->needs_input_grad(e)) out[4] = at::mm(dh.t(), rows_of(x));
+      }
+      if (ctx->needs_input_grad(e + 1)) out[5] = at::mm(gy.t(), h);
     }
-    if (ctx->needs_input_grad(e + 1)) out[5] = at::mm(gy.t(), h);
-    if (e == 4 && ctx->needs_input_grad(3)) out[3] = sum_rows(gy);
+    refuse_second(out, {g[0], x, a, b}, "mx4_lora_linear");
+    if (e == 4 && ctx->needs_input_grad(3)) out[3] = sum_rows(g[0]);
     return out;
   }
 };
@@ -423,11 +457,14 @@ struct BucketBiasAttention : torch::autograd::Function<BucketBiasAttention> {
     std::array<bool, 4> want;
     for (int i = 0; i < 4; ++i) want[i] = ctx->needs_input_grad(i);
     const std::optional<at::Tensor> mask = s[6].defined() ? std::optional<at::Tensor>(s[6]) : std::nullopt;
-    auto [dq, dk, dv, dt] = bias_attn_bwd(g[0], s[0], s[1], s[2], s[3], s[4], s[5], mask, d["max_distance"].toInt(),
-                                          d["bidirectional"].toBool(), d["causal"].toBool(), d["scale"].toDouble(),
-                                          d["q_offset"].toInt(), want);
     variable_list out(10);
-    out[0] = dq, out[1] = dk, out[2] = dv, out[3] = dt;
+    {
+      at::NoGradGuard plain;
+      std::tie(out[0], out[1], out[2], out[3]) =
+          bias_attn_bwd(g[0], s[0], s[1], s[2], s[3], s[4], s[5], mask, d["max_distance"].toInt(), d["bidirectional"].toBool(),
+                        d["causal"].toBool(), d["scale"].toDouble(), d["q_offset"].toInt(), want);
+    }
+    refuse_second(out, {g[0], s[0], s[1], s[2], s[5]}, "bucket_bias_attention");
     return out;
   }
 };

@@ -25,6 +25,8 @@ import torch.nn.functional as F
 
 import torch_vulkan_b200 as tv
 
+from ._refuse import refuse_second
+
 
 class Int8Linear(nn.Module):
     """Frozen int8 weight [out, in] with a per-output-row fp32 scale; y = x (W*s)^T + b."""
@@ -196,28 +198,38 @@ class _StackedMx4LoRA(torch.autograd.Function):
         if not x2.is_contiguous():
             x2 = x2.contiguous()
         y, h = torch.ops.b2.mx4_lora_fwd(x2, codes, scales, bias, grp.a, grp.b_bd)
-        ctx.save_for_backward(x2, codes, scales, h)
-        ctx.grp, ctx.x_shape = grp, x.shape
+        ctx.save_for_backward(x, codes, scales, h)
+        ctx.grp, ctx.params = grp, params
         return y.view(*x.shape[:-1], codes.shape[0])
 
     @staticmethod
     def backward(ctx, gy):
-        x2, codes, scales, h = ctx.saved_tensors
+        sources = (gy, ctx.saved_tensors[0], *ctx.params)
+        gx, *rest = refuse_second("stacked mx4_lora_linear", _StackedMx4LoRA.gradients(ctx, gy), sources)
+        return (gx, None, None, None, None, *rest)
+
+    @staticmethod
+    @torch.no_grad()
+    def gradients(ctx, gy):
+        x, codes, scales, h = ctx.saved_tensors
         grp = ctx.grp
+        x2 = x.reshape(-1, x.shape[-1])
+        if not x2.is_contiguous():
+            x2 = x2.contiguous()
         gy2 = gy.reshape(-1, gy.shape[-1])
         if not gy2.is_contiguous():
             gy2 = gy2.contiguous()
         dh = torch.mm(gy2, grp.b_bd)
         gx = None
         if ctx.needs_input_grad[0]:
-            gx = torch.ops.b2.mx4_lora_dx(gy2, codes, scales, x2.shape[1], dh, grp.a).view(ctx.x_shape)
+            gx = torch.ops.b2.mx4_lora_dx(gy2, codes, scales, x2.shape[1], dh, grp.a).view(x.shape)
         ga = torch.mm(dh.t(), x2)
         gb = grp.diag_blocks(torch.mm(gy2.t(), h))
         if grp.scale != 1.0:
             gb.mul_(grp.scale)
         gdown = [ga[i * grp.r:(i + 1) * grp.r] for i in range(grp.g)]
         gup = [gb[i * grp.n:(i + 1) * grp.n] for i in range(grp.g)]
-        return (gx, None, None, None, None, *gdown, *gup)
+        return [gx, *gdown, *gup]
 
 
 def stacked_mx4_lora_forward(x, codes, scales, bias, grp: LoRAGroup, whole=False):

@@ -3,7 +3,8 @@ power-of-two scale (E8M0) per 32 columns, 4.25 bits a value.
 
 ``mx4_quantize`` / ``mx4_dequantize`` make and read an ``Mx4``; ``mx4_linear`` multiplies by a frozen ``Mx4`` weight,
 quantising its activation in the call; ``mx4_lora_linear`` adds the LoRA side path in the same product. The backward
-passes are straight-through: dX = dY W with the quantised weight and an unquantised dY. CUDA tensors only."""
+passes are straight-through: dX = dY W with the quantised weight and an unquantised dY; gradients cannot be differentiated
+again (an error says so). CUDA tensors only."""
 
 from __future__ import annotations
 
