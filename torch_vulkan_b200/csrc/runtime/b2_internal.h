@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <mutex>
 #include <string>
 
 #include "../../../include/b2rt.h"
@@ -77,16 +78,20 @@ int launch_pdl(const char* name, void (*kernel)(KArgs...), dim3 grid, dim3 block
 }
 
 // Raises a kernel's dynamic shared-memory limit, once per kernel and device (and again only for a larger size): the
-// attribute call costs about as much host time as a launch. KERNEL is a template parameter, so each has its own record.
+// attribute call costs about as much host time as a launch. KERNEL is a template parameter, so each has its own record. The
+// attribute can go down as well as up, so threads that ask for different sizes set it and record it one at a time.
 template <auto KERNEL>
 int allow_smem(int bytes, const char* what) {
   static std::atomic<int> have[64];
+  static std::mutex one_at_a_time;
   int dev = 0;
   if (int rc = check_cuda(cudaGetDevice(&dev), what)) return rc;
   const bool known = dev >= 0 && dev < 64;
+  if (known && have[dev].load(std::memory_order_acquire) >= bytes) return 0;
+  std::lock_guard<std::mutex> lock(one_at_a_time);
   if (known && have[dev].load(std::memory_order_relaxed) >= bytes) return 0;
   if (int rc = check_cuda(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), what)) return rc;
-  if (known) have[dev].store(bytes, std::memory_order_relaxed);
+  if (known) have[dev].store(bytes, std::memory_order_release);
   return 0;
 }
 
