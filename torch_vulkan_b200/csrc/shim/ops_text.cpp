@@ -85,10 +85,10 @@ at::Tensor rows_of(const at::Tensor& t) {
 
 // LoRA side operands: h [rows, r] and the weight-side matrix ([N, r] forward, [r, K] in dX), both bf16.
 void lora_operands(b2_mx4_gemm_args& g, const at::Tensor* h, const at::Tensor* w, at::Tensor& hc, at::Tensor& wc,
-                   int64_t rows, int64_t width, const char* what) {
+                   int64_t rows, int64_t width, c10::Device device, const char* what) {
   if (!h) return;
-  TORCH_CHECK(h->is_cuda() && w->is_cuda() && h->scalar_type() == at::kBFloat16 && w->scalar_type() == at::kBFloat16, what,
-              ": bf16 CUDA LoRA operands required");
+  TORCH_CHECK(h->device() == device && w->device() == device && h->scalar_type() == at::kBFloat16 &&
+                  w->scalar_type() == at::kBFloat16, what, ": the LoRA operands must be bf16 tensors on x's device");
   hc = rows_of(*h), wc = w->contiguous();
   const int64_t r = hc.size(1);
   TORCH_CHECK(hc.size(0) == rows && r >= 8 && r <= 64 && r % 8 == 0, what,
@@ -119,8 +119,9 @@ at::Tensor mx4_fwd(const at::Tensor& x0, const at::Tensor& codes, const at::Tens
   at::Tensor bias;
   if (bias0.has_value() && bias0->defined()) {
     bias = bias0->contiguous();
-    TORCH_CHECK(bias.is_cuda() && bias.scalar_type() == at::kBFloat16 && bias.numel() == N, name,
-                ": bias must be a bf16 CUDA tensor of ", N, " elements");
+    TORCH_CHECK(bias.device() == x0.device() && bias.scalar_type() == at::kBFloat16 && bias.numel() == N, name,
+                ": bias must be a bf16 tensor of ", N, " elements on x's device, got ", bias.scalar_type(), " ", bias.sizes(), " on ",
+                bias.device());
   }
   at::Tensor out = at::empty(osz, x0.options());
   if (out.numel() == 0) return out;
@@ -139,7 +140,7 @@ at::Tensor mx4_fwd(const at::Tensor& x0, const at::Tensor& codes, const at::Tens
   g.out = out.data_ptr();
   g.M = x.size(0), g.N = N, g.K = K, g.out_ld = N;
   at::Tensor hc, wc;
-  lora_operands(g, h, b, hc, wc, g.M, N, name);
+  lora_operands(g, h, b, hc, wc, g.M, N, x.device(), name);
   at::Tensor ws = workspace(b2_mx4_gemm_workspace_bytes(&g), x);
   g.workspace = ws.defined() ? ws.data_ptr() : nullptr;
   b2_check(b2_mx4_gemm(&g, cur_stream()), name);
@@ -167,7 +168,7 @@ at::Tensor mx4_dx(const at::Tensor& dy0, const at::Tensor& codes, const at::Tens
   g.M = dy.size(0), g.N = d.rows, g.K = K, g.x_ld = d.rows, g.out_ld = K;
   g.transpose_w = 1;
   at::Tensor hc, wc;
-  lora_operands(g, h, a, hc, wc, g.M, K, name);
+  lora_operands(g, h, a, hc, wc, g.M, K, dy.device(), name);
   at::Tensor ws = workspace(b2_mx4_gemm_workspace_bytes(&g), dy);
   g.workspace = ws.defined() ? ws.data_ptr() : nullptr;
   b2_check(b2_mx4_gemm(&g, cur_stream()), name);
@@ -245,8 +246,8 @@ std::tuple<at::Tensor, at::Tensor> mx4_lora_fwd(const at::Tensor& x, const at::T
                                                 const at::Tensor& b) {
   const char* name = "b2::mx4_lora_linear";
   TORCH_CHECK(x.is_cuda() && x.scalar_type() == at::kBFloat16 && x.dim() >= 1, name, ": x must be a bfloat16 CUDA tensor");
-  TORCH_CHECK(a.dim() == 2 && b.dim() == 2 && a.is_cuda() && a.scalar_type() == at::kBFloat16 && a.size(1) == x.size(-1), name,
-              ": a must be a bf16 CUDA matrix [r, ", x.size(-1), "], got ", a.scalar_type(), " ", a.sizes());
+  TORCH_CHECK(a.dim() == 2 && b.dim() == 2 && a.device() == x.device() && a.scalar_type() == at::kBFloat16 && a.size(1) == x.size(-1), name,
+              ": a must be a bf16 matrix [r, ", x.size(-1), "] on x's device, got ", a.scalar_type(), " ", a.sizes(), " on ", a.device());
   c10::cuda::CUDAGuard guard(x.device());
   at::Tensor h = at::mm(rows_of(x), a.t());  // of the unquantised activation
   at::Tensor y = mx4_fwd(x, codes, scales, bias, &h, &b, name);
