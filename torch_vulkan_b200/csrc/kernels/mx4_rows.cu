@@ -139,9 +139,10 @@ __global__ void __launch_bounds__(NWARP * 32, 2) mx4_rows_kernel(const __grid_co
 #pragma unroll
           for (int m = 0; m < M; ++m) s[m] = __dp4a(pos, xv[m][q], s[m]), t[m] = __dp4a(neg, xv[m][q], t[m]);
         }
+        // the weight's scale first: a sum of 32 products passes fp32's range under the scale of activations above 2^119
         const float ws = mx4::e8m0_to_f32(csc[r]);
 #pragma unroll
-        for (int m = 0; m < M; ++m) acc[r][m] = fmaf((float)(s[m] - t[m]) * xsc[m * p.nblk + blk], ws, acc[r][m]);
+        for (int m = 0; m < M; ++m) acc[r][m] = fmaf((float)(s[m] - t[m]) * ws, xsc[m * p.nblk + blk], acc[r][m]);
       }
     }
     if (p.r) {  // the LoRA term: two columns of h and b a lane
