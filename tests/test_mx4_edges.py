@@ -19,3 +19,17 @@ def test_the_largest_activations(m):
     xq, wq = ot.mx4_round(x), ot.mx4_round((w.float() * 2.0 ** -10).to(BF))
     assert (xq.abs() @ wq.abs().t()).max() < 3e38
     _close(y, xq @ wq.t(), xq.abs() @ wq.abs().t())
+
+
+@pytest.mark.gpu
+def test_no_output_features_and_no_rows():
+    import torch_vulkan_b200 as tv
+
+    for m, n in ((5, 0), (0, 40), (0, 0)):
+        w = tv.mx4_quantize(torch.randn(n, 64, device="cuda"))
+        x = torch.randn(m, 64, device="cuda").bfloat16().requires_grad_(True)
+        a, b, bias = (torch.randn(*s, device="cuda").bfloat16().requires_grad_(True) for s in ((8, 64), (n, 8), (n,)))
+        for y, leaf in ((tv.mx4_linear(x, w, bias), (x, bias)), (tv.mx4_lora_linear(x, w, bias, a, b), (x, a, b, bias))):
+            assert y.shape == (m, n)
+            for t, g in zip(leaf, torch.autograd.grad(y, leaf, torch.ones_like(y))):
+                assert g.shape == t.shape and not g.any()

@@ -79,7 +79,9 @@ at::Tensor mx4_dequantize(const at::Tensor& codes, const at::Tensor& scales, int
 }
 
 at::Tensor rows_of(const at::Tensor& t) {
-  at::Tensor m = t.reshape({-1, t.size(-1)});
+  int64_t rows = 1;  // counted: -1 says nothing about a tensor without elements
+  for (int64_t i = 0; i + 1 < t.dim(); ++i) rows *= t.size(i);
+  at::Tensor m = t.reshape({rows, t.size(-1)});
   return m.is_contiguous() ? m : m.contiguous();
 }
 
