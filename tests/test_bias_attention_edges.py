@@ -157,3 +157,29 @@ def test_bias_gradient_is_as_good_as_its_output(dt, Sq, Sk, D, mask, causal):
     kw = dict(causal=causal, bidirectional=not causal, q_offset=Sk - Sq if causal else 0)
     ref = ot.bias_attention(q, k, v, table, key_mask=m, go=go, **kw)
     _tight(_run(q, k, v, table, m, go, **kw), ref, [31] if causal else [15, 31])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("D", [64, 128, 20])
+def test_a_row_with_one_key_has_no_gradient_of_its_scores(dt, D):
+    """P is 1 there whatever the score: dq and the bias gradient are exactly zero, and a NaN is not lost."""
+    Sq, Sk = 200, 300
+    q, k, v, go, table, _ = _case(2, 4, 2, Sq, Sk, D, dt, D)
+    m = torch.zeros(2, Sk, dtype=torch.bool)
+    m[0, 123] = m[1, 299] = True
+    got = _check(q, k, v, go, table, m)
+    assert not got["dq"].any() and not got["dtable"].any()
+    m[1, 7] = True  # the second sample's queries choose between two keys
+    got = _check(q, k, v, go, table, m)
+    assert not got["dq"][0].any() and got["dq"][1].any() and got["dtable"].any()
+    kw = dict(causal=True, bidirectional=False, q_offset=0)
+    m[0, 5:] = True
+    got = _check(q, k, v, go, table, m, **kw)  # none for rows 0..4 of the first sample, one for row 5; one for the second's rows 7..
+    assert not got["dq"][0, :, :6].any() and got["dq"][0, :, 6:].any(-1).all() and not got["dq"][1].any()
+    got = _check(q, k, v, go, table, None, **kw)
+    assert not got["dq"][:, :, 0].any() and got["dq"][:, :, 1:].any(-1).all()
+    v = v.clone()
+    v[0, 0, 0, 1] = NAN
+    got = _run(q, k, v, table, None, go, **kw)
+    assert torch.isnan(got["dq"][0, 0, 0]).any() and torch.isnan(got["dtable"][:, 0]).any()

@@ -93,10 +93,9 @@ __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ Para
   if (lane == 0) delta[row] = s;
 }
 
-// dtable[n][h] = sum over batch and query tiles of the partial sums, one warp per (n, h), a fixed order. With a single key P
-// is 1 and dS zero: what dP - delta left there by rounding is dropped, infinities and NaN are not.
+// dtable[n][h] = sum over batch and query tiles of the partial sums, one warp per (n, h), a fixed order.
 __global__ void __launch_bounds__(256) dtable_kernel(const float* __restrict__ part, float* __restrict__ dtable, int B,
-                                                     int H, int nt, int nb, int Sk) {
+                                                     int H, int nt, int nb) {
   const int lane = threadIdx.x & 31;
   const int w = blockIdx.x * 8 + (threadIdx.x >> 5);
   tc::pdl_wait();
@@ -107,7 +106,7 @@ __global__ void __launch_bounds__(256) dtable_kernel(const float* __restrict__ p
   for (int64_t i = lane; i < (int64_t)B * nt; i += 32)
     s += part[((i / nt * H + h) * nt + i % nt) * nb + n];
   s = warp_sum(s);
-  if (lane == 0) dtable[n * H + h] = Sk == 1 ? 0.f * s : s;
+  if (lane == 0) dtable[n * H + h] = s;
 }
 
 __global__ void __launch_bounds__(256) zero_rows_kernel(uint8_t* o, int64_t s0, int64_t s1, int64_t s2, int H, int64_t S,
@@ -348,7 +347,7 @@ extern "C" int b2_bias_attn_bwd(const b2_bias_attn_args* a, b2_stream_t stream) 
   }
   if (a->dtable) {
     return launch_pdl("bias_attn_dtable", dtable_kernel, dim3((unsigned)((p.nb * p.H + 7) / 8)), dim3(256), 0, st,
-                      (const float*)p.dtab, a->dtable, p.B, p.H, pl.ntq, p.nb, p.Sk);
+                      (const float*)p.dtab, a->dtable, p.B, p.H, pl.ntq, p.nb);
   }
   return 0;
 }

@@ -85,6 +85,49 @@ __device__ __forceinline__ int key_end(const Params& p, int64_t last_row) {
   return e < 0 ? 0 : (e < p.Sk ? (int)e : p.Sk);
 }
 
+// What the mask leaves of the keys below `end`: one past the last, how many there are, how many up to key lo and from key hi on,
+// and the first two (INT_MAX: there is none). Every thread of the block calls it and gets the same; the row of the mask is read at
+// once, in one trip to memory. slot: six ints of shared memory.
+struct Visible {
+  int last, total, past, ahead, first, second;
+};
+__device__ __forceinline__ Visible visible_keys(const Params& p, int b, int end, int lo, int hi, int nthreads, int* slot) {
+  constexpr int NONE = 0x7fffffff;
+  if (p.mask == nullptr)
+    return {end, end, max(0, min(end, lo + 1)), max(0, end - max(0, hi)), end > 0 ? 0 : NONE, end > 1 ? 1 : NONE};
+  const uint8_t* m = p.mask + (int64_t)b * p.mask_sb;
+  if (threadIdx.x < 6) slot[threadIdx.x] = threadIdx.x < 4 ? 0 : NONE;
+  Visible v = {0, 0, 0, 0, NONE, NONE};
+#pragma unroll 8
+  for (int j = (int)threadIdx.x; j < end; j += nthreads) {
+    const bool on = m[j] != 0;
+    v.last = on ? j + 1 : v.last;
+    v.total += on, v.past += on && j <= lo, v.ahead += on && j >= hi;
+    v.second = on ? min(v.second, max(v.first, j)) : v.second;
+    v.first = on ? min(v.first, j) : v.first;
+  }
+  __syncthreads();
+  const unsigned all = 0xffffffffu;
+  const bool lead = (threadIdx.x & 31) == 0;
+  v.last = __reduce_max_sync(all, v.last), v.total = __reduce_add_sync(all, v.total);
+  v.past = __reduce_add_sync(all, v.past), v.ahead = __reduce_add_sync(all, v.ahead);
+  const int first = __reduce_min_sync(all, v.first);
+  const int second = __reduce_min_sync(all, v.first == first ? v.second : v.first);
+  if (lead && v.total > 0) {
+    atomicMax(slot, v.last), atomicMin(slot + 4, first);
+    atomicAdd(slot + 1, v.total), atomicAdd(slot + 2, v.past), atomicAdd(slot + 3, v.ahead);
+  }
+  __syncthreads();
+  if (lead && v.total > 0) atomicMin(slot + 5, first == slot[4] ? second : first);
+  __syncthreads();
+  return {slot[0], slot[1], slot[2], slot[3], slot[4], slot[5]};
+}
+// Whether query row i sees exactly one key. P is 1 there whatever the score, so dS is zero.
+__device__ __forceinline__ bool sees_one(const Params& p, int i, int first, int second) {
+  const int lim = p.causal ? i + p.q_off : p.Sk - 1;
+  return first <= lim && second > lim;
+}
+
 int simt_fwd(const Params& p, int dtype, cudaStream_t st);   // bias_attn_simt.cu
 int simt_bwd(const Params& p, int dtype, cudaStream_t st);
 constexpr int kSimtTile = 32, kSimtWalk = 64;

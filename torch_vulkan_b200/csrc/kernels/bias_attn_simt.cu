@@ -240,6 +240,8 @@ __device__ __forceinline__ void dq_side(const Params& p, int block, int xtiles) 
   load_tile<T, DP, OWN>(Qs, p.q, p.q_s, b, h, q0, p.Sq, p.D, p.scale * kLog2e, nullptr);
   load_tile<T, DP, OWN>(Gs, p.d_o, p.do_s, b, h, q0, p.Sq, p.D, 1.f, nullptr);
   float L[4], dl[4], acc[4][DP / 16];
+  const int end = key_end(p, min(q0 + OWN, p.Sq) - 1), nt = (end + T64 - 1) / T64;
+  const Visible seen = visible_keys(p, b, end, 0, 0, NTH, reinterpret_cast<int*>(diag));
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int qi = q0 + ty * 4 + i;
@@ -248,11 +250,11 @@ __device__ __forceinline__ void dq_side(const Params& p, int block, int xtiles) 
     L[i] = qi < p.Sq ? p.lse[row] * kLog2e : INFINITY;
     if (L[i] == -INFINITY) L[i] = INFINITY;
     dl[i] = qi < p.Sq ? p.delta[row] : 0.f;
+    if (sees_one(p, qi, seen.first, seen.second) && isfinite(L[i] + dl[i])) L[i] = INFINITY;  // dS = 0; a NaN goes its way
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) acc[i][c] = 0.f;
   }
   float db = 0.f;  // thread n: sum of dS over bucket n
-  const int end = key_end(p, min(q0 + OWN, p.Sq) - 1), nt = (end + T64 - 1) / T64;
   for (int t = 0; t < nt; ++t) {
     const int k0 = t * T64;
     __syncthreads();

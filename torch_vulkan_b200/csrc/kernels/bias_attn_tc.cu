@@ -82,36 +82,19 @@ __device__ __forceinline__ int trim_end(const Params& p, int b, int end, int nth
   return *slot;
 }
 
-// The same for the query side of the backward, and into *big the bucket whose sum is taken from the others' (see the end of
+// The same for the query side of the backward. row_keys[0]: the bucket whose sum is taken from the others' (see the end of
 // bwd_side), or -1: the far bucket of one side where it holds more than half of the keys that the block's middle row sees. Only
-// visible keys count, so that the bucket has a pair. slot: four ints of shared memory.
-__device__ __forceinline__ int trim_end_and_pick(const Params& p, int b, int end, int mid, int nthreads, int* slot, volatile int* big) {
+// visible keys count, so that the bucket has a pair. row_keys[1], [2]: the first two visible keys. slot: six ints of shared memory.
+__device__ __forceinline__ int trim_end_and_pick(const Params& p, int b, int end, int mid, int nthreads, int* slot,
+                                                 volatile int* row_keys) {
   const int side = p.bidir ? p.nb / 2 : p.nb, beyond = p.thr[side - 2];
-  const int lo = mid - beyond, hi = p.bidir ? mid + beyond : mid;  // one-sided: keys after the query share bucket 0
-  int last = end, total = end, past = max(0, min(end, lo + 1)), ahead = max(0, end - max(0, hi));
-  if (p.mask != nullptr) {
-    const uint8_t* m = p.mask + (int64_t)b * p.mask_sb;
-    if (threadIdx.x < 4) slot[threadIdx.x] = 0;
-    last = total = past = ahead = 0;
-#pragma unroll 8
-    for (int j = (int)threadIdx.x; j < end; j += nthreads) {
-      const bool on = m[j] != 0;
-      last = on ? j + 1 : last;
-      total += on, past += on && j <= lo, ahead += on && j >= hi;
-    }
-    __syncthreads();
-    last = __reduce_max_sync(0xffffffffu, last);
-    total = __reduce_add_sync(0xffffffffu, total), past = __reduce_add_sync(0xffffffffu, past);
-    ahead = __reduce_add_sync(0xffffffffu, ahead);
-    if ((threadIdx.x & 31) == 0 && total > 0) {
-      atomicMax(slot, last);
-      atomicAdd(slot + 1, total), atomicAdd(slot + 2, past), atomicAdd(slot + 3, ahead);
-    }
-    __syncthreads();
-    last = slot[0], total = slot[1], past = slot[2], ahead = slot[3];
+  // one-sided: keys after the query share bucket 0
+  const Visible v = visible_keys(p, b, end, mid - beyond, p.bidir ? mid + beyond : mid, nthreads, slot);
+  if (threadIdx.x == 0) {
+    row_keys[0] = 2 * v.past > v.total ? side - 1 : !p.causal && 2 * v.ahead > v.total ? (p.bidir ? p.nb - 1 : 0) : -1;
+    row_keys[1] = v.first, row_keys[2] = v.second;
   }
-  if (threadIdx.x == 0) *big = 2 * past > total ? side - 1 : !p.causal && 2 * ahead > total ? (p.bidir ? p.nb - 1 : 0) : -1;
-  return last;
+  return v.last;
 }
 
 // A warp's 32 rows of O (TMEM, relative to the maximum m) and their earlier part (relative to run_m): in TMEM columns of its own
@@ -621,7 +604,7 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
   uint64_t* acc_full = pd_full + NB;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(acc_full + 2);
-  volatile int* big_bucket = abort_flag + 1;  // !KEYS
+  volatile int* row_keys = abort_flag + 1;  // !KEYS: [3], see trim_end_and_pick
   const int vlen4 = (vec_len(p) + 3) / 4 * 4, dlen = (2 * p.R + 1 + 3) / 4 * 4;
   float* vec = reinterpret_cast<float*>(smem + C::OFF_VEC);  // KEYS: one per team (the head changes along the walk)
   float* darr = vec + vlen4;                                 // !KEYS: diagonal sums, one array per warp
@@ -658,7 +641,7 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
     tiles = any ? nt - first : 0;
   } else {
     end = trim_end_and_pick(p, b, key_end(p, min(x0 + C::BX, p.Sq) - 1), x0 + min(C::BX, p.Sq - x0) / 2 + p.q_off, C::THREADS,
-                            reinterpret_cast<int*>(vec), big_bucket);
+                            reinterpret_cast<int*>(vec), row_keys);
     tiles = (end + NT - 1) / NT;
   }
   tc::tc_fence_before();
@@ -765,6 +748,7 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
     if (!KEYS) {  // while the first tiles are loaded and multiplied
       const float2 ld = lsed[((int64_t)b * p.H + hx) * sq_pad + x0 + r];
       nL = ld.x, nd = ld.y;
+      if (sees_one(p, x0 + r, row_keys[1], row_keys[2]) && isfinite(nL + nd)) nL = -INFINITY;  // dS = 0; a NaN goes its way
       fill_vec(p, hx, vec, (int)threadIdx.x - 64, C::EW);
       if (p.dtab)
         for (int i = (int)threadIdx.x - 64; i < 16 * dlen; i += C::EW) darr[i] = 0.f;
@@ -935,7 +919,7 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
       // on one side) that bucket's sum is minus the others': what an error of delta leaves in a bucket goes with the share of P
       // there. A NaN or infinity that only the bucket itself has stays
       if (w16 == 0) {
-        const int big = *big_bucket;
+        const int big = row_keys[0];
         float rest = 0.f;
         for (int i = lane; i < p.nb; i += 32) rest += i == big ? 0.f : dscr[i];
         rest = warp_sum(rest);
