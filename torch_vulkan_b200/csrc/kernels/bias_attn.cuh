@@ -87,7 +87,7 @@ __device__ __forceinline__ int key_end(const Params& p, int64_t last_row) {
 
 // What the mask leaves of the keys below `end`: one past the last, how many there are, how many up to key lo and from key hi on,
 // and the first two (INT_MAX: there is none). Every thread of the block calls it and gets the same; the row of the mask is read at
-// once, in one trip to memory. slot: six ints of shared memory.
+// once, in one trip to memory. slot: six ints of shared memory per warp, free again after the block's next barrier.
 struct Visible {
   int last, total, past, ahead, first, second;
 };
@@ -96,7 +96,6 @@ __device__ __forceinline__ Visible visible_keys(const Params& p, int b, int end,
   if (p.mask == nullptr)
     return {end, end, max(0, min(end, lo + 1)), max(0, end - max(0, hi)), end > 0 ? 0 : NONE, end > 1 ? 1 : NONE};
   const uint8_t* m = p.mask + (int64_t)b * p.mask_sb;
-  if (threadIdx.x < 6) slot[threadIdx.x] = threadIdx.x < 4 ? 0 : NONE;
   Visible v = {0, 0, 0, 0, NONE, NONE};
 #pragma unroll 8
   for (int j = (int)threadIdx.x; j < end; j += nthreads) {
@@ -106,21 +105,23 @@ __device__ __forceinline__ Visible visible_keys(const Params& p, int b, int end,
     v.second = on ? min(v.second, max(v.first, j)) : v.second;
     v.first = on ? min(v.first, j) : v.first;
   }
-  __syncthreads();
-  const unsigned all = 0xffffffffu;
-  const bool lead = (threadIdx.x & 31) == 0;
-  v.last = __reduce_max_sync(all, v.last), v.total = __reduce_add_sync(all, v.total);
-  v.past = __reduce_add_sync(all, v.past), v.ahead = __reduce_add_sync(all, v.ahead);
-  const int first = __reduce_min_sync(all, v.first);
-  const int second = __reduce_min_sync(all, v.first == first ? v.second : v.first);
-  if (lead && v.total > 0) {
-    atomicMax(slot, v.last), atomicMin(slot + 4, first);
-    atomicAdd(slot + 1, v.total), atomicAdd(slot + 2, v.past), atomicAdd(slot + 3, v.ahead);
+  // the lanes' into one, then the warps', which every warp joins for itself
+  auto join = [](Visible a, bool counts) -> Visible {
+    const unsigned all = 0xffffffffu;
+    const int first = __reduce_min_sync(all, a.first);
+    return {__reduce_max_sync(all, a.last), __reduce_add_sync(all, counts ? a.total : 0),
+            __reduce_add_sync(all, counts ? a.past : 0), __reduce_add_sync(all, counts ? a.ahead : 0), first,
+            __reduce_min_sync(all, a.first == first ? a.second : a.first)};
+  };
+  v = join(v, true);
+  const int lane = threadIdx.x & 31, warps = nthreads / 32;
+  if (lane == 0) {
+    int* s = slot + (threadIdx.x >> 5) * 6;
+    s[0] = v.last, s[1] = v.total, s[2] = v.past, s[3] = v.ahead, s[4] = v.first, s[5] = v.second;
   }
   __syncthreads();
-  if (lead && v.total > 0) atomicMin(slot + 5, first == slot[4] ? second : first);
-  __syncthreads();
-  return {slot[0], slot[1], slot[2], slot[3], slot[4], slot[5]};
+  const int* s = slot + min(lane, warps - 1) * 6;
+  return join(Visible{s[0], s[1], s[2], s[3], s[4], s[5]}, lane < warps);
 }
 // Whether query row i sees exactly one key. P is 1 there whatever the score, so dS is zero.
 __device__ __forceinline__ bool sees_one(const Params& p, int i, int first, int second) {

@@ -82,19 +82,12 @@ __device__ __forceinline__ int trim_end(const Params& p, int b, int end, int nth
   return *slot;
 }
 
-// The same for the query side of the backward. row_keys[0]: the bucket whose sum is taken from the others' (see the end of
-// bwd_side), or -1: the far bucket of one side where it holds more than half of the keys that the block's middle row sees. Only
-// visible keys count, so that the bucket has a pair. row_keys[1], [2]: the first two visible keys. slot: six ints of shared memory.
-__device__ __forceinline__ int trim_end_and_pick(const Params& p, int b, int end, int mid, int nthreads, int* slot,
-                                                 volatile int* row_keys) {
-  const int side = p.bidir ? p.nb / 2 : p.nb, beyond = p.thr[side - 2];
-  // one-sided: keys after the query share bucket 0
-  const Visible v = visible_keys(p, b, end, mid - beyond, p.bidir ? mid + beyond : mid, nthreads, slot);
-  if (threadIdx.x == 0) {
-    row_keys[0] = 2 * v.past > v.total ? side - 1 : !p.causal && 2 * v.ahead > v.total ? (p.bidir ? p.nb - 1 : 0) : -1;
-    row_keys[1] = v.first, row_keys[2] = v.second;
-  }
-  return v.last;
+// The bucket whose sum the query side of the backward takes from the others' (see the end of bwd_side), or -1: the far bucket of
+// one side where it holds more than half of the keys that the block's middle row sees. Only visible keys count, so that the
+// bucket has a pair.
+__device__ __forceinline__ int big_bucket(const Params& p, const Visible& v) {
+  const int side = p.bidir ? p.nb / 2 : p.nb;
+  return 2 * v.past > v.total ? side - 1 : !p.causal && 2 * v.ahead > v.total ? (p.bidir ? p.nb - 1 : 0) : -1;
 }
 
 // A warp's 32 rows of O (TMEM, relative to the maximum m) and their earlier part (relative to run_m): in TMEM columns of its own
@@ -604,7 +597,7 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
   uint64_t* acc_full = pd_full + NB;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(acc_full + 2);
-  volatile int* row_keys = abort_flag + 1;  // !KEYS: [3], see trim_end_and_pick
+  volatile int* big_slot = abort_flag + 1;  // !KEYS: big_bucket of this block, and one past its last key
   const int vlen4 = (vec_len(p) + 3) / 4 * 4, dlen = (2 * p.R + 1 + 3) / 4 * 4;
   float* vec = reinterpret_cast<float*>(smem + C::OFF_VEC);  // KEYS: one per team (the head changes along the walk)
   float* darr = vec + vlen4;                                 // !KEYS: diagonal sums, one array per warp
@@ -631,6 +624,7 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
     tc::tmem_alloc(tmem_slot, C::TMEM_COLS);
     tc::tmem_relinquish();
   }
+  Visible seen = {};
   int first = 0, tiles, end = p.Sk;  // tiles first .. first + tiles of every walked head; !KEYS: one past the last key
   if (KEYS) {
     const int any = p.mask == nullptr ||
@@ -640,8 +634,12 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
     if (p.causal) first = (int)min((int64_t)nt, max((int64_t)0, (int64_t)x0 - p.q_off) / NT);
     tiles = any ? nt - first : 0;
   } else {
-    end = trim_end_and_pick(p, b, key_end(p, min(x0 + C::BX, p.Sq) - 1), x0 + min(C::BX, p.Sq - x0) / 2 + p.q_off, C::THREADS,
-                            reinterpret_cast<int*>(vec), row_keys);
+    // far from the block's middle row; one-sided: keys after the query share bucket 0
+    const int beyond = p.thr[(p.bidir ? p.nb / 2 : p.nb) - 2], mid = x0 + min(C::BX, p.Sq - x0) / 2 + p.q_off;
+    seen = visible_keys(p, b, key_end(p, min(x0 + C::BX, p.Sq) - 1), mid - beyond, p.bidir ? mid + beyond : mid, C::THREADS,
+                        reinterpret_cast<int*>(vec));
+    end = seen.last;
+    if (threadIdx.x == 0) big_slot[1] = end;
     tiles = (end + NT - 1) / NT;
   }
   tc::tc_fence_before();
@@ -748,11 +746,12 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
     if (!KEYS) {  // while the first tiles are loaded and multiplied
       const float2 ld = lsed[((int64_t)b * p.H + hx) * sq_pad + x0 + r];
       nL = ld.x, nd = ld.y;
-      if (sees_one(p, x0 + r, row_keys[1], row_keys[2]) && isfinite(nL + nd)) nL = -INFINITY;  // dS = 0; a NaN goes its way
+      if (w16 == 0 && lane == 0) *big_slot = big_bucket(p, seen);
       fill_vec(p, hx, vec, (int)threadIdx.x - 64, C::EW);
       if (p.dtab)
         for (int i = (int)threadIdx.x - 64; i < 16 * dlen; i += C::EW) darr[i] = 0.f;
       tc::named_bar_sync(1, C::EW);
+      if (sees_one(p, x0 + r, seen.first, seen.second) && isfinite(nL + nd)) nL = -INFINITY;  // dS = 0; a NaN goes its way
     }
     float far_lo = 0.f, far_hi = 0.f;
     int cur = -1;  // KEYS: the head whose bias is in myvec
@@ -783,7 +782,7 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
         bits = (uint64_t)b0 | ((uint64_t)b1 << 32);
         full = (~bits & ((1ull << HC) - 1)) == 0;
       }
-      if (!KEYS && t + 2 >= wholes) keys = key_bytes(p, b, y0 + 2 * NT + hh * HC, end);  // this team's next tile's, on their way
+      if (!KEYS && t + 2 >= wholes) keys = key_bytes(p, b, y0 + 2 * NT + hh * HC, big_slot[1]);  // this team's next tile's, on their way
       // relative position of column 0 against row 0, and how it moves: -row + column (queries own the rows) or +row - column
       const int rel0 = KEYS ? x0 - y0 - p.q_off : y0 - x0 - p.q_off;
       const bool near = KEYS ? (rel0 - (NT - 1) < p.R && rel0 + 127 > -p.R) : (rel0 - 127 < p.R && rel0 + (NT - 1) > -p.R);
@@ -866,7 +865,7 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
         if (KEYS || full) walk(no{}, no{});
         else walk(no{}, std::integral_constant<bool, !KEYS>{});
       }
-      if (!KEYS && !full && (p.mask != nullptr || end < p.Sk)) {
+      if (!KEYS && !full) {
         // hidden keys may hold anything, and 0 * NaN is NaN in the dS K product: clear their rows of K
         for (int i = lane; i < HC; i += 32)
           if (!((bits >> i) & 1ull) && quarter < 2 * C::DCH) {
@@ -919,7 +918,7 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
       // on one side) that bucket's sum is minus the others': what an error of delta leaves in a bucket goes with the share of P
       // there. A NaN or infinity that only the bucket itself has stays
       if (w16 == 0) {
-        const int big = row_keys[0];
+        const int big = *big_slot;
         float rest = 0.f;
         for (int i = lane; i < p.nb; i += 32) rest += i == big ? 0.f : dscr[i];
         rest = warp_sum(rest);
