@@ -183,3 +183,25 @@ def test_a_row_with_one_key_has_no_gradient_of_its_scores(dt, D):
     v[0, 0, 0, 1] = NAN
     got = _run(q, k, v, table, None, go, **kw)
     assert torch.isnan(got["dq"][0, 0, 0]).any() and torch.isnan(got["dtable"][:, 0]).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("up", [-24, -16, -12, 0, 9])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("causal", [False, True])
+def test_half_gradients_of_any_magnitude(up, D, causal):
+    """Gradients of an f16 call are as good for a loss that was not scaled as for one that was: relative to their norm, and to
+    half a step of f16's smallest numbers."""
+    Sq, Sk, dt = 260, 900, torch.float16
+    q, k, v, go, table, m = _case(2, 4, 2, Sq, Sk, D, dt, D + 100, "tail")
+    if up > 0:  # rows that look at one key: dS as large as dP
+        q, v = q * 6, v * 4
+    go = torch.ldexp(go.float(), torch.tensor(up)).to(dt)
+    kw = dict(causal=causal, bidirectional=not causal, q_offset=Sk - Sq if causal else 0)
+    ref = ot.bias_attention(q, k, v, table, key_mask=m, go=go, **kw)
+    got = _run(q, k, v, table, m, go, **kw)
+    for n in ("dq", "dk", "dv"):
+        assert ref[n].abs().max() < 60000
+        mags = 0.0 if n == "dv" else 2.0 ** -20 * ref[n + "_abs"].norm().item()
+        _near(got[n], ref[n], GRAD[dt], n, 1e-9 * 2.0 ** up + mags + 2.0 ** -25 * ref[n].numel() ** 0.5)
+    _tight(got, ref, [15, 31])

@@ -157,7 +157,7 @@ struct Plan {
   int nsplit = 1;
   int ntq = 0;               // query tiles of the bias-gradient partial sums
   int sq_pad = 0;            // tensor-core backward: rows of (lse, delta) per head
-  uint64_t part_o = 0, part_ml = 0, delta = 0, dtab = 0, bytes = 0;  // offsets into the workspace
+  uint64_t part_o = 0, part_ml = 0, delta = 0, dtab = 0, norms = 0, bytes = 0;  // offsets into the workspace
 };
 
 uint64_t up16(uint64_t v) { return (v + 15) / 16 * 16; }
@@ -206,7 +206,8 @@ Plan make_plan(const b2_bias_attn_args* a, bool bwd) {
     pl.delta = 0;
     pl.sq_pad = (int)((a->Sq + kTcPad - 1) / kTcPad * kTcPad);
     pl.dtab = pl.tc ? (uint64_t)(a->B * a->H) * pl.sq_pad * 8 : up16((uint64_t)rows * 4);
-    pl.bytes = pl.dtab + (a->dtable ? up16((uint64_t)(a->B * a->H * tq) * a->num_buckets * 4) : 0);
+    pl.norms = pl.dtab + (a->dtable ? up16((uint64_t)(a->B * a->H * tq) * a->num_buckets * 4) : 0);
+    pl.bytes = pl.norms + (pl.tc && a->dtype == B2_F16 ? up16((uint64_t)(a->B * a->Hk) * 8) : 0);
   }
   if (pl.nsplit > 1) {
     pl.part_o = 0;
@@ -340,6 +341,10 @@ extern "C" int b2_bias_attn_bwd(const b2_bias_attn_args* a, b2_stream_t stream) 
   p.delta = delta;
   p.dtab = a->dtable ? (float*)((char*)a->workspace + pl.dtab) : nullptr;
   if (pl.tc) {
+    if (a->dtype == B2_F16) {
+      p.norms = (uint32_t*)((char*)a->workspace + pl.norms);
+      if (int rc = check_cuda(cudaMemsetAsync(p.norms, 0, (size_t)(a->B * a->Hk) * 8, st), "bias_attn_bwd memset")) return rc;
+    }
     if (int rc = tc_bwd(p, a->dtype == B2_BF16, (float2*)delta, pl.sq_pad, st)) return rc;
   } else {
     if (int rc = by_dtype<Delta>(a->dtype, p, delta, st)) return rc;

@@ -32,6 +32,7 @@ struct Params {
   void* dk;
   void* dv;
   const float* delta;   // [B*H*Sq] rowsum(dO * O)
+  uint32_t* norms;      // [B*Hk][2] bits of the largest squared norms of a dO row and of a V row, f16 on the tensor cores
   float* dtab;          // [B*H][query tiles][num_buckets] partial sums, NULL: not wanted
   float* part_o;        // [nsplit][B*H*Sq][D] unnormalised outputs of the key splits
   float2* part_ml;      // [nsplit][B*H*Sq] (running maximum in log2 units, sum)

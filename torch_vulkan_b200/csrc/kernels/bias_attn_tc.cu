@@ -579,6 +579,16 @@ __device__ __forceinline__ void add_diagonals(const float* v, float* arr, int re
   add_at(arr, rel + lane - 31, lane < 15 ? scratch[lane] : 0.f, lane < 15, R, lane);
 }
 
+// f16: the exponent of the factor that dS is rounded under, as large as it can be: |dS| <= |dP| + |delta| <= 2 max |dO_i| max |V_j|,
+// which it brings to 2^13.5 .. 2^15 for the rows of a key/value head. Without it the gradients of a loss that was not scaled lose
+// bits: dq of 1000 keys is 0.37 % off at dO = 2^-12 and 5.6 % at 2^-16, where the rounding to f16 alone leaves 0.04 % and 0.5 %.
+__device__ __forceinline__ int ds_up(const Params& p, int b, int hk) {
+  const uint2 n = *reinterpret_cast<const uint2*>(p.norms + 2 * ((int64_t)b * p.Hk + hk));
+  const int exps = (int)(n.x >> 23) + (int)(n.y >> 23) - 2 * 127;  // of the two squared norms together
+  return n.x && n.y ? max(-40, min(60, 13 - ((exps + 1) >> 1))) : 0;
+}
+__device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+
 // block: index among the blocks of this side, xtiles of them per head.
 template <int D, bool BF16, bool KEYS>
 __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensorMap& tmX2, const CUtensorMap& tmY1,
@@ -736,9 +746,10 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
     const uint32_t buf0 = tbase + hh * HC + lane_off;  // this warp's columns of S (and, + T_DP, of dP) in the first buffer
     const float sl2 = p.scale * kLog2e;
     const float2 sl22 = make_float2(sl2, sl2);
-    // f16: P carries a factor of 2^8 (in its bias) so that 1 / Sk stays clear of the subnormals; dS does not
+    // f16: P carries a factor of 2^8 (in its bias) so that 1 / Sk stays clear of the subnormals; dS carries 2^ds_up
     constexpr float PUP = BF16 ? 0.f : 8.f;
     constexpr float PDOWN = BF16 ? 1.f : 1.f / 256.f;
+    float ds_mul = PDOWN;
     float* myvec = KEYS ? vec + g * vlen4 : vec;
     float* mydarr = darr + w16 * dlen + p.R;         // centred on relative position 0
     float* myscr = dscr + w16 * 16;
@@ -752,6 +763,7 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
         for (int i = (int)threadIdx.x - 64; i < 16 * dlen; i += C::EW) darr[i] = 0.f;
       tc::named_bar_sync(1, C::EW);
       if (sees_one(p, x0 + r, seen.first, seen.second) && isfinite(nL + nd)) nL = -INFINITY;  // dS = 0; a NaN goes its way
+      if (!BF16) nL += (float)ds_up(p, b, hx / G);  // P times 2^ds_up: this side needs it for dS alone
     }
     float far_lo = 0.f, far_hi = 0.f;
     int cur = -1;  // KEYS: the head whose bias is in myvec
@@ -772,6 +784,7 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
         tc::named_bar_sync(2 + g, 256);
         cur = gi;
         b_lo = myvec[0], b_hi = myvec[vec_len(p) - 1];
+        if (!BF16) ds_mul = PDOWN * exp2i(ds_up(p, b, hx));
       }
       // after a wait that ran out the tiles are still counted off, so that the team meets at the barriers above
       if (!ok) continue;
@@ -825,7 +838,7 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
             const float2 x = __ffma2_rn(make_float2(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), sl22, off);
             const float2 pr = make_float2(ex2(x.x), ex2(x.y));
             float2 dd = __fadd2_rn(make_float2(__uint_as_float(dp[2 * e]), __uint_as_float(dp[2 * e + 1])), del);
-            if (KEYS && !BF16) dd = __fmul2_rn(dd, make_float2(PDOWN, PDOWN));
+            if (KEYS && !BF16) dd = __fmul2_rn(dd, make_float2(ds_mul, ds_mul));
             float2 ds = __fmul2_rn(pr, dd);
             if (MASK) {
               if (!((bits >> col) & 1ull)) ds.x = 0.f;
@@ -882,6 +895,7 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&pd_full[bi]);
     }
+    const float ds_down = BF16 ? 1.f : exp2i(-ds_up(p, b, KEYS ? hx : hx / G));
     if (!KEYS && p.dtab) {
       // this warp's far tiles join the ends of its array; then the arrays are added and cut into buckets
       const float lo = warp_sum(far_lo), hi = warp_sum(far_hi);
@@ -911,7 +925,7 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
             for (int d = 1 + lane; d <= p.R; d += 32) s += vec[p.R + d];
         }
         s = warp_sum(s);
-        if (lane == 0) dscr[bk] = s;
+        if (lane == 0) dscr[bk] = s * ds_down;
       }
       tc::named_bar_sync(1, C::EW);
       // A row of dS adds up to zero over its keys. Where most visible keys of the block lie in one bucket (beyond the last threshold
@@ -940,7 +954,7 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
         const int which = job / CH, c = job % CH;  // KEYS: dV, then dK
         const bool wanted = KEYS ? (which ? p.dk != nullptr : p.dv != nullptr) : p.dq != nullptr;
         if (!wanted) continue;
-        const float mul = KEYS ? (which ? p.scale : PDOWN) : p.scale;
+        const float mul = KEYS && !which ? PDOWN : p.scale * ds_down;
         const CUtensorMap* tm = which ? &tmG2 : &tmG1;
         uint32_t v[32], w[16];
         __syncwarp();
@@ -995,19 +1009,59 @@ __global__ void __launch_bounds__(608, 1)
     bwd_side<D, BF16, false>(m.qx, m.gx, m.ky, m.vy, m.dq, m.dq, p, lsed, sq_pad, (int)blockIdx.x - key_blocks, query_tiles);
 }
 
+// Sum over eight lanes (a row of the prepared tensors).
+__device__ __forceinline__ float sum8(float s) {
+  s += __shfl_xor_sync(0xffffffffu, s, 1);
+  s += __shfl_xor_sync(0xffffffffu, s, 2);
+  return s + __shfl_xor_sync(0xffffffffu, s, 4);
+}
+// The block's largest finite value of x >= 0, into *at: floats without a sign are ordered as their bits, and a maximum does not
+// depend on the order.
+__device__ __forceinline__ void block_max(float x, uint32_t* at) {
+  __shared__ uint32_t top[8];
+  const uint32_t m = __reduce_max_sync(0xffffffffu, x <= 3.4e38f ? __float_as_uint(x) : 0u);
+  if ((threadIdx.x & 31) == 0) top[threadIdx.x >> 5] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    uint32_t t = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t = max(t, top[i]);
+    if (t) atomicMax(at, t);
+  }
+}
+
 // lsed[bh][q] = (-lse log2 e, -sum_d dO O) for q < Sq, (-inf, 0) for padding and for rows without a key: exp2(x - inf) = 0.
-// Eight lanes a row, 16-byte loads.
+// Eight lanes a row, 16-byte loads, 32 rows of one head a block. With p.norms (f16), the blocks from row_blocks on take the rows
+// of V that some query sees, and both kinds record their largest norm.
 template <typename T>
-__global__ void __launch_bounds__(256) bias_bwd_prep(const __grid_constant__ Params p, float2* __restrict__ lsed, int sq_pad) {
+__global__ void __launch_bounds__(256) bias_bwd_prep(const __grid_constant__ Params p, float2* __restrict__ lsed, int sq_pad,
+                                                     int64_t row_blocks) {
   tc::pdl_wait();
   tc::pdl_trigger();
-  const int64_t idx = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 3;
-  const int part = threadIdx.x & 7;
-  const int64_t bh = idx / sq_pad;
+  const int part = threadIdx.x & 7, r = threadIdx.x >> 3;
+  if ((int64_t)blockIdx.x >= row_blocks) {
+    const int tiles = (p.Sk + 31) / 32;
+    const int64_t vb = blockIdx.x - row_blocks, bh = vb / tiles;
+    const int j = (int)(vb - bh * tiles) * 32 + r, b = (int)(bh / p.Hk);
+    float s = 0.f;
+    if (j < key_end(p, p.Sq - 1) && (p.mask == nullptr || p.mask[(int64_t)b * p.mask_sb + j] != 0)) {
+      const T* v = row_of<T>(p.v, p.v_s, b, (int)(bh % p.Hk), j);
+      for (int d = part * 8; d < p.D; d += 64) {
+        const uint4 raw = *reinterpret_cast<const uint4*>(v + d);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float x = to_f32<T>(reinterpret_cast<const T*>(&raw)[i]);
+          s = fmaf(x, x, s);
+        }
+      }
+    }
+    block_max(sum8(s), p.norms + 2 * bh + 1);
+    return;
+  }
+  const int64_t idx = (int64_t)blockIdx.x * 32 + r, bh = idx / sq_pad;
   const int q = (int)(idx - bh * sq_pad);
-  if (bh >= (int64_t)p.B * p.H) return;  // whole groups of eight lanes; warps of the last block may be partial
   const int b = (int)(bh / p.H), h = (int)(bh % p.H);
-  float s = 0.f;
+  float s = 0.f, g2 = 0.f;
   if (q < p.Sq) {
     const T* o = row_of<T>((const void*)p.o, p.o_s, b, h, q);
     const T* g = row_of<T>(p.d_o, p.do_s, b, h, q);
@@ -1026,15 +1080,18 @@ __global__ void __launch_bounds__(256) bias_bwd_prep(const __grid_constant__ Par
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) s = fmaf(a[i], to_f32<T>(c[i]), s);
+      if (std::is_same<T, __half>::value) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g2 = fmaf(to_f32<T>(c[i]), to_f32<T>(c[i]), g2);
+      }
     }
   }
-  const uint32_t m = __activemask();
-  s += __shfl_xor_sync(m, s, 1);
-  s += __shfl_xor_sync(m, s, 2);
-  s += __shfl_xor_sync(m, s, 4);
-  if (part == 0) {
-    const float lse = q < p.Sq ? p.lse[bh * p.Sq + q] : -INFINITY;
-    lsed[idx] = lse == -INFINITY ? make_float2(-INFINITY, 0.f) : make_float2(-lse * kLog2e, -s);
+  s = sum8(s);
+  const float lse = q < p.Sq ? p.lse[bh * p.Sq + q] : -INFINITY;
+  if (part == 0) lsed[idx] = lse == -INFINITY ? make_float2(-INFINITY, 0.f) : make_float2(-lse * kLog2e, -s);
+  if (std::is_same<T, __half>::value) {
+    g2 = sum8(g2);
+    block_max(lse == -INFINITY ? 0.f : g2, p.norms + 2 * ((int64_t)b * p.Hk + h / (p.H / p.Hk)));
   }
 }
 
@@ -1084,9 +1141,11 @@ int bwd_smem(const Params& p) {
 template <int D, bool BF16>
 int bwd_t(const Params& p, float2* lsed, int sq_pad, cudaStream_t st) {
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
-  const int64_t rows = (int64_t)p.B * p.H * sq_pad;
-  if (int rc = launch_pdl("bias_attn_bwd_prep", bias_bwd_prep<T>, dim3((unsigned)((rows * 8 + 255) / 256)), dim3(256), 0, st, p,
-                          lsed, sq_pad))
+  static_assert(kTcPad % 32 == 0, "whole blocks of rows per head");
+  const int64_t row_blocks = (int64_t)p.B * p.H * (sq_pad / 32), v_blocks = BF16 ? 0 : (int64_t)p.B * p.Hk * ((p.Sk + 31) / 32);
+  if (row_blocks + v_blocks >= (1ll << 31)) return fail(B2_ERR_ARG, "bias_attn_bwd: too many rows");
+  if (int rc = launch_pdl("bias_attn_bwd_prep", bias_bwd_prep<T>, dim3((unsigned)(row_blocks + v_blocks)), dim3(256), 0, st, p,
+                          lsed, sq_pad, row_blocks))
     return rc;
   using Q = Bwd<D, false>;
   using K = Bwd<D, true>;
