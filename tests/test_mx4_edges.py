@@ -33,3 +33,30 @@ def test_no_output_features_and_no_rows():
             assert y.shape == (m, n)
             for t, g in zip(leaf, torch.autograd.grad(y, leaf, torch.ones_like(y))):
                 assert g.shape == t.shape and not g.any()
+
+
+def test_lora_ranks_that_do_not_fit_are_refused_by_the_constructors():
+    """Before anything is built: on the CPU."""
+    from torch_vulkan_b200.dit import DiTBlock, LoRAMx4Linear
+    from torch_vulkan_b200.text_encoder import TextEncoder
+
+    for rank in (0, 4, 12, 24, 32, 128):
+        with pytest.raises(ValueError, match="at most 16 where 3"):
+            DiTBlock(hidden=256, heads=2, text_dim=128, mlp=512, rank=rank, base="mx4", device="cpu")
+    for rank in (4, 40, 64):
+        with pytest.raises(ValueError, match="at most 32 where 2"):
+            TextEncoder(blocks=1, hidden=256, heads=4, mlp=512, rank=rank, device="cpu")
+    for rank in (4, 72):
+        with pytest.raises(ValueError, match="at most 64"):
+            LoRAMx4Linear(64, 64, rank=rank, device="cpu")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rank", [8, 16])
+def test_lora_ranks_that_fit(rank):
+    from torch_vulkan_b200.dit import DiTBlock, synthetic_batch
+    from torch_vulkan_b200.text_encoder import TextEncoder
+
+    x, text, cond, _ = synthetic_batch(tokens=64, text_tokens=32, hidden=256, text_dim=128, seed=7)
+    assert torch.isfinite(DiTBlock(hidden=256, heads=2, text_dim=128, mlp=512, rank=rank, base="mx4")(x, text, cond)).all()
+    assert torch.isfinite(TextEncoder(blocks=1, hidden=256, heads=4, mlp=512, rank=2 * rank)(x)).all()

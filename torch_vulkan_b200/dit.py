@@ -85,11 +85,19 @@ class Mx4Linear(nn.Module):
         return tv.mx4_linear(x, self.weight, self.bias)
 
 
+def check_mx4_rank(rank, modules=1):
+    """The LoRA term of a 4-bit product has 8 to 64 columns in whole groups of 8, of all modules that share the product."""
+    if rank < 8 or rank % 8 or rank * modules > 64:
+        raise ValueError(f"LoRA rank {rank}: over a 4-bit base it must be a multiple of 8 and at most {64 // modules // 8 * 8}"
+                         + (f" where {modules} projections share one product" if modules > 1 else ""))
+
+
 class LoRAMx4Linear(nn.Module):
     """Frozen 4-bit base + trainable LoRA: y = base(x) + (x A^T) B^T * alpha / r, the LoRA term in the same product."""
 
     def __init__(self, in_f, out_f, rank=16, alpha=16.0, generator=None, device="cuda", dtype=torch.bfloat16):
         super().__init__()
+        check_mx4_rank(rank)
         self.base = Mx4Linear(in_f, out_f, bias=True, generator=generator, device=device)
         gdev = generator.device if generator else device
         self.lora_down = nn.Parameter((torch.randn(rank, in_f, generator=generator, device=gdev) / math.sqrt(in_f)).to(dtype).to(device))
@@ -278,7 +286,8 @@ class _StackedSDPA(torch.autograd.Function):
 
 class DiTBlock(nn.Module):
     """base="int8": frozen int8 weights (the default); base="mx4": frozen 4-bit weights, half the memory, whose products
-    run on the block-scaled tensor cores with the activations quantised per call (hidden a multiple of 128)."""
+    run on the block-scaled tensor cores with the activations quantised per call (hidden a multiple of 128, LoRA rank 8 or 16:
+    three projections share a product, which takes 64 columns of LoRA)."""
 
     def __init__(self, hidden=2048, heads=16, text_dim=1024, mlp=8192, rank=16, alpha=16.0, seed=0, device="cuda", base="int8"):
         super().__init__()
@@ -286,6 +295,8 @@ class DiTBlock(nn.Module):
             raise ValueError(f"DiTBlock: base must be 'int8' or 'mx4', got {base!r}")
         if base == "mx4" and hidden % 128:
             raise ValueError(f"DiTBlock: a 4-bit base stacks its projections by 128 rows; hidden {hidden} is no multiple")
+        if base == "mx4":
+            check_mx4_rank(rank, 3)
         self.base = base
         frozen = Int8Linear if base == "int8" else Mx4Linear
         lora = LoRAInt8Linear if base == "int8" else LoRAMx4Linear

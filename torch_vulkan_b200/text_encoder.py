@@ -14,7 +14,7 @@ import torch.nn.functional as F
 
 import torch_vulkan_b200 as tv
 
-from .dit import LoRAGroup, LoRAMx4Linear, Mx4Linear, make_optimizer, stacked_mx4_lora_forward
+from .dit import LoRAGroup, LoRAMx4Linear, Mx4Linear, check_mx4_rank, make_optimizer, stacked_mx4_lora_forward
 
 
 class TextEncoderBlock(nn.Module):
@@ -22,6 +22,7 @@ class TextEncoderBlock(nn.Module):
         super().__init__()
         if hidden % heads or hidden % 128:
             raise ValueError(f"TextEncoderBlock: hidden {hidden} must be a multiple of 128 and of the {heads} heads")
+        check_mx4_rank(rank, 2)  # k and v share a product
         g = torch.Generator(device=device).manual_seed(seed)
         mk = lambda: LoRAMx4Linear(hidden, hidden, rank, alpha, generator=g, device=device)  # noqa: E731
         self.h, self.heads, self.d, self.max_distance = hidden, heads, hidden // heads, max_distance
