@@ -60,3 +60,11 @@ def test_lora_ranks_that_fit(rank):
     x, text, cond, _ = synthetic_batch(tokens=64, text_tokens=32, hidden=256, text_dim=128, seed=7)
     assert torch.isfinite(DiTBlock(hidden=256, heads=2, text_dim=128, mlp=512, rank=rank, base="mx4")(x, text, cond)).all()
     assert torch.isfinite(TextEncoder(blocks=1, hidden=256, heads=4, mlp=512, rank=2 * rank)(x)).all()
+
+
+def test_lowered_scales_keep_a_nan():
+    from torch_vulkan_b200.text_encoder import _shift_scales
+
+    s = torch.tensor([0, 1, 2, 3, 4, 100, 252, 255], dtype=torch.uint8)
+    assert _shift_scales(s, 64).tolist() == [0, 0, 0, 0, 1, 97, 249, 255]
+    assert _shift_scales(s, 16).tolist() == [0, 0, 0, 1, 2, 98, 250, 255]

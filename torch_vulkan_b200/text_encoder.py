@@ -62,7 +62,8 @@ class TextEncoder(nn.Module):
         g = torch.Generator().manual_seed(seed + 1000)
         self.table = nn.Parameter((0.1 * torch.randn(num_buckets, heads, generator=g)).to(device))
         self.register_buffer("ln", torch.ones(hidden, dtype=torch.bfloat16, device=device))
-        # an encoder without a score scale carries 1 / sqrt(d) in its query weights: here in the normalisation they read
+        # an encoder without a score scale carries 1 / sqrt(d) in its query weights: here a power of two near it, which the scales
+        # of a 4-bit weight take exactly (1/8 for a head dim from 64 to 255)
         for b in self.blocks:
             with torch.no_grad():
                 b.q.base.scales.copy_(_shift_scales(b.q.base.scales, b.d))
@@ -83,8 +84,9 @@ def _half_log2(d: int) -> int:
 
 
 def _shift_scales(scales: torch.Tensor, d: int) -> torch.Tensor:
-    """MXFP4 scale codes of W / 2^(log2(d) / 2): the exponents lowered (not below 2^-127)."""
-    return (scales.to(torch.int16) - _half_log2(d)).clamp_(min=0).to(torch.uint8)
+    """MXFP4 scale codes of W / 2^_half_log2(d): the exponents lowered (not below 2^-127); the NaN scale (255) stays."""
+    lower = (scales.to(torch.int16) - _half_log2(d)).clamp_(min=0).to(torch.uint8)
+    return torch.where(scales == 255, scales, lower)
 
 
 class ConditionedTrainer:
