@@ -212,14 +212,14 @@ class _StackedMx4LoRA(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, gy):
-        sources = (gy, ctx.saved_tensors[0], *ctx.params)
-        gx, *rest = refuse_second("stacked mx4_lora_linear", _StackedMx4LoRA.gradients(ctx, gy), sources)
+        saved = ctx.saved_tensors  # once: activation checkpointing hands them out a single time
+        grads = _StackedMx4LoRA.gradients(ctx, gy, *saved)
+        gx, *rest = refuse_second("stacked mx4_lora_linear", grads, (gy, saved[0], *ctx.params))
         return (gx, None, None, None, None, *rest)
 
     @staticmethod
     @torch.no_grad()
-    def gradients(ctx, gy):
-        x, codes, scales, h = ctx.saved_tensors
+    def gradients(ctx, gy, x, codes, scales, h):
         grp = ctx.grp
         x2 = x.reshape(-1, x.shape[-1])
         if not x2.is_contiguous():
