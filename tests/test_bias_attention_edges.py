@@ -205,3 +205,40 @@ def test_half_gradients_of_any_magnitude(up, D, causal):
         mags = 0.0 if n == "dv" else 2.0 ** -20 * ref[n + "_abs"].norm().item()
         _near(got[n], ref[n], GRAD[dt], n, 1e-9 * 2.0 ** up + mags + 2.0 ** -25 * ref[n].numel() ** 0.5)
     _tight(got, ref, [15, 31])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("Sq,D", [(1, 64), (8, 128), (150, 64), (150, 128), (150, 20)])
+@pytest.mark.parametrize("low", [-torch.finfo(torch.float32).max, -INF])
+def test_a_bucket_of_the_lowest_bias_is_left_out(dt, Sq, D, low):
+    """A table entry of fp32's lowest value hides its keys as -inf does; a row that has no others gets zeros."""
+    q, k, v, go, table, _ = _case(2, 2, 2, Sq, 300, D, dt, D)
+    table[3], table[7, 0], table[12:16], table[20:] = low, low, low, low
+    kw = dict(q_offset=40)
+    ref = ot.bias_attention(q, k, v, table.clamp(min=-INF if low == -INF else -1e30), go=go, **kw)
+    got = _run(q, k, v, table, None, go, **kw)
+    _near(got["o"], ref["o"], OUT[dt], "o")
+    _near(_infer(q, k, v, table, None, **kw), ref["o"], OUT[dt], "o")
+    for n in ("dq", "dk", "dv"):
+        _near(got[n], ref[n], GRAD[dt], n, 1e-9 if n == "dv" else 1e-9 + 2.0 ** -20 * ref[n + "_abs"].norm().item())
+    for i in [3, *range(12, 16), *range(20, 32)]:
+        assert not got["dtable"][i].any()
+    table[:, 1] = low
+    got = _run(q, k, v, table, None, go, **kw)
+    assert not got["o"][:, 1].any() and not got["dq"][:, 1].any() and not got["dk"][:, 1].any() and not got["dv"][:, 1].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("bidirectional,off", [(True, 1300), (True, 0), (False, 1300)])
+def test_a_far_bucket_of_little_weight_keeps_its_own_accuracy(dt, D, bidirectional, off):
+    """A table that has learned to look nearby: the far buckets hold most keys and almost no weight, and their small gradients
+    are not made from the large ones."""
+    Sq, Sk = 200, 1500
+    q, k, v, go, table, _ = _case(1, 2, 2, Sq, Sk, D, dt, D)
+    table[[15, 31] if bidirectional else [31]] = -16.0
+    kw = dict(q_offset=off, bidirectional=bidirectional, causal=not bidirectional)
+    ref = ot.bias_attention(q, k, v, table, go=go, **kw)
+    _tight(_run(q, k, v, table, None, go, **kw), ref, [])

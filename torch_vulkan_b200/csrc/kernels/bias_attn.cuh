@@ -86,23 +86,23 @@ __device__ __forceinline__ int key_end(const Params& p, int64_t last_row) {
   return e < 0 ? 0 : (e < p.Sk ? (int)e : p.Sk);
 }
 
-// What the mask leaves of the keys below `end`: one past the last, how many there are, how many up to key lo and from key hi on,
-// and the first two (INT_MAX: there is none). Every thread of the block calls it and gets the same; the row of the mask is read at
-// once, in one trip to memory. slot: six ints of shared memory per warp, free again after the block's next barrier.
+// What the mask leaves of the keys below `end`: one past the last, how many up to key lo and from key hi on, and the first two
+// (INT_MAX: there is none). Every thread of the block calls it and gets the same; the row of the mask is read at
+// once, in one trip to memory. slot: five ints of shared memory per warp, free again after the block's next barrier.
 struct Visible {
-  int last, total, past, ahead, first, second;
+  int last, past, ahead, first, second;
 };
 __device__ __forceinline__ Visible visible_keys(const Params& p, int b, int end, int lo, int hi, int nthreads, int* slot) {
   constexpr int NONE = 0x7fffffff;
   if (p.mask == nullptr)
-    return {end, end, max(0, min(end, lo + 1)), max(0, end - max(0, hi)), end > 0 ? 0 : NONE, end > 1 ? 1 : NONE};
+    return {end, max(0, min(end, lo + 1)), max(0, end - max(0, hi)), end > 0 ? 0 : NONE, end > 1 ? 1 : NONE};
   const uint8_t* m = p.mask + (int64_t)b * p.mask_sb;
-  Visible v = {0, 0, 0, 0, NONE, NONE};
+  Visible v = {0, 0, 0, NONE, NONE};
 #pragma unroll 8
   for (int j = (int)threadIdx.x; j < end; j += nthreads) {
     const bool on = m[j] != 0;
     v.last = on ? j + 1 : v.last;
-    v.total += on, v.past += on && j <= lo, v.ahead += on && j >= hi;
+    v.past += on && j <= lo, v.ahead += on && j >= hi;
     v.second = on ? min(v.second, max(v.first, j)) : v.second;
     v.first = on ? min(v.first, j) : v.first;
   }
@@ -110,19 +110,18 @@ __device__ __forceinline__ Visible visible_keys(const Params& p, int b, int end,
   auto join = [](Visible a, bool counts) -> Visible {
     const unsigned all = 0xffffffffu;
     const int first = __reduce_min_sync(all, a.first);
-    return {__reduce_max_sync(all, a.last), __reduce_add_sync(all, counts ? a.total : 0),
-            __reduce_add_sync(all, counts ? a.past : 0), __reduce_add_sync(all, counts ? a.ahead : 0), first,
-            __reduce_min_sync(all, a.first == first ? a.second : a.first)};
+    return {__reduce_max_sync(all, a.last), __reduce_add_sync(all, counts ? a.past : 0),
+            __reduce_add_sync(all, counts ? a.ahead : 0), first, __reduce_min_sync(all, a.first == first ? a.second : a.first)};
   };
   v = join(v, true);
   const int lane = threadIdx.x & 31, warps = nthreads / 32;
   if (lane == 0) {
-    int* s = slot + (threadIdx.x >> 5) * 6;
-    s[0] = v.last, s[1] = v.total, s[2] = v.past, s[3] = v.ahead, s[4] = v.first, s[5] = v.second;
+    int* s = slot + (threadIdx.x >> 5) * 5;
+    s[0] = v.last, s[1] = v.past, s[2] = v.ahead, s[3] = v.first, s[4] = v.second;
   }
   __syncthreads();
-  const int* s = slot + min(lane, warps - 1) * 6;
-  return join(Visible{s[0], s[1], s[2], s[3], s[4], s[5]}, lane < warps);
+  const int* s = slot + min(lane, warps - 1) * 5;
+  return join(Visible{s[0], s[1], s[2], s[3], s[4]}, lane < warps);
 }
 // Whether query row i sees exactly one key. P is 1 there whatever the score, so dS is zero.
 __device__ __forceinline__ bool sees_one(const Params& p, int i, int first, int second) {

@@ -82,12 +82,26 @@ __device__ __forceinline__ int trim_end(const Params& p, int b, int end, int nth
   return *slot;
 }
 
+// One past the last threshold's distance: where a side's far bucket begins.
+__device__ __forceinline__ int far_from(const Params& p) { return p.thr[(p.bidir ? p.nb / 2 : p.nb) - 2]; }
+
 // The bucket whose sum the query side of the backward takes from the others' (see the end of bwd_side), or -1: the far bucket of
-// one side where it holds more than half of the keys that the block's middle row sees. Only visible keys count, so that the
-// bucket has a pair.
-__device__ __forceinline__ int big_bucket(const Params& p, const Visible& v) {
-  const int side = p.bidir ? p.nb / 2 : p.nb;
-  return 2 * v.past > v.total ? side - 1 : !p.causal && 2 * v.ahead > v.total ? (p.bidir ? p.nb - 1 : 0) : -1;
+// one side where it has more than half of the weight of what the block's middle row sees, exp(bias) for each visible key (v counts
+// the far ones; one-sided, keys after the query share bucket 0). So it has a pair, and a bucket that the table all but hides is
+// left alone. vec: the head's bias. A whole warp calls it.
+__device__ __forceinline__ int big_bucket(const Params& p, const Visible& v, const float* vec, int b, int mid, int end) {
+  const int side = p.bidir ? p.nb / 2 : p.nb, far = far_from(p), lane = threadIdx.x & 31;
+  const float* at = vec + p.R + kPad;  // centred on relative position 0
+  const uint8_t* m = p.mask ? p.mask + (int64_t)b * p.mask_sb : nullptr;
+  const float past = v.past > 0 ? at[-far] : -INFINITY, ahead = v.ahead > 0 ? at[p.bidir ? far : 1] : -INFINITY;
+  const int first = max(1 - far, -mid), last = min(p.bidir ? far - 1 : p.causal ? 0 : -1, end - 1 - mid);
+  const float top = fmaxf(past, ahead);
+  if (top == -INFINITY) return -1;
+  float near = 0.f;  // infinite where the far keys weigh next to nothing beside it
+#pragma unroll 8
+  for (int r = first + lane; r <= last; r += 32) near += m == nullptr || m[mid + r] != 0 ? ex2(at[r] - top) : 0.f;
+  const float wp = v.past * ex2(past - top), wa = v.ahead * ex2(ahead - top), half = 0.5f * (warp_sum(near) + wp + wa);
+  return wp > half ? side - 1 : wa > half ? (p.bidir ? p.nb - 1 : 0) : -1;
 }
 
 // A warp's 32 rows of O (TMEM, relative to the maximum m) and their earlier part (relative to run_m): in TMEM columns of its own
@@ -635,6 +649,7 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
     tc::tmem_relinquish();
   }
   Visible seen = {};
+  const int mid = x0 + min(C::BX, p.Sq - x0) / 2 + p.q_off;  // !KEYS: the position of the block's middle row
   int first = 0, tiles, end = p.Sk;  // tiles first .. first + tiles of every walked head; !KEYS: one past the last key
   if (KEYS) {
     const int any = p.mask == nullptr ||
@@ -644,10 +659,8 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
     if (p.causal) first = (int)min((int64_t)nt, max((int64_t)0, (int64_t)x0 - p.q_off) / NT);
     tiles = any ? nt - first : 0;
   } else {
-    // far from the block's middle row; one-sided: keys after the query share bucket 0
-    const int beyond = p.thr[(p.bidir ? p.nb / 2 : p.nb) - 2], mid = x0 + min(C::BX, p.Sq - x0) / 2 + p.q_off;
-    seen = visible_keys(p, b, key_end(p, min(x0 + C::BX, p.Sq) - 1), mid - beyond, p.bidir ? mid + beyond : mid, C::THREADS,
-                        reinterpret_cast<int*>(vec));
+    seen = visible_keys(p, b, key_end(p, min(x0 + C::BX, p.Sq) - 1), mid - far_from(p), p.bidir ? mid + far_from(p) : mid,
+                        C::THREADS, reinterpret_cast<int*>(vec));
     end = seen.last;
     if (threadIdx.x == 0) big_slot[1] = end;
     tiles = (end + NT - 1) / NT;
@@ -757,11 +770,14 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
     if (!KEYS) {  // while the first tiles are loaded and multiplied
       const float2 ld = lsed[((int64_t)b * p.H + hx) * sq_pad + x0 + r];
       nL = ld.x, nd = ld.y;
-      if (w16 == 0 && lane == 0) *big_slot = big_bucket(p, seen);
       fill_vec(p, hx, vec, (int)threadIdx.x - 64, C::EW);
       if (p.dtab)
         for (int i = (int)threadIdx.x - 64; i < 16 * dlen; i += C::EW) darr[i] = 0.f;
       tc::named_bar_sync(1, C::EW);
+      if (w16 == 15 && p.dtab) {  // of the team whose first tile comes later
+        const int big = big_bucket(p, seen, vec, b, mid, end);
+        if (lane == 0) *big_slot = big;
+      }
       if (sees_one(p, x0 + r, seen.first, seen.second) && isfinite(nL + nd)) nL = -INFINITY;  // dS = 0; a NaN goes its way
       if (!BF16) nL += (float)ds_up(p, b, hx / G);  // P times 2^ds_up: this side needs it for dS alone
     }
@@ -928,9 +944,9 @@ __device__ __forceinline__ void bwd_side(const CUtensorMap& tmX1, const CUtensor
         if (lane == 0) dscr[bk] = s * ds_down;
       }
       tc::named_bar_sync(1, C::EW);
-      // A row of dS adds up to zero over its keys. Where most visible keys of the block lie in one bucket (beyond the last threshold
-      // on one side) that bucket's sum is minus the others': what an error of delta leaves in a bucket goes with the share of P
-      // there. A NaN or infinity that only the bucket itself has stays
+      // A row of dS adds up to zero over its keys. Where most of the block's weight lies in one bucket (beyond the last threshold on
+      // one side) that bucket's sum is minus the others': what an error of delta leaves in a bucket goes with the share of P there.
+      // A NaN or infinity that only the bucket itself has stays
       if (w16 == 0) {
         const int big = *big_slot;
         float rest = 0.f;
