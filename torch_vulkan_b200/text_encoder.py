@@ -70,10 +70,14 @@ class TextEncoder(nn.Module):
                 b.q.lora_up.mul_(2.0 ** -_half_log2(b.d))
 
     def forward(self, x, key_mask=None):
+        # what a padded position holds (it may be anything) reaches neither the other positions nor, times zero, a gradient
+        pad = None if key_mask is None else ~key_mask.unsqueeze(-1)
+        if pad is not None:
+            x = x.masked_fill(pad, 0.0)
         for b in self.blocks:
             x = b(x, self.table, key_mask)
         x = F.layer_norm(x, (x.shape[-1],), weight=self.ln, eps=1e-6)
-        return x if key_mask is None else x * key_mask.unsqueeze(-1).to(x.dtype)
+        return x if pad is None else x.masked_fill(pad, 0.0)
 
     def trainable_parameters(self):
         return [p for n, p in self.named_parameters() if "lora_" in n] + [self.table]
