@@ -21,7 +21,9 @@ def bucket_bias_attention(q, k, v, table, key_mask=None, max_distance=128, bidir
     """softmax(scale * q k^T + table[bucket(j - i - q_offset)]) v.
 
     q [B, H, Sq, D], k and v [B, Hk, Sk, D] with H a multiple of Hk (query head h reads key/value head h // (H // Hk)),
-    D at most 128, bf16, f16 or fp32, any strides; table [num_buckets, H], float. key_mask bool [B, Sk], true where a
+    D at most 128, bf16, f16 or fp32, any strides; table [num_buckets, H], float, where an entry of -inf (or below -2.3e38)
+    hides its bucket. The 16-bit backward is many times slower where max_distance is above 591 (D up to 64) or 471 and the
+    table wants its gradient. key_mask bool [B, Sk], true where a
     key may be attended to; causal hides keys after the query's position i + q_offset (a decoder's new token against a
     cache of Sk keys has q_offset = Sk - Sq). scale defaults to 1 / sqrt(D). A query whose keys are all masked gets
     zeros and zero gradients; what k and v hold at masked positions, or (causal) past the last query's, is never used.

@@ -145,7 +145,7 @@ __device__ __forceinline__ void add_run(uint32_t t_o, uint32_t t_sum, float* par
 // scores are multiplied while a softmax runs. Two blocks share an SM (256 TMEM columns, half of the shared memory each), so
 // that one's set-up, softmax and output run beside the other's. The softmax bounds it: 1800 cycles a tile, 800 of them
 // exponentials of two warps on one scheduler (scores are always ready when they are asked for). 16 heads x 4096 x 4096 x 64:
-// 134 us, for a backward (below) 177. One block to an SM with two softmax groups took 24.5 us against 20.8 at B4 H16 S512
+// 135 us, for a backward (below) 170. One block to an SM with two softmax groups took 24.5 us against 20.8 at B4 H16 S512
 // D64 and 110 against 94 at B8 H16 S1024 D128 (padded); tiles of 128 with one score buffer 165 us against 151; two threads
 // to a row, 32 columns each, 213 against 174 (for a backward).
 // ==================================================================================================
@@ -168,8 +168,8 @@ struct Fwd {
 // rounded once, the bias gradient (a sum of dS over many rows) keeps errors of a few 1e-3 of itself. The tensor core also
 // truncates each of its sums towards zero: after 4096 keys (512 of them) O is 8.3e-6 of itself short, and the gradient of a far
 // bucket adds that up over all rows (1e-5 of it). So every RUN tiles the sum joins a sum kept in fp32 elsewhere and the next one
-// starts from zero: 1.1e-6 short at D = 64 (2.0e-6 at D = 128), gradient 2e-6 to 4e-6 off; 163 -> 177 us and, through memory,
-// 183 -> 224 us (16 heads x 4096 x 4096).
+// starts from zero: 1.1e-6 short at D = 64 (2.0e-6 at D = 128), gradient 1e-6 to 2.5e-6 off; 9 % more time and, through memory,
+// 22 % (16 heads x 4096 x 4096).
 template <int D, bool BF16, bool PREC>
 __global__ void __launch_bounds__(192, 2)
     bias_fwd_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -537,8 +537,8 @@ __global__ void __launch_bounds__(192, 2)
 // owner: no atomics, no accumulator in memory, the same bits on every run. Two teams of eight warps take the tiles in turn;
 // in a team, two warps share a lane quarter and split its columns. P and dS (16 bits) replace the scores a warp has read and
 // are the A operands of the gradient MMAs, 8 columns per 16 of the reduction at any place. At D = 64 TMEM holds three tiles,
-// so that the MMAs of one run while both teams work (4 x 16 heads x 512 x 512: 60 us, with two tiles of 96 columns 67). Issue
-// slots bound it: an issuing thread among element-wise warps takes 80 to 140 cycles for a product of 48 (16 heads x 4096 x
+// so that the MMAs of one run while both teams work (4 x 16 heads x 512 x 512: 60 us, with two tiles of 96 columns 67). The two
+// issuing threads bound it: one among element-wise warps takes 80 to 140 cycles for a product of 48 (16 heads x 4096 x
 // 4096: 366 us at D = 64, 464 at 128). Eight element-wise warps, half as many, took 357 us instead of 285 for the key side alone.
 // ==================================================================================================
 template <int D, bool KEYS>
